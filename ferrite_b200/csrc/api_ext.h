@@ -180,6 +180,17 @@ int fb_mla_expand(void* kp, void* vp, const void* kvx, const void* lat, long row
 int fb_mla_qpad(void* qp, const void* q, long q_stride, const void* qabs, long rows, int nq, int dn, int L, int R, int HP,
                 float scale, cudaStream_t s);
 
+// ---- mla_cache.cu, mla_cache_attn.cu: the same over a cache of 4- or 8-bit rows (mla_cache.cuh). `pages`: pages of the cache; a table entry outside
+// them sets ST_BOUNDS and reads as no page. Bytes of a row, or -1 where (L, R, bits) has no such row ----
+int fb_latent_row_bytes(int L, int R, int bits);
+int fb_mla_prep_q(void* cache, long pages, int bits, void* qabs, const void* kva, long kva_stride, const void* q, long q_stride, const void* norm_w,
+                  const float* inv_freq, const int* row_slot, const int* row_pos, const int* block_table, int max_blocks, int kv_block, int rows, int nq,
+                  int dn, int L, int R, float eps, int* status, cudaStream_t s);
+int fb_mla_rows(void* out, long rows, const void* cache, long pages, int bits, const int* seg_slot, const int* seg_pos0, const int* seg_nrows, int nseg,
+                const int* block_table, int max_blocks, int kv_block, int L, int R, int whole, int align, int* status, cudaStream_t s);
+int fb_mla_attn_q(void* out, const void* qabs, const void* cache, long pages, int bits, const int* row_slot, const int* row_kvlen,
+                  const int* block_table, int max_blocks, int kv_block, int rows, int nq, int L, int R, float scale, int* status, cudaStream_t s);
+
 // ---- latent.cu ----
 int fb_embed_grams(float* x, void* xb, int copies, const void* table, const void* grams, const int* tok, const int* slot, const int* pos,
                    const int* block_table, int max_blocks, int kv_block, int* tok_pages, int rows, int width, int vocab, float scale,

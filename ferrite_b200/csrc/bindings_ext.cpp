@@ -1,5 +1,6 @@
 // Python bindings, second part (fused collectives, quantised formats, MoE, MLA, drafter ops).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
 
@@ -582,6 +583,69 @@ void mla_qpad(Tensor qp, Tensor q, Tensor qabs, int64_t nq, int64_t dn, int64_t 
                     (int)L, (int)R, (int)qp.size(-1), (float)scale, cur_stream()), "mla_qpad");
 }
 
+// ---- latent caches in 4 and 8 bits (mla_cache.cu). Launched on the current stream of the cache's device.
+void check_latent_cache(const Tensor& cache, const Tensor& block_table, int64_t kv_block, int64_t L, int64_t R, int64_t bits, const char* what) {
+  const int row = fb_latent_row_bytes((int)L, (int)R, (int)bits);
+  TORCH_CHECK(row > 0, what, ": no row of ", bits, " bits for widths ", L, " and ", R, " (4 or 8 bits, L a multiple of 64 up to 512, R 64)");
+  TORCH_CHECK(cache.is_cuda() && cache.is_contiguous() && cache.scalar_type() == torch::kUInt8 && cache.dim() >= 3 && cache.size(1) == kv_block &&
+              cache.numel() == cache.size(0) * kv_block * row, what, ": cache is not [pages, ", kv_block, ", ", row, "] bytes");
+  TORCH_CHECK(block_table.is_contiguous() && block_table.dim() == 2 && block_table.scalar_type() == torch::kInt32 &&
+              block_table.device() == cache.device(), what, ": block_table");
+}
+void check_ints(const Tensor& t, int64_t n, const Tensor& beside, const char* what) {
+  TORCH_CHECK(t.is_contiguous() && t.scalar_type() == torch::kInt32 && t.numel() == n && t.device() == beside.device(), what, ": ", n,
+              " int32 on the cache's device");
+}
+bool is_bf16(const Tensor& t) { return t.scalar_type() == torch::kBFloat16; }
+
+void mla_prep_q(Tensor cache, Tensor qabs, Tensor kva, Tensor q, Tensor norm_w, Tensor inv_freq, Tensor row_slot, Tensor row_pos, Tensor block_table,
+                int64_t kv_block, int64_t nq, int64_t dn, int64_t L, int64_t R, double eps, int64_t bits, Tensor status) {
+  check_latent_cache(cache, block_table, kv_block, L, R, bits, "mla_prep_q");
+  const int64_t T = q.size(0);
+  const auto dev = cache.device();
+  TORCH_CHECK(is_bf16(q) && q.dim() == 2 && q.size(1) == nq * (dn + R) && q.stride(1) == 1 && q.device() == dev, "mla_prep_q: q");
+  TORCH_CHECK(is_bf16(kva) && kva.dim() == 2 && kva.size(0) == T && kva.size(1) >= L + R && kva.stride(1) == 1 && kva.device() == dev, "mla_prep_q: kva");
+  TORCH_CHECK(is_bf16(qabs) && qabs.is_contiguous() && qabs.numel() == T * nq * (L + R) && qabs.device() == dev, "mla_prep_q: qabs");
+  TORCH_CHECK(is_bf16(norm_w) && norm_w.is_contiguous() && norm_w.numel() == L && norm_w.device() == dev, "mla_prep_q: norm_w");
+  TORCH_CHECK(inv_freq.scalar_type() == torch::kFloat32 && inv_freq.is_contiguous() && inv_freq.numel() == R / 2 && inv_freq.device() == dev,
+              "mla_prep_q: inv_freq");
+  check_ints(row_slot, T, cache, "mla_prep_q: row_slot");
+  check_ints(row_pos, T, cache, "mla_prep_q: row_pos");
+  const c10::cuda::CUDAGuard guard(dev);
+  check(fb_mla_prep_q(cache.data_ptr(), (long)cache.size(0), (int)bits, qabs.data_ptr(), kva.data_ptr(), (long)kva.stride(0), q.data_ptr(),
+                      (long)q.stride(0), norm_w.data_ptr(), inv_freq.data_ptr<float>(), row_slot.data_ptr<int>(), row_pos.data_ptr<int>(),
+                      block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)dn, (int)L, (int)R, (float)eps,
+                      status.data_ptr<int>(), cur_stream()), "mla_prep_q");
+}
+
+void mla_rows(Tensor out, Tensor cache, Tensor seg_slot, Tensor seg_pos0, Tensor seg_nrows, Tensor block_table, int64_t kv_block, int64_t L, int64_t R,
+              int64_t bits, bool whole, int64_t align, Tensor status) {
+  check_latent_cache(cache, block_table, kv_block, L, R, bits, "mla_rows");
+  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.dim() == 2 && out.size(1) == L + R && out.device() == cache.device(), "mla_rows: out");
+  const int64_t n = seg_slot.numel();
+  check_ints(seg_slot, n, cache, "mla_rows: seg_slot");
+  check_ints(seg_pos0, n, cache, "mla_rows: seg_pos0");
+  check_ints(seg_nrows, n, cache, "mla_rows: seg_nrows");
+  const c10::cuda::CUDAGuard guard(cache.device());
+  check(fb_mla_rows(out.data_ptr(), (long)out.size(0), cache.data_ptr(), (long)cache.size(0), (int)bits, seg_slot.data_ptr<int>(),
+                    seg_pos0.data_ptr<int>(), seg_nrows.data_ptr<int>(), (int)n, block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block,
+                    (int)L, (int)R, whole ? 1 : 0, (int)align, status.data_ptr<int>(), cur_stream()), "mla_rows");
+}
+
+void mla_attn_q(Tensor out, Tensor qabs, Tensor cache, Tensor row_slot, Tensor row_kvlen, Tensor block_table, int64_t kv_block, int64_t L, int64_t R,
+                int64_t bits, double scale, Tensor status) {
+  check_latent_cache(cache, block_table, kv_block, L, R, bits, "mla_attn_q");
+  TORCH_CHECK(is_bf16(qabs) && qabs.is_contiguous() && qabs.dim() == 3 && qabs.size(2) == L + R && qabs.device() == cache.device(), "mla_attn_q: qabs");
+  const int64_t T = qabs.size(0), nq = qabs.size(1);
+  TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.numel() == T * nq * L && out.device() == cache.device(), "mla_attn_q: out");
+  check_ints(row_slot, T, cache, "mla_attn_q: row_slot");
+  check_ints(row_kvlen, T, cache, "mla_attn_q: row_kvlen");
+  const c10::cuda::CUDAGuard guard(cache.device());
+  check(fb_mla_attn_q(out.data_ptr(), qabs.data_ptr(), cache.data_ptr(), (long)cache.size(0), (int)bits, row_slot.data_ptr<int>(),
+                      row_kvlen.data_ptr<int>(), block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)L, (int)R,
+                      (float)scale, status.data_ptr<int>(), cur_stream()), "mla_attn_q");
+}
+
 // ---- models of listed layers (latent.cu). The element type of activations and cache (bf16 / fp32) is read off the tensors.
 void* optr(const c10::optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
@@ -955,6 +1019,10 @@ void register_ext(pybind11::module_& m) {
   m.def("dynconv", &dynconv);
   m.def("mla_expand", &mla_expand);
   m.def("mla_qpad", &mla_qpad);
+  m.def("latent_row_bytes", &fb_latent_row_bytes);
+  m.def("mla_prep_q", &mla_prep_q);
+  m.def("mla_rows", &mla_rows);
+  m.def("mla_attn_q", &mla_attn_q);
   m.def("hc_norm", &hc_norm);
   m.def("hc_mix", &hc_mix);
   m.def("hc_combine", &hc_combine);

@@ -16,6 +16,7 @@ import os
 import contextlib
 import gc
 import math
+import warnings
 from collections import OrderedDict
 from dataclasses import dataclass, field
 from typing import Dict, List, Optional, Sequence, Tuple
@@ -25,6 +26,7 @@ import torch
 from ..config import EngineConfig, ModelConfig
 from ..models.weights import Weights, delta_dims, gqa_dims, latent_dims, ssm_dims
 from ..ops.latent import SegGroup, seg_groups
+from ..ops.mla_cache import fits, latent_bits, row_bytes
 from ..ops.qweight import QWeight
 
 
@@ -152,6 +154,9 @@ class Executor:
         self.kv8 = kd in ("fp8", "int4", "int6")
         self.kv_bits = {"fp8": 8, "int4": 4, "int6": 6}.get(kd, 16)
         self.kv4 = kd in ("int4", "int6")                   # group scales (one per 32 elements)
+        self.latent_bits = self.latent_cache_bits()         # MLA layers: bits of a cached latent
+        if c.kv_lora > 0 and self.kv8 and self.latent_bits == 16:
+            warnings.warn(f"kv_dtype {ecfg.kv_dtype!r}: latents of width {c.kv_lora} beside {c.rope_head_dim} stay in the compute dtype")
         self.kv_scale: Dict[int, torch.Tensor] = {}
         self.k_cache: Dict[int, torch.Tensor] = {}
         self.v_cache: Dict[int, torch.Tensor] = {}
@@ -169,8 +174,13 @@ class Executor:
                     ns = 2 * (c.head_dim // 32) if self.kv4 else 2
                     self.kv_scale[i] = torch.ones(n_blocks, ecfg.kv_block, c.n_kv, ns, dtype=torch.float32, device=dev)
             elif kind == "mla":
-                # one latent row [kv_lora | rope] per token; the value cache slot stays empty
-                self.k_cache[i] = torch.zeros(n_blocks, ecfg.kv_block, 1, c.kv_lora + c.rope_head_dim, dtype=dt, device=dev)
+                # one latent row [kv_lora | rope] per token; the value cache slot stays empty. Quantised: bytes of codes and scales on the
+                # GPU, the values they stand for on the CPU
+                if self.latent_bits != 16 and dev.type == "cuda":
+                    self.k_cache[i] = torch.zeros(n_blocks, ecfg.kv_block, row_bytes(c.kv_lora, c.rope_head_dim, self.latent_bits),
+                                                  dtype=torch.uint8, device=dev)
+                else:
+                    self.k_cache[i] = torch.zeros(n_blocks, ecfg.kv_block, 1, c.kv_lora + c.rope_head_dim, dtype=dt, device=dev)
                 self.v_cache[i] = torch.zeros(n_blocks, 0, dtype=dt, device=dev)
             elif kind == "gdn":
                 self.rec_state[i] = torch.zeros(ecfg.n_slots, c.lin_v_heads, c.lin_dk, c.lin_dv, dtype=torch.float32, device=dev)
@@ -344,6 +354,11 @@ class Executor:
             self.moe_merged[i] = torch.cat([router, gate.to(router.dtype)]).contiguous() if gate is not None else router
 
     # ---- sizes -----------------------------------------------------------------------------------
+    def latent_cache_bits(self) -> int:
+        """Bits of a cached latent of the MLA layers: 4 (kv_dtype int4), 8 (fp8), or 16 where that has no form for latents or for these widths."""
+        c, bits = self.cfg, latent_bits(self.ecfg.kv_dtype)
+        return bits if c.kv_lora > 0 and fits(c.kv_lora, c.rope_head_dim, bits) else 16
+
     def kv_block_bytes(self) -> int:
         c, e = self.cfg, self.ecfg
         kd = e.kv_dtype[:-1] if e.kv_dtype.endswith("h") else e.kv_dtype
@@ -351,7 +366,7 @@ class Executor:
         if kd in ("int4", "int6"):
             per = 2 * e.kv_block * c.n_kv * (c.head_dim * int(kd[3]) // 8 + c.head_dim // 32 * 4)
         if c.kv_lora > 0:
-            per = e.kv_block * (c.kv_lora + c.rope_head_dim) * 2
+            per = e.kv_block * row_bytes(c.kv_lora, c.rope_head_dim, self.latent_cache_bits())
         if c.layers:
             item = torch.empty(0, dtype=self.dtype).element_size()
             dims = [(gqa_dims if c.layers[r.layer].mixer == "gqa" else latent_dims)(c, r.layer) for r in c.layer_runs if c.layers[r.layer].cached]
@@ -974,21 +989,23 @@ class Executor:
                 expand = (ops.name == "cuda" and max_seg_rows > FLASH_MIN_ROWS and self._step_segments is not None
                           and self.ecfg.kv_block % 64 == 0 and max(c.nope_head_dim + R, c.v_head_dim) <= 256
                           and isinstance(w[p + "kv_b"], torch.Tensor))
+                cache = self.k_cache[i].view(-1, self.ecfg.kv_block, self.k_cache[i].shape[-1])
+                kvq = {"kv_bits": self.latent_bits} if self.latent_bits != 16 else {}
                 qabs = ops.mla_prep(q, kva, w[p + "kv_a_norm"], w_uk_t, self.inv_freq_mla, mv["slot"], mv["pos"],
-                                    self.block_table, self.k_cache[i].view(-1, self.ecfg.kv_block, L + R),
+                                    self.block_table, cache,
                                     self.ecfg.kv_block, c.n_q, c.nope_head_dim, L, R, eps,
-                                    **({"absorb": False} if expand else {}))
+                                    **({"absorb": False} if expand else {}), **kvq)
                 if expand:
                     o = ops.mla_attention_prefill(q, qabs, self.k_cache[i], w[p + "kv_b"], self._step_segments, mv["srow0"],
                                                   mv["snrows"], mv["spos0"], self.block_table, self.ecfg.kv_block, c.n_q,
-                                                  c.nope_head_dim, c.v_head_dim, L, R)
+                                                  c.nope_head_dim, c.v_head_dim, L, R, **kvq, **({"seg_slot": mv["sslot"]} if kvq else {}))
                 else:
-                    ol = ops.mla_attention(qabs, self.k_cache[i].view(-1, self.ecfg.kv_block, L + R), mv["slot"], mv["kvlen"],
+                    ol = ops.mla_attention(qabs, cache, mv["slot"], mv["kvlen"],
                                            self.block_table, self.ecfg.kv_block, c.n_q, L, R,
                                            1.0 / math.sqrt(c.nope_head_dim + R),
                                            nsplit=nsplit if max_seg_rows <= FLASH_MIN_ROWS else 1,
                                            segs=(mv["sslot"], mv["srow0"], mv["snrows"], max_seg_rows),
-                                           picked=self.ecfg.attn_splits <= 0)
+                                           picked=self.ecfg.attn_splits <= 0, **kvq)
                     o = ops.mla_out(ol, w_uv)
                 x = row(o, w[p + "out_proj"], x)
             else:

@@ -745,24 +745,41 @@ class CudaOps(CudaLatent, CudaMixers, CudaExtras):
 
     # ---- multi-head latent attention (absorbed form) ----------------------------------------------------
     def mla_prep(self, q, kva, norm_w, w_uk_t, inv_freq, row_slot, row_pos, block_table, cache, kv_block, nq, dn, L, R, eps,
-                 absorb=True):
+                 absorb=True, kv_bits=16):
         """Latent rows into the paged cache and the absorbed queries [T, nq, L + R]. `absorb=False` leaves the first L
-        columns of every query unwritten (the expanded prompt path only reads the rotated rope tail)."""
+        columns of every query unwritten (the expanded prompt path only reads the rotated rope tail). `kv_bits` 4 or 8: the
+        cache holds rows of codes ([blocks, kv_block, `mla_cache.row_bytes`] uint8), quantised as they are written."""
         T = q.shape[0]
         qabs = self.empty(T, nq, L + R, dtype=self.dtype, device=self.device)
         self.launches += 1
-        self.C.mla_prep(cache, qabs, kva, q, norm_w, inv_freq, row_slot, row_pos, block_table, kv_block, nq, dn, L, R, eps,
-                        self.status_word)
+        if kv_bits != 16:
+            if q.dim() != 2 or q.stride(1) != 1 or q.stride(0) % 4 or q.data_ptr() % 8:      # the kernel reads query parts by 8 bytes
+                q = q.reshape(T, nq * (dn + R)).clone()
+            self.C.mla_prep_q(cache, qabs, kva if kva.stride(1) == 1 else kva.contiguous(), q, norm_w, inv_freq, row_slot, row_pos, block_table,
+                              kv_block, nq, dn, L, R, eps, kv_bits, self.status_word)
+        else:
+            self.C.mla_prep(cache, qabs, kva, q, norm_w, inv_freq, row_slot, row_pos, block_table, kv_block, nq, dn, L, R, eps,
+                            self.status_word)
         if absorb:
             # key up-projection folded into the query: one small linear per head
             self.head_linear(q.view(T, nq, dn + R)[:, :, :dn], w_uk_t, out=qabs[:, :, :L])
         return qabs
 
+    def mla_rows(self, cache, seg_slot, seg_pos0, seg_nrows, block_table, kv_block, L, R, total, whole=False, kv_bits=8):
+        """Rows of segments read back from a paged latent cache of 4- or 8-bit codes, bf16 [total, L + R], segment after segment: a segment's own
+        rows (positions seg_pos0 and on, seg_nrows of them), or (`whole`) its context from the first token to its last row, each from a multiple of
+        `kv_block` on. Zeros between and behind them."""
+        out = self.empty(total, L + R, dtype=torch.bfloat16, device=self.device)
+        self.launches += 1
+        self.C.mla_rows(out, cache, seg_slot, seg_pos0, seg_nrows, block_table, kv_block, L, R, kv_bits, whole, kv_block if whole else 1,
+                        self.status_word)
+        return out
+
     def mla_attention_prefill(self, q, qabs, cache, kv_b, segs, seg_row0, seg_nrows, seg_pos0, block_table, kv_block,
-                              nq, dn, dv, L, R):
+                              nq, dn, dv, L, R, kv_bits=16, seg_slot=None):
         """Latent attention of prompt segments in the expanded form on the tcgen05 flash kernel. `segs`: host list of
-        (slot, pos0, rows) per segment; the context's latent rows are gathered through the block table, expanded to
-        per-head keys / values by one GEMM with `kv_b` [nq (dn + dv), L], packed (padded to the kernel's head width) into
+        (slot, pos0, rows) per segment; the context's latent rows are gathered through the block table (`kv_bits` 4 or 8, with
+        `seg_slot`: read back from their codes), expanded to per-head keys / values by one GEMM with `kv_b` [nq (dn + dv), L], packed (padded to the kernel's head width) into
         a scratch laid out segment after segment, and read through a step-local page table. Returns [T, nq * dv]."""
         T = q.shape[0]
         HP = 64 if max(dn + R, dv) <= 64 else 128 if max(dn + R, dv) <= 128 else 256
@@ -772,8 +789,11 @@ class CudaOps(CudaLatent, CudaMixers, CudaExtras):
             starts.append((slot, tot, nb))
             tot += nb
         max_nb = max(nb for _, _, nb in starts)
-        pages = torch.cat([block_table[slot, :nb] for slot, _, nb in starts]).long()
-        lat = cache.view(-1, kv_block, L + R)[pages].view(tot * kv_block, L + R)            # the segments' latent rows
+        if kv_bits != 16:
+            lat = self.mla_rows(cache, seg_slot, seg_pos0, seg_nrows, block_table, kv_block, L, R, tot * kv_block, whole=True, kv_bits=kv_bits)
+        else:
+            pages = torch.cat([block_table[slot, :nb] for slot, _, nb in starts]).long()
+            lat = cache.view(-1, kv_block, L + R)[pages].view(tot * kv_block, L + R)        # the segments' latent rows
         kvx = self.linear(lat[:, :L].contiguous(), kv_b)                                     # [rows, nq (dn + dv)]
         kp = self.empty(tot, kv_block, nq, HP, dtype=self.dtype, device=self.device)
         vp = self.empty(tot, kv_block, nq, HP, dtype=self.dtype, device=self.device)
@@ -788,12 +808,19 @@ class CudaOps(CudaLatent, CudaMixers, CudaExtras):
                                    nq, nq, HP, False, max(n for _, _, n in segs))
         return o.view(T, nq, HP)[:, :, :dv].contiguous().view(T, nq * dv)
 
-    def mla_attention(self, qabs, cache, row_slot, row_kvlen, block_table, kv_block, nq, L, R, scale, nsplit=1, segs=None, picked=False):
+    def mla_attention(self, qabs, cache, row_slot, row_kvlen, block_table, kv_block, nq, L, R, scale, nsplit=1, segs=None, picked=False,
+                      kv_bits=16):
         """Every head attends the cached latents. With `segs` = (seg_slot, seg_row0, seg_nrows, max rows per segment) and pages of whole
         64-key tiles the tensor-core kernel of the listed models runs, heads of a row sharing every pass over the latents. Rows of segments of
         up to 32 rows share nothing and, with `picked` splits (see `attention`), are split by their own context: a row has the same bits
-        decoded, verified and among other streams. Callers without segment tables and other page sizes take the CUDA-core kernel."""
+        decoded, verified and among other streams. Callers without segment tables and other page sizes take the CUDA-core kernel.
+        `kv_bits` 4 or 8: the cache holds rows of codes (`mla_prep`)."""
         T = qabs.shape[0]
+        if kv_bits != 16:
+            out = self.empty(T, nq, L, dtype=torch.bfloat16, device=self.device)
+            self.launches += 1
+            self.C.mla_attn_q(out, qabs.contiguous(), cache, row_slot, row_kvlen, block_table, kv_block, L, R, kv_bits, scale, self.status_word)
+            return out
         if segs is not None and kv_block % 64 == 0 and R == 64 and L in (64, 128, 512):
             if qabs.dtype != torch.bfloat16:
                 return self.latent_attention(qabs, cache.view(-1, kv_block, L + R), SegGroup(0, segs[0].numel(), 0, T, segs[3]), row_slot, row_kvlen,

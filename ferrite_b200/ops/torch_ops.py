@@ -15,6 +15,7 @@ import torch.nn.functional as F
 from .extras import TorchExtras
 from .latent import TORCH_ACTS, TorchLatent
 from .mixers import TorchMixers
+from .mla_cache import quantised
 
 
 def _softplus(x):
@@ -269,30 +270,48 @@ class TorchOps(TorchLatent, TorchMixers, TorchExtras):
         return y
 
     # ---- multi-head latent attention (absorbed form) ----------------------------------------------------
-    def mla_prep(self, q, kva, norm_w, w_uk_t, inv_freq, row_slot, row_pos, block_table, cache, kv_block, nq, dn, L, R, eps):
+    def mla_prep(self, q, kva, norm_w, w_uk_t, inv_freq, row_slot, row_pos, block_table, cache, kv_block, nq, dn, L, R, eps, absorb=True,
+                 kv_bits=16):
         """Latent RMSNorm + key RoPE into the paged cache [blocks, kv_block, L + R]; returns the absorbed queries
-        [T, nq, L + R] = [q_nope W_uk | rope(q_rope)]."""
+        [T, nq, L + R] = [q_nope W_uk | rope(q_rope)] (`absorb=False`: zeros in front). `kv_bits` 4 or 8: the cache takes the values that a cache
+        of so many bits returns (`mla_cache.quantised`), norm and angles in 64 bits."""
         T = q.shape[0]
-        q3 = q.reshape(T, nq, dn + R).float()
-        kf = kva.float()
-        lat = kf[:, :L] * torch.rsqrt(kf[:, :L].pow(2).mean(-1, keepdim=True) + eps) * (1.0 + norm_w.float())
-        ang = row_pos.float()[:, None] * inv_freq.float()[None, :]
+        wide = torch.float32 if kv_bits == 16 else torch.float64
+        q3 = q.reshape(T, nq, dn + R).to(wide)
+        kf = kva.to(wide)
+        lat = kf[:, :L] * torch.rsqrt(kf[:, :L].pow(2).mean(-1, keepdim=True) + eps) * (1.0 + norm_w.to(wide))
+        if kv_bits != 16:
+            lat = quantised(lat, kv_bits)
+        ang = row_pos.to(wide)[:, None] * inv_freq.to(wide)[None, :]
         cos, sin = ang.cos(), ang.sin()
         half = R // 2
 
         def rope(v, c, s):
             a, b = v[..., :half], v[..., half:]
             return torch.cat([a * c - b * s, b * c + a * s], -1)
-        kr = rope(kf[:, L:], cos, sin)
+        kr = rope(kf[:, L:L + R], cos, sin)
         qr = rope(q3[..., dn:], cos[:, None, :], sin[:, None, :])
-        rows = torch.cat([lat, kr], -1).to(cache.dtype)
+        rows = torch.cat([lat, kr], -1).to(cache.dtype).view(T, *cache.shape[2:])
         for t in range(T):
             slot, pos = int(row_slot[t]), int(row_pos[t])
             cache[int(block_table[slot, pos // kv_block]), pos % kv_block] = rows[t]
-        qn = torch.einsum("thd,hld->thl", q3[..., :dn], w_uk_t.float())
-        return torch.cat([qn, qr], -1).to(self.dtype)
+        qn = torch.einsum("thd,hld->thl", q3[..., :dn].float(), w_uk_t.float()) if absorb else qr.new_zeros(T, nq, L)
+        return torch.cat([qn.to(wide), qr], -1).to(self.dtype)
 
-    def mla_attention(self, qabs, cache, row_slot, row_kvlen, block_table, kv_block, nq, L, R, scale, nsplit=1, segs=None, picked=False):
+    def mla_rows(self, cache, seg_slot, seg_pos0, seg_nrows, block_table, kv_block, L, R, total, whole=False, kv_bits=16):
+        """Rows of segments read back from the paged cache, [total, L + R], segment after segment: a segment's own rows, or (`whole`) its context from
+        the first token on, each from a multiple of `kv_block` on. Zeros between and behind them."""
+        out = torch.zeros(total, L + R, dtype=cache.dtype, device=cache.device)
+        at = 0
+        for slot, pos0, n in zip(seg_slot.tolist(), seg_pos0.tolist(), seg_nrows.tolist()):
+            lo, hi = (0 if whole else pos0), pos0 + n
+            pos = torch.arange(lo, hi, device=cache.device)
+            rows = cache.reshape(-1, L + R)[block_table[slot, pos // kv_block].long() * kv_block + pos % kv_block]
+            out[at:at + len(rows)] = rows[:max(0, total - at)]
+            at += (hi + kv_block - 1) // kv_block * kv_block if whole else n
+        return out.to(self.dtype)
+
+    def mla_attention(self, qabs, cache, row_slot, row_kvlen, block_table, kv_block, nq, L, R, scale, nsplit=1, segs=None, picked=False, kv_bits=16):
         T = qabs.shape[0]
         out = torch.zeros(T, nq, L, dtype=torch.float32, device=qabs.device)
         for t in range(T):
