@@ -632,18 +632,22 @@ void mla_rows(Tensor out, Tensor cache, Tensor seg_slot, Tensor seg_pos0, Tensor
                     (int)L, (int)R, whole ? 1 : 0, (int)align, status.data_ptr<int>(), cur_stream()), "mla_rows");
 }
 
-void mla_attn_q(Tensor out, Tensor qabs, Tensor cache, Tensor row_slot, Tensor row_kvlen, Tensor block_table, int64_t kv_block, int64_t L, int64_t R,
-                int64_t bits, double scale, Tensor status) {
+void mla_attn_q(Tensor out, Tensor ws, Tensor qabs, Tensor cache, Tensor seg_slot, Tensor seg_row0, Tensor seg_nrows, int64_t max_rows, Tensor row_kvlen,
+                Tensor block_table, int64_t kv_block, int64_t L, int64_t R, int64_t bits, double scale, int64_t ctas, Tensor status) {
   check_latent_cache(cache, block_table, kv_block, L, R, bits, "mla_attn_q");
   TORCH_CHECK(is_bf16(qabs) && qabs.is_contiguous() && qabs.dim() == 3 && qabs.size(2) == L + R && qabs.device() == cache.device(), "mla_attn_q: qabs");
-  const int64_t T = qabs.size(0), nq = qabs.size(1);
+  const int64_t T = qabs.size(0), nq = qabs.size(1), n = seg_slot.numel();
   TORCH_CHECK(is_bf16(out) && out.is_contiguous() && out.numel() == T * nq * L && out.device() == cache.device(), "mla_attn_q: out");
-  check_ints(row_slot, T, cache, "mla_attn_q: row_slot");
+  TORCH_CHECK(is_f32(ws) && ws.is_contiguous() && ws.device() == cache.device(), "mla_attn_q: workspace");
+  check_ints(seg_slot, n, cache, "mla_attn_q: seg_slot");
+  check_ints(seg_row0, n, cache, "mla_attn_q: seg_row0");
+  check_ints(seg_nrows, n, cache, "mla_attn_q: seg_nrows");
   check_ints(row_kvlen, T, cache, "mla_attn_q: row_kvlen");
   const c10::cuda::CUDAGuard guard(cache.device());
-  check(fb_mla_attn_q(out.data_ptr(), qabs.data_ptr(), cache.data_ptr(), (long)cache.size(0), (int)bits, row_slot.data_ptr<int>(),
-                      row_kvlen.data_ptr<int>(), block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)L, (int)R,
-                      (float)scale, status.data_ptr<int>(), cur_stream()), "mla_attn_q");
+  check(fb_mla_attn_q(out.data_ptr(), ws.data_ptr<float>(), (long)ws.numel(), qabs.data_ptr(), cache.data_ptr(), (long)cache.size(0), (int)bits,
+                      seg_slot.data_ptr<int>(), seg_row0.data_ptr<int>(), seg_nrows.data_ptr<int>(), (int)n, (int)max_rows, row_kvlen.data_ptr<int>(),
+                      block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)L, (int)R, (float)scale, (int)ctas,
+                      status.data_ptr<int>(), cur_stream()), "mla_attn_q");
 }
 
 // ---- models of listed layers (latent.cu). The element type of activations and cache (bf16 / fp32) is read off the tensors.
@@ -1023,6 +1027,7 @@ void register_ext(pybind11::module_& m) {
   m.def("mla_prep_q", &mla_prep_q);
   m.def("mla_rows", &mla_rows);
   m.def("mla_attn_q", &mla_attn_q);
+  m.def("mla_attn_q_floats", &fb_mla_attn_q_floats);
   m.def("hc_norm", &hc_norm);
   m.def("hc_mix", &hc_mix);
   m.def("hc_combine", &hc_combine);

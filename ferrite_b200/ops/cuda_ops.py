@@ -817,9 +817,14 @@ class CudaOps(CudaLatent, CudaMixers, CudaExtras):
         `kv_bits` 4 or 8: the cache holds rows of codes (`mla_prep`)."""
         T = qabs.shape[0]
         if kv_bits != 16:
+            if segs is None:                              # every row a segment of its own
+                row0 = torch.arange(T, dtype=torch.int32, device=self.device)
+                segs = (row_slot, row0, torch.ones_like(row0), 1)
             out = self.empty(T, nq, L, dtype=torch.bfloat16, device=self.device)
-            self.launches += 1
-            self.C.mla_attn_q(out, qabs.contiguous(), cache, row_slot, row_kvlen, block_table, kv_block, L, R, kv_bits, scale, self.status_word)
+            ws = self.empty(self.C.mla_attn_q_floats(segs[3], nq, L, self.sm_count), dtype=torch.float32, device=self.device)
+            self.launches += 2
+            self.C.mla_attn_q(out, ws, qabs.contiguous(), cache, *segs, row_kvlen, block_table, kv_block, L, R, kv_bits, scale, self.sm_count,
+                              self.status_word)
             return out
         if segs is not None and kv_block % 64 == 0 and R == 64 and L in (64, 128, 512):
             if qabs.dtype != torch.bfloat16:
