@@ -9,7 +9,8 @@
 //
 // Warps 0..7 unpack (two threads a key, 32 of every 64 values each): a word of eight 4-bit codes takes a shift, a mask and one fma per two values, fp16(16 +
 // code + 8) * s - 24 s, exact in fp16 as the value itself is (a power of two times seven bits). The codes of the next tile are in flight in registers meanwhile.
-// Warps 8..15 run the softmax: a thread has a key (its TMEM lane) and half of the pairs. Warp 16 issues the products.
+// Warps 8..15 run the softmax: a thread has a key (its TMEM lane) and half of the pairs. Warp 16 issues the products, 17 and 18 copy the key parts, 19 looks
+// up the keys' pages.
 // The values' products run in fp16, so that a weight keeps 11 bits; a query is brought to 2^10 by a power of two of its own, which keeps its bf16 bits down
 // to 2^-27 of its largest value. The key part stays in bf16 (its products go to the same sums).
 //
@@ -24,14 +25,15 @@
 // A key of which a group is no number gets the score NaN and a finite place in the tile, so that rows ahead of it, whose weight for it is zero, stay clean.
 // Every wait is bounded: one that runs out sets the status word and an abort flag, all roles leave and the CTA frees its TMEM.
 #include "api_ext.h"
-#include "gemm_core.cuh"
 #include "mla_cache.cuh"
 
 namespace fb {
 
 constexpr int LA_KT = 128;                       // keys of a tile
 constexpr int LA_CH = LA_KT * 128;               // bytes of 64 values of all of them
-constexpr int LA_THREADS = 17 * 32;
+constexpr int LA_UNPACK = 16, LA_SOFT = LA_UNPACK + 8;             // warps up to which these roles go
+constexpr int LA_THREADS = (LA_SOFT + 4) * 32;              // eight warps unpack, eight run the softmax, one issues the products, two copy key parts, one looks keys up
+constexpr int LA_AHEAD = 4;                      // tiles whose keys are looked up ahead
 constexpr float LA_TOP = 4.f, LA_LIMIT = 15.f;   // log2 of a piece's first largest weight; of the largest one that a weight may be
 
 template <int BITS, int NC, int N>
@@ -40,7 +42,7 @@ struct LatentAttn {
   static constexpr int NP = (NC + 1) / 2;                          // pairs of 64 values: rows of 128 of O^T
   static constexpr int NB = NC == 8 ? (N == 64 ? 4 : 5) : 2 * NP;  // buffers of them
   static constexpr bool SHARE = NC == 8 && N == 64;                // the weights take the place of the tile's key part
-  static constexpr int PD = BITS == 8 && NC == 8 ? 4 : NC;         // 64s of values in flight
+  static constexpr int PD = BITS == 8 && NP == 4 ? 2 : NP;         // pairs of codes in flight
   static constexpr int Q_BYTES = (NC + 1) * N * 128, P_BYTES = LA_KT * N * 2;
   static constexpr int K_AT = Q_BYTES, R_AT = K_AT + NB * 2 * LA_CH, P_AT = SHARE ? R_AT : R_AT + LA_CH;
   static constexpr int MISC_AT = SHARE ? R_AT + LA_CH : P_AT + P_BYTES;
@@ -52,10 +54,11 @@ struct LatentAttnMisc {
   float c[2][N], nr[2][N];                       // by the piece's parity: what leads from a score to log2, minus the reference
   int see[2][N];                                 // keys that a pair sees
   float mx[4][N], d[N];
-  uint32_t bad[4][8];                            // of the last tiles: keys that are no number, two bits a key
-  long long scan[18];
+  uint32_t bad[4][16];                           // of the last tiles: keys that are no number, four bits a key
+  long long scan[LA_THREADS / 32];
   int start[4];
-  uint64_t bars[2 * 5 + 7];
+  int rows[LA_AHEAD][LA_KT];                     // ring of tiles: their keys' rows of the cache, -1 where there is none
+  uint64_t bars[2 * 5 + 7 + 2 * LA_AHEAD];
   uint32_t tmem;
   int abort, fail;
 };
@@ -66,10 +69,10 @@ struct LatentSegs {
   long limit;                                    // keys that a table has room for
 };
 struct LatentWalk {                              // a place in the list of tiles
-  int s, u, t, units, nt, kv, row0, nrows;
+  int s, u, t, units, nt, kv, row0, nrows, slot;
   template <int N>
   __device__ __forceinline__ void load(const LatentSegs& g) {
-    nrows = g.nrows[s]; row0 = g.row0[s];
+    nrows = g.nrows[s]; row0 = g.row0[s]; slot = g.slot[s];
     kv = nrows > 0 ? (int)min((long)max(g.kvlen[row0 + nrows - 1], 0), g.limit) : 0;
     units = (int)(((long)max(nrows, 0) * g.nq + N - 1) / N);
     nt = max(1, (kv + LA_KT - 1) / LA_KT);
@@ -95,6 +98,17 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Bounded wait that leaves the issue slots to others: the hardware holds the warp for up to 20 us a poll.
+__device__ __forceinline__ bool la_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (int i = 0; i < (1 << 16); ++i) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+  }
+  return false;
+}
 template <int W>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[W]) {
   if constexpr (W == 8) tmem_ld8(addr, r);
@@ -116,16 +130,14 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[W]) {
 // Per column of a warp's 32 rows: op over the rows. Lane `lane` ends with column lane % W. Halves change hands, so that W columns cost W - 1 exchanges.
 template <int W, typename Op>
 __device__ __forceinline__ float columns(const float (&v)[W], int lane, Op op) {
-  float a[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) a[i] = v[i];
+  float a[W / 2];
 #pragma unroll
   for (int off = W / 2; off > 0; off >>= 1) {
     const bool up = lane & off;
 #pragma unroll
     for (int i = 0; i < off; ++i) {
-      const float keep = up ? a[i + off] : a[i], give = up ? a[i] : a[i + off];
-      a[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, off));
+      const float lo = off == W / 2 ? v[i] : a[i], hi = off == W / 2 ? v[i + off] : a[i + off];
+      a[i] = op(up ? hi : lo, __shfl_xor_sync(0xffffffffu, up ? lo : hi, off));
     }
   }
 #pragma unroll
@@ -140,36 +152,50 @@ __device__ __forceinline__ bool softmax_any(bool p) {
   return r != 0;
 }
 
-// 32 values of a key: codes -> fp16 in four 16-byte places of the key's 128 bytes
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// 32 values of a key: codes -> fp16 in four 16-byte places of the key's row(s) of 128 bytes. Lanes 4 r + p have key r, part p of a pair of 64 values.
+// Eight lanes' stores fall on eight different places: the swizzle tells keys apart, the order within a part tells the pair's halves apart.
+//   4 bits: part p is half p % 2 of 64 number p / 2; sc: the scale bytes of its two groups. Places of the words in their order (p < 2) or 2, 3, 0, 1
+//   8 bits: part p is 16 values of each 64, from 16 p on; sc: the scale bytes of the two 64s. Places of the first 64, then of the second
 template <int BITS>
-__device__ __forceinline__ void unpack32(const uint4 (&raw)[BITS / 4], uint32_t sb0, uint32_t sb1, unsigned char* row, int first, int turn) {
+__device__ __forceinline__ void unpack32(const uint4 (&raw)[BITS / 4], uint32_t sc, uint32_t base, const uint32_t (&at)[4], bool up, bool second) {
   if constexpr (BITS == 4) {
-    const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+    const uint32_t w[4] = {up ? raw[0].z : raw[0].x, up ? raw[0].w : raw[0].y, up ? raw[0].x : raw[0].z, up ? raw[0].y : raw[0].w};
+    const uint32_t sb = up ? __byte_perm(sc, 0, 0x4401) : sc;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const __half2 s = __float2half2_rn(latent_scale<4>(q < 2 ? sb0 : sb1)), m = __hmul2(s, __float2half2_rn(-24.f));
-      uint32_t o[4];
+    for (int h = 0; h < 2; ++h) {
+      const __half2 s = __float2half2_rn(latent_scale<4>(h ? sb >> 8 & 255u : sb & 255u)), m = __hmul2(s, __float2half2_rn(-24.f));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t t = ((i == 0 ? w[q] << 6 : i == 1 ? w[q] << 2 : i == 2 ? w[q] >> 2 : w[q] >> 6) & 0x03c003c0u) | 0x4c004c00u;
-        const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&t), s, m);
-        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int q = 2 * h; q < 2 * h + 2; ++q) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t t = ((i == 0 ? w[q] << 6 : i == 1 ? w[q] << 2 : i == 2 ? w[q] >> 2 : w[q] >> 6) & 0x03c003c0u) | 0x4c004c00u;
+          const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&t), s, m);
+          o[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        st_shared_v4(base + at[q], o);
       }
-      *reinterpret_cast<uint4*>(row + (((first + q) ^ turn) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   } else {
-    const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
-    const __half2 s = __float2half2_rn(latent_scale<8>(sb0));
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t o[4];
+    for (int e = 0; e < 2; ++e) {
+      if (e == 1 && !second) break;
+      const uint32_t w[4] = {raw[e].x, raw[e].y, raw[e].z, raw[e].w};
+      const __half2 s = __float2half2_rn(latent_scale<8>(sc >> (8 * e) & 255u));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[2 * q + i / 2] >> (16 * (i % 2))), __NV_E4M3);
-        const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&r), s);
-        o[i] = *reinterpret_cast<const uint32_t*>(&h);
+      for (int q = 0; q < 2; ++q) {
+        uint32_t o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[2 * q + i / 2] >> (16 * (i % 2))), __NV_E4M3);
+          const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&r), s);
+          o[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        st_shared_v4(base + at[2 * e + q], o);
       }
-      *reinterpret_cast<uint4*>(row + (((first + q) ^ turn) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
@@ -187,14 +213,15 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   extern __shared__ __align__(1024) unsigned char smem[];
   LatentAttnMisc<N>& ms = *reinterpret_cast<LatentAttnMisc<N>*>(smem + C::MISC_AT);
   uint64_t *kfull = ms.bars, *kempty = kfull + 5, *rfull = kempty + 5, *rempty = rfull + 1, *sfull = rempty + 1, *pfull = sfull + 1, *qfull = pfull + 1,
-           *ofull = qfull + 1, *oempty = ofull + 1;
+           *ofull = qfull + 1, *oempty = ofull + 1, *xfull = oempty + 1, *xempty = xfull + LA_AHEAD;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &ms.abort;
   pdl_launch_dependents();
   if (tid == 0) {
     ms.abort = 0; ms.fail = 0;
-    for (int i = 0; i < NB; ++i) { mbar_init(&kfull[i], 8); mbar_init(&kempty[i], 1); }
-    mbar_init(rfull, 8); mbar_init(rempty, 1); mbar_init(sfull, 1); mbar_init(pfull, 8); mbar_init(qfull, 8); mbar_init(ofull, 1); mbar_init(oempty, 8);
+    for (int i = 0; i < NB; ++i) { mbar_init(&kfull[i], LA_UNPACK); mbar_init(&kempty[i], 1); }
+    mbar_init(rfull, 2); mbar_init(rempty, 1); mbar_init(sfull, 1); mbar_init(pfull, 8); mbar_init(qfull, 8); mbar_init(ofull, 1); mbar_init(oempty, 8);
+    for (int i = 0; i < LA_AHEAD; ++i) { mbar_init(&xfull[i], 1); mbar_init(&xempty[i], LA_UNPACK + 2); }
     fence_mbar_init();
   }
   pdl_wait();
@@ -253,7 +280,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     }
     ms.start[0] = w.s; ms.start[1] = at / w.nt; ms.start[2] = at % w.nt; ms.start[3] = unit + at / w.nt;
   }
-  if (warp == 16) {
+  if (warp == LA_SOFT) {
     tmem_alloc(&ms.tmem, C::TMEM);
     tmem_relinquish();
   }
@@ -264,178 +291,119 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   w.s = ms.start[0]; w.u = ms.start[1]; w.t = ms.start[2];
   w.load<N>(g);
 
-  if (warp < 8) {
-    // ---- unpack: thread = (key, half of every 64 values) ---------------------------------------------------------------------------------------
-    const int row = warp * 16 + (lane >> 1), half = lane & 1;
-    unsigned char* const krow = smem + C::K_AT + row * 128;
-    unsigned char* const rrow = smem + C::R_AT + row * 128;
-    const int turn = row & 7;
-    constexpr int CB = BITS * 4, SW = Row::per_half * NC;            // bytes of 32 codes; of this half's scales
-    // page of a key of the walk's tile, -1 where there is none
-    auto page_of = [&](int& off) -> int {
-      const int key = w.t * LA_KT + row;
-      off = 0;
-      if (w.s >= g.nseg || key >= w.kv) return -2;
-      const int p = key / kv_block;
-      off = key - p * kv_block;
-      return block_table[(size_t)g.slot[w.s] * max_blocks + p];
-    };
-    auto place = [&](int blk, int off) -> const uint8_t* {
-      if (blk >= 0 && blk < pages) return cache + ((size_t)blk * kv_block + off) * RB;
-      if (blk != -2) set_status(status, ST_BOUNDS);
-      return nullptr;
-    };
-    auto step = [&] { if (w.s < g.nseg && ++w.t == w.nt) w.next_unit<N>(g); };
+  // launched with 72 registers for 896 threads (64512); sixteen warps of 56, eight of 112 and four of 56 are as many
+  if (warp < LA_UNPACK) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    // ---- unpack: lanes 4 r + p of a warp have key r of its eight, part p of every pair of 64 values (unpack32), so that a load takes 64 bytes of eight
+    // rows each. Codes and scales are a tile ahead in registers. A key that is not there reads row 0 in 4 bits, where any byte is some
+    // number: it has no weight. (8 bits have codes that are none: zeros.)
+    const int r8 = lane >> 2, p = lane & 3;
+    const bool up = BITS == 4 && p >= 2;
+    uint32_t at[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      at[q] = (warp * 8 + r8) * 128 + (BITS == 4 ? (p / 2) * LA_CH + ((((p & 1) * 4 + (up ? 2 : 0)) ^ r8 ^ q) << 4)
+                                                  : (q / 2) * LA_CH + (((2 * p) ^ r8 ^ (q & 1)) << 4));
+    const uint32_t ak = smem_u32(smem + C::K_AT);
+    const uint8_t* const codes = cache + p * 16;
+    const uint8_t* const bytes = cache + Row::scale_at(L) + (BITS == 4 ? (p & 1) * 2 * NC : (p >> 1) * NC);
     uint4 raw[C::PD][BITS / 4];
-    auto fetch = [&](uint4 (&r)[BITS / 4], const uint8_t* p, int c) {
-#pragma unroll
-      for (int i = 0; i < BITS / 4; ++i)
-        r[i] = p ? ldg_stream(p + c * 2 * CB + half * CB + i * 16) : BITS == 4 ? make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u) : make_uint4(0, 0, 0, 0);
-    };
-    constexpr int SCW = (SW + 3) / 4;
-    auto scales = [&](uint32_t (&v)[SCW], const uint8_t* p) {
-#pragma unroll
-      for (int i = 0; i < SCW; ++i) v[i] = 0;
-      if (!p) return;
-      const uint8_t* at = p + Row::scale_at(L) + half * SW;
-      if constexpr (SW >= 4) {
-#pragma unroll
-        for (int i = 0; i < SCW; ++i) v[i] = *reinterpret_cast<const uint32_t*>(at + 4 * i);
-      } else if constexpr (SW == 2) {
-        v[0] = *reinterpret_cast<const uint16_t*>(at);
+    auto fetch = [&](uint4 (&r)[BITS / 4], int row, int j) {
+      if constexpr (BITS == 4) {
+        if (2 * j + 1 < NC || p < 2) r[0] = ldg_stream(codes + (size_t)max(row, 0) * RB + j * 64);
       } else {
-        v[0] = *at;
+        const uint8_t* from = codes + (size_t)max(row, 0) * RB + j * 128;
+        r[0] = row >= 0 ? ldg_stream(from) : make_uint4(0, 0, 0, 0);
+        if (2 * j + 1 < NC) r[1] = row >= 0 ? ldg_stream(from + 64) : make_uint4(0, 0, 0, 0);
       }
     };
-    int off;
-    int blk = page_of(off);
-    const uint8_t* p0 = place(blk, off);
+    // scale bytes of a key, as they come (arithmetic on them here would wait for them): a word has those of two pairs
+    constexpr int SRW = NC == 8 && BITS == 4 ? 4 : NC == 8 ? 2 : NP, SCW = (NP + 1) / 2;
+    auto scales = [&](uint32_t (&v)[SRW], int row) {
+      const uint8_t* from = bytes + (size_t)max(row, 0) * RB;
+      if constexpr (NC == 8 && BITS == 4) {
+        const uint4 u = ldg_stream(from);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else if constexpr (NC == 8) {
+        const uint2 u = ldg_stream8(from);
+        v[0] = u.x; v[1] = u.y;
+      } else {
 #pragma unroll
-    for (int c = 0; c < C::PD; ++c) fetch(raw[c], p0, c);
-    uint32_t sc0[SCW], sc1[SCW];
-    scales(sc0, p0);
-    step();
-    blk = page_of(off);
-    const uint8_t* p1 = place(blk, off);
+        for (int j = 0; j < NP; ++j) {
+          v[j] = 0;
+          if constexpr (BITS == 4) {
+            if (2 * j + 1 < NC || p < 2) asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v[j]) : "l"(from + 4 * j + (p >> 1) * 2));
+          } else if (2 * j + 1 < NC) {
+            asm volatile("ld.global.nc.u16 %0, [%1];" : "=r"(v[j]) : "l"(from + 2 * j));
+          } else {
+            asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v[j]) : "l"(from + 2 * j));
+          }
+        }
+      }
+    };
+    auto pairs_of_bytes = [&](uint32_t (&v)[SCW], const uint32_t (&u)[SRW]) {
+      if constexpr (NC == 8 && BITS == 4) {
+        const uint32_t pick = p >= 2 ? 0x7632u : 0x5410u;
+        v[0] = __byte_perm(u[0], u[1], pick);
+        v[1] = __byte_perm(u[2], u[3], pick);
+      } else if constexpr (NC == 8) {
+        v[0] = u[0]; v[1] = u[1];
+      } else {
+#pragma unroll
+        for (int j = 0; j < NP; j += 2) v[j / 2] = j + 1 < NP ? u[j] | u[j + 1] << 16 : u[j];
+      }
+    };
+    bool ok = true;
+    auto look = [&](int i) -> int {                                      // the key's row of the cache, from the warp that looks them up
+      ok = ok && la_wait(&xfull[i % LA_AHEAD], i / LA_AHEAD & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      const int row = ms.rows[i % LA_AHEAD][warp * 8 + r8];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&xempty[i % LA_AHEAD]);
+      return ok ? row : -1;
+    };
+    int row0 = look(0), row1 = -1;
+    uint32_t sraw[SRW];
+#pragma unroll
+    for (int j = 0; j < C::PD; ++j) fetch(raw[j], row0, j);
+    scales(sraw, row0);
     int buf = 0;
     uint32_t kph = 1;                                                // (a fresh barrier passes a wait for parity 1)
-    bool ok = true;
     for (int i = 0; i < tiles; ++i) {
-      step();
-      blk = i + 2 < tiles ? page_of(off) : -2;
-      uint4 rope[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) rope[j] = p0 ? ldg_stream(p0 + Row::rope_at(L) + half * 64 + j * 16) : make_uint4(0, 0, 0, 0);
-      scales(sc1, i + 1 < tiles ? p1 : nullptr);
-      uint32_t nan = 0;
+      if (i + 1 < tiles) row1 = look(i + 1);
+      uint32_t sc[SCW], nan = 0;
+      pairs_of_bytes(sc, sraw);
+      scales(sraw, row1);
 #pragma unroll
       for (int j = 0; j < SCW; ++j) {
-        const uint32_t m = __vcmpgeu4(sc0[j], BITS == 4 ? 0xf8f8f8f8u : 0x87878787u);
+        const uint32_t m = __vcmpgeu4(sc[j], BITS == 4 ? 0xf8f8f8f8u : 0x87878787u);
         nan |= m;
-        sc0[j] &= ~m;
+        sc[j] &= ~m;
       }
       nan = __ballot_sync(0xffffffffu, nan != 0);
       if (lane == 0) ms.bad[i & 3][warp] = nan;
 #pragma unroll
       for (int j = 0; j < NP; ++j) {
-        ok = ok && mbar_wait_or_flag(&kempty[buf], kph, abort_flag);
+        ok = ok && la_wait(&kempty[buf], kph, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = 2 * j + e;
-          if (c < NC) {
-            uint32_t b0, b1;
-            if constexpr (BITS == 4) { b0 = sc0[c / 2] >> (16 * (c % 2)) & 255u; b1 = sc0[c / 2] >> (16 * (c % 2) + 8) & 255u; }
-            else { b0 = sc0[c / 4] >> (8 * (c % 4)) & 255u; b1 = b0; }
-            unpack32<BITS>(raw[c % C::PD], b0, b1, krow + buf * 2 * LA_CH + e * LA_CH, half * 4, turn);
-            if (c + C::PD < NC) fetch(raw[c % C::PD], p0, c + C::PD);
-            else if (i + 1 < tiles) fetch(raw[c % C::PD], p1, c + C::PD - NC);
-          }
-        }
+        if (BITS == 8 || 2 * j + 1 < NC || p < 2)
+          unpack32<BITS>(raw[j % C::PD], sc[j / 2] >> (16 * (j % 2)) & 0xffffu, ak + buf * 2 * LA_CH, at, up, 2 * j + 1 < NC);
+        if (j + C::PD < NP) fetch(raw[j % C::PD], row0, j + C::PD);
+        else fetch(raw[j % C::PD], row1, j + C::PD - NP);
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(&kfull[buf]);
         if (++buf == NB) { buf = 0; kph ^= 1; }
       }
       if (!ok) break;
-      ok = mbar_wait_or_flag(rempty, (i & 1) ^ 1, abort_flag);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(rrow + (((half * 4 + j) ^ turn) << 4)) = rope[j];
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(rfull);
-      p0 = p1;
-      p1 = place(blk, off);
-#pragma unroll
-      for (int j = 0; j < SCW; ++j) sc0[j] = sc1[j];
+      row0 = row1;
     }
     if (!ok) { set_status(status, ST_MBAR_TIMEOUT); *abort_flag = 1; }
-  } else if (warp == 16) {
-    // ---- products: the whole warp, one lane of it by predicate ------------------------------------------------------------------------------------
-    constexpr uint32_t id_s = umma_idesc(0, 0, 128, N), id_r = umma_idesc(1, 1, 128, N), id_o = umma_idesc(0, 0, 128, N) | 1u << 15 | 1u << 16;
-    constexpr uint32_t P_ROW = N * 2, P_SW = N == 64 ? 2 : N == 32 ? 4 : 6;        // the weights' rows: swizzled over 128, 64 or 32 bytes
-    const uint32_t aq = smem_u32(smem), ak = smem_u32(smem + C::K_AT), ar = smem_u32(smem + C::R_AT), ap = smem_u32(smem + C::P_AT);
-    const uint32_t ts = tmem + NP * N;
-    const bool issue = elect_one();
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_or_flag(bar, parity, abort_flag)); };
-    int buf = 0, i = 0, piece = 0;
-    uint32_t kph = 0;
-    bool ok = true;
-    while (ok && i < tiles) {
-      const int n = min(w.nt - w.t, tiles - i);
-      ok = wait(qfull, piece & 1);
-      for (int k = 0; ok && k < n; ++k, ++i) {
-        const int b0 = buf;
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-          if (!ok || !wait(&kfull[buf], kph)) { ok = false; break; }
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const int c = 2 * j + kk / 4;
-            if (c < NC)
-              tc_mma_f16_if(issue, ts, umma_desc_k128(ak + buf * 2 * LA_CH + (kk / 4) * LA_CH + (kk & 3) * 32),
-                            umma_desc_k128(aq + c * N * 128 + (kk & 3) * 32), id_s, j > 0 || kk > 0);
-          }
-          if (++buf == NB) { buf = 0; kph ^= 1; }
-        }
-        if (!ok || !wait(rfull, i & 1)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          tc_mma_f16_if(issue, ts, umma_desc_k128(ar + kk * 32), umma_desc_k128(aq + NC * N * 128 + kk * 32), id_r, 1u);
-        tc_commit_if(issue, sfull);
-        if (!C::SHARE) tc_commit_if(issue, rempty);
-        if (!wait(pfull, i & 1) || (k == 0 && piece > 0 && !wait(oempty, (piece - 1) & 1))) { ok = false; break; }
-        tc_fence_after();
-        int b = b0;
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            tc_mma_f16_if(issue, tmem + j * N, umma_desc_mn(ak + b * 2 * LA_CH + kk * 2048, LA_CH, 1024, 2),
-                          umma_desc_mn(ap + kk * 16 * P_ROW, 0, 8 * P_ROW, P_SW), id_o, k > 0 || kk > 0);
-          tc_commit_if(issue, &kempty[b]);
-          if (++b == NB) b = 0;
-        }
-        if (C::SHARE) tc_commit_if(issue, rempty);
-      }
-      if (!ok) break;
-      tc_commit_if(issue, ofull);
-      ++piece;
-      if (w.t + n == w.nt) w.next_unit<N>(g);                        // (else the list ends here)
-    }
-    if (!ok) {
-      set_status(status, ST_MBAR_TIMEOUT);
-      *abort_flag = 1;
-      // products in flight end before their TMEM goes: a commit behind all of them, on a barrier that nobody else waits for any more
-      tc_commit_if(issue, ofull);
-      mbar_wait(ofull, piece & 1, 1u << 20);
-    }
-  } else {
+  } else if (warp < LA_SOFT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ---- softmax: thread = (key, half of the pairs) ----------------------------------------------------------------------------------------------
-    const int quad = warp & 3, hc = (warp - 8) >> 2, st = tid - 256, key = quad * 32 + lane;
+    constexpr int W = CW < 16 ? CW : 16;                             // pairs in registers at a time
+    const int quad = warp & 3, hc = (warp - LA_UNPACK) >> 2, st = tid - LA_UNPACK * 32, key = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, ts = tmem + lanes + NP * N + hc * CW, to = tmem + lanes + hc * CW;
     auto fmx = [](float a, float b) { return fmaxf(a, b); };
     auto fad = [](float a, float b) { return a + b; };
@@ -451,7 +419,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         uint4 v[AT_ONCE][UV], r[AT_ONCE];
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
-          const int n = (b + k) * 8 + warp - 8;
+          const int n = (b + k) * 8 + warp - LA_UNPACK;
           const uint4* src = reinterpret_cast<const uint4*>(q0 + (size_t)n * D);
 #pragma unroll
           for (int x = 0; x < UV; ++x) v[k][x] = n < np && x * 32 + lane < L / 8 ? __ldg(src + x * 32 + lane) : make_uint4(0, 0, 0, 0);
@@ -459,7 +427,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         }
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
-          const int n = (b + k) * 8 + warp - 8;
+          const int n = (b + k) * 8 + warp - LA_UNPACK;
           float top = 0.f;
           auto look = [&](const uint4& u) {
             const uint32_t a[4] = {u.x, u.y, u.z, u.w};
@@ -495,6 +463,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
           }
           if (lane == 0) {
             ms.c[par][n] = scale_log2 * __uint_as_float((uint32_t)(ex - 10 + 127) << 23);
+            ms.nr[par][n] = 0.f;
             ms.see[par][n] = n < np ? min(max(g.kvlen[w.row0 + (int)(((long)w.u * N + n) / g.nq)], 0), w.kv) : w.kv;
           }
         }
@@ -504,138 +473,130 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       if (lane == 0) mbar_arrive(qfull);
     };
 
-    int i = 0, piece = 0, unit = ms.start[3];
-    int flat = f0;
+    int i = 0, piece = 0, unit = ms.start[3], flat = f0;
     bool broke = false;
-    load_q(0);
-    while (i < tiles) {
-      const int par = piece & 1, n = min(w.nt - w.t, tiles - i), t0 = w.t, nt = w.nt, np = pairs_of(w);
+    // once round per piece: its tiles, the next one's queries (no score needs this one's any more), its end
+    for (int n = 0;; ++piece) {
+      const int par = piece & 1, t0 = w.t, nt = w.nt, np = pairs_of(w);
       const size_t base = (size_t)w.row0 * g.nq + (size_t)w.u * N;
-      softmax_sync();                                                // what load_q wrote beside the queries
-      const int least = ms.see[par][0];                              // rows of a segment see no fewer keys than those ahead of them
       uint64_t sum[CW / 2];
+      if (piece > 0) {
+        n = min(nt - t0, tiles - i);
+        softmax_sync();                                              // what load_q wrote beside the queries
+        const int least = ms.see[par][0];                            // rows of a segment see no fewer keys than those ahead of them
 #pragma unroll
-      for (int e = 0; e < CW / 2; ++e) sum[e] = f2_pack(0.f, 0.f);
-      for (int k = 0; k < n; ++k, ++i) {
-        bool ok = mbar_wait_or_flag(sfull, i & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        float v[CW];
-        {
-          uint32_t s[CW];
-          tc_fence_after();
-          tmem_ld<CW>(ts, s);
-          tmem_ld_wait();
-          tc_fence_before();
-#pragma unroll
-          for (int e = 0; e < CW; ++e) v[e] = __uint_as_float(s[e]);
-        }
-        const int at = (t0 + k) * LA_KT + key;
-        if (ms.bad[i & 3][key >> 4] >> (2 * (key & 15)) & 3u) {
-#pragma unroll
-          for (int e = 0; e < CW; ++e) v[e] = __uint_as_float(0x7fc00000u);
-        }
-        const bool edge = (t0 + k + 1) * LA_KT > least;
-        if (k == 0) {
-          float x[CW];
-#pragma unroll
-          for (int e = 0; e < CW; ++e) {
-            x[e] = v[e] * ms.c[par][hc * CW + e];
-            if (edge && at >= ms.see[par][hc * CW + e]) x[e] = -INFINITY;
-          }
-          const float m = columns<CW>(x, lane, fmx);
-          if (lane < CW) ms.mx[quad][hc * CW + lane] = m;
-          softmax_sync();
-          if (st < N) {
-            const float top = fmaxf(fmaxf(ms.mx[0][st], ms.mx[1][st]), fmaxf(ms.mx[2][st], ms.mx[3][st]));
-            ms.nr[par][st] = top == -INFINITY ? 0.f : LA_TOP - top;
-          }
-          softmax_sync();
-        }
-        bool past = !ok;
-#pragma unroll
-        for (int e = 0; e < CW; e += 2) {
-          const float2 c = *reinterpret_cast<const float2*>(&ms.c[par][hc * CW + e]), nr = *reinterpret_cast<const float2*>(&ms.nr[par][hc * CW + e]);
-          const float2 x = f2_unpack(f2_fma(f2_pack(v[e], v[e + 1]), f2_pack(c.x, c.y), f2_pack(nr.x, nr.y)));
-          v[e] = x.x; v[e + 1] = x.y;
-        }
-        if (edge) {
-#pragma unroll
-          for (int e = 0; e < CW; ++e)
-            if (at >= ms.see[par][hc * CW + e]) v[e] = -INFINITY;
-        }
-        float top = v[0];
-#pragma unroll
-        for (int e = 1; e < CW; ++e) top = fmaxf(top, v[e]);
-        past |= top > LA_LIMIT;
-        if (softmax_any(past)) {
-          if (!ok) ms.fail = 1;
-          const float m = columns<CW>(v, lane, fmx);
-          if (lane < CW) ms.mx[quad][hc * CW + lane] = m;
-          softmax_sync();
-          if (ms.fail) { broke = true; break; }
-          if (st < N) {
-            const float most = fmaxf(fmaxf(ms.mx[0][st], ms.mx[1][st]), fmaxf(ms.mx[2][st], ms.mx[3][st]));
-            const float d = most > LA_TOP ? most - LA_TOP : 0.f;
-            ms.d[st] = d;
-            ms.nr[par][st] -= d;
-          }
-          softmax_sync();
-          float f[CW];
-#pragma unroll
-          for (int e = 0; e < CW; ++e) {
-            const float d = ms.d[hc * CW + e];
-            v[e] -= d;
-            f[e] = ex2(-d);
-          }
-#pragma unroll
-          for (int e = 0; e < CW / 2; ++e) sum[e] = f2_mul(sum[e], f2_pack(f[2 * e], f[2 * e + 1]));
-          if (k > 0) {                                               // (the tile's scores are complete, so the products ahead of them are)
+        for (int e = 0; e < CW / 2; ++e) sum[e] = f2_pack(0.f, 0.f);
 #pragma unroll 1
-            for (int j = 0; j < NP; ++j) {
-              uint32_t o[CW];
-              tmem_ld<CW>(to + j * N, o);
-              tmem_ld_wait();
+        for (int k = 0; k < n; ++k, ++i) {
+          bool ok = la_wait(sfull, i & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          tc_fence_after();
+          const int at = (t0 + k) * LA_KT + key;
+          const bool edge = (t0 + k + 1) * LA_KT > least, none = ms.bad[i & 3][key >> 3] >> (4 * (key & 7)) & 15u;
+          // log2 of the thread's weights, up to the reference
+          auto scores = [&](float (&x)[CW]) {
+            uint32_t r[CW];
+            tmem_ld<CW>(ts, r);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < CW; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f[e]);
-              tmem_st<CW>(to + j * N, o);
+            for (int e = 0; e < CW; e += 4) {
+              const float4 c = *reinterpret_cast<const float4*>(&ms.c[par][hc * CW + e]), nr = *reinterpret_cast<const float4*>(&ms.nr[par][hc * CW + e]);
+              const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), f2_pack(c.x, c.y), f2_pack(nr.x, nr.y)));
+              const float2 b = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), f2_pack(c.z, c.w), f2_pack(nr.z, nr.w)));
+              x[e] = a.x; x[e + 1] = a.y; x[e + 2] = b.x; x[e + 3] = b.y;
             }
-            tmem_st_wait();
-            tc_fence_before();
+            if (none) {
+#pragma unroll
+              for (int e = 0; e < CW; ++e) x[e] = __uint_as_float(0x7fc00000u);
+            }
+            if (edge) {
+#pragma unroll
+              for (int e = 0; e < CW; ++e)
+                if (at >= ms.see[par][hc * CW + e]) x[e] = -INFINITY;
+            }
+          };
+          unsigned char* prow = smem + C::P_AT + key * N * 2;
+          const int pturn = N == 64 ? key & 7 : N == 32 ? key >> 1 & 3 : key >> 2 & 1;
+          // Weights by the reference there is; a tile whose scores pass the limit (all 256 threads look) and a piece's first (load_q left zeros) get one anew
+          // and go round again.
+          bool anew = k == 0, done = false;
+#pragma unroll 1
+          while (!done) {
+            float x[CW];
+            scores(x);
+            if (anew) {
+              if (!ok) ms.fail = 1;
+              const float m = columns<CW>(x, lane, fmx);
+              if (lane < CW) ms.mx[quad][hc * CW + lane] = m;
+              softmax_sync();
+              if (ms.fail) break;
+              if (st < N) {
+                const float most = fmaxf(fmaxf(ms.mx[0][st], ms.mx[1][st]), fmaxf(ms.mx[2][st], ms.mx[3][st]));
+                const float d = k == 0 ? (most == -INFINITY ? 0.f : most - LA_TOP) : most > LA_TOP ? most - LA_TOP : 0.f;
+                ms.d[st] = d;
+                ms.nr[par][st] -= d;
+              }
+              softmax_sync();
+              anew = false;
+              if (k > 0) {                                           // (the tile's scores are complete, so the products ahead of them are)
+#pragma unroll
+                for (int e = 0; e < CW; e += 2) {
+                  // the weights of this tile leave the sums again; what they rounded off is 2^-24 of the new largest weight. Sums of 2^-100 of that are none.
+                  const float2 d = *reinterpret_cast<const float2*>(&ms.d[hc * CW + e]), l = f2_unpack(sum[e / 2]);
+                  sum[e / 2] = f2_pack(d.x > 100.f ? 0.f : (l.x - ex2(x[e])) * ex2(-d.x), d.y > 100.f ? 0.f : (l.y - ex2(x[e + 1])) * ex2(-d.y));
+                }
+#pragma unroll 1
+                for (int j = 0; j < NP * CW; j += W) {
+                  uint32_t o[W];
+                  tmem_ld<W>(to + j / CW * N + j % CW, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < W; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * ex2(-ms.d[hc * CW + j % CW + e]));
+                  tmem_st<W>(to + j / CW * N + j % CW, o);
+                }
+                tmem_st_wait();
+              }
+              continue;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int h = 0; h < CW; h += 8) {
+              uint32_t pw[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                top = fmaxf(top, fmaxf(x[h + 2 * e], x[h + 2 * e + 1]));
+                const float a = ex2(x[h + 2 * e]), b = ex2(x[h + 2 * e + 1]);
+                sum[h / 2 + e] = f2_add(sum[h / 2 + e], f2_pack(a, b));
+                const __half2 p2 = __floats2half2_rn(a, b);
+                pw[e] = *reinterpret_cast<const uint32_t*>(&p2);
+              }
+              *reinterpret_cast<uint4*>(prow + (((hc * (CW / 8) + h / 8) ^ pturn) << 4)) = make_uint4(pw[0], pw[1], pw[2], pw[3]);
+            }
+            anew = softmax_any(!ok || top > LA_LIMIT);
+            done = !anew;
           }
+          if (!done) { broke = true; break; }
+          tc_fence_before();
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pfull);
         }
-        uint32_t pw[CW / 2];
+        if (broke) break;
+        float a[CW];
 #pragma unroll
         for (int e = 0; e < CW / 2; ++e) {
-          const float a = ex2(v[2 * e]), b = ex2(v[2 * e + 1]);
-          sum[e] = f2_add(sum[e], f2_pack(a, b));
-          const __half2 h = __floats2half2_rn(a, b);
-          pw[e] = *reinterpret_cast<const uint32_t*>(&h);
+          const float2 x = f2_unpack(sum[e]);
+          a[2 * e] = x.x; a[2 * e + 1] = x.y;
         }
-        unsigned char* prow = smem + C::P_AT + key * N * 2;
-        const int pturn = N == 64 ? key & 7 : N == 32 ? key >> 1 & 3 : key >> 2 & 1;
-#pragma unroll
-        for (int e = 0; e < CW / 8; ++e)
-          *reinterpret_cast<uint4*>(prow + (((hc * (CW / 8) + e) ^ pturn) << 4)) = make_uint4(pw[4 * e], pw[4 * e + 1], pw[4 * e + 2], pw[4 * e + 3]);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pfull);
+        const float l = columns<CW>(a, lane, fad);
+        if (lane < CW) ms.mx[quad][hc * CW + lane] = l;
+        if (t0 + n == nt) w.next_unit<N>(g);
       }
-      if (broke) break;
-      // ---- the piece's end; the next one's queries first (its scores no longer need this one's) ------------------------------------------------
+      if (i < tiles) load_q(piece + 1 & 1);
+      if (piece == 0) continue;
+      // ---- the piece's end
       const bool whole = t0 == 0 && n == nt;
-      const int my_unit = unit, first_flat = flat - t0;
-      flat += n;
-      if (t0 + n == nt) { w.next_unit<N>(g); ++unit; }
-      if (i < tiles) load_q(par ^ 1);
-      float a[CW];
-#pragma unroll
-      for (int e = 0; e < CW / 2; ++e) {
-        const float2 x = f2_unpack(sum[e]);
-        a[2 * e] = x.x; a[2 * e + 1] = x.y;
-      }
-      const float l = columns<CW>(a, lane, fad);
-      if (lane < CW) ms.mx[quad][hc * CW + lane] = l;
-      bool ok = mbar_wait_or_flag(ofull, piece & 1, abort_flag);
+      bool ok = la_wait(ofull, piece - 1 & 1, abort_flag);
       if (!__all_sync(0xffffffffu, ok)) ms.fail = 1;
       softmax_sync();
       if (ms.fail) { broke = true; break; }
@@ -650,42 +611,153 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
           ml[1] = lt;
         }
       }
-      if (st == 0) {
-        if (t0 == 0 && (by_unit || !whole))
-          join[by_unit ? my_unit : (int)blockIdx.x] = make_int4((int)base, whole ? 0 : np, rec, (first_flat + nt - 1) / share);
-      }
+      if (st == 0 && t0 == 0 && (by_unit || !whole))
+        join[by_unit ? unit : (int)blockIdx.x] = make_int4((int)base, whole ? 0 : np, rec, (flat + nt - 1) / share);
+      if (t0 + n == nt) ++unit;
+      flat += n;
       softmax_sync();
       tc_fence_after();
 #pragma unroll 1
-      for (int j = 0; j < NP; ++j) {
-        uint32_t o[CW];
-        tmem_ld<CW>(to + j * N, o);
+      for (int j = 0; j < NP * CW; j += W) {
+        uint32_t o[W];
+        const int n0 = hc * CW + j % CW, e0 = j / CW * 128 + quad * 32 + lane;
+        tmem_ld<W>(to + j / CW * N + j % CW, o);
         tmem_ld_wait();
-        const int e0 = j * 128 + quad * 32 + lane;
         if (e0 < L) {
           if (whole) {
-            __nv_bfloat16* dst = out + (base + hc * CW) * L + e0;
+            __nv_bfloat16* dst = out + (base + n0) * L + e0;
 #pragma unroll
-            for (int e = 0; e < CW; ++e)
-              if (hc * CW + e < np) dst[(size_t)e * L] = f2bf(__uint_as_float(o[e]) * ms.d[hc * CW + e]);
+            for (int e = 0; e < W; ++e)
+              if (n0 + e < np) dst[(size_t)e * L] = f2bf(__uint_as_float(o[e]) * ms.d[n0 + e]);
           } else {
-            float* dst = o_part + ((size_t)rec * N + hc * CW) * L + e0;
+            float* dst = o_part + ((size_t)rec * N + n0) * L + e0;
 #pragma unroll
-            for (int e = 0; e < CW; ++e)
-              if (hc * CW + e < np) dst[(size_t)e * L] = __uint_as_float(o[e]);
+            for (int e = 0; e < W; ++e)
+              if (n0 + e < np) dst[(size_t)e * L] = __uint_as_float(o[e]);
           }
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(oempty);
-      ++piece;
+      if (i >= tiles) break;
     }
     if (broke && st == 0) { set_status(status, ST_MBAR_TIMEOUT); *abort_flag = 1; }
+    } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == LA_SOFT) {
+      // ---- products: the whole warp, one lane of it by predicate ------------------------------------------------------------------------------------
+      constexpr uint32_t id_s = umma_idesc(0, 0, 128, N), id_r = umma_idesc(1, 1, 128, N), id_o = umma_idesc(0, 0, 128, N) | 1u << 15 | 1u << 16;
+      constexpr uint32_t P_ROW = N * 2, P_SW = N == 64 ? 2 : N == 32 ? 4 : 6;        // the weights' rows: swizzled over 128, 64 or 32 bytes
+      const uint32_t aq = smem_u32(smem), ak = smem_u32(smem + C::K_AT), ar = smem_u32(smem + C::R_AT), ap = smem_u32(smem + C::P_AT);
+      const uint32_t ts = tmem + NP * N;
+      const bool issue = elect_one();
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, la_wait(bar, parity, abort_flag)); };
+      int buf = 0, i = 0, piece = 0;
+      uint32_t kph = 0;
+      bool ok = true;
+      while (ok && i < tiles) {
+        const int n = min(w.nt - w.t, tiles - i);
+        ok = wait(qfull, piece & 1);
+        for (int k = 0; ok && k < n; ++k, ++i) {
+          const int b0 = buf;
+#pragma unroll 1
+          for (int j = 0; j < NP; ++j) {
+            if (!ok || !wait(&kfull[buf], kph)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t da = umma_desc_k128(ak + buf * 2 * LA_CH), db = umma_desc_k128(aq + j * 2 * N * 128);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              if (kk < 4 || 2 * j + 1 < NC)
+                tc_mma_f16_if(issue, ts, da + ((kk / 4) * LA_CH + (kk & 3) * 32 >> 4), db + ((kk / 4) * N * 128 + (kk & 3) * 32 >> 4), id_s, j > 0 || kk > 0);
+            if (++buf == NB) { buf = 0; kph ^= 1; }
+          }
+          if (!ok || !wait(rfull, i & 1)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            tc_mma_f16_if(issue, ts, umma_desc_k128(ar + kk * 32), umma_desc_k128(aq + NC * N * 128 + kk * 32), id_r, 1u);
+          tc_commit_if(issue, sfull);
+          if (!C::SHARE) tc_commit_if(issue, rempty);
+          if (!wait(pfull, i & 1) || (k == 0 && piece > 0 && !wait(oempty, (piece - 1) & 1))) { ok = false; break; }
+          tc_fence_after();
+          int b = b0;
+          const uint64_t dp = umma_desc_mn(ap, 0, 8 * P_ROW, P_SW);
+#pragma unroll 1
+          for (int j = 0; j < NP; ++j) {
+            const uint64_t dv = umma_desc_mn(ak + b * 2 * LA_CH, LA_CH, 1024, 2);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_f16_if(issue, tmem + j * N, dv + (kk * 2048 >> 4), dp + (kk * 16 * P_ROW >> 4), id_o, k > 0 || kk > 0);
+            tc_commit_if(issue, &kempty[b]);
+            if (++b == NB) b = 0;
+          }
+          if (C::SHARE) tc_commit_if(issue, rempty);
+        }
+        if (!ok) break;
+        tc_commit_if(issue, ofull);
+        ++piece;
+        if (w.t + n == w.nt) w.next_unit<N>(g);                        // (else the list ends here)
+      }
+      if (!ok) {
+        set_status(status, ST_MBAR_TIMEOUT);
+        *abort_flag = 1;
+        // products in flight end before their TMEM goes: a commit behind all of them, on a barrier that nobody else waits for any more
+        tc_commit_if(issue, ofull);
+        mbar_wait(ofull, piece & 1, 1u << 20);
+      }
+    } else if (warp == LA_SOFT + 3) {
+      // ---- rows of the cache of the tiles' keys, four a lane
+      bool ok = true;
+      for (int i = 0; i < tiles; ++i) {
+        int row[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int key = w.t * LA_KT + k * 32 + lane;
+          row[k] = -1;
+          if (key < w.kv) {
+            const int at = key / kv_block, blk = block_table[(size_t)w.slot * max_blocks + at];
+            if (blk >= 0 && blk < pages) row[k] = blk * kv_block + key - at * kv_block;      // (rows of a cache are fewer than 2^31)
+            else set_status(status, ST_BOUNDS);
+          }
+        }
+        ok = la_wait(&xempty[i % LA_AHEAD], (i / LA_AHEAD & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ms.rows[i % LA_AHEAD][k * 32 + lane] = row[k];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xfull[i % LA_AHEAD]);
+        if (++w.t == w.nt) w.next_unit<N>(g);
+      }
+      if (!ok) { set_status(status, ST_MBAR_TIMEOUT); *abort_flag = 1; }
+    } else {
+      // ---- key parts: a warp copies those of 64 keys as they are, eight lanes a row. Their place is free late and they are needed last, so they go straight
+      // to shared memory.
+      bool ok = true;
+      for (int i = 0; i < tiles; ++i) {
+        ok = la_wait(&xfull[i % LA_AHEAD], i / LA_AHEAD & 1, abort_flag) && la_wait(rempty, (i & 1) ^ 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll 4
+        for (int m = 0; m < 16; ++m) {
+          const int key = (warp - LA_SOFT - 1) * 64 + m * 4 + (lane >> 3), r = ms.rows[i % LA_AHEAD][key];
+          const uint32_t to = smem_u32(smem + C::R_AT) + key * 128 + (((lane & 7) ^ (key & 7)) << 4);
+          // (no bytes, zeros in their place, where there is no row)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(to), "l"(cache + (size_t)max(r, 0) * RB + Row::rope_at(L) + (lane & 7) * 16), "r"(r >= 0 ? 16 : 0) : "memory");
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&xempty[i % LA_AHEAD]);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(rfull);
+      }
+      if (!ok) { set_status(status, ST_MBAR_TIMEOUT); *abort_flag = 1; }
+    }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 16) tmem_dealloc(tmem, C::TMEM);
+  if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);
 }
 
 // Units that span CTAs. grid (entries, N), 128 threads: a CTA a pair, its records in the order of their keys.
@@ -747,6 +819,7 @@ extern "C" int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* q
                              int max_blocks, int kv_block, int rows, int nq, int L, int R, float scale, int ctas, int* status, cudaStream_t s) {
   if (R != LC_R || (bits != 4 && bits != 8) || nq < 1 || kv_block < 1 || ctas < 1 || max_rows < 0) return -1;
   if (((uintptr_t)qabs | (uintptr_t)cache | (uintptr_t)ws) % 16 || (uintptr_t)out % 8) return -2;
+  if (pages < 1 || pages * kv_block > 0x7fffffffl) return -2;
   if (rows <= 0 || nseg <= 0 || max_rows == 0) return 0;
   if (ws_floats < fb_mla_attn_q_floats(max_rows, nq, L, ctas)) return -3;
   const int N = latent_pairs((long)max_rows * nq);
