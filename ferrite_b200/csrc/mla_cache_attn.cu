@@ -55,8 +55,6 @@ struct LatentAttnMisc {
   int see[2][N];                                 // keys that a pair sees
   float mx[4][N], d[N];
   uint32_t bad[4][16];                           // of the last tiles: keys that are no number, four bits a key
-  long long scan[LA_THREADS / 32];
-  int start[4];
   int rows[LA_AHEAD][LA_KT];                     // ring of tiles: their keys' rows of the cache, -1 where there is none
   uint64_t bars[2 * 5 + 7 + 2 * LA_AHEAD];
   uint32_t tmem;
@@ -74,7 +72,7 @@ struct LatentWalk {                              // a place in the list of tiles
   __device__ __forceinline__ void load(const LatentSegs& g) {
     nrows = g.nrows[s]; row0 = g.row0[s]; slot = g.slot[s];
     kv = nrows > 0 ? (int)min((long)max(g.kvlen[row0 + nrows - 1], 0), g.limit) : 0;
-    units = (int)(((long)max(nrows, 0) * g.nq + N - 1) / N);
+    units = (int)(((uint32_t)max(nrows, 0) * g.nq + N - 1) / N);       // (rows times heads are fewer than 2^30)
     nt = max(1, (kv + LA_KT - 1) / LA_KT);
   }
   template <int N>
@@ -83,6 +81,7 @@ struct LatentWalk {                              // a place in the list of tiles
     if (++u < units) return;
     u = 0;
     units = 0;
+#pragma unroll 1
     while (++s < g.nseg) {
       load<N>(g);
       if (units) break;
@@ -98,16 +97,20 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Bounded wait that leaves the issue slots to others: the hardware holds the warp for up to 20 us a poll.
+// Wait of at most 2^31 cycles (about a second) that leaves the issue slots to others: the hardware holds the warp for up to 20 us a poll.
+__device__ __forceinline__ bool la_poll(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+  return ok;
+}
 __device__ __forceinline__ bool la_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  for (int i = 0; i < (1 << 16); ++i) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
-    if (ok) return true;
-    if (*abort_flag) return false;
-  }
-  return false;
+  if (la_poll(bar, parity)) return true;
+  const long long t0 = clock64();
+#pragma unroll 1
+  while (!la_poll(bar, parity))
+    if (*abort_flag || clock64() - t0 > 1ll << 31) return false;
+  return true;
 }
 template <int W>
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[W]) {
@@ -217,68 +220,16 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &ms.abort;
   pdl_launch_dependents();
+  if (smem_u32(smem) & 1023u) {                                      // the swizzled tiles need the 1024-byte base
+    if (tid == 0) set_status(status, ST_BOUNDS);
+    return;
+  }
   if (tid == 0) {
     ms.abort = 0; ms.fail = 0;
     for (int i = 0; i < NB; ++i) { mbar_init(&kfull[i], LA_UNPACK); mbar_init(&kempty[i], 1); }
     mbar_init(rfull, 2); mbar_init(rempty, 1); mbar_init(sfull, 1); mbar_init(pfull, 8); mbar_init(qfull, 8); mbar_init(ofull, 1); mbar_init(oempty, 8);
     for (int i = 0; i < LA_AHEAD; ++i) { mbar_init(&xfull[i], 1); mbar_init(&xempty[i], LA_UNPACK + 2); }
     fence_mbar_init();
-  }
-  pdl_wait();
-  qabs = after_wait(qabs); cache = after_wait(cache); block_table = after_wait(block_table);
-  g.slot = after_wait(g.slot); g.row0 = after_wait(g.row0); g.nrows = after_wait(g.nrows); g.kvlen = after_wait(g.kvlen);
-
-  // ---- this CTA's share of the list: prefix sums of the segments' tiles (low 40 bits) and units (the rest) -----------------------------------------
-  const int per_thread = (g.nseg + LA_THREADS - 1) / LA_THREADS;
-  const int s_lo = min(tid * per_thread, g.nseg), s_hi = min(s_lo + per_thread, g.nseg);
-  LatentWalk w;
-  long long mine = 0;
-  for (w.s = s_lo; w.s < s_hi; ++w.s) {
-    w.load<N>(g);
-    mine += (long long)w.units * w.nt + ((long long)w.units << 40);
-    if (blockIdx.x == 0 && w.nrows > 0 && (long)g.kvlen[w.row0 + w.nrows - 1] > g.limit) set_status(status, ST_BOUNDS);
-  }
-  long long before = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += v;
-  }
-  if (lane == 31) ms.scan[warp] = before;
-  __syncthreads();
-  long long total = 0;
-  before -= mine;
-  for (int i = 0; i < LA_THREADS / 32; ++i) {
-    if (i < warp) before += ms.scan[i];
-    total += ms.scan[i];
-  }
-  constexpr long long TILES = (1ll << 40) - 1;
-  const int all = (int)(total & TILES), share = max(1, (all + (int)gridDim.x - 1) / (int)gridDim.x);
-  const int f0 = min((int)blockIdx.x * share, all), f1 = min(f0 + share, all), tiles = f1 - f0;
-  if (by_unit) {
-    if (blockIdx.x == 0)
-      for (int i = (int)(total >> 40) + tid; i < entries; i += LA_THREADS) join[i] = make_int4(0, 0, 0, 0);
-  } else if (tid == 0) {
-    join[blockIdx.x] = make_int4(0, 0, 0, 0);
-  }
-  if (by_unit && (int)(total >> 40) > entries) {                     // segments of more rows than the caller said
-    if (tid == 0) set_status(status, ST_CAPACITY);
-    return;
-  }
-  if (tiles == 0) return;                                            // the same for the whole CTA, before any allocation
-  if (smem_u32(smem) & 1023u) {                                      // the swizzled tiles need the 1024-byte base
-    if (tid == 0) set_status(status, ST_BOUNDS);
-    return;
-  }
-  if (f0 >= (before & TILES) && f0 < (before & TILES) + (mine & TILES)) {
-    int at = f0 - (int)(before & TILES), unit = (int)(before >> 40);
-    for (w.s = s_lo; w.s < s_hi; ++w.s) {
-      w.load<N>(g);
-      if (at < w.units * w.nt) break;
-      at -= w.units * w.nt;
-      unit += w.units;
-    }
-    ms.start[0] = w.s; ms.start[1] = at / w.nt; ms.start[2] = at % w.nt; ms.start[3] = unit + at / w.nt;
   }
   if (warp == LA_SOFT) {
     tmem_alloc(&ms.tmem, C::TMEM);
@@ -288,8 +239,72 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = ms.tmem;
-  w.s = ms.start[0]; w.u = ms.start[1]; w.t = ms.start[2];
-  w.load<N>(g);
+  pdl_wait();
+  qabs = after_wait(qabs); cache = after_wait(cache); block_table = after_wait(block_table);
+  g.slot = after_wait(g.slot); g.row0 = after_wait(g.row0); g.nrows = after_wait(g.nrows); g.kvlen = after_wait(g.kvlen);
+
+  // ---- this CTA's share of the list, by every warp for itself (no barrier stands between the lengths and a role's first load): sums over the segments, a
+  // lane each, of their tiles (low 40 bits) and units (the rest)
+  constexpr long long TILES = (1ll << 40) - 1;
+  LatentWalk w;
+  auto count = [&](int seg) -> long long {
+    if (seg >= g.nseg) return 0;
+    w.s = seg;
+    w.load<N>(g);
+    return (long long)w.units * w.nt + ((long long)w.units << 40);
+  };
+  long long mine = 0, total = 0;
+#pragma unroll 1
+  for (int seg = lane; seg < g.nseg; seg += 32) total += mine = count(seg);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  const int all = (int)(total & TILES), share = max(1, (int)((uint32_t)(all + (int)gridDim.x - 1) / gridDim.x));
+  const int f0 = min((int)blockIdx.x * share, all), f1 = min(f0 + share, all), tiles = f1 - f0;
+  if (by_unit) {
+    if (blockIdx.x == 0)
+#pragma unroll 1
+      for (int i = (int)(total >> 40) + tid; i < entries; i += LA_THREADS) join[i] = make_int4(0, 0, 0, 0);
+  } else if (tid == LA_UNPACK * 32) {                                // (the thread that may write another one there)
+    join[blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
+  if (blockIdx.x == 0 && warp == 0)
+#pragma unroll 1
+    for (int seg = lane; seg < g.nseg; seg += 32)
+      if (g.nrows[seg] > 0 && (long)g.kvlen[g.row0[seg] + g.nrows[seg] - 1] > g.limit) set_status(status, ST_BOUNDS);
+  const bool much = by_unit && (int)(total >> 40) > entries;         // segments of more rows than the caller said
+  if (tiles == 0 || much) {                                          // the same for the whole CTA
+    if (tid == 0 && much) set_status(status, ST_CAPACITY);
+    if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);
+    return;
+  }
+  int unit = 0;
+  {
+    long long done = 0;
+#pragma unroll 1
+    for (int seg0 = 0; seg0 < g.nseg; seg0 += 32) {
+      if (g.nseg > 32) mine = count(seg0 + lane);
+      long long end = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += v;
+      }
+      end += done;
+      const uint32_t hit = __ballot_sync(0xffffffffu, f0 < (int)(end & TILES));
+      if (hit) {
+        const int from = __ffs(hit) - 1;
+        auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
+        const int at = of(f0 - (int)(end - mine & TILES));
+        unit = of((int)(end - mine >> 40));
+        w.s = seg0 + from; w.units = of(w.units); w.nt = of(w.nt); w.kv = of(w.kv); w.row0 = of(w.row0); w.nrows = of(w.nrows); w.slot = of(w.slot);
+        w.u = (int)((uint32_t)at / (uint32_t)w.nt);
+        w.t = at - w.u * w.nt;
+        unit += w.u;
+        break;
+      }
+      done = __shfl_sync(0xffffffffu, end, 31);
+    }
+  }
 
   // launched with 72 registers for 896 threads (64512); sixteen warps of 56, eight of 112 and four of 56 are as many
   if (warp < LA_UNPACK) {
@@ -407,65 +422,55 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, ts = tmem + lanes + NP * N + hc * CW, to = tmem + lanes + hc * CW;
     auto fmx = [](float a, float b) { return fmaxf(a, b); };
     auto fad = [](float a, float b) { return a + b; };
-    auto pairs_of = [&](const LatentWalk& x) { return (int)min((long)N, (long)x.nrows * g.nq - (long)x.u * N); };
+    auto pairs_of = [&](const LatentWalk& x) { return min(N, x.nrows * g.nq - x.u * N); };
 
-    // queries of the walk's unit -> shared memory, and what belongs to each pair
+    // queries of the walk's unit -> shared memory, and what belongs to each pair. Eight lanes have a pair; a thread turns the 16-byte pieces that it copied
+    // itself, in their places. (Loops, not unrolled ones: a CTA comes by once or twice, and code that is new to the SM costs more than its instructions.)
     auto load_q = [&](int par) {
-      const int np = pairs_of(w);
-      const __nv_bfloat16* q0 = qabs + ((size_t)w.row0 * g.nq + (size_t)w.u * N) * D;
-      constexpr int PER = N / 8, AT_ONCE = PER < 4 ? PER : 4, UV = (L / 8 + 31) / 32;
+      const int np = pairs_of(w), n0 = (warp - LA_UNPACK) * 4 + (lane >> 3);
+      const __nv_bfloat16* q0 = qabs + ((size_t)w.row0 * g.nq + (size_t)w.u * N) * D + (lane & 7) * 8;
+      auto place = [&](int n, int c) { return smem + (c * N + n) * 128 + (((lane & 7) ^ (n & 7)) << 4); };
 #pragma unroll 1
-      for (int b = 0; b < PER; b += AT_ONCE) {
-        uint4 v[AT_ONCE][UV], r[AT_ONCE];
+      for (int n = n0; n < N; n += 32)
+#pragma unroll 3
+        for (int c = 0; c <= NC; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(smem_u32(place(n, c))), "l"(q0 + (size_t)(n < np ? n : 0) * D + c * 64), "r"(n < np ? 16 : 0) : "memory");
+      asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+      for (int n = n0; n < N; n += 32) {
+        __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+#pragma unroll 3
+        for (int c = 0; c <= NC; ++c) {
+          const uint4 u = *reinterpret_cast<const uint4*>(place(n, c));
+          const uint32_t a[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) {
-          const int n = (b + k) * 8 + warp - LA_UNPACK;
-          const uint4* src = reinterpret_cast<const uint4*>(q0 + (size_t)n * D);
-#pragma unroll
-          for (int x = 0; x < UV; ++x) v[k][x] = n < np && x * 32 + lane < L / 8 ? __ldg(src + x * 32 + lane) : make_uint4(0, 0, 0, 0);
-          r[k] = n < np && lane < 8 ? __ldg(src + L / 8 + lane) : make_uint4(0, 0, 0, 0);
+          for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&a[e])));
         }
+        float top = fmaxf(__low2float(most), __high2float(most));
 #pragma unroll
-        for (int k = 0; k < AT_ONCE; ++k) {
-          const int n = (b + k) * 8 + warp - LA_UNPACK;
-          float top = 0.f;
-          auto look = [&](const uint4& u) {
-            const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        int ex = (int)(__float_as_uint(top) >> 23) - 127;
+        ex = top == 0.f || ex > 127 ? 10 : max(ex, -110);                           // (a value that is no number stays one)
+        const float mul = __uint_as_float((uint32_t)(10 - ex + 127) << 23);
+#pragma unroll 1
+        for (int c = 0; c <= NC; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(place(n, c));
+          const uint4 u = *at;
+          const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+          uint32_t o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) top = fmaxf(top, fmaxf(fabsf(bf_lo(a[e])), fabsf(bf_hi(a[e]))));
-          };
-#pragma unroll
-          for (int x = 0; x < UV; ++x) look(v[k][x]);
-          look(r[k]);
-          top = warp_max(top);
-          int ex = (int)(__float_as_uint(top) >> 23) - 127;
-          ex = top == 0.f || ex > 127 ? 10 : max(ex, -110);                         // (a value that is no number stays one)
-          const float mul = __uint_as_float((uint32_t)(10 - ex + 127) << 23);
-#pragma unroll
-          for (int x = 0; x < UV; ++x) {
-            const int at = x * 32 + lane;
-            const uint32_t a[4] = {v[k][x].x, v[k][x].y, v[k][x].z, v[k][x].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const __half2 h = __floats2half2_rn(bf_lo(a[e]) * mul, bf_hi(a[e]) * mul);
-              o[e] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            if (at < L / 8)
-              *reinterpret_cast<uint4*>(smem + (at / 8) * N * 128 + n * 128 + (((at & 7) ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          for (int e = 0; e < 4; ++e) {
+            const float lo = bf_lo(a[e]) * mul, hi = bf_hi(a[e]) * mul;
+            const __half2 h = __floats2half2_rn(lo, hi);
+            o[e] = c < NC ? *reinterpret_cast<const uint32_t*>(&h) : pack_bf2(lo, hi);
           }
-          if (lane < 8) {
-            const uint32_t a[4] = {r[k].x, r[k].y, r[k].z, r[k].w};
-            uint32_t o[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = pack_bf2(bf_lo(a[e]) * mul, bf_hi(a[e]) * mul);
-            *reinterpret_cast<uint4*>(smem + NC * N * 128 + n * 128 + ((lane ^ (n & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          }
-          if (lane == 0) {
-            ms.c[par][n] = scale_log2 * __uint_as_float((uint32_t)(ex - 10 + 127) << 23);
-            ms.nr[par][n] = 0.f;
-            ms.see[par][n] = n < np ? min(max(g.kvlen[w.row0 + (int)(((long)w.u * N + n) / g.nq)], 0), w.kv) : w.kv;
-          }
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if ((lane & 7) == 0) {
+          ms.c[par][n] = scale_log2 * __uint_as_float((uint32_t)(ex - 10 + 127) << 23);
+          ms.nr[par][n] = 0.f;
+          ms.see[par][n] = n < np ? min(max(g.kvlen[w.row0 + (int)((uint32_t)(w.u * N + n) / (uint32_t)g.nq)], 0), w.kv) : w.kv;
         }
       }
       fence_proxy_async();
@@ -473,7 +478,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       if (lane == 0) mbar_arrive(qfull);
     };
 
-    int i = 0, piece = 0, unit = ms.start[3], flat = f0;
+    int i = 0, piece = 0, flat = f0;
     bool broke = false;
     // once round per piece: its tiles, the next one's queries (no score needs this one's any more), its end
     for (int n = 0;; ++piece) {
@@ -518,8 +523,8 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
           unsigned char* prow = smem + C::P_AT + key * N * 2;
           const int pturn = N == 64 ? key & 7 : N == 32 ? key >> 1 & 3 : key >> 2 & 1;
           // Weights by the reference there is; a tile whose scores pass the limit (all 256 threads look) and a piece's first (load_q left zeros) get one anew
-          // and go round again.
-          bool anew = k == 0, done = false;
+          // and go round again, once: scores so large that their difference to it is still past the limit, for rounding, weigh the limit.
+          bool anew = k == 0, again = false, done = false;
 #pragma unroll 1
           while (!done) {
             float x[CW];
@@ -538,6 +543,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
               }
               softmax_sync();
               anew = false;
+              again = true;
               if (k > 0) {                                           // (the tile's scores are complete, so the products ahead of them are)
 #pragma unroll
                 for (int e = 0; e < CW; e += 2) {
@@ -557,6 +563,10 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
                 tmem_st_wait();
               }
               continue;
+            }
+            if (again) {
+#pragma unroll
+              for (int e = 0; e < CW; ++e) x[e] = x[e] > LA_LIMIT ? LA_LIMIT : x[e];
             }
             float top = x[0];
 #pragma unroll
@@ -612,7 +622,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         }
       }
       if (st == 0 && t0 == 0 && (by_unit || !whole))
-        join[by_unit ? unit : (int)blockIdx.x] = make_int4((int)base, whole ? 0 : np, rec, (flat + nt - 1) / share);
+        join[by_unit ? unit : (int)blockIdx.x] = make_int4((int)base, whole ? 0 : np, rec, (int)((uint32_t)(flat + nt - 1) / (uint32_t)share));
       if (t0 + n == nt) ++unit;
       flat += n;
       softmax_sync();
@@ -762,43 +772,49 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
 
 // Units that span CTAs. grid (entries, N), 128 threads: a CTA a pair, its records in the order of their keys.
 __global__ void __launch_bounds__(128) mla_attn_q_join_kernel(__nv_bfloat16* __restrict__ out, const float* o_part, const float* ml_part, const int4* join,
-                                                              int N, int L, const int* row_kvlen, int nq) {
-  extern __shared__ float wt[];                                      // [records]
-  __shared__ float red[32];
-  const int n = blockIdx.y, tid = threadIdx.x;
+                                                              int N, int L, const int* row_kvlen, long pairs, int nq, int ctas) {
+  const int n = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   pdl_launch_dependents();
   pdl_wait();
   o_part = after_wait(o_part); ml_part = after_wait(ml_part); row_kvlen = after_wait(row_kvlen);
   const int4 job = after_wait(join)[blockIdx.x];
-  if (n >= job.y) return;
+  // (where a wait ran out in the kernel ahead, jobs are whatever was there)
   const int c0 = job.z >> 1, count = job.w - c0 + 1;
+  if (n >= job.y || job.x < 0 || (long)job.x + n >= pairs || job.z < 0 || job.w >= ctas || count < 1 || count > ctas) return;
   auto record = [&](int i) { return (size_t)(i == 0 ? job.z : 2 * (c0 + i)) * N + n; };
-  float m = -INFINITY;
-  for (int i = tid; i < count; i += 128) {
-    wt[i] = ml_part[record(i) * 2];
-    m = fmaxf(m, wt[i]);
+  // The sums of eight records are on their way while the weights are worked out, by every warp for itself, 32 records at a time.
+  constexpr int AT_ONCE = 8;
+  const int e = tid * 4;
+  float4 v[AT_ONCE], a = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (i0 + k < count && e < L) v[k] = *reinterpret_cast<const float4*>(o_part + record(i0 + k) * L + e);
+  };
+  load(0);
+  float m = -INFINITY, l = 0.f, x = 0.f;
+#pragma unroll 1
+  for (int i = lane; i < count; i += 32) m = fmaxf(m, ml_part[record(i) * 2]);
+  m = warp_max(m);
+#pragma unroll 1
+  for (int i0 = 0; i0 < count; i0 += AT_ONCE) {
+    if (i0 % 32 == 0) {
+      // a record without weight has -inf there; a reference of +inf comes with sums that are no numbers
+      const float2 ml = i0 + lane < count ? *reinterpret_cast<const float2*>(ml_part + record(i0 + lane) * 2) : make_float2(-INFINITY, 0.f);
+      x = ml.x == -INFINITY ? 0.f : ml.x == m ? 1.f : exp2f(ml.x - m);
+      l += x == 0.f ? 0.f : x * ml.y;
+    }
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const float y = __shfl_sync(0xffffffffu, x, (i0 + k) % 32);    // (zero where there is no record)
+      if (y != 0.f) { a.x = fmaf(y, v[k].x, a.x); a.y = fmaf(y, v[k].y, a.y); a.z = fmaf(y, v[k].z, a.z); a.w = fmaf(y, v[k].w, a.w); }
+    }
+    load(i0 + AT_ONCE);
   }
-  m = block_max(m, red);
-  float l = 0.f;
-  for (int i = tid; i < count; i += 128) {
-    // a record without weight has -inf there; a reference of +inf comes with sums that are no numbers
-    const float x = wt[i] == -INFINITY ? 0.f : wt[i] == m ? 1.f : exp2f(wt[i] - m);
-    wt[i] = x;
-    l += x == 0.f ? 0.f : x * ml_part[record(i) * 2 + 1];
-  }
-  l = block_sum(l, red);                                             // (its barriers publish wt)
+  l = warp_sum(l);
   const size_t pair = (size_t)job.x + n;
   const float inv = row_kvlen[pair / nq] > 0 ? 1.f / l * (l == 0.f ? 0.f : 1.f) : 0.f;
-  for (int e = tid * 4; e < L; e += 512) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int i = 0; i < count; ++i) {
-      const float x = wt[i];
-      const float4 v = *reinterpret_cast<const float4*>(o_part + record(i) * L + e);
-      if (x != 0.f) { a.x = fmaf(x, v.x, a.x); a.y = fmaf(x, v.y, a.y); a.z = fmaf(x, v.z, a.z); a.w = fmaf(x, v.w, a.w); }
-    }
-    *reinterpret_cast<uint2*>(out + pair * L + e) = make_uint2(pack_bf2(a.x * inv, a.y * inv), pack_bf2(a.z * inv, a.w * inv));
-  }
+  if (e < L) *reinterpret_cast<uint2*>(out + pair * L + e) = make_uint2(pack_bf2(a.x * inv, a.y * inv), pack_bf2(a.z * inv, a.w * inv));
 }
 
 }  // namespace fb
@@ -819,7 +835,7 @@ extern "C" int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* q
                              int max_blocks, int kv_block, int rows, int nq, int L, int R, float scale, int ctas, int* status, cudaStream_t s) {
   if (R != LC_R || (bits != 4 && bits != 8) || nq < 1 || kv_block < 1 || ctas < 1 || max_rows < 0) return -1;
   if (((uintptr_t)qabs | (uintptr_t)cache | (uintptr_t)ws) % 16 || (uintptr_t)out % 8) return -2;
-  if (pages < 1 || pages * kv_block > 0x7fffffffl) return -2;
+  if (pages < 1 || pages * kv_block > 0x7fffffffl || (long)rows * nq > 0x3fffffffl) return -2;
   if (rows <= 0 || nseg <= 0 || max_rows == 0) return 0;
   if (ws_floats < fb_mla_attn_q_floats(max_rows, nq, L, ctas)) return -3;
   const int N = latent_pairs((long)max_rows * nq);
@@ -845,6 +861,6 @@ extern "C" int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* q
 #undef FB_LA
   if (!known) return -2;
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(mla_attn_q_join_kernel, dim3(entries, N), dim3(128), (size_t)ctas * 4, s, (__nv_bfloat16*)out, (const float*)op,
-                         (const float*)ml, (const int4*)join, N, L, row_kvlen, nq);
+  return (int)launch_pdl(mla_attn_q_join_kernel, dim3(entries, N), dim3(128), 0, s, (__nv_bfloat16*)out, (const float*)op,
+                         (const float*)ml, (const int4*)join, N, L, row_kvlen, (long)rows * nq, nq, ctas);
 }
