@@ -24,6 +24,8 @@
 //
 // A key of which a group is no number gets the score NaN and a finite place in the tile, so that rows ahead of it, whose weight for it is zero, stay clean.
 // Every wait is bounded: one that runs out sets the status word and an abort flag, all roles leave and the CTA frees its TMEM.
+#include <algorithm>
+
 #include "api_ext.h"
 #include "mla_cache.cuh"
 
@@ -227,7 +229,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   if (tid == 0) {
     ms.abort = 0; ms.fail = 0;
     for (int i = 0; i < NB; ++i) { mbar_init(&kfull[i], LA_UNPACK); mbar_init(&kempty[i], 1); }
-    mbar_init(rfull, 2); mbar_init(rempty, 1); mbar_init(sfull, 1); mbar_init(pfull, 8); mbar_init(qfull, 8); mbar_init(ofull, 1); mbar_init(oempty, 8);
+    mbar_init(rfull, 2); mbar_init(rempty, 1); mbar_init(sfull, 1); mbar_init(pfull, 8); mbar_init(qfull, LA_UNPACK); mbar_init(ofull, 1); mbar_init(oempty, 8);
     for (int i = 0; i < LA_AHEAD; ++i) { mbar_init(&xfull[i], 1); mbar_init(&xempty[i], LA_UNPACK + 2); }
     fence_mbar_init();
   }
@@ -306,6 +308,64 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     }
   }
 
+  // Queries of the walk's unit -> shared memory, and what belongs to each pair. Eight lanes have a pair; a thread turns the 16-byte pieces that it copied
+  // itself, in their places. The first piece's are brought by the unpacking warps, while their first codes are on their way (before: copies, after: the
+  // rest), the others' by the softmax. (Loops, not unrolled ones: a CTA comes by once or twice, and code that is new to the SM costs more than its instructions.)
+  auto pairs_of = [&](const LatentWalk& x) { return min(N, x.nrows * g.nq - x.u * N); };
+  auto place = [&](int n, int c) { return smem + (c * N + n) * 128 + (((lane & 7) ^ (n & 7)) << 4); };
+  auto copy_q = [&](int n0, int step) {
+    const int np = pairs_of(w);
+    const __nv_bfloat16* q0 = qabs + ((size_t)w.row0 * g.nq + (size_t)w.u * N) * D + (lane & 7) * 8;
+#pragma unroll 1
+    for (int n = n0; n < N; n += step)
+#pragma unroll 3
+      for (int c = 0; c <= NC; ++c)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                     ::"r"(smem_u32(place(n, c))), "l"(q0 + (size_t)(n < np ? n : 0) * D + c * 64), "r"(n < np ? 16 : 0) : "memory");
+  };
+  auto turn_q = [&](int n0, int step, int par) {
+    const int np = pairs_of(w);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 1
+    for (int n = n0; n < N; n += step) {
+      __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+#pragma unroll 3
+      for (int c = 0; c <= NC; ++c) {
+        const uint4 u = *reinterpret_cast<const uint4*>(place(n, c));
+        const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&a[e])));
+      }
+      float top = fmaxf(__low2float(most), __high2float(most));
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      int ex = (int)(__float_as_uint(top) >> 23) - 127;
+      ex = top == 0.f || ex > 127 ? 10 : max(ex, -110);                           // (a value that is no number stays one)
+      const float mul = __uint_as_float((uint32_t)(10 - ex + 127) << 23);
+#pragma unroll 3
+      for (int c = 0; c <= NC; ++c) {
+        uint4* at = reinterpret_cast<uint4*>(place(n, c));
+        const uint4 u = *at;
+        const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float lo = bf_lo(a[e]) * mul, hi = bf_hi(a[e]) * mul;
+          const __half2 h = __floats2half2_rn(lo, hi);
+          o[e] = c < NC ? *reinterpret_cast<const uint32_t*>(&h) : pack_bf2(lo, hi);
+        }
+        *at = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      if ((lane & 7) == 0) {
+        ms.c[par][n] = scale_log2 * __uint_as_float((uint32_t)(ex - 10 + 127) << 23);
+        ms.nr[par][n] = 0.f;
+        ms.see[par][n] = n < np ? min(max(g.kvlen[w.row0 + (int)((uint32_t)(w.u * N + n) / (uint32_t)g.nq)], 0), w.kv) : w.kv;
+      }
+    }
+    fence_proxy_async();
+    __syncwarp();
+  };
+
   // launched with 72 registers for 896 threads (64512); sixteen warps of 56, eight of 112 and four of 56 are as many
   if (warp < LA_UNPACK) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -377,11 +437,14 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       if (lane == 0) mbar_arrive(&xempty[i % LA_AHEAD]);
       return ok ? row : -1;
     };
+    if (warp * 4 < N) copy_q(warp * 4 + (lane >> 3), N);
     int row0 = look(0), row1 = -1;
     uint32_t sraw[SRW];
 #pragma unroll
     for (int j = 0; j < C::PD; ++j) fetch(raw[j], row0, j);
     scales(sraw, row0);
+    if (warp * 4 < N) turn_q(warp * 4 + (lane >> 3), N, 1);
+    if (lane == 0) mbar_arrive(qfull);
     int buf = 0;
     uint32_t kph = 1;                                                // (a fresh barrier passes a wait for parity 1)
     for (int i = 0; i < tiles; ++i) {
@@ -422,72 +485,16 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, ts = tmem + lanes + NP * N + hc * CW, to = tmem + lanes + hc * CW;
     auto fmx = [](float a, float b) { return fmaxf(a, b); };
     auto fad = [](float a, float b) { return a + b; };
-    auto pairs_of = [&](const LatentWalk& x) { return min(N, x.nrows * g.nq - x.u * N); };
-
-    // queries of the walk's unit -> shared memory, and what belongs to each pair. Eight lanes have a pair; a thread turns the 16-byte pieces that it copied
-    // itself, in their places. (Loops, not unrolled ones: a CTA comes by once or twice, and code that is new to the SM costs more than its instructions.)
-    auto load_q = [&](int par) {
-      const int np = pairs_of(w), n0 = (warp - LA_UNPACK) * 4 + (lane >> 3);
-      const __nv_bfloat16* q0 = qabs + ((size_t)w.row0 * g.nq + (size_t)w.u * N) * D + (lane & 7) * 8;
-      auto place = [&](int n, int c) { return smem + (c * N + n) * 128 + (((lane & 7) ^ (n & 7)) << 4); };
-#pragma unroll 1
-      for (int n = n0; n < N; n += 32)
-#pragma unroll 3
-        for (int c = 0; c <= NC; ++c)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
-                       ::"r"(smem_u32(place(n, c))), "l"(q0 + (size_t)(n < np ? n : 0) * D + c * 64), "r"(n < np ? 16 : 0) : "memory");
-      asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 1
-      for (int n = n0; n < N; n += 32) {
-        __nv_bfloat162 most = __float2bfloat162_rn(0.f);
-#pragma unroll 3
-        for (int c = 0; c <= NC; ++c) {
-          const uint4 u = *reinterpret_cast<const uint4*>(place(n, c));
-          const uint32_t a[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&a[e])));
-        }
-        float top = fmaxf(__low2float(most), __high2float(most));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        int ex = (int)(__float_as_uint(top) >> 23) - 127;
-        ex = top == 0.f || ex > 127 ? 10 : max(ex, -110);                           // (a value that is no number stays one)
-        const float mul = __uint_as_float((uint32_t)(10 - ex + 127) << 23);
-#pragma unroll 1
-        for (int c = 0; c <= NC; ++c) {
-          uint4* at = reinterpret_cast<uint4*>(place(n, c));
-          const uint4 u = *at;
-          const uint32_t a[4] = {u.x, u.y, u.z, u.w};
-          uint32_t o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lo = bf_lo(a[e]) * mul, hi = bf_hi(a[e]) * mul;
-            const __half2 h = __floats2half2_rn(lo, hi);
-            o[e] = c < NC ? *reinterpret_cast<const uint32_t*>(&h) : pack_bf2(lo, hi);
-          }
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
-        }
-        if ((lane & 7) == 0) {
-          ms.c[par][n] = scale_log2 * __uint_as_float((uint32_t)(ex - 10 + 127) << 23);
-          ms.nr[par][n] = 0.f;
-          ms.see[par][n] = n < np ? min(max(g.kvlen[w.row0 + (int)((uint32_t)(w.u * N + n) / (uint32_t)g.nq)], 0), w.kv) : w.kv;
-        }
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(qfull);
-    };
-
-    int i = 0, piece = 0, flat = f0;
+    int i = 0, flat = f0;
     bool broke = false;
+    la_wait(qfull, 0, abort_flag);                                   // what came with the first piece's queries (if they don't come, no score does either)
     // once round per piece: its tiles, the next one's queries (no score needs this one's any more), its end
-    for (int n = 0;; ++piece) {
-      const int par = piece & 1, t0 = w.t, nt = w.nt, np = pairs_of(w);
+    for (int piece = 1;; ++piece) {
+      const int par = piece & 1, t0 = w.t, nt = w.nt, np = pairs_of(w), n = min(nt - t0, tiles - i);
       const size_t base = (size_t)w.row0 * g.nq + (size_t)w.u * N;
       uint64_t sum[CW / 2];
-      if (piece > 0) {
-        n = min(nt - t0, tiles - i);
-        softmax_sync();                                              // what load_q wrote beside the queries
+      {
+        softmax_sync();                                              // what came with later pieces' queries, from these warps
         const int least = ms.see[par][0];                            // rows of a segment see no fewer keys than those ahead of them
 #pragma unroll
         for (int e = 0; e < CW / 2; ++e) sum[e] = f2_pack(0.f, 0.f);
@@ -602,8 +609,11 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         if (lane < CW) ms.mx[quad][hc * CW + lane] = l;
         if (t0 + n == nt) w.next_unit<N>(g);
       }
-      if (i < tiles) load_q(piece + 1 & 1);
-      if (piece == 0) continue;
+      if (i < tiles) {
+        copy_q((warp - LA_UNPACK) * 4 + (lane >> 3), 32);
+        turn_q((warp - LA_UNPACK) * 4 + (lane >> 3), 32, piece + 1 & 1);
+        if (lane < 2) mbar_arrive(qfull);
+      }
       // ---- the piece's end
       const bool whole = t0 == 0 && n == nt;
       bool ok = la_wait(ofull, piece - 1 & 1, abort_flag);
@@ -821,11 +831,17 @@ __global__ void __launch_bounds__(128) mla_attn_q_join_kernel(__nv_bfloat16* __r
 
 using namespace fb;
 
-// Pairs of a unit: the fewest of 16, 32 and 64 that hold a segment's; more are several units (an unpacked tile serves as many as it can).
-static int latent_pairs(long pairs) { return pairs <= 16 ? 16 : pairs <= 32 ? 32 : 64; }
+// Pairs of a unit: the fewest of 16, 32 and 64 that hold a segment's; more are several units (an unpacked tile serves as many as it can). Fewer where even
+// then every tile that the table has room for finds a CTA of its own: its products, its softmax and the sums that it leaves are shorter, and nobody
+// waits for the unpacking that is done again.
+static int latent_pairs(long pairs, long tiles, int ctas) {
+  int N = 16;
+  while (N < 64 && N < pairs && (pairs + N - 1) / N * tiles > ctas) N *= 2;
+  return N;
+}
 
 extern "C" long fb_mla_attn_q_floats(int max_rows, int nq, int L, int ctas) {
-  const long N = latent_pairs((long)max_rows * nq);
+  const long N = latent_pairs((long)max_rows * nq, 1l << 31, ctas);       // (the most that they can be)
   return 4l * ctas + 2l * ctas * N * (L + 2);
 }
 
@@ -838,7 +854,7 @@ extern "C" int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* q
   if (pages < 1 || pages * kv_block > 0x7fffffffl || (long)rows * nq > 0x3fffffffl) return -2;
   if (rows <= 0 || nseg <= 0 || max_rows == 0) return 0;
   if (ws_floats < fb_mla_attn_q_floats(max_rows, nq, L, ctas)) return -3;
-  const int N = latent_pairs((long)max_rows * nq);
+  const int N = latent_pairs((long)max_rows * nq, nseg * std::max(1l, ((long)max_blocks * kv_block + LA_KT - 1) / LA_KT), ctas);
   const long units = (long)nseg * (((long)max_rows * nq + N - 1) / N);
   const int by_unit = units <= ctas, entries = by_unit ? (int)units : ctas;
   int4* join = reinterpret_cast<int4*>(ws);
