@@ -25,43 +25,45 @@ __device__ __forceinline__ void four_digits(double x, int& q, int& e) {
   if (q == 16) { q = 8; ++e; }
 }
 
-__device__ __forceinline__ double block_sum_f64(double v, double* red) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double r = 0.0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r += red[i];
-  return r;
-}
+constexpr int LP_ROWS = 8;             // cache rows of a CTA
 
-// grid (rows, 1 + groups of `per` heads), 256 threads. y = 0: the cache row, two values a thread; else the heads' query parts, four rotated pairs a thread
-// (8-byte accesses), whose angles serve all of its heads.
+// grid ceil(rows / LP_ROWS) + rows * kinds, kinds: groups of `per` heads (32 or 128), 256 threads. The first CTAs write cache rows, a warp each: 16 values a
+// lane (the 64-bit square root and quotients of a row are then worked out once, not by eight warps). The others turn the heads' query parts of a row,
+// four pairs a thread (8-byte accesses), whose angles serve all of its heads; queries are on their way before the position is known.
 template <int BITS>
-__global__ void __launch_bounds__(256) mla_prep_q_kernel(uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ qabs, const __nv_bfloat16* kva,
+__global__ void __launch_bounds__(256, 4) mla_prep_q_kernel(uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ qabs, const __nv_bfloat16* kva,
                                                          long kva_stride, const __nv_bfloat16* q, long q_stride,
                                                          const __nv_bfloat16* __restrict__ norm_w, const float* __restrict__ inv_freq,
                                                          const int* row_slot, const int* row_pos, const int* block_table, int max_blocks, long pages,
-                                                         int kv_block, int nq, int dn, int L, float eps, int* status, int per) {
+                                                         int kv_block, int nq, int dn, int L, float eps, int* status, int rows, int per, int kinds) {
   using Row = LatentRow<BITS>;
   constexpr int R = LC_R, half = R / 2;
-  __shared__ double red[8];
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, writers = (rows + LP_ROWS - 1) / LP_ROWS, turner = (int)blockIdx.x - writers;
   pdl_launch_dependents();
   pdl_wait();
   kva = after_wait(kva); q = after_wait(q);
-  const int pos = after_wait(row_pos)[row];
-  if (blockIdx.y > 0) {
-    const int h_end = min((int)blockIdx.y * per, nq), i = tid % 8 * 4;
-    float s[4], c[4];
+  if (turner >= 0) {
+    const int row = turner / kinds, kind = turner % kinds, h0 = kind * per + tid / 8, h_end = min((kind + 1) * per, nq), i = tid % 8 * 4;
+    const int pos = after_wait(row_pos)[row];
+    const __nv_bfloat16* from = q + (size_t)row * q_stride + dn + i;
+    uint2 u[4], v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) turn(pos, inv_freq[i + j], s[j], c[j]);
-    for (int h = (blockIdx.y - 1) * per + tid / 8; h < h_end; h += 32) {
-      const __nv_bfloat16* from = q + (size_t)row * q_stride + (size_t)h * (dn + R) + dn + i;
+    for (int k = 0; k < 4; ++k)
+      if (h0 + 32 * k < h_end) {
+        u[k] = *reinterpret_cast<const uint2*>(from + (size_t)(h0 + 32 * k) * (dn + R));
+        v[k] = *reinterpret_cast<const uint2*>(from + (size_t)(h0 + 32 * k) * (dn + R) + half);
+      }
+    __shared__ __align__(16) float sn[half], cs[half];
+    if (tid < half) turn(pos, inv_freq[tid], sn[tid], cs[tid]);
+    __syncthreads();
+    const float4 s4 = *reinterpret_cast<const float4*>(sn + i), c4 = *reinterpret_cast<const float4*>(cs + i);
+    const float s[4] = {s4.x, s4.y, s4.z, s4.w}, c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int h = h0 + 32 * k;
+      if (h >= h_end) break;
       __nv_bfloat16* to = qabs + ((size_t)row * nq + h) * (L + R) + L + i;
-      const uint2 u = *reinterpret_cast<const uint2*>(from), v = *reinterpret_cast<const uint2*>(from + half);
-      const float a[4] = {bf_lo(u.x), bf_hi(u.x), bf_lo(u.y), bf_hi(u.y)}, b[4] = {bf_lo(v.x), bf_hi(v.x), bf_lo(v.y), bf_hi(v.y)};
+      const float a[4] = {bf_lo(u[k].x), bf_hi(u[k].x), bf_lo(u[k].y), bf_hi(u[k].y)}, b[4] = {bf_lo(v[k].x), bf_hi(v[k].x), bf_lo(v[k].y), bf_hi(v[k].y)};
       float x[4], y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -73,125 +75,167 @@ __global__ void __launch_bounds__(256) mla_prep_q_kernel(uint8_t* __restrict__ c
     }
     return;
   }
-  const int slot = after_wait(row_slot)[row], page = pos / kv_block;
+  const int row = blockIdx.x * LP_ROWS + (tid >> 5);
+  if (row >= rows) return;
+  const int pos = after_wait(row_pos)[row], slot = after_wait(row_slot)[row], page = pos / kv_block;
+  const __nv_bfloat16* kr = kva + (size_t)row * kva_stride;
+  const int e0 = lane * 16;
+  const bool in = e0 < L;
+  uint4 xu[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}, wu[2] = {xu[0], xu[0]};
+  if (in) {
+    auto take = [&](uint4 (&u)[2], const __nv_bfloat16* p) {             // 16 values, by 16 bytes where they lie so
+      if ((uintptr_t)p % 16 == 0) {
+        u[0] = reinterpret_cast<const uint4*>(p)[0];
+        u[1] = reinterpret_cast<const uint4*>(p)[1];
+      } else {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+        uint32_t* o = reinterpret_cast<uint32_t*>(u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = h[2 * j] | (uint32_t)h[2 * j + 1] << 16;
+      }
+    };
+    take(xu, kr + e0);
+    take(wu, norm_w + e0);
+  }
+  const float ka = bf2f(kr[L + lane]), kb = bf2f(kr[L + half + lane]);
   const int blk = pos < 0 || page >= max_blocks ? -1 : after_wait(block_table)[(size_t)slot * max_blocks + page];
-  if (blk < 0 || blk >= pages) {                                         // (the same for all threads)
-    if (tid == 0) set_status(status, ST_BOUNDS);
+  if (blk < 0 || blk >= pages) {                                         // (the same for the whole warp)
+    if (lane == 0) set_status(status, ST_BOUNDS);
     return;
   }
   uint8_t* crow = cache + ((size_t)blk * kv_block + pos % kv_block) * Row::bytes(L);
-  const __nv_bfloat16* kr = kva + (size_t)row * kva_stride;
-  const int e0 = tid * 2;
-  const bool in = e0 < L;
-  double x[2] = {0.0, 0.0};
-  if (in) { x[0] = bf2f(kr[e0]); x[1] = bf2f(kr[e0 + 1]); }
-  const double ss = block_sum_f64(x[0] * x[0] + x[1] * x[1], red);
+  const uint32_t* xw = reinterpret_cast<const uint32_t*>(xu);
+  const uint32_t* ww = reinterpret_cast<const uint32_t*>(wu);
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ss += (double)bf_lo(xw[j]) * bf_lo(xw[j]) + (double)bf_hi(xw[j]) * bf_hi(xw[j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const double r = 1.0 / sqrt(ss / L + (double)eps);
-  if (in) {
-    double y[2], top = 0.0;
-    bool bad = false;
+  double y[16], top = 0.0;
+  bool bad = false;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      y[j] = x[j] * r * (1.0 + (double)bf2f(norm_w[e0 + j]));
-      bad |= !isfinite(y[j]);
-      top = fmax(top, fabs(y[j]));                                       // (fmax drops a NaN; `bad` has it)
-    }
-    const unsigned here = __activemask();                                // whole warps: L is a multiple of 64
-#pragma unroll
-    for (int o = Row::group / 4; o > 0; o >>= 1) {
-      top = fmax(top, __shfl_xor_sync(here, top, o));
-      bad |= __shfl_xor_sync(here, (int)bad, o) != 0;
-    }
-    int byte;
-    if constexpr (BITS == 4) {
-      int f = 8, e = -20;
-      const double want = top / 7.0;
-      if (want > 0x1p-20 && !bad) {
-        four_digits(want, f, e);
-        if (e > 10) { f = 15; e = 10; }
-      }
-      byte = (e + 20) << 3 | (f - 8);
-      const double scale = ldexp((double)f, e - 3);
-      uint32_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int code = bad ? 0 : (int)fmin(fmax(rint(y[j] / scale), -7.0), 7.0);
-        w |= (uint32_t)(code + 8) << (16 * j + 4 * (tid % 4));           // value 2 (tid % 4) + j of the word
-      }
-      w |= __shfl_xor_sync(here, w, 1);
-      w |= __shfl_xor_sync(here, w, 2);
-      if (tid % 4 == 0) *reinterpret_cast<uint32_t*>(crow + e0 / 2) = w;
-    } else {
-      int k = -15;
-      const double want = top / 448.0;
-      if (want > 0x1p-15 && !bad) {
-        const long long b = __double_as_longlong(want);
-        k = min((int)(b >> 52) - 1023 + ((b & 0xfffffffffffffll) ? 1 : 0), 7);
-      }
-      byte = k + 127;
-      const double inv = ldexp(1.0, -k);
-      uint32_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // rounded to odd on the way to 32 bits, so that the rounding to e4m3 is the only one
-        const double v = bad ? 0.0 : y[j] * inv;
-        float f = __double2float_rz(v);
-        if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
-        w |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3) << (8 * j);
-      }
-      *reinterpret_cast<uint16_t*>(crow + e0) = (uint16_t)w;
-    }
-    if (e0 % Row::group == 0) crow[Row::scale_of(L, e0)] = (uint8_t)(bad ? LC_NAN : byte);
+  for (int j = 0; j < 16; ++j) {
+    y[j] = (double)(j % 2 ? bf_hi(xw[j / 2]) : bf_lo(xw[j / 2])) * r * (1.0 + (double)(j % 2 ? bf_hi(ww[j / 2]) : bf_lo(ww[j / 2])));
+    bad |= !isfinite(y[j]);
+    top = fmax(top, fabs(y[j]));                                         // (fmax drops a NaN; `bad` has it)
   }
-  if (tid < half) {
-    float s, c;
-    turn(pos, inv_freq[tid], s, c);
-    const float a = bf2f(kr[L + tid]), b = bf2f(kr[L + half + tid]);
-    __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(crow + Row::rope_at(L)) + tid;
-    to[0] = f2bf(fmaf(a, c, -__fmul_rn(b, s)));
-    to[half] = f2bf(fmaf(b, c, __fmul_rn(a, s)));
+  if constexpr (BITS == 8) {                                             // a group is two lanes'
+    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    bad |= __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;
   }
+  int byte;
+  if constexpr (BITS == 4) {
+    int f = 8, e = -20;
+    const double want = top / 7.0;
+    if (want > 0x1p-20 && !bad) {
+      four_digits(want, f, e);
+      if (e > 10) { f = 15; e = 10; }
+    }
+    byte = (e + 20) << 3 | (f - 8);
+    const double scale = ldexp((double)f, e - 3), inv = 1.0 / scale;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      // the product is off by 2^-51 of itself: only next to a half does it take the quotient
+      const double t = y[j] * inv;
+      double c = rint(t);
+      if (fabs(fabs(t - c) - 0.5) < 1e-9) c = rint(y[j] / scale);
+      const int code = bad ? 0 : (int)fmin(fmax(c, -7.0), 7.0);
+      w[j / 8] |= (uint32_t)(code + 8) << (16 * (j % 2) + 4 * (j % 8 / 2));
+    }
+    if (in) *reinterpret_cast<uint2*>(crow + lane * 8) = make_uint2(w[0], w[1]);
+  } else {
+    int k = -15;
+    const double want = top / 448.0;
+    if (want > 0x1p-15 && !bad) {
+      const long long b = __double_as_longlong(want);
+      k = min((int)(b >> 52) - 1023 + ((b & 0xfffffffffffffll) ? 1 : 0), 7);
+    }
+    byte = k + 127;
+    const double inv = ldexp(1.0, -k);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      // rounded to odd on the way to 32 bits, so that the rounding to e4m3 is the only one
+      const double v = bad ? 0.0 : y[j] * inv;
+      float f = __double2float_rz(v);
+      if ((double)f != v) f = __uint_as_float(__float_as_uint(f) | 1u);
+      w[j / 4] |= (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3) << (8 * (j % 4));
+    }
+    if (in) *reinterpret_cast<uint4*>(crow + e0) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (in && e0 % Row::group == 0) crow[Row::scale_of(L, e0)] = (uint8_t)(bad ? LC_NAN : byte);
+  float s, c;
+  turn(pos, inv_freq[lane], s, c);
+  __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(crow + Row::rope_at(L)) + lane;
+  to[0] = f2bf(fmaf(ka, c, -__fmul_rn(kb, s)));
+  to[half] = f2bf(fmaf(kb, c, __fmul_rn(ka, s)));
   const int end = Row::scale_at(L) + L / Row::group;
-  if (tid < Row::bytes(L) - end) crow[end + tid] = 0;
+  if (lane < Row::bytes(L) - end) crow[end + lane] = 0;
 }
 
-constexpr int LR_ROWS = 16;            // output rows of a CTA
+constexpr int LR_ROWS = 16, LR_THREADS = 288;                            // output rows of a CTA at most
 
-// grid ceil(rows / LR_ROWS), 288 threads: eight values of a row a thread. Output rows: segment after segment, each from a multiple of `align` on; `whole`:
+// grid ceil(rows / per), 288 threads: eight values of a row a thread. Output rows: segment after segment, each from a multiple of `align` on; `whole`:
 // positions 0 .. pos0 + nrows of a segment, else its own rows pos0 .. pos0 + nrows. Rows between them are zeros.
 template <int BITS>
-__global__ void __launch_bounds__(288) mla_rows_kernel(__nv_bfloat16* __restrict__ out, long rows, const uint8_t* cache, const int* seg_slot,
-                                                       const int* seg_pos0, const int* seg_nrows, int nseg, const int* block_table, int max_blocks,
-                                                       long pages, int kv_block, int L, int whole, int align, int* status) {
+__global__ void __launch_bounds__(LR_THREADS) mla_rows_kernel(__nv_bfloat16* __restrict__ out, long rows, const uint8_t* cache, const int* seg_slot,
+                                                              const int* seg_pos0, const int* seg_nrows, int nseg, const int* block_table,
+                                                              int max_blocks, long pages, int kv_block, int L, int whole, int align, int* status,
+                                                              int per) {
   using Row = LatentRow<BITS>;
   __shared__ const uint8_t* from[LR_ROWS];
   const int tid = threadIdx.x;
-  const long r0 = (long)blockIdx.x * LR_ROWS;
+  const long r0 = (long)blockIdx.x * per;
   pdl_launch_dependents();
   pdl_wait();
   cache = after_wait(cache); seg_slot = after_wait(seg_slot); seg_pos0 = after_wait(seg_pos0); seg_nrows = after_wait(seg_nrows);
   block_table = after_wait(block_table);
-  if (tid < LR_ROWS) {
-    long at = r0 + tid;
+  if (tid < 32) {
+    // a lane a segment, 32 at a time: where each ends; then a lane a row looks its own up
+    const bool mine = tid < per;
+    const long at = r0 + tid;
+    long base = 0;
+    bool found = false;
     const uint8_t* p = nullptr;
-    for (int s = 0; s < nseg; ++s) {
-      const int pos0 = seg_pos0[s], n = seg_nrows[s], count = max(whole ? pos0 + n : n, 0);
-      const long room = ((long)count + align - 1) / align * align;
-      if (at >= room) { at -= room; continue; }
-      if (at < count) {
-        const long pos = whole ? at : pos0 + at, page = pos / kv_block;
-        const int blk = pos < 0 || page >= max_blocks ? -1 : block_table[(size_t)seg_slot[s] * max_blocks + page];
-        if (blk < 0 || blk >= pages) set_status(status, ST_BOUNDS);
-        else p = cache + ((size_t)blk * kv_block + pos % kv_block) * Row::bytes(L);
+    for (int s0 = 0; s0 < nseg; s0 += 32) {
+      const bool there = s0 + tid < nseg;
+      const int pos0 = there ? seg_pos0[s0 + tid] : 0, n = there ? seg_nrows[s0 + tid] : 0, slot = there ? seg_slot[s0 + tid] : 0;
+      const int count = max(whole && there ? pos0 + n : n, 0);
+      long end = align == 1 ? count : (long)((uint32_t)(count + align - 1) / (uint32_t)align) * align;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long v = __shfl_up_sync(0xffffffffu, end, o);
+        if (tid >= o) end += v;
       }
-      break;
+      end += base;
+      int k = 0;                                                         // the first segment that ends behind the row, if it is one of these
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        if (__shfl_sync(0xffffffffu, end, k + o - 1) <= at) k += o;
+      const long stop = __shfl_sync(0xffffffffu, end, k), room_before = __shfl_up_sync(0xffffffffu, end, 1);
+      const long start = __shfl_sync(0xffffffffu, tid == 0 ? base : room_before, k);
+      const int c = __shfl_sync(0xffffffffu, count, k), q0 = __shfl_sync(0xffffffffu, pos0, k), sl = __shfl_sync(0xffffffffu, slot, k);
+      if (mine && !found && at < stop) {
+        found = true;
+        if (at - start < c) {
+          const int pos = (int)(at - start) + (whole ? 0 : q0), page = pos < 0 ? -1 : (int)((uint32_t)pos / (uint32_t)kv_block);
+          const int blk = page < 0 || page >= max_blocks ? -1 : block_table[(size_t)sl * max_blocks + page];
+          if (blk < 0 || blk >= pages) set_status(status, ST_BOUNDS);
+          else p = cache + ((size_t)blk * kv_block + (pos - page * kv_block)) * Row::bytes(L);
+        }
+      }
+      base = __shfl_sync(0xffffffffu, end, 31);
+      if (base > r0 + per - 1) break;
     }
-    from[tid] = p;
+    if (mine) from[tid] = p;
   }
   __syncthreads();
-  const int units = (L + LC_R) / 8;
-  for (int i = tid; i < LR_ROWS * units; i += blockDim.x) {
-    const int r = i / units, u = i % units;
+  const int units = (L + LC_R) / 8, step = LR_THREADS / units, u = tid % units;
+  if (tid >= step * units) return;
+#pragma unroll 4
+  for (int r = tid / units; r < per; r += step) {
     if (r0 + r >= rows) break;
     const uint8_t* p = from[r];
     uint4 v = make_uint4(0, 0, 0, 0);
@@ -236,11 +280,12 @@ extern "C" int fb_mla_prep_q(void* cache, long pages, int bits, void* qabs, cons
   if (dn % 4 || q_stride % 4 || ((uintptr_t)q | (uintptr_t)qabs) % 8 || (uintptr_t)cache % 16) return -2;
   if (rows <= 0) return 0;
   // heads a CTA: 32 (one pass of the threads) as long as the SMs hold all CTAs at once, else all heads of a row, whose angles are then taken once
-  const int per = (long)rows * (1 + (nq + 31) / 32) <= 8 * 148 ? 32 : 128;
+  const int per = (long)rows * ((nq + 31) / 32) <= 8 * 148 ? 32 : 128, kinds = (nq + per - 1) / per;
+  if ((long)rows * (kinds + 1) > 0x7fffffffl) return -2;
   auto kern = bits == 4 ? mla_prep_q_kernel<4> : mla_prep_q_kernel<8>;
-  return (int)launch_pdl(kern, dim3(rows, 1 + (nq + per - 1) / per), dim3(256), (size_t)0, s, (uint8_t*)cache, (__nv_bfloat16*)qabs,
+  return (int)launch_pdl(kern, dim3((rows + LP_ROWS - 1) / LP_ROWS + rows * kinds), dim3(256), (size_t)0, s, (uint8_t*)cache, (__nv_bfloat16*)qabs,
                          (const __nv_bfloat16*)kva, kva_stride, (const __nv_bfloat16*)q, q_stride, (const __nv_bfloat16*)norm_w, inv_freq, row_slot,
-                         row_pos, block_table, max_blocks, pages, kv_block, nq, dn, L, eps, status, per);
+                         row_pos, block_table, max_blocks, pages, kv_block, nq, dn, L, eps, status, rows, per, kinds);
 }
 
 extern "C" int fb_mla_rows(void* out, long rows, const void* cache, long pages, int bits, const int* seg_slot, const int* seg_pos0, const int* seg_nrows,
@@ -249,7 +294,10 @@ extern "C" int fb_mla_rows(void* out, long rows, const void* cache, long pages, 
   if (!latent_shape_ok(L, R, bits) || kv_block < 1 || align < 1) return -1;
   if (((uintptr_t)out | (uintptr_t)cache) % 16) return -2;
   if (rows <= 0) return 0;
+  // rows a CTA: the fewest of 4, 8 and 16 with which the SMs hold all CTAs at once
+  int per = 4;
+  while (per < LR_ROWS && (rows + per - 1) / per > 148 * (2048 / LR_THREADS)) per *= 2;
   auto kern = bits == 4 ? mla_rows_kernel<4> : mla_rows_kernel<8>;
-  return (int)launch_pdl(kern, dim3((unsigned)((rows + LR_ROWS - 1) / LR_ROWS)), dim3(288), (size_t)0, s, (__nv_bfloat16*)out, rows,
-                         (const uint8_t*)cache, seg_slot, seg_pos0, seg_nrows, nseg, block_table, max_blocks, pages, kv_block, L, whole, align, status);
+  return (int)launch_pdl(kern, dim3((unsigned)((rows + per - 1) / per)), dim3(LR_THREADS), (size_t)0, s, (__nv_bfloat16*)out, rows,
+                         (const uint8_t*)cache, seg_slot, seg_pos0, seg_nrows, nseg, block_table, max_blocks, pages, kv_block, L, whole, align, status, per);
 }
