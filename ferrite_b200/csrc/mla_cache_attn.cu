@@ -755,7 +755,15 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       // to shared memory.
       bool ok = true;
       for (int i = 0; i < tiles; ++i) {
-        ok = la_wait(&xfull[i % LA_AHEAD], i / LA_AHEAD & 1, abort_flag) && la_wait(rempty, (i & 1) ^ 1, abort_flag);
+        ok = la_wait(&xfull[i % LA_AHEAD], i / LA_AHEAD & 1, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+        for (int m = 0; m < 64; m += 32) {                             // the way to L2 while the place is taken (a row's part may lie in two lines)
+          const int r = ms.rows[i % LA_AHEAD][(warp - LA_SOFT - 1) * 64 + m + lane];
+          const uint8_t* from = cache + (size_t)max(r, 0) * RB + Row::rope_at(L);
+          asm volatile("prefetch.global.L2 [%0];\n\tprefetch.global.L2 [%1];" ::"l"(from), "l"(from + 2 * LC_R - 1) : "memory");
+        }
+        ok = la_wait(rempty, (i & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
 #pragma unroll 4
         for (int m = 0; m < 16; ++m) {
