@@ -7,10 +7,10 @@
 //   S^T [128 keys x N]  = [K | key part] Q^T     A: the tile's values, rows of keys; B: the pairs' queries
 //   O^T [L x N]        += V^T P^T                A: the SAME tile in shared memory, read along its columns; B: the weights, written by the softmax
 //
-// Warps 0..7 unpack (two threads a key, 32 of every 64 values each): a word of eight 4-bit codes takes a shift, a mask and one fma per two values, fp16(16 +
-// code + 8) * s - 24 s, exact in fp16 as the value itself is (a power of two times seven bits). The codes of the next tile are in flight in registers meanwhile.
-// Warps 8..15 run the softmax: a thread has a key (its TMEM lane) and half of the pairs. Warp 16 issues the products, 17 and 18 copy the key parts, 19 looks
-// up the keys' pages.
+// Warps 0..15 unpack (four threads a key, 32 of every 128 values each): a word of eight 4-bit codes takes a shift, a mask and one fma per two values,
+// fp16(16 + code + 8) * s - 24 s, exact in fp16 as the value itself is (a power of two times seven bits). The codes of the next tile are in flight in
+// registers meanwhile. Warps 16..23 run the softmax: a thread has a key (its TMEM lane) and half of the pairs. Warp 24 issues the products, 25 and 26
+// copy the key parts, 27 looks up the keys' pages.
 // The values' products run in fp16, so that a weight keeps 11 bits; a query is brought to 2^10 by a power of two of its own, which keeps its bf16 bits down
 // to 2^-27 of its largest value. The key part stays in bf16 (its products go to the same sums).
 //
@@ -23,6 +23,14 @@
 // and a second kernel joins them in order. A row's bits therefore depend on what else is in the step, and on nothing else.
 //
 // A key of which a group is no number gets the score NaN and a finite place in the tile, so that rows ahead of it, whose weight for it is zero, stay clean.
+// What bounds it: shared memory, 128 bytes a cycle. A tile of 64 pairs moves 36 * 6 KB for S, 32 * 6 KB for O, 128 KB as it is unpacked and 52 KB as its codes
+// come: 4600 cycles; it takes 8700, of which 3700 are S beside the unpacking (107 bytes a cycle), 2100 O (91) and 2000 the softmax, during which the tile has
+// to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 4200 of 6200. Measured, 512 values, 4 bits: 24 streams of up to
+// 16000 keys, 128 heads 159 us (43 would be the products alone), 32 of 16 heads 87 us (22: the bytes), one of 100000, 128 heads 93 us; one of 2048 25 us, a
+// fixed cost: 13 us here, of which 7 until the first scores (code that is new to every SM), 6 in the join, the rest between launches.
+// Tried and slower: tiles of 64 keys in two places (S costs 65 cycles where 48 do for 128 keys), tiles in tensor memory for S, unpacking by two groups
+// of warps in turn (32 streams of 16 heads 87 -> 93 us), whole rows brought to L2 ahead (one request a row: 114 us).
+//
 // Every wait is bounded: one that runs out sets the status word and an abort flag, all roles leave and the CTA frees its TMEM.
 #include <algorithm>
 
@@ -34,7 +42,7 @@ namespace fb {
 constexpr int LA_KT = 128;                       // keys of a tile
 constexpr int LA_CH = LA_KT * 128;               // bytes of 64 values of all of them
 constexpr int LA_UNPACK = 16, LA_SOFT = LA_UNPACK + 8;             // warps up to which these roles go
-constexpr int LA_THREADS = (LA_SOFT + 4) * 32;              // eight warps unpack, eight run the softmax, one issues the products, two copy key parts, one looks keys up
+constexpr int LA_THREADS = (LA_SOFT + 4) * 32;   // and one that issues the products, two that copy key parts, one that looks keys up
 constexpr int LA_AHEAD = 4;                      // tiles whose keys are looked up ahead
 constexpr float LA_TOP = 4.f, LA_LIMIT = 15.f;   // log2 of a piece's first largest weight; of the largest one that a weight may be
 
@@ -663,7 +671,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       if (i >= tiles) break;
     }
     if (broke && st == 0) { set_status(status, ST_MBAR_TIMEOUT); *abort_flag = 1; }
-    } else {
+  } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == LA_SOFT) {
       // ---- products: the whole warp, one lane of it by predicate ------------------------------------------------------------------------------------
@@ -841,7 +849,7 @@ using namespace fb;
 
 // Pairs of a unit: the fewest of 16, 32 and 64 that hold a segment's; more are several units (an unpacked tile serves as many as it can). Fewer where even
 // then every tile that the table has room for finds a CTA of its own: its products, its softmax and the sums that it leaves are shorter, and nobody
-// waits for the unpacking that is done again.
+// waits for the unpacking that is done again (one stream of 2048 with 128 heads: 25 us in units of 16, 27 of 64).
 static int latent_pairs(long pairs, long tiles, int ctas) {
   int N = 16;
   while (N < 64 && N < pairs && (pairs + N - 1) / N * tiles > ctas) N *= 2;
