@@ -23,13 +23,15 @@
 // and a second kernel joins them in order. A row's bits therefore depend on what else is in the step, and on nothing else.
 //
 // A key of which a group is no number gets the score NaN and a finite place in the tile, so that rows ahead of it, whose weight for it is zero, stay clean.
-// What bounds it: shared memory, 128 bytes a cycle. A tile of 64 pairs moves 36 * 6 KB for S, 32 * 6 KB for O, 128 KB as it is unpacked and 52 KB as its codes
-// come: 4600 cycles; it takes 8700, of which 3700 are S beside the unpacking (107 bytes a cycle), 2100 O (91) and 2000 the softmax, during which the tile has
-// to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 4200 of 6200. Measured, 512 values, 4 bits: 24 streams of up to
-// 16000 keys, 128 heads 159 us (43 would be the products alone), 32 of 16 heads 87 us (22: the bytes), one of 100000, 128 heads 93 us; one of 2048 25 us, a
-// fixed cost: 13 us here, of which 7 until the first scores (code that is new to every SM), 6 in the join, the rest between launches.
+//
+// What bounds it: the way to shared memory, 128 bytes a cycle. For a tile of 64 pairs the products read 36 * 6 KB (S) and 32 * 6 KB (O), 3260 cycles; stores
+// of the unpacked tile, codes that come in sectors of 32 bytes, key parts and scores take 4300 more (the counters' wavefronts): 7560 of the tile's
+// 8700. The rest is the softmax, during which the tile has to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 6200
+// cycles a tile. Measured, 512 values in 4 bits, cold caches: 24 streams of up to 16000 keys with 128 heads 157 us (43: the products at the card's rate),
+// 32 with 16 heads 87 us (22: the bytes), one of 100000 with 128 heads 91 us (17), one of 2048 25 us: 13 here, of which 7 until the first scores (code
+// that is new to every SM comes slowly), 6 in the join, the rest between launches.
 // Tried and slower: tiles of 64 keys in two places (S costs 65 cycles where 48 do for 128 keys), tiles in tensor memory for S, unpacking by two groups
-// of warps in turn (32 streams of 16 heads 87 -> 93 us), whole rows brought to L2 ahead (one request a row: 114 us).
+// of warps in turn (32 streams of 16 heads 87 -> 93 us), rows brought to L2 ahead one by one (114 us; a page's in one request costs nothing).
 //
 // Every wait is bounded: one that runs out sets the status word and an abort flag, all roles leave and the CTA frees its TMEM.
 #include <algorithm>
@@ -744,9 +746,16 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
           const int key = w.t * LA_KT + k * 32 + lane;
           row[k] = -1;
           if (key < w.kv) {
-            const int at = key / kv_block, blk = block_table[(size_t)w.slot * max_blocks + at];
-            if (blk >= 0 && blk < pages) row[k] = blk * kv_block + key - at * kv_block;      // (rows of a cache are fewer than 2^31)
-            else set_status(status, ST_BOUNDS);
+            const int at = key / kv_block, in = key - at * kv_block, blk = block_table[(size_t)w.slot * max_blocks + at];
+            if (blk >= 0 && blk < pages) {
+              row[k] = blk * kv_block + in;                            // (rows of a cache are fewer than 2^31)
+              if (i > 0 && (in == 0 || k * 32 + lane == 0)) {          // the tile's rows of a page lie together: one request brings them to L2
+                const int n = min(kv_block - in, min((w.t + 1) * LA_KT, w.kv) - key);
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(cache + (size_t)row[k] * RB), "r"(n * RB) : "memory");
+              }
+            } else {
+              set_status(status, ST_BOUNDS);
+            }
           }
         }
         ok = la_wait(&xempty[i % LA_AHEAD], (i / LA_AHEAD & 1) ^ 1, abort_flag);
@@ -765,12 +774,6 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       for (int i = 0; i < tiles; ++i) {
         ok = la_wait(&xfull[i % LA_AHEAD], i / LA_AHEAD & 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-        for (int m = 0; m < 64; m += 32) {                             // the way to L2 while the place is taken (a row's part may lie in two lines)
-          const int r = ms.rows[i % LA_AHEAD][(warp - LA_SOFT - 1) * 64 + m + lane];
-          const uint8_t* from = cache + (size_t)max(r, 0) * RB + Row::rope_at(L);
-          asm volatile("prefetch.global.L2 [%0];\n\tprefetch.global.L2 [%1];" ::"l"(from), "l"(from + 2 * LC_R - 1) : "memory");
-        }
         ok = la_wait(rempty, (i & 1) ^ 1, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
 #pragma unroll 4
