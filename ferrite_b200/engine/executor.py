@@ -26,7 +26,7 @@ import torch
 from ..config import EngineConfig, ModelConfig
 from ..models.weights import Weights, delta_dims, gqa_dims, latent_dims, ssm_dims
 from ..ops.latent import SegGroup, seg_groups
-from ..ops.mla_cache import fits, latent_bits, row_bytes
+from ..ops.mla_cache import ATTENDED, fits, latent_bits, row_bytes
 from ..ops.qweight import QWeight
 
 
@@ -357,7 +357,7 @@ class Executor:
     def latent_cache_bits(self) -> int:
         """Bits of a cached latent of the MLA layers: 4 (kv_dtype int4), 8 (fp8), or 16 where that has no form for latents or for these widths."""
         c, bits = self.cfg, latent_bits(self.ecfg.kv_dtype)
-        return bits if c.kv_lora > 0 and fits(c.kv_lora, c.rope_head_dim, bits) else 16
+        return bits if c.kv_lora in ATTENDED and fits(c.kv_lora, c.rope_head_dim, bits) else 16
 
     def kv_block_bytes(self) -> int:
         c, e = self.cfg, self.ecfg

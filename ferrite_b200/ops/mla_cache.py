@@ -14,6 +14,7 @@ import torch
 
 BITS = {"int4": 4, "fp8": 8}             # kv_dtype -> bits of a latent; every other kv_dtype keeps latents in the compute dtype
 GROUP = {4: 16, 8: 32}
+ATTENDED = (64, 128, 256, 512)           # latent widths that the attention kernel takes; rows are written and read back at every width that fits
 
 
 def latent_bits(kv_dtype: str) -> int:

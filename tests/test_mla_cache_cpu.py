@@ -1,4 +1,5 @@
 """Latent cache of the MLA models in 4 and 8 bits: what a row stands for, and the engine over it, on the CPU."""
+import dataclasses
 import warnings
 
 import latent_rows as lr
@@ -106,3 +107,11 @@ def test_engine_says_where_latents_stay_as_they_are():
     with warnings.catch_warnings():
         warnings.simplefilter("error")
         Engine(cfg, init_weights(cfg, seed=0), EngineConfig(n_slots=1, max_ctx=128, kv_dtype="int4"), device="cpu")
+
+
+def test_widths_that_no_kernel_attends_stay_as_they_are():
+    cfg = dataclasses.replace(tiny_mla(moe=False), kv_lora=192)
+    assert mla_cache.fits(192, 64, 4) and 192 not in mla_cache.ATTENDED
+    with pytest.warns(UserWarning, match="latents"):
+        eng = Engine(cfg, init_weights(cfg, seed=0), EngineConfig(n_slots=1, max_ctx=128, kv_dtype="int4"), device="cpu")
+    assert eng.ex.latent_bits == 16
