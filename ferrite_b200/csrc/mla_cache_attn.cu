@@ -515,16 +515,19 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
           tc_fence_after();
           const int at = (t0 + k) * LA_KT + key;
           const bool edge = (t0 + k + 1) * LA_KT > least, none = ms.bad[i & 3][key >> 3] >> (4 * (key & 7)) & 15u;
-          // log2 of the thread's weights, up to the reference
-          auto scores = [&](float (&x)[CW]) {
+          // log2 of the thread's weights, up to the reference or (`bare`) without it. The product is rounded ahead of the sum: the largest score minus itself
+          // is then nothing, however large it is (in one fma the product's rounding would be left, 2^-24 of the score, as if it were a weight).
+          auto scores = [&](float (&x)[CW], bool bare) {
+            const uint64_t zero = f2_pack(0.f, 0.f);                 // (a product and a sum that follows may be made one; a sum of two may not)
             uint32_t r[CW];
             tmem_ld<CW>(ts, r);
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < CW; e += 4) {
-              const float4 c = *reinterpret_cast<const float4*>(&ms.c[par][hc * CW + e]), nr = *reinterpret_cast<const float4*>(&ms.nr[par][hc * CW + e]);
-              const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), f2_pack(c.x, c.y), f2_pack(nr.x, nr.y)));
-              const float2 b = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), f2_pack(c.z, c.w), f2_pack(nr.z, nr.w)));
+              const float4 c = *reinterpret_cast<const float4*>(&ms.c[par][hc * CW + e]);
+              const float4 nr = bare ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(&ms.nr[par][hc * CW + e]);
+              const float2 a = f2_unpack(f2_add(f2_fma(f2_pack(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), f2_pack(c.x, c.y), zero), f2_pack(nr.x, nr.y)));
+              const float2 b = f2_unpack(f2_add(f2_fma(f2_pack(__uint_as_float(r[e + 2]), __uint_as_float(r[e + 3])), f2_pack(c.z, c.w), zero), f2_pack(nr.z, nr.w)));
               x[e] = a.x; x[e + 1] = a.y; x[e + 2] = b.x; x[e + 3] = b.y;
             }
             if (none) {
@@ -545,18 +548,26 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
 #pragma unroll 1
           while (!done) {
             float x[CW];
-            scores(x);
+            scores(x, anew);
             if (anew) {
               if (!ok) ms.fail = 1;
+              if (k > 0) {                                           // the tile's weights leave the sums again: what they rounded off is 2^-24 of the largest
+#pragma unroll
+                for (int e = 0; e < CW; e += 2) {
+                  const float2 nr = *reinterpret_cast<const float2*>(&ms.nr[par][hc * CW + e]), l = f2_unpack(sum[e / 2]);
+                  sum[e / 2] = f2_pack(l.x - ex2(x[e] + nr.x), l.y - ex2(x[e + 1] + nr.y));
+                }
+              }
               const float m = columns<CW>(x, lane, fmx);
               if (lane < CW) ms.mx[quad][hc * CW + lane] = m;
               softmax_sync();
               if (ms.fail) break;
               if (st < N) {
                 const float most = fmaxf(fmaxf(ms.mx[0][st], ms.mx[1][st]), fmaxf(ms.mx[2][st], ms.mx[3][st]));
-                const float d = k == 0 ? (most == -INFINITY ? 0.f : most - LA_TOP) : most > LA_TOP ? most - LA_TOP : 0.f;
-                ms.d[st] = d;
-                ms.nr[par][st] -= d;
+                const float was = -ms.nr[par][st], to = most - LA_TOP;
+                const bool up = k == 0 ? most > -INFINITY : to > was;
+                ms.d[st] = up ? to - was : 0.f;
+                if (up) ms.nr[par][st] = -to;
               }
               softmax_sync();
               anew = false;
@@ -564,9 +575,8 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
               if (k > 0) {                                           // (the tile's scores are complete, so the products ahead of them are)
 #pragma unroll
                 for (int e = 0; e < CW; e += 2) {
-                  // the weights of this tile leave the sums again; what they rounded off is 2^-24 of the new largest weight. Sums of 2^-100 of that are none.
-                  const float2 d = *reinterpret_cast<const float2*>(&ms.d[hc * CW + e]), l = f2_unpack(sum[e / 2]);
-                  sum[e / 2] = f2_pack(d.x > 100.f ? 0.f : (l.x - ex2(x[e])) * ex2(-d.x), d.y > 100.f ? 0.f : (l.y - ex2(x[e + 1])) * ex2(-d.y));
+                  const float2 d = *reinterpret_cast<const float2*>(&ms.d[hc * CW + e]), l = f2_unpack(sum[e / 2]);       // (sums of 2^-100 are none)
+                  sum[e / 2] = f2_pack(d.x > 100.f ? 0.f : l.x * ex2(-d.x), d.y > 100.f ? 0.f : l.y * ex2(-d.y));
                 }
 #pragma unroll 1
                 for (int j = 0; j < NP * CW; j += W) {

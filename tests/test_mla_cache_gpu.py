@@ -1,5 +1,7 @@
 """Latent cache of the MLA models in 4 and 8 bits on the GPU: the step that writes it, its rows read back and the attention over it against the plain
 statement in 64 bits (`latent_rows.py`), alone and as the engine runs them."""
+import functools
+import sys
 import zlib
 
 import latent_rows as lr
@@ -431,3 +433,77 @@ def test_engine_over_quantised_latents(ext, kv):
     kl = torch.nn.functional.kl_div(torch.log_softmax(got, -1), torch.log_softmax(want, -1), log_target=True, reduction="batchmean").item()
     assert kl < (8e-2 if kv == "int4" else 3e-2), kl             # bf16 activations, and codes that fall on the other side of a border for them
     eng.check()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nq", [128, 24])
+def test_attention_in_wide_tables(ops, bits, nq, monkeypatch):
+    """Tables with room for far more keys than there are: units of 64 and 32 pairs, where narrow tables have units of 16."""
+    monkeypatch.setattr(sys.modules[__name__], "tables", functools.partial(tables, width=300))
+    for L in (512, 256, 128, 64):
+        for lens, rows, page in (((1, 127, 128, 129, 64), 1, 64), ((1000, 300), 5, 64)):
+            test_attention(ops, bits, L, nq, lens, rows, page)
+    test_attention_with_scores_that_grow(ops, bits, nq)
+    test_values_that_are_no_numbers_reach_who_sees_them(ops, bits, nq)
+    test_attention_of_rows_that_see_nothing(ops, bits)
+    test_attention_scales_of_queries(ops, bits)
+
+
+@pytest.mark.parametrize("width", [0, 100])
+def test_attention_of_many_segments(ops, width):
+    """More segments than a warp has lanes, some without rows, some that see nothing."""
+    g = gen("many", width)
+    n, L, nq = 71, 512, 16
+    lens = [(i * 37) % 200 for i in range(n)]
+    nrows = [0 if i % 9 == 4 else 1 + i % 3 for i in range(n)]
+    table, pages = tables(lens, 64, g, width=width)
+    cache = random_cache(4, L, pages, 64, g)
+    slot = [s for s in range(n) for _ in range(nrows[s])]
+    kvlen = [max(0, lens[s] - nrows[s] + 1 + r) for s in range(n) for r in range(nrows[s])]
+    row0 = [sum(nrows[:s]) for s in range(n)]
+    check_attention(ops, 4, L, nq, 64, slot, kvlen, table, cache, bf(g, len(slot), nq, L + R), 0.05, (i32(list(range(n))), i32(row0), i32(nrows), 3))
+    seg = i32(list(range(n))), i32([max(0, lens[s] - nrows[s]) for s in range(n)]), i32([min(lens[s], nrows[s]) for s in range(n)])
+    vals = lr.unpack(cache.view(-1, cache.shape[-1]), L, 4)
+    total = sum(min(a, b) for a, b in zip(lens, nrows))
+    got = ops.mla_rows(cache, *seg, table, 64, L, R, total, kv_bits=4).cpu().double()
+    want = [int(table[s, p // 64]) * 64 + p % 64 for s in range(n) for p in range(max(0, lens[s] - nrows[s]), lens[s])]
+    assert torch.equal(got, vals[want])
+    got = ops.mla_rows(cache, *seg, table, 64, L, R, sum((m + 63) // 64 * 64 for m in lens), whole=True, kv_bits=4).cpu().double()
+    lo = 0
+    for s, m in enumerate(lens):
+        assert torch.equal(got[lo:lo + m], vals[[int(table[s, p // 64]) * 64 + p % 64 for p in range(m)]])
+        lo += (m + 63) // 64 * 64
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prep_reads_rows_on_any_address(ops, bits):
+    g = gen("address", bits)
+    T, L = 9, 512
+    table, pages = tables([T], 64, g)
+    wide = bf(g, T, L + R + 5)
+    slot, pos = [0] * T, list(range(T))
+    _, odd, before, q, kva, w = prep(ops, bits, L, 2, 16, slot, pos, table, pages, 64, g, kva=wide[:, 3:3 + L + R])
+    even = before.clone()
+    ops.mla_prep(q, kva.contiguous(), w, None, inv_freq(), i32(slot), i32(pos), table, even, 64, 2, 16, L, R, 1e-6, absorb=False, kv_bits=bits)
+    assert torch.equal(odd, even) and not torch.equal(odd, before)
+
+
+@pytest.mark.parametrize("width", [0, 300])
+@pytest.mark.parametrize("falling", [False, True])
+def test_attention_with_scores_past_what_32_bits_tell_apart(ops, width, falling):
+    """Scores of 4e9 a step, rising or falling along the keys: all weight is one key's, whose value comes back, off by its rounding to bf16 and
+    by that of its weight (2^-8 and 2^-11)."""
+    g = gen("huge", width)
+    n, L, nq = 256, 512, 128
+    table, pages = tables([n], 64, g, width=width)
+    cache = random_cache(4, L, pages, 64, g)
+    p = torch.arange(n, device=DEV)
+    flat = table[0, p // 64].long() * 64 + p % 64
+    rope = torch.zeros(n, R, dtype=torch.bfloat16, device=DEV)
+    rope[:, 0] = n - 1 - p if falling else p
+    cache.view(-1, cache.shape[-1])[flat, L // 2:L // 2 + 2 * R] = rope.view(torch.uint8).view(n, 2 * R)
+    q = torch.zeros(1, nq, L + R, dtype=torch.bfloat16, device=DEV)
+    q[..., L] = 2.0 ** 36
+    got = ops.mla_attention(q, cache, i32([0]), i32([n]), table, 64, nq, L, R, 1 / 16, segs=segments(1, 1), kv_bits=4)
+    want = lr.unpack(cache.view(-1, cache.shape[-1])[flat[0 if falling else -1]][None], L, 4)[:, :L].to(DEV)
+    assert ((got[0].double() - want).abs() <= want.abs() * (2 ** -8 + 2 ** -11)).all()
