@@ -682,6 +682,7 @@ class EngineConfig:
     fused_layers: Optional[bool] = None   # plain decode rows: one persistent kernel per layer (None = when tensor parallel)
     # "bf16" | "fp8" (e4m3, one scale per (token, kv head)) | "int6" | "int4" (integer codes, one scale per 32 elements);
     # "fp8h" / "int6h" / "int4h": the same with keys stored in a Walsh-Hadamard rotated basis
+    # latents of MLA models: "int4" (one scale per 16 values) and "fp8" (e4m3, one power of two per 32); the others leave them in the compute dtype
     kv_dtype: str = "bf16"
     seq_parallel: bool = True          # TP prompts: row-sharded residual stream, all-gather/reduce-scatter fused into the GEMMs
     graph_max: int = 128               # LRU size of the CUDA-graph cache (reference GRAPH_MAX)

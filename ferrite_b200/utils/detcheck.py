@@ -76,6 +76,14 @@ def cases(ops, dev):
     qm, lat = rnd(1, 16, 576), rnd(nb, kvb, 576)
     out["latent_mma: 1 row, 16 key splits"] = lambda: ops.mla_attention(qm, lat, i32(0), i32(ctx), bt, kvb, 16, 512, 64, 0.05, nsplit=16,
                                                                         segs=(i32(0), i32(0), i32(1), 1))
+    # latents in 4 bits: units of three rows that span CTAs, joined by a second kernel
+    from ..ops.mla_cache import row_bytes
+    lat4 = torch.zeros(nb, kvb, row_bytes(512, 64, 4), device=dev, dtype=torch.uint8)
+    ops.mla_prep(rnd(ctx, 128), rnd(ctx, 576), rnd(512, scale=0.1), None, torch.rand(32, generator=g, device=dev), i32(*[0] * ctx), i32(*range(ctx)), bt,
+                 lat4, kvb, 1, 64, 512, 64, 1e-6, absorb=False, kv_bits=4)
+    qm3, kv3 = rnd(3, 128, 576), i32(ctx - 2, ctx - 1, ctx)
+    out["mla_attn_q: 3 rows of 128 heads, 4 bits"] = lambda: ops.mla_attention(qm3, lat4, i32(0, 0, 0), kv3, bt, kvb, 128, 512, 64, 0.05,
+                                                                              segs=(i32(0), i32(0), i32(3), 3), kv_bits=4)
     # chunked Gated DeltaNet scan
     nk, nv, dk, dv, T = 4, 8, 128, 128, 300
     conv_dim = 2 * nk * dk + nv * dv
