@@ -26,12 +26,13 @@
 //
 // What bounds it: the way to shared memory, 128 bytes a cycle. For a tile of 64 pairs the products read 36 * 6 KB (S) and 32 * 6 KB (O), 3260 cycles; stores
 // of the unpacked tile, codes that come in sectors of 32 bytes, key parts and scores take 4300 more (the counters' wavefronts): 7560 of the tile's
-// 8700. The rest is the softmax, during which the tile has to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 6200
-// cycles a tile. Measured, 512 values in 4 bits, cold caches: 24 streams of up to 16000 keys with 128 heads 157 us (43: the products at the card's rate),
-// 32 with 16 heads 87 us (22: the bytes), one of 100000 with 128 heads 91 us (17), one of 2048 25 us: 13 here, of which 7 until the first scores (code
+// 8700. During the softmax's 2000 no product runs: the tile has to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 6200
+// cycles a tile. Measured, 512 values in 4 bits, cold caches: 24 streams of up to 16000 keys with 128 heads 161 us (43: the products at the card's rate),
+// 32 with 16 heads 87 us (22: the bytes), one of 100000 with 128 heads 93 us (17), one of 2048 25 us: 13 here, of which 7 until the first scores (code
 // that is new to every SM comes slowly), 6 in the join, the rest between launches.
 // Tried and slower: tiles of 64 keys in two places (S costs 65 cycles where 48 do for 128 keys), tiles in tensor memory for S, unpacking by two groups
-// of warps in turn (32 streams of 16 heads 87 -> 93 us), rows brought to L2 ahead one by one (114 us; a page's in one request costs nothing).
+// of warps in turn (32 streams of 16 heads 87 -> 93 us), the softmax in halves with the next one's load under
+// way (registers: 161 -> 171 us), rows brought to L2 ahead one by one (114 us; a page's in one request costs nothing).
 //
 // Every wait is bounded: one that runs out sets the status word and an abort flag, all roles leave and the CTA frees its TMEM.
 #include <algorithm>
