@@ -846,8 +846,9 @@ __global__ void __launch_bounds__(128) mla_attn_q_join_kernel(__nv_bfloat16* __r
     }
 #pragma unroll
     for (int k = 0; k < AT_ONCE; ++k) {
-      const float y = __shfl_sync(0xffffffffu, x, (i0 + k) % 32);    // (zero where there is no record)
-      if (y != 0.f) { a.x = fmaf(y, v[k].x, a.x); a.y = fmaf(y, v[k].y, a.y); a.z = fmaf(y, v[k].z, a.z); a.w = fmaf(y, v[k].w, a.w); }
+      // (a record that weighs nothing is multiplied all the same: sums that are no numbers have seen a key that is none, and so has the row)
+      const float y = __shfl_sync(0xffffffffu, x, (i0 + k) % 32);
+      if (i0 + k < count) { a.x = fmaf(y, v[k].x, a.x); a.y = fmaf(y, v[k].y, a.y); a.z = fmaf(y, v[k].z, a.z); a.w = fmaf(y, v[k].w, a.w); }
     }
     load(i0 + AT_ONCE);
   }
