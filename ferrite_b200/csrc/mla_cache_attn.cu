@@ -273,10 +273,11 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   const int all = (int)(total & TILES), share = max(1, (int)((uint32_t)(all + (int)gridDim.x - 1) / gridDim.x));
   const int f0 = min((int)blockIdx.x * share, all), f1 = min(f0 + share, all), tiles = f1 - f0;
+  const bool much = by_unit && (int)(total >> 40) > entries;         // segments of more rows than the caller said: nothing is written
   if (by_unit) {
     if (blockIdx.x == 0)
 #pragma unroll 1
-      for (int i = (int)(total >> 40) + tid; i < entries; i += LA_THREADS) join[i] = make_int4(0, 0, 0, 0);
+      for (int i = (much ? 0 : (int)(total >> 40)) + tid; i < entries; i += LA_THREADS) join[i] = make_int4(0, 0, 0, 0);
   } else if (tid == LA_UNPACK * 32) {                                // (the thread that may write another one there)
     join[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
@@ -284,7 +285,6 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
 #pragma unroll 1
     for (int seg = lane; seg < g.nseg; seg += 32)
       if (g.nrows[seg] > 0 && (long)g.kvlen[g.row0[seg] + g.nrows[seg] - 1] > g.limit) set_status(status, ST_BOUNDS);
-  const bool much = by_unit && (int)(total >> 40) > entries;         // segments of more rows than the caller said
   if (tiles == 0 || much) {                                          // the same for the whole CTA
     if (tid == 0 && much) set_status(status, ST_CAPACITY);
     if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);

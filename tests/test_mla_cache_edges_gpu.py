@@ -57,3 +57,23 @@ def test_a_key_that_is_no_number_is_not_lost_when_scores_rise(ops, bits):
     assert call().isfinite().all()
     cache.view(-1, cache.shape[-1])[flat[7], L * bits // 8 + 2 * R] = 255
     assert call().isnan().all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_segments_of_more_rows_than_said_leave_the_output_alone(ops, bits):
+    """A workspace that an earlier call has used, and a segment of five rows where one was said: the status says so and nothing is written."""
+    g = gen("capacity", bits)
+    L, nq, page, n, T = 512, 16, 64, 1000, 5
+    table, pages = tables([n], page, g)
+    cache = random_cache(bits, L, pages, page, g)
+    q, out = bf(g, T, nq, L + R), torch.full((T, nq, L), 7.0, dtype=torch.bfloat16, device=DEV)
+    ws = torch.zeros(ops.C.mla_attn_q_floats(1, nq, L, ops.sm_count), device=DEV)
+    call = lambda rows: ops.C.mla_attn_q(out, ws, q, cache, i32([0]), i32([0]), i32([rows]), 1, i32([n] * T), table, page, L, R, bits, 0.05, ops.sm_count,
+                                         ops.status_word)
+    call(1)
+    assert ops.status() == 0 and not (out[0] == 7).any() and (out[1:] == 7).all()
+    out.fill_(7)
+    call(T)
+    assert ops.status() == 5
+    ops.status_word.zero_()
+    assert (out == 7).all()
