@@ -185,7 +185,7 @@ int fb_mla_qpad(void* qp, const void* q, long q_stride, const void* qabs, long r
 int fb_latent_row_bytes(int L, int R, int bits);
 int fb_mla_prep_q(void* cache, long pages, int bits, void* qabs, const void* kva, long kva_stride, const void* q, long q_stride, const void* norm_w,
                   const float* inv_freq, const int* row_slot, const int* row_pos, const int* block_table, int max_blocks, int kv_block, int rows, int nq,
-                  int dn, int L, int R, float eps, int* status, cudaStream_t s);
+                  int dn, int L, int R, double eps, int* status, cudaStream_t s);
 int fb_mla_rows(void* out, long rows, const void* cache, long pages, int bits, const int* seg_slot, const int* seg_pos0, const int* seg_nrows, int nseg,
                 const int* block_table, int max_blocks, int kv_block, int L, int R, int whole, int align, int* status, cudaStream_t s);
 // attention of segments' rows; ws: as many 32-bit words as fb_mla_attn_q_floats says for the most rows of a segment; row_kvlen does not fall along a segment

@@ -614,7 +614,7 @@ void mla_prep_q(Tensor cache, Tensor qabs, Tensor kva, Tensor q, Tensor norm_w, 
   const c10::cuda::CUDAGuard guard(dev);
   check(fb_mla_prep_q(cache.data_ptr(), (long)cache.size(0), (int)bits, qabs.data_ptr(), kva.data_ptr(), (long)kva.stride(0), q.data_ptr(),
                       (long)q.stride(0), norm_w.data_ptr(), inv_freq.data_ptr<float>(), row_slot.data_ptr<int>(), row_pos.data_ptr<int>(),
-                      block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)dn, (int)L, (int)R, (float)eps,
+                      block_table.data_ptr<int>(), (int)block_table.size(1), (int)kv_block, (int)T, (int)nq, (int)dn, (int)L, (int)R, eps,
                       status.data_ptr<int>(), cur_stream()), "mla_prep_q");
 }
 

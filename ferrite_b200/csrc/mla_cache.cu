@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256, 4) mla_prep_q_kernel(uint8_t* __restrict_
                                                          long kva_stride, const __nv_bfloat16* q, long q_stride,
                                                          const __nv_bfloat16* __restrict__ norm_w, const float* __restrict__ inv_freq,
                                                          const int* row_slot, const int* row_pos, const int* block_table, int max_blocks, long pages,
-                                                         int kv_block, int nq, int dn, int L, float eps, int* status, int rows, int kinds) {
+                                                         int kv_block, int nq, int dn, int L, double eps, int* status, int rows, int kinds) {
   using Row = LatentRow<BITS>;
   constexpr int R = LC_R, half = R / 2;
   const int tid = threadIdx.x, lane = tid & 31, writers = (rows + LP_ROWS - 1) / LP_ROWS, turner = (int)blockIdx.x - writers;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256, 4) mla_prep_q_kernel(uint8_t* __restrict_
   for (int j = 0; j < 8; ++j) ss += (double)bf_lo(xw[j]) * bf_lo(xw[j]) + (double)bf_hi(xw[j]) * bf_hi(xw[j]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  const double r = 1.0 / sqrt(ss / L + (double)eps);
+  const double r = 1.0 / sqrt(ss / L + eps);
   double y[16], top = 0.0;
   bool bad = false;
 #pragma unroll
@@ -277,7 +277,7 @@ extern "C" int fb_latent_row_bytes(int L, int R, int bits) { return latent_shape
 
 extern "C" int fb_mla_prep_q(void* cache, long pages, int bits, void* qabs, const void* kva, long kva_stride, const void* q, long q_stride,
                              const void* norm_w, const float* inv_freq, const int* row_slot, const int* row_pos, const int* block_table,
-                             int max_blocks, int kv_block, int rows, int nq, int dn, int L, int R, float eps, int* status, cudaStream_t s) {
+                             int max_blocks, int kv_block, int rows, int nq, int dn, int L, int R, double eps, int* status, cudaStream_t s) {
   if (!latent_shape_ok(L, R, bits) || nq < 1 || dn < 0 || kv_block < 1) return -1;
   if (dn % 4 || q_stride % 4 || ((uintptr_t)q | (uintptr_t)qabs) % 8 || (uintptr_t)cache % 16) return -2;
   if (rows <= 0) return 0;

@@ -1,7 +1,10 @@
 """Latents in 4 and 8 bits where steps, pages and values go to their limits."""
+import latent_rows as lr
 import pytest
 import torch
-from test_mla_cache_gpu import DEV, R, bf, check_attention, clean, gen, i32, ops, random_cache, segments, tables  # noqa: F401
+from test_mla_cache_gpu import DEV, R, bf, check_attention, clean, gen, i32, inv_freq, ops, random_cache, segments, tables  # noqa: F401
+
+from ferrite_b200.ops import mla_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +80,21 @@ def test_segments_of_more_rows_than_said_leave_the_output_alone(ops, bits):
     assert ops.status() == 5
     ops.status_word.zero_()
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prep_takes_eps_in_64_bits(ops, bits):
+    """A row whose mean square is about eps: mean square + eps is 2^-18 (1 + 2^-30), so a value that would lie on the border of two codes (3.5 of 4 bits;
+    15.5 of e4m3) lies below it, by less than eps has in 32 bits."""
+    L, nq, dn, page = 64, 2, 32, 64
+    u = 2.0 ** -9
+    kva = torch.zeros(1, L + R, dtype=torch.bfloat16, device=DEV)
+    kva[0, :3] = torch.tensor([7.0, 3.5, 31 / 128]) * u
+    eps = u * u * (1 + 2.0 ** -30) - float(kva[0, :L].double().square().sum()) / L
+    assert float(torch.tensor(eps)) != eps
+    w, q = torch.zeros(L, dtype=torch.bfloat16, device=DEV), torch.zeros(1, nq * (dn + R), dtype=torch.bfloat16, device=DEV)
+    cache = torch.zeros(1, page, lr.row_bytes(L, bits), dtype=torch.uint8, device=DEV)
+    ops.mla_prep(q, kva, w, None, inv_freq(), i32([0]), i32([0]), i32([[0]]), cache, page, nq, dn, L, R, eps, absorb=False, kv_bits=bits)
+    want = mla_cache.quantised(lr.normed(kva, w, L, eps), bits).cpu()
+    assert want[0, 1 if bits == 4 else 2] == (3.0 if bits == 4 else 15 / 64)
+    assert torch.equal(lr.unpack(cache[0, :1], L, bits)[:, :L], want)
