@@ -47,6 +47,7 @@ constexpr int LA_CH = LA_KT * 128;               // bytes of 64 values of all of
 constexpr int LA_UNPACK = 16, LA_SOFT = LA_UNPACK + 8;             // warps up to which these roles go
 constexpr int LA_THREADS = (LA_SOFT + 4) * 32;   // and one that issues the products, two that copy key parts, one that looks keys up
 constexpr int LA_AHEAD = 4;                      // tiles whose keys are looked up ahead
+constexpr int LA_ROWS = 64;                      // rows whose units walk the same keys; a segment of more, a prompt, is cut into blocks of so many
 constexpr float LA_TOP = 4.f, LA_LIMIT = 15.f;   // log2 of a piece's first largest weight; of the largest one that a weight may be
 
 template <int BITS, int NC, int N>
@@ -79,14 +80,33 @@ struct LatentSegs {
   int nseg, nq;
   long limit;                                    // keys that a table has room for
 };
-struct LatentWalk {                              // a place in the list of tiles
-  int s, u, t, units, nt, kv, row0, nrows, slot;
+// A place in the list of tiles: of segment s, block row0 .. row0 + nrows of its rows, `left` rows behind them, unit u of the block, tile t of the unit. A
+// prompt's blocks end where their own last rows do (2048 rows of 128 heads from position 0: 1282 us; 2215 with every unit as long as the prompt). Its units
+// count a place more than they have tiles (`extra`): the queries, the output and the gaps of a unit take 6 us where a tile takes 4.5, and the first rows'
+// units are short (without it the CTA that has those is the last by far: 2354 us).
+struct LatentWalk {
+  int s, u, t, units, nt, kv, row0, nrows, slot, left, extra;
   template <int N>
-  __device__ __forceinline__ void load(const LatentSegs& g) {
-    nrows = g.nrows[s]; row0 = g.row0[s]; slot = g.slot[s];
+  __device__ __forceinline__ void block(const LatentSegs& g) {
     kv = nrows > 0 ? (int)min((long)max(g.kvlen[row0 + nrows - 1], 0), g.limit) : 0;
-    units = (int)(((uint32_t)max(nrows, 0) * g.nq + N - 1) / N);       // (rows times heads are fewer than 2^30)
+    units = (int)(((uint32_t)nrows * g.nq + N - 1) / N);               // (rows times heads are fewer than 2^30; those of a whole block fill its units)
     nt = max(1, (kv + LA_KT - 1) / LA_KT);
+  }
+  template <int N>
+  __device__ __forceinline__ void segment(const LatentSegs& g) {
+    const int n = max(g.nrows[s], 0);
+    row0 = g.row0[s]; slot = g.slot[s];
+    nrows = min(n, LA_ROWS);
+    left = n - nrows;
+    extra = left > 0;
+    block<N>(g);
+  }
+  template <int N>
+  __device__ __forceinline__ void next_block(const LatentSegs& g) {
+    row0 += LA_ROWS;
+    nrows = min(left, LA_ROWS);
+    left -= nrows;
+    block<N>(g);
   }
   template <int N>
   __device__ __forceinline__ void next_unit(const LatentSegs& g) {
@@ -94,9 +114,13 @@ struct LatentWalk {                              // a place in the list of tiles
     if (++u < units) return;
     u = 0;
     units = 0;
+    if (left > 0) {
+      next_block<N>(g);
+      return;
+    }
 #pragma unroll 1
     while (++s < g.nseg) {
-      load<N>(g);
+      segment<N>(g);
       if (units) break;
     }
   }
@@ -257,22 +281,41 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   g.slot = after_wait(g.slot); g.row0 = after_wait(g.row0); g.nrows = after_wait(g.nrows); g.kvlen = after_wait(g.kvlen);
 
   // ---- this CTA's share of the list, by every warp for itself (no barrier stands between the lengths and a role's first load): sums over the segments, a
-  // lane each, of their tiles (low 40 bits) and units (the rest)
-  constexpr long long TILES = (1ll << 40) - 1;
+  // lane each (a prompt's further blocks by the whole warp), of their places (low 40 bits) and units (the rest)
+  constexpr long long PLACES = (1ll << 40) - 1;
   LatentWalk w;
-  auto count = [&](int seg) -> long long {
-    if (seg >= g.nseg) return 0;
-    w.s = seg;
-    w.load<N>(g);
-    return (long long)w.units * w.nt + ((long long)w.units << 40);
+  bool prompts = false;
+  auto count = [&](int seg0) -> long long {                          // of segment seg0 + lane, at whose first block the lane's walk is then
+    w.units = w.nrows = w.nt = w.left = w.extra = 0;
+    if (seg0 + lane < g.nseg) {
+      w.s = seg0 + lane;
+      w.segment<N>(g);
+    }
+    long long sum = (long long)w.units * (w.nt + w.extra) + ((long long)w.units << 40);
+#pragma unroll 1
+    for (uint32_t more = __ballot_sync(0xffffffffu, w.left > 0); more; more &= more - 1) {
+      const int from = __ffs(more) - 1;
+      LatentWalk x;
+      x.row0 = __shfl_sync(0xffffffffu, w.row0, from);
+      x.left = __shfl_sync(0xffffffffu, w.left, from);
+      long long rest = 0;
+#pragma unroll 1
+      while (x.left > 0) {
+        x.next_block<N>(g);
+        rest += (long long)x.units * (x.nt + 1) + ((long long)x.units << 40);
+      }
+      if (lane == from) sum += rest;
+      prompts = true;
+    }
+    return sum;
   };
   long long mine = 0, total = 0;
 #pragma unroll 1
-  for (int seg = lane; seg < g.nseg; seg += 32) total += mine = count(seg);
+  for (int seg0 = 0; seg0 < g.nseg; seg0 += 32) total += mine = count(seg0);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  const int all = (int)(total & TILES), share = max(1, (int)((uint32_t)(all + (int)gridDim.x - 1) / gridDim.x));
-  const int f0 = min((int)blockIdx.x * share, all), f1 = min(f0 + share, all), tiles = f1 - f0;
+  const int all = (int)(total & PLACES), share = max(1, (int)((uint32_t)(all + (int)gridDim.x - 1) / gridDim.x));
+  const int f0 = min((int)blockIdx.x * share, all), f1 = min(f0 + share, all);
   const bool much = by_unit && (int)(total >> 40) > entries;         // segments of more rows than the caller said: nothing is written
   if (by_unit) {
     if (blockIdx.x == 0)
@@ -285,17 +328,21 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
 #pragma unroll 1
     for (int seg = lane; seg < g.nseg; seg += 32)
       if (g.nrows[seg] > 0 && (long)g.kvlen[g.row0[seg] + g.nrows[seg] - 1] > g.limit) set_status(status, ST_BOUNDS);
-  if (tiles == 0 || much) {                                          // the same for the whole CTA
+  if (f0 == f1 || much) {                                          // the same for the whole CTA
     if (tid == 0 && much) set_status(status, ST_CAPACITY);
     if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);
     return;
   }
-  int unit = 0;
-  {
+  // Where the share starts, and how many tiles it has: its places without those that a prompt's units count beside their tiles, of which `gone` lie ahead of
+  // a place (of f1 first, then of f0, where the walk stays)
+  int unit = 0, gone1 = 0, gone = 0;
+#pragma unroll 1
+  for (int f = prompts ? f1 : f0;; f = f0) {
     long long done = 0;
+    gone = 0;
 #pragma unroll 1
     for (int seg0 = 0; seg0 < g.nseg; seg0 += 32) {
-      if (g.nseg > 32) mine = count(seg0 + lane);
+      if (g.nseg > 32 || prompts) mine = count(seg0);
       long long end = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -303,20 +350,43 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         if (lane >= o) end += v;
       }
       end += done;
-      const uint32_t hit = __ballot_sync(0xffffffffu, f0 < (int)(end & TILES));
+      const uint32_t hit = __ballot_sync(0xffffffffu, f < (int)(end & PLACES));
+      const int from = hit ? __ffs(hit) - 1 : 32;
+      if (prompts) gone += __reduce_add_sync(0xffffffffu, lane < from && w.extra ? (int)(mine >> 40) : 0);
       if (hit) {
-        const int from = __ffs(hit) - 1;
         auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
-        const int at = of(f0 - (int)(end - mine & TILES));
+        int at = of(f - (int)(end - mine & PLACES));
         unit = of((int)(end - mine >> 40));
         w.s = seg0 + from; w.units = of(w.units); w.nt = of(w.nt); w.kv = of(w.kv); w.row0 = of(w.row0); w.nrows = of(w.nrows); w.slot = of(w.slot);
-        w.u = (int)((uint32_t)at / (uint32_t)w.nt);
-        w.t = at - w.u * w.nt;
+        w.left = of(w.left); w.extra = of(w.extra);
+#pragma unroll 1
+        while (w.left > 0 && at >= w.units * (w.nt + 1)) {
+          at -= w.units * (w.nt + 1);
+          unit += w.units;
+          gone += w.units;
+          w.next_block<N>(g);
+        }
+        w.u = (int)((uint32_t)at / (uint32_t)(w.nt + w.extra));
+        w.t = at - w.u * (w.nt + w.extra);
         unit += w.u;
+        if (w.extra) gone += w.u;
         break;
       }
       done = __shfl_sync(0xffffffffu, end, 31);
     }
+    if (f == f0) break;
+    gone1 = gone;
+  }
+  int flat = f0;
+  if (w.t == w.nt) {                                                 // (a place that is no tile)
+    w.next_unit<N>(g);
+    ++unit;
+    ++flat;
+  }
+  const int tiles = prompts ? f1 - f0 - (gone1 - gone) : f1 - f0;
+  if (tiles <= 0) {                                                  // the same for the whole CTA
+    if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);
+    return;
   }
 
   // Queries of the walk's unit -> shared memory, and what belongs to each pair. Eight lanes have a pair; a thread turns the 16-byte pieces that it copied
@@ -496,12 +566,12 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     const uint32_t lanes = (uint32_t)(quad * 32) << 16, ts = tmem + lanes + NP * N + hc * CW, to = tmem + lanes + hc * CW;
     auto fmx = [](float a, float b) { return fmaxf(a, b); };
     auto fad = [](float a, float b) { return a + b; };
-    int i = 0, flat = f0;
+    int i = 0;
     bool broke = false;
     la_wait(qfull, 0, abort_flag);                                   // what came with the first piece's queries (if they don't come, no score does either)
     // once round per piece: its tiles, the next one's queries (no score needs this one's any more), its end
     for (int piece = 1;; ++piece) {
-      const int par = piece & 1, t0 = w.t, nt = w.nt, np = pairs_of(w), n = min(nt - t0, tiles - i);
+      const int par = piece & 1, t0 = w.t, nt = w.nt, np = pairs_of(w), n = min(nt - t0, tiles - i), places = n + (t0 + n == nt ? w.extra : 0);
       const size_t base = (size_t)w.row0 * g.nq + (size_t)w.u * N;
       uint64_t sum[CW / 2];
       {
@@ -655,7 +725,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       if (st == 0 && t0 == 0 && (by_unit || !whole))
         join[by_unit ? unit : (int)blockIdx.x] = make_int4((int)base, whole ? 0 : np, rec, (int)((uint32_t)(flat + nt - 1) / (uint32_t)share));
       if (t0 + n == nt) ++unit;
-      flat += n;
+      flat += places;
       softmax_sync();
       tc_fence_after();
 #pragma unroll 1

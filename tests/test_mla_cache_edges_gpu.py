@@ -1,4 +1,6 @@
 """Latents in 4 and 8 bits where steps, pages and values go to their limits."""
+import dataclasses
+
 import latent_rows as lr
 import pytest
 import torch
@@ -98,3 +100,63 @@ def test_prep_takes_eps_in_64_bits(ops, bits):
     want = mla_cache.quantised(lr.normed(kva, w, L, eps), bits).cpu()
     assert want[0, 1 if bits == 4 else 2] == (3.0 if bits == 4 else 15 / 64)
     assert torch.equal(lr.unpack(cache[0, :1], L, bits)[:, :L], want)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_of_a_prompt_walk_tiles_of_their_own_contexts(ops, bits):
+    """A causal segment of 140 rows, 64 heads: a unit is a row, and walks as many tiles as the last row of its 64 sees. The CTAs share the tiles, and a place
+    more for each unit, evenly. What the kernel leaves for the join says in which CTA each unit starts and ends."""
+    g = gen("units", bits)
+    L, nq, page, rows, ctas = 64, 64, 64, 140, ops.sm_count
+    assert rows <= ctas
+    table, pages = tables([128 * rows], page, g)
+    cache = random_cache(bits, L, pages, page, g)
+    kvlen = [128 * (r + 1) for r in range(rows)]
+    q, out = bf(g, rows, nq, L + R), torch.empty(rows, nq, L, dtype=torch.bfloat16, device=DEV)
+    segs = (i32([0]), i32([0]), i32([rows]), rows)
+    ws = torch.zeros(ops.C.mla_attn_q_floats(rows, nq, L, ctas), device=DEV)
+    ops.C.mla_attn_q(out, ws, q, cache, *segs, i32(kvlen), table, page, L, R, bits, 0.1, ctas, ops.status_word)
+    jobs = ws[:4 * rows].view(torch.int32).view(rows, 4).cpu()
+    own = [min(rows, r // 64 * 64 + 64) for r in range(rows)]              # tiles of a row's unit
+    start = [sum(n + 1 for n in own[:r]) for r in range(rows)]
+    share = -(-(start[-1] + own[-1] + 1) // ctas)
+    assert jobs[:, 0].tolist() == [r * nq for r in range(rows)]
+    assert (jobs[:, 2] // 2).tolist() == [s // share for s in start]
+    assert jobs[:, 3].tolist() == [(s + n - 1) // share for s, n in zip(start, own)]
+    assert torch.equal(out, check_attention(ops, bits, L, nq, page, [0] * rows, kvlen, table, cache, q, 0.1, segs))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nq", [128, 16, 3, 1])
+@pytest.mark.parametrize("width", [0, 300])
+def test_attention_of_prompts_on_small_pages(ops, bits, nq, width):
+    """Causal segments of hundreds of rows beside short ones and single rows, on pages of 24 tokens."""
+    g = gen("prompts", bits, nq, width)
+    lens, nrows, L = [700, 90, 333, 0, 20, 512], [400, 1, 333, 0, 5, 40], 64
+    table, pages = tables(lens, 24, g, width=width)
+    cache = random_cache(bits, L, pages, 24, g)
+    slot = [s for s, r in enumerate(nrows) for _ in range(r)]
+    kvlen = [lens[s] - r + 1 + i for s, r in enumerate(nrows) for i in range(r)]
+    row0 = [sum(nrows[:s]) for s in range(len(nrows))]
+    check_attention(ops, bits, L, nq, 24, slot, kvlen, table, cache, bf(g, len(slot), nq, L + R), (L + R) ** -0.5,
+                    (i32(list(range(len(nrows)))), i32(row0), i32(nrows), max(nrows)))
+
+
+@pytest.mark.parametrize("latent", [64, 512])
+@pytest.mark.parametrize("kv", ["int4", "fp8"])
+def test_engine_prompts_on_small_pages(ext, kv, latent):
+    """Pages of 16 tokens: prompts take the absorbed form, causal rows over codes; against the CPU engine over the same format, as near as the expanded
+    form on pages of 64 has to be."""
+    from ferrite_b200.config import EngineConfig, tiny_mla
+    from ferrite_b200.engine.engine import Engine
+    from ferrite_b200.engine.executor import Segment
+    from ferrite_b200.models.weights import init_weights
+    cfg = dataclasses.replace(tiny_mla(), kv_lora=latent)
+    w = init_weights(cfg, seed=0)
+    p = torch.randint(0, cfg.vocab, (200,), generator=torch.Generator().manual_seed(4)).tolist()
+    want = Engine(cfg, w, EngineConfig(n_slots=1, max_ctx=256, kv_dtype=kv), device="cpu").forward([Segment(0, 0, p, "all")])[0]
+    eng = Engine(cfg, w, EngineConfig(n_slots=1, max_ctx=256, kv_dtype=kv, kv_block=16), device=DEV)
+    got = torch.cat([eng.forward([Segment(0, 0, p[:150], "all")])[0].clone(), eng.forward([Segment(0, 150, p[150:], "all")])[0].clone()]).float().cpu()
+    eng.check()
+    kl = torch.nn.functional.kl_div(torch.log_softmax(got, -1), torch.log_softmax(want, -1), log_target=True, reduction="batchmean").item()
+    assert kl < (8e-2 if kv == "int4" else 3e-2), kl
