@@ -188,7 +188,7 @@ int fb_mla_prep_q(void* cache, long pages, int bits, void* qabs, const void* kva
                   int dn, int L, int R, double eps, int* status, cudaStream_t s);
 int fb_mla_rows(void* out, long rows, const void* cache, long pages, int bits, const int* seg_slot, const int* seg_pos0, const int* seg_nrows, int nseg,
                 const int* block_table, int max_blocks, int kv_block, int L, int R, int whole, int align, int* status, cudaStream_t s);
-// attention of segments' rows; ws: as many 32-bit words as fb_mla_attn_q_floats says for the most rows of a segment; row_kvlen does not fall along a segment
+// attention of segments' rows; ws: as many 32-bit words as fb_mla_attn_q_floats says for the most rows of a segment
 long fb_mla_attn_q_floats(int max_rows, int nq, int L, int ctas);
 int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* qabs, const void* cache, long pages, int bits, const int* seg_slot,
                   const int* seg_row0, const int* seg_nrows, int nseg, int max_rows, const int* row_kvlen, const int* block_table, int max_blocks,

@@ -86,20 +86,34 @@ struct LatentSegs {
 // units are short (without it the CTA that has those is the last by far: 2354 us).
 struct LatentWalk {
   int s, u, t, units, nt, kv, row0, nrows, slot, left, extra;
-  template <int N>
+  bool over = false;                             // a row that sees more than the table has room for has come by
+  // rows of a block may stand in any order: it is as long as the longest of their contexts, which a warp looks for, or (APART) a lane for itself
+  template <int N, bool APART = false>
   __device__ __forceinline__ void block(const LatentSegs& g) {
-    kv = nrows > 0 ? (int)min((long)max(g.kvlen[row0 + nrows - 1], 0), g.limit) : 0;
+    int most = 0;
+    if constexpr (APART) {
+#pragma unroll 4
+      for (int r = 0; r < nrows; ++r) most = max(most, g.kvlen[row0 + r]);
+    } else {
+      const int lane = threadIdx.x & 31;
+      static_assert(LA_ROWS == 64, "two rows a lane");
+      if (lane < nrows) most = max(most, g.kvlen[row0 + lane]);
+      if (lane + 32 < nrows) most = max(most, g.kvlen[row0 + 32 + lane]);
+      most = __reduce_max_sync(0xffffffffu, most);
+    }
+    over |= most > g.limit;
+    kv = (int)min((long)most, g.limit);
     units = (int)(((uint32_t)nrows * g.nq + N - 1) / N);               // (rows times heads are fewer than 2^30; those of a whole block fill its units)
     nt = max(1, (kv + LA_KT - 1) / LA_KT);
   }
-  template <int N>
+  template <int N, bool APART = false>
   __device__ __forceinline__ void segment(const LatentSegs& g) {
     const int n = max(g.nrows[s], 0);
     row0 = g.row0[s]; slot = g.slot[s];
     nrows = min(n, LA_ROWS);
     left = n - nrows;
     extra = left > 0;
-    block<N>(g);
+    block<N, APART>(g);
   }
   template <int N>
   __device__ __forceinline__ void next_block(const LatentSegs& g) {
@@ -283,21 +297,21 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   // ---- this CTA's share of the list, by every warp for itself (no barrier stands between the lengths and a role's first load): sums over the segments, a
   // lane each (a prompt's further blocks by the whole warp), of their places (low 40 bits) and units (the rest)
   constexpr long long PLACES = (1ll << 40) - 1;
-  LatentWalk w;
+  LatentWalk c;                                                      // a lane's segment, at its first block
   bool prompts = false;
-  auto count = [&](int seg0) -> long long {                          // of segment seg0 + lane, at whose first block the lane's walk is then
-    w.units = w.nrows = w.nt = w.left = w.extra = 0;
+  auto count = [&](int seg0) -> long long {                          // of segment seg0 + lane, where the lane's walk is then
+    c.units = c.nrows = c.nt = c.left = c.extra = 0;
     if (seg0 + lane < g.nseg) {
-      w.s = seg0 + lane;
-      w.segment<N>(g);
+      c.s = seg0 + lane;
+      c.segment<N, true>(g);
     }
-    long long sum = (long long)w.units * (w.nt + w.extra) + ((long long)w.units << 40);
+    long long sum = (long long)c.units * (c.nt + c.extra) + ((long long)c.units << 40);
 #pragma unroll 1
-    for (uint32_t more = __ballot_sync(0xffffffffu, w.left > 0); more; more &= more - 1) {
+    for (uint32_t more = __ballot_sync(0xffffffffu, c.left > 0); more; more &= more - 1) {
       const int from = __ffs(more) - 1;
       LatentWalk x;
-      x.row0 = __shfl_sync(0xffffffffu, w.row0, from);
-      x.left = __shfl_sync(0xffffffffu, w.left, from);
+      x.row0 = __shfl_sync(0xffffffffu, c.row0, from);
+      x.left = __shfl_sync(0xffffffffu, c.left, from);
       long long rest = 0;
 #pragma unroll 1
       while (x.left > 0) {
@@ -305,6 +319,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
         rest += (long long)x.units * (x.nt + 1) + ((long long)x.units << 40);
       }
       if (lane == from) sum += rest;
+      c.over |= x.over;
       prompts = true;
     }
     return sum;
@@ -324,10 +339,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   } else if (tid == LA_UNPACK * 32) {                                // (the thread that may write another one there)
     join[blockIdx.x] = make_int4(0, 0, 0, 0);
   }
-  if (blockIdx.x == 0 && warp == 0)
-#pragma unroll 1
-    for (int seg = lane; seg < g.nseg; seg += 32)
-      if (g.nrows[seg] > 0 && (long)g.kvlen[g.row0[seg] + g.nrows[seg] - 1] > g.limit) set_status(status, ST_BOUNDS);
+  if (blockIdx.x == 0 && warp == 0 && c.over) set_status(status, ST_BOUNDS);
   if (f0 == f1 || much) {                                          // the same for the whole CTA
     if (tid == 0 && much) set_status(status, ST_CAPACITY);
     if (warp == LA_SOFT) tmem_dealloc(tmem, C::TMEM);
@@ -335,6 +347,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
   }
   // Where the share starts, and how many tiles it has: its places without those that a prompt's units count beside their tiles, of which `gone` lie ahead of
   // a place (of f1 first, then of f0, where the walk stays)
+  LatentWalk w;
   int unit = 0, gone1 = 0, gone = 0;
 #pragma unroll 1
   for (int f = prompts ? f1 : f0;; f = f0) {
@@ -342,7 +355,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
     gone = 0;
 #pragma unroll 1
     for (int seg0 = 0; seg0 < g.nseg; seg0 += 32) {
-      if (g.nseg > 32 || prompts) mine = count(seg0);
+      if (g.nseg > 32) mine = count(seg0);
       long long end = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -352,13 +365,13 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       end += done;
       const uint32_t hit = __ballot_sync(0xffffffffu, f < (int)(end & PLACES));
       const int from = hit ? __ffs(hit) - 1 : 32;
-      if (prompts) gone += __reduce_add_sync(0xffffffffu, lane < from && w.extra ? (int)(mine >> 40) : 0);
+      if (prompts) gone += __reduce_add_sync(0xffffffffu, lane < from && c.extra ? (int)(mine >> 40) : 0);
       if (hit) {
         auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, from); };
         int at = of(f - (int)(end - mine & PLACES));
         unit = of((int)(end - mine >> 40));
-        w.s = seg0 + from; w.units = of(w.units); w.nt = of(w.nt); w.kv = of(w.kv); w.row0 = of(w.row0); w.nrows = of(w.nrows); w.slot = of(w.slot);
-        w.left = of(w.left); w.extra = of(w.extra);
+        w.s = seg0 + from; w.units = of(c.units); w.nt = of(c.nt); w.kv = of(c.kv); w.row0 = of(c.row0); w.nrows = of(c.nrows); w.slot = of(c.slot);
+        w.left = of(c.left); w.extra = of(c.extra);
 #pragma unroll 1
         while (w.left > 0 && at >= w.units * (w.nt + 1)) {
           at -= w.units * (w.nt + 1);
@@ -576,7 +589,7 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       uint64_t sum[CW / 2];
       {
         softmax_sync();                                              // what came with later pieces' queries, from these warps
-        const int least = ms.see[par][0];                            // rows of a segment see no fewer keys than those ahead of them
+        const int least = __reduce_min_sync(0xffffffffu, min(ms.see[par][lane % N], ms.see[par][(lane + 32) % N]));      // keys that all pairs see
 #pragma unroll
         for (int e = 0; e < CW / 2; ++e) sum[e] = f2_pack(0.f, 0.f);
 #pragma unroll 1
@@ -946,7 +959,7 @@ extern "C" long fb_mla_attn_q_floats(int max_rows, int nq, int L, int ctas) {
   return 4l * ctas + 2l * ctas * N * (L + 2);
 }
 
-// ws: fb_mla_attn_q_floats of 32 bits; row_kvlen does not fall along a segment
+// ws: fb_mla_attn_q_floats of 32 bits
 extern "C" int fb_mla_attn_q(void* out, float* ws, long ws_floats, const void* qabs, const void* cache, long pages, int bits, const int* seg_slot,
                              const int* seg_row0, const int* seg_nrows, int nseg, int max_rows, const int* row_kvlen, const int* block_table,
                              int max_blocks, int kv_block, int rows, int nq, int L, int R, float scale, int ctas, int* status, cudaStream_t s) {

@@ -160,3 +160,33 @@ def test_engine_prompts_on_small_pages(ext, kv, latent):
     eng.check()
     kl = torch.nn.functional.kl_div(torch.log_softmax(got, -1), torch.log_softmax(want, -1), log_target=True, reduction="batchmean").item()
     assert kl < (8e-2 if kv == "int4" else 3e-2), kl
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("nq", [128, 16, 3])
+@pytest.mark.parametrize("width", [0, 300])
+@pytest.mark.parametrize("rows", [17, 150])
+def test_rows_of_a_segment_in_any_order(ops, bits, nq, width, rows):
+    """Contexts that fall along a segment, or come in no order, some of them empty."""
+    g = gen("order", bits, nq, width, rows)
+    lens, L = [700, 300, 130], 512 if rows == 17 else 64
+    table, pages = tables(lens, 64, g, width=width)
+    cache = random_cache(bits, L, pages, 64, g)
+    slot = [s for s in range(3) for _ in range(rows)]
+    kvlen = [700 - 600 * r // rows for r in range(rows)]
+    kvlen += torch.randint(0, 301, (rows,), generator=torch.Generator().manual_seed(nq)).tolist()
+    kvlen += [130 if r % 3 == 1 else 0 if r % 3 == 0 else 129 for r in range(rows)]
+    check_attention(ops, bits, L, nq, 64, slot, kvlen, table, cache, bf(g, 3 * rows, nq, L + R), 0.05, segments(rows, 3))
+
+
+@pytest.mark.parametrize("rows", [3, 90])
+@pytest.mark.parametrize("at", [0, 1, -1])
+def test_any_row_that_sees_past_the_table_sets_the_status(ops, rows, at):
+    g = gen("past", rows, at)
+    table, pages = tables([128], 64, g)
+    cache = random_cache(4, 64, pages, 64, g)
+    kvlen = [100] * rows
+    kvlen[at] = 200
+    ops.mla_attention(bf(g, rows, 4, 64 + R), cache, i32([0] * rows), i32(kvlen), table, 64, 4, 64, R, 0.05, segs=segments(rows, 1), kv_bits=4)
+    assert ops.status() == 3
+    ops.status_word.zero_()
