@@ -20,7 +20,10 @@
 //
 // Work is cut evenly, not by row: the tiles of all (segment, group of N pairs) units form one list, every CTA takes the same number of consecutive
 // ones, from what the lengths on the device say (so a captured call follows its contexts). Units that span CTAs leave their sums in 32 bits,
-// and a second kernel joins them in order. A row's bits therefore depend on what else is in the step, and on nothing else.
+// and a second kernel joins them in order. Where a row's keys are cut, and so how its sums round, therefore follows the other rows of the step, the
+// number of SMs, and N: the most rows of a segment, the heads, and the keys that the block table has room for. The same call gives the same bits. (Cuts
+// that follow a row's own context alone, as in the 16-bit cache, have to be fine enough for one stream on all SMs, and then leave 32-bit sums of 2 KB a
+// head for every few tiles of a loaded step.)
 //
 // A key of which a group is no number gets the score NaN and a finite place in the tile, so that rows ahead of it, whose weight for it is zero, stay clean.
 //

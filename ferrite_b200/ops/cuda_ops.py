@@ -814,8 +814,9 @@ class CudaOps(CudaLatent, CudaMixers, CudaExtras):
         64-key tiles the tensor-core kernel of the listed models runs, heads of a row sharing every pass over the latents. Rows of segments of
         up to 32 rows share nothing and, with `picked` splits (see `attention`), are split by their own context: a row has the same bits
         decoded, verified and among other streams. Callers without segment tables and other page sizes take the CUDA-core kernel.
-        `kv_bits` 4 or 8: the cache holds rows of codes (`mla_prep`); L is 64, 128, 256 or 512, a segment's rows stand in any order, and a row's bits
-        depend on what else is in the step, which the tiles are shared out over."""
+        `kv_bits` 4 or 8: the cache holds rows of codes (`mla_prep`); L is 64, 128, 256 or 512 and a segment's rows stand in any order. `nsplit` and
+        `picked` say nothing there: the tiles of the step are shared out evenly, so a row may round differently (by less than the result's bf16
+        rounding and that of weights of 11 bits) decoded, verified, beside other streams and under another `max_ctx`; the same call gives the same bits."""
         T = qabs.shape[0]
         if kv_bits != 16:
             if segs is None:                              # every row a segment of its own

@@ -190,3 +190,81 @@ def test_any_row_that_sees_past_the_table_sets_the_status(ops, rows, at):
     ops.mla_attention(bf(g, rows, 4, 64 + R), cache, i32([0] * rows), i32(kvlen), table, 64, 4, 64, R, 0.05, segs=segments(rows, 1), kv_bits=4)
     assert ops.status() == 3
     ops.status_word.zero_()
+
+
+def bounds(bits, L, page, slot, kvlen, table, cache, q, scale):
+    """How far `check_attention` lets every output be from 64 bits."""
+    vals = lr.unpack(cache.view(-1, cache.shape[-1]), L, bits).to(DEV)
+    out = []
+    for r, (s, n) in enumerate(zip(slot, kvlen)):
+        p = torch.arange(n, device=DEV)
+        keys, qr = vals[table[s, p // page].long() * page + p % page], q[r].double()
+        w = torch.softmax(qr @ keys.t() * scale, -1)
+        ds = (qr.abs() @ keys.abs().t() * scale).amax(-1, keepdim=True) * (L + R) / 16 * 2 ** -23
+        out.append(2 ** -8 * (w @ keys[:, :L]).abs() + (w @ keys[:, :L].abs()) * (2 ** -11 + 2 * ds) + 1e-30)
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("L,nq", [(512, 128), (512, 16), (64, 4)])
+@pytest.mark.parametrize("first", [30, 2040])
+def test_how_far_a_row_moves_from_step_to_step(ops, bits, L, nq, first):
+    """A row decoded alone, verified among seventeen and beside other streams: its keys are cut at other places, so it may round differently. Each is within
+    `check_attention`'s distance of 64 bits, so two of them are within twice that of each other; the same step again gives the same bits."""
+    g = gen("moves", bits, L, nq, first)
+    rows, lens, page = 17, [first + 17, 60, 5000], 64
+    table, pages = tables(lens, page, g)
+    cache = random_cache(bits, L, pages, page, g)
+    q, scale = bf(g, rows + 2, nq, L + R), (L + R) ** -0.5
+
+    def step(parts):                                         # (stream, first row, rows) of each segment
+        at = [r for _, r, n in parts for r in range(r, r + n)]
+        own = [first + 1 + r if s == 0 else lens[s] for s, a, n in parts for r in range(a, a + n)]
+        slot, row0 = [s for s, _, n in parts for _ in range(n)], [sum(n for _, _, n in parts[:i]) for i in range(len(parts))]
+        segs = (i32([s for s, _, _ in parts]), i32(row0), i32([n for _, _, n in parts]), max(n for _, _, n in parts))
+        got = check_attention(ops, bits, L, nq, page, slot, own, table, cache, q[at], scale, segs)
+        again = ops.mla_attention(q[at], cache, i32(slot), i32(own), table, page, nq, L, R, scale, segs=segs, kv_bits=bits)
+        assert torch.equal(got, again)
+        return got.double()
+
+    tol = 2 * bounds(bits, L, page, [0] * rows + [1, 2], list(range(first + 1, first + rows + 1)) + lens[1:], table, cache, q, scale)
+    whole = step([(0, 0, rows)])
+    beside = step([(1, rows, 1), (0, 0, rows), (2, rows + 1, 1)])
+    assert ((beside[1:1 + rows] - whole).abs() <= tol[:rows]).all()
+    for r in (0, 8, 16):
+        assert ((step([(0, r, 1)])[0] - whole[r]).abs() <= tol[r]).all()
+    assert ((step([(1, rows, 1)])[0] - beside[0]).abs() <= tol[rows]).all() and ((step([(2, rows + 1, 1)])[0] - beside[-1]).abs() <= tol[rows + 1]).all()
+
+
+@pytest.mark.parametrize("latent", [64, 512])
+@pytest.mark.parametrize("kv", ["int4", "fp8"])
+def test_engine_row_alone_beside_others_and_verified(ext, kv, latent):
+    """A token behind the same context, decoded alone, beside other streams and as the first of verified rows, and the rows behind it against decoding
+    them one by one. Only the step's own rows can differ (bf16 roundings of its products, its cuts of the keys, its own latents' codes next to a border):
+    less than what holding ALL latents of the context in codes instead of 16 bits changes."""
+    from ferrite_b200.config import EngineConfig, tiny_mla
+    from ferrite_b200.engine.engine import Engine
+    from ferrite_b200.engine.executor import Segment
+    from ferrite_b200.models.weights import init_weights
+    cfg = dataclasses.replace(tiny_mla(moe=False), kv_lora=latent)
+    w = init_weights(cfg, seed=0)
+    g = torch.Generator().manual_seed(3)
+    p, other, new = (torch.randint(0, cfg.vocab, (n,), generator=g).tolist() for n in (300, 60, 5))
+
+    def run(kv):
+        eng = Engine(cfg, w, EngineConfig(n_slots=5, max_ctx=512, kv_dtype=kv), device=DEV)
+        eng.forward([Segment(0, 0, p, "none")])
+        eng.forward([Segment(4, 0, other, "none")])
+        for s in (1, 2, 3):
+            eng.ex.copy_slot(0, s, len(p))
+        alone = torch.cat([eng.forward([Segment(1, 300 + i, [t], "last")])[0].clone() for i, t in enumerate(new)])
+        beside = eng.forward([Segment(4, 60, [7], "last"), Segment(2, 300, [new[0]], "last"), Segment(0, 300, [9], "last")])[0].clone()
+        verified = eng.forward([Segment(3, 300, new, "all")], commit=False)[0].clone()
+        eng.check()
+        return alone.double(), beside[1].double(), verified.double()
+
+    alone, beside, verified = run(kv)
+    format_moves = (alone - run("bf16")[0]).norm(dim=1)
+    assert (format_moves > 0).all()
+    assert (beside - alone[0]).norm() <= format_moves[0]
+    assert ((verified - alone).norm(dim=1) <= format_moves).all()
