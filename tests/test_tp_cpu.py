@@ -98,6 +98,49 @@ def test_moe_latent_attention_model_under_tp2(plen):
     assert torch.equal(outs[0][1], outs[1][1]) and torch.equal(outs[0][3], outs[1][3])
 
 
+def _quantised_worker(rank, world, port, prompt, q, kv):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world, timeout=datetime.timedelta(seconds=60))
+    from ferrite_b200.parallel.tp import TensorParallel
+    cfg = PRESETS["tiny-mla"]()
+    eng = Engine(cfg, init_weights(cfg, seed=0), EngineConfig(n_slots=1, max_ctx=128, kv_dtype=kv), device="cpu",
+                 tp=TensorParallel(dist.group.WORLD, "cpu", fused=False))
+    logits = eng.forward([Segment(0, 0, prompt, "all")])[0]
+    l2 = eng.forward([Segment(0, len(prompt), [7], "last")])[0]
+    q.put((rank, logits.numpy(), l2.numpy(), eng.ex.k_cache[0].numpy()))
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("kv", ["int4", "fp8"])
+def test_quantised_latents_under_tp2(kv):
+    """Latents in codes on two gloo ranks, each with half of the heads: both hold the same cache and logits, bit for bit, and give the single-rank logits up
+    to values that a sum over the ranks puts on the other side of a code's border, which move logits by less than the format itself does."""
+    cfg = PRESETS["tiny-mla"]()
+    w = init_weights(cfg, seed=0)
+    prompt = torch.randint(0, cfg.vocab, (24,), generator=torch.Generator().manual_seed(6)).tolist()
+
+    def alone(kv):
+        eng = Engine(cfg, w, EngineConfig(n_slots=1, max_ctx=128, kv_dtype=kv), device="cpu")
+        return (eng.forward([Segment(0, 0, prompt, "all")])[0], eng.forward([Segment(0, len(prompt), [7], "last")])[0])
+
+    want, plain = alone(kv), alone("bf16")
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    procs = [ctx.Process(target=_quantised_worker, args=(r, 2, port, prompt, q, kv)) for r in range(2)]
+    for p in procs:
+        p.start()
+    outs = gather(q, 2)
+    for p in procs:
+        p.join(timeout=60)
+    for rank, logits, l2, cache in outs:
+        assert cache.any()
+        for got, own, other in ((logits, want[0], plain[0]), (l2, want[1], plain[1])):
+            assert 0 < (own - other).norm() and (got - own).norm() < 0.5 * (own - other).norm(), rank
+    assert all(torch.equal(a, b) for a, b in zip(outs[0][1:], outs[1][1:]))
+
+
 def _lonely(rank, world, port, q):
     os.environ["MASTER_ADDR"] = "127.0.0.1"
     os.environ["MASTER_PORT"] = str(port)
