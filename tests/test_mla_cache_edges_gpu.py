@@ -268,3 +268,21 @@ def test_engine_row_alone_beside_others_and_verified(ext, kv, latent):
     assert (format_moves > 0).all()
     assert (beside - alone[0]).norm() <= format_moves[0]
     assert ((verified - alone).norm(dim=1) <= format_moves).all()
+
+
+@pytest.mark.parametrize("ctas", [1, 7, 61, 148])
+@pytest.mark.parametrize("nq,n", [(16, 9), (3, 45), (40, 45)])
+def test_prompts_and_single_rows_cut_anywhere(ops, nq, n, ctas, monkeypatch):
+    """Prompts of up to 200 rows among single and verified rows, more segments than a warp has lanes, shared out over few CTAs and many."""
+    g = gen("cut", nq, n)
+    L, page = 64, 24
+    nrows = [0 if i % 7 == 3 else 65 + 27 * (i % 6) if i % 4 == 1 else 1 + i % 5 for i in range(n)]
+    lens = [r + (i * 53) % 150 for i, r in enumerate(nrows)]
+    table, pages = tables(lens, page, g, width=11 * (nq == 16))
+    cache = random_cache(4, L, pages, page, g)
+    slot = [s for s, r in enumerate(nrows) for _ in range(r)]
+    kvlen = [lens[s] - r + 1 + i for s, r in enumerate(nrows) for i in range(r)]
+    row0 = [sum(nrows[:s]) for s in range(n)]
+    monkeypatch.setattr(ops, "sm_count", ctas)
+    check_attention(ops, 4, L, nq, page, slot, kvlen, table, cache, bf(g, len(slot), nq, L + R), (L + R) ** -0.5,
+                    (i32(list(range(n))), i32(row0), i32(nrows), max(nrows)))
