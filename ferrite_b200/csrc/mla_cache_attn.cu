@@ -75,6 +75,7 @@ struct LatentAttnMisc {
   int rows[LA_AHEAD][LA_KT];                     // ring of tiles: their keys' rows of the cache, -1 where there is none
   uint64_t bars[2 * 5 + 7 + 2 * LA_AHEAD];
   uint32_t tmem;
+  int least[8];                                  // of the piece: keys that all pairs of a softmax warp see
   int abort, fail;
 };
 
@@ -592,7 +593,9 @@ mla_attn_q_kernel(__nv_bfloat16* __restrict__ out, float* __restrict__ o_part, f
       uint64_t sum[CW / 2];
       {
         softmax_sync();                                              // what came with later pieces' queries, from these warps
-        const int least = __reduce_min_sync(0xffffffffu, min(ms.see[par][lane % N], ms.see[par][(lane + 32) % N]));      // keys that all pairs see
+        if (const int m = __reduce_min_sync(0xffffffffu, ms.see[par][hc * CW + lane % CW]); lane == 0) ms.least[warp - LA_UNPACK] = m;
+        __syncwarp();
+        const int least = ms.least[warp - LA_UNPACK];                // (read where it is needed: a register more, and eight-bit variants spill 300 bytes)
 #pragma unroll
         for (int e = 0; e < CW / 2; ++e) sum[e] = f2_pack(0.f, 0.f);
 #pragma unroll 1
