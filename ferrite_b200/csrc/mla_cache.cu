@@ -30,7 +30,9 @@ constexpr int LP_ROWS = 8, LP_HEADS = 128;             // cache rows, heads of a
 // grid ceil(rows / LP_ROWS) + rows * kinds, kinds: groups of LP_HEADS heads, 256 threads. The first CTAs write cache rows, a warp each: 16 values a lane (the
 // 64-bit square root and quotients of a row are then worked out once, not by eight warps: 2048 rows 36 -> 25 us with their reading back). The others turn
 // the heads' query parts of a row, four pairs a thread (8-byte accesses), whose angles serve all of its heads (groups of 32 heads: 34 us); queries are on
-// their way before the position is known. Bound by the queries' bytes: 67 MB, 10 us, of 19.
+// their way before the position is known. 2048 rows of 128 heads take 15 us by the profiler's clock (17 captured, cold caches) where the queries' 67 MB are 10
+// at the copy rate. It is not the bytes (DRAM 32 % busy) but the chain of a row's CTA, four a SM and four waves of them: of a warp's 12.9 cycles between
+// instructions 3.9 go to the barrier behind the 32 threads that turn the angles in 64 bits, 2.0 to loads; a quarter of the time SMs start or run dry.
 template <int BITS>
 __global__ void __launch_bounds__(256, 4) mla_prep_q_kernel(uint8_t* __restrict__ cache, __nv_bfloat16* __restrict__ qabs, const __nv_bfloat16* kva,
                                                          long kva_stride, const __nv_bfloat16* q, long q_stride,

@@ -30,9 +30,9 @@
 // What bounds it: the way to shared memory, 128 bytes a cycle. For a tile of 64 pairs the products read 36 * 6 KB (S) and 32 * 6 KB (O), 3260 cycles; stores
 // of the unpacked tile, codes that come in sectors of 32 bytes, key parts and scores take 4300 more (the counters' wavefronts): 7560 of the tile's
 // 8700. During the softmax's 2000 no product runs: the tile has to stay and none of the next has room (128 KB of tile, 72 KB of queries). 16 pairs: 6200
-// cycles a tile. Measured, 512 values in 4 bits, cold caches: 24 streams of up to 16000 keys with 128 heads 161 us (43: the products at the card's rate),
-// 32 with 16 heads 87 us (22: the bytes), one of 100000 with 128 heads 93 us (17), one of 2048 25 us: 13 here, of which 7 until the first scores (code
-// that is new to every SM comes slowly), 6 in the join, the rest between launches.
+// cycles a tile. Measured, 512 values in 4 bits, captured, cold caches: 24 streams of up to 16000 keys with 128 heads 154 us (43: the products at the card's
+// rate), 32 with 16 heads 82 us (22: the bytes), one of 100000 with 128 heads 89 us (17), one of 2048 21 to 25 us by the table's room (latent_pairs): 13 here,
+// of which 7 until the first scores (code that is new to every SM comes slowly), 6 in the join, the rest between launches.
 // Tried and slower: tiles of 64 keys in two places (S costs 65 cycles where 48 do for 128 keys), tiles in tensor memory for S, unpacking by two groups
 // of warps in turn (32 streams of 16 heads 87 -> 93 us), the softmax in halves with the next one's load under
 // way (registers: 161 -> 171 us), rows brought to L2 ahead one by one (114 us; a page's in one request costs nothing).
@@ -953,7 +953,8 @@ using namespace fb;
 
 // Pairs of a unit: the fewest of 16, 32 and 64 that hold a segment's; more are several units (an unpacked tile serves as many as it can). Fewer where even
 // then every tile that the table has room for finds a CTA of its own: its products, its softmax and the sums that it leaves are shorter, and nobody
-// waits for the unpacking that is done again (one stream of 2048 with 128 heads: 25 us in units of 16, 27 of 64).
+// waits for the unpacking that is done again. It is the TABLE's room that counts, not the context, which only the device knows: one stream of 2048 with 128
+// heads takes 21.0 us in a table for no more (units of 16), 21.9 in one for 4096 tokens (32), 24.6 from 8192 on (64).
 static int latent_pairs(long pairs, long tiles, int ctas) {
   int N = 16;
   while (N < 64 && N < pairs && (pairs + N - 1) / N * tiles > ctas) N *= 2;
