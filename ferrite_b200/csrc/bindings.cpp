@@ -441,6 +441,7 @@ void kv_move_rows(Tensor k, c10::optional<Tensor> v, c10::optional<Tensor> sc, T
 
 void register_ext(pybind11::module_& m);
 void register_listed(pybind11::module_& m);
+void register_shared(pybind11::module_& m);
 void register_host(pybind11::module_& m);
 void register_oracle(pybind11::module_& m);
 void register_gguf_host(pybind11::module_& m);
@@ -497,6 +498,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_move_rows", &kv_move_rows);
   register_ext(m);
   register_listed(m);
+  register_shared(m);
   register_host(m);
   register_oracle(m);
   register_gguf_host(m);

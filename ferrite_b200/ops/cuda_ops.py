@@ -19,6 +19,7 @@ from .extras import CudaExtras
 from .latent import CudaLatent, SegGroup
 from .mixers import CudaMixers
 from .qweight import Exl3Weight, ExpertsFP4, GgufWeight, QWeight, StackWeight
+from .shared_kv import CudaShared
 
 GEMV_MAX_ROWS = 8
 MOE_PAIR_ROWS = 64     # up to this many rows (the largest graph-captured step) the experts run as per-pair GEMVs,
@@ -45,7 +46,7 @@ TAIL_STREAMS = 4       # streams that keep the scratch of a prompt GEMM's last t
 FP4_TC_UNITS = 2560
 
 
-class CudaOps(CudaLatent, CudaMixers, CudaExtras):
+class CudaOps(CudaLatent, CudaMixers, CudaExtras, CudaShared):
     name = "cuda"
 
     def __init__(self, device, dtype=torch.bfloat16):

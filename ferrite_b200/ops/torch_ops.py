@@ -16,13 +16,14 @@ from .extras import TorchExtras
 from .latent import TORCH_ACTS, TorchLatent
 from .mixers import TorchMixers
 from .mla_cache import quantised
+from .shared_kv import TorchShared
 
 
 def _softplus(x):
     return torch.where(x > 20, x, torch.log1p(torch.exp(torch.clamp(x, max=20.0))))
 
 
-class TorchOps(TorchLatent, TorchMixers, TorchExtras):
+class TorchOps(TorchLatent, TorchMixers, TorchExtras, TorchShared):
     name = "torch"
 
     def __init__(self, device="cpu", dtype=torch.float32):
