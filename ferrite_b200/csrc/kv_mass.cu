@@ -55,13 +55,16 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(float* out, const float* m
 
 using namespace fb;
 
-extern "C" long fb_attention_mass_floats(int rows, int, int, int, int nq, int, int) { return (long)rows * nq; }
+extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int ctas) {
+  return ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, 64, ctas, 0);
+}
 
 extern "C" int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride,
                                  const void* k, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
   if (st.rows <= 0 || st.nseg <= 0) return 0;
   if (!lse) {
-    const int rc = fb_attention_shared(nullptr, ws, nullptr, 0, q, q_stride, k, k, nullptr, 0, st, nq, nkv, hd, ctas, status, s);
+    const long used = ((long)st.rows * nq + 3) / 4 * 4;
+    const int rc = fb_attention_shared(nullptr, ws, ws + used, ws_floats - used, q, q_stride, k, k, nullptr, 0, st, nq, nkv, hd, ctas, status, s);
     if (rc) return rc;
     lse = ws;
   }

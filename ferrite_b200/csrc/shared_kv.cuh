@@ -1,11 +1,37 @@
-// A step over a paged cache whose streams may share pages: which slot a row's keys are read through.
+// A step over a paged cache whose streams may share pages, as lists of equal pieces of work: what a kernel needs to find its own piece from the lengths
+// on the device, so that a captured call follows its contexts.
+//
+// Spans: the shared tokens of a group, [0, len) through the table of its first segment, for the rows of all its segments; and what follows them of a segment,
+// [len, longest context) through its own table, for its own rows. A span's rows are cut into blocks of R (what fills the 128 rows of a product, share query
+// heads a row), and a (block, kv head) walks the key tiles of its span that one of its rows sees.
 #pragma once
 #include "api_shared.h"
 #include "common.cuh"
 
 namespace fb {
 
-// Row of the cache that holds token j of a slot, or -1 (with a status) where the table has none.
+constexpr int SK_SEGS = 4096;                    // segments, and groups, of a step
+constexpr int SK_BLOCKS = 12000;                 // blocks of a step
+constexpr int SK_PLAN_BYTES = (3 * SK_SEGS + 2 * SK_BLOCKS) * 4;   // shared memory that the plan takes while it is made
+
+// What a block is. kmin: keys that all of its rows see. tile0: key tiles of the blocks ahead of it (of one kv head).
+struct __align__(16) SharedBlock {
+  int row0, nrows, slot, k0;
+  int k1, kmin, tile0, nt;
+};
+
+__device__ __forceinline__ long table_limit(const FbSharedStep& st) { return (long)st.max_blocks * st.kv_block; }
+// Row of the cache where a tile's first token lies; one far outside (a load from there reads zeros) where the table has none.
+__device__ __forceinline__ int tile_row(const FbSharedStep& st, int slot, int token, int* status) {
+  const int blk = st.table[(size_t)slot * st.max_blocks + token / st.kv_block];
+  if (blk < 0 || blk >= st.pages) {
+    set_status(status, ST_BOUNDS);
+    return -1024;
+  }
+  return blk * st.kv_block + token % st.kv_block;
+}
+__device__ __forceinline__ bool rows_fit(const FbSharedStep& st, int row0, int nrows) { return row0 >= 0 && nrows >= 0 && nrows <= st.rows - row0; }
+
 __device__ __forceinline__ long cache_row(const FbSharedStep& st, int slot, int j, int* status) {
   const int blk = slot < 0 || slot >= st.slots || j / st.kv_block >= st.max_blocks ? -1 : st.table[(size_t)slot * st.max_blocks + j / st.kv_block];
   if (blk < 0 || blk >= st.pages) {
@@ -13,12 +39,6 @@ __device__ __forceinline__ long cache_row(const FbSharedStep& st, int slot, int 
     return -1;
   }
   return (long)blk * st.kv_block + j % st.kv_block;
-}
-// Segment of a row, or -1; group of a segment, or -1.
-__device__ __forceinline__ int segment_of_row(const FbSharedStep& st, int row) {
-  for (int s = 0; s < st.nseg; ++s)
-    if (row >= st.seg_row0[s] && row < st.seg_row0[s] + st.seg_nrows[s]) return s;
-  return -1;
 }
 __device__ __forceinline__ bool group_fits(const FbSharedStep& st, int g, int* status) {
   if (st.grp_seg0[g] >= 0 && st.grp_nsegs[g] >= 0 && st.grp_nsegs[g] <= st.nseg - st.grp_seg0[g]) return true;
@@ -29,6 +49,204 @@ __device__ __forceinline__ int group_of_segment(const FbSharedStep& st, int seg,
   for (int g = 0; g < st.ngrp; ++g)
     if (group_fits(st, g, status) && seg >= st.grp_seg0[g] && seg < st.grp_seg0[g] + st.grp_nsegs[g]) return g;
   return -1;
+}
+
+// a[0 .. n) -> sums of what lies ahead, in place; returns the sum of all. Every thread of the CTA calls it; tmp: a place for each warp and one more.
+template <int THREADS>
+__device__ __forceinline__ long long scan_ahead(int* a, int n, long long* tmp) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, per = (n + THREADS - 1) / THREADS;
+  const int lo = min(n, tid * per), hi = min(n, lo + per);
+  long long sum = 0;
+  for (int i = lo; i < hi; ++i) sum += a[i];
+  long long x = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) tmp[warp] = x;
+  __syncthreads();
+  if (tid == 0) {
+    long long all = 0;
+    for (int w = 0; w < THREADS / 32; ++w) {
+      const long long y = tmp[w];
+      tmp[w] = all;
+      all += y;
+    }
+    tmp[THREADS / 32] = all;
+  }
+  __syncthreads();
+  long long at = tmp[warp] + x - sum;
+  for (int i = lo; i < hi; ++i) {
+    const int v = a[i];
+    a[i] = (int)min(at, 0x7fffffffll);
+    at += v;
+  }
+  const long long all = tmp[THREADS / 32];
+  __syncthreads();
+  return all;
+}
+
+// The plan of a step, made by all threads of a CTA in shared memory. start: first block of every span (groups, then segments) and, behind them, the group of
+// every segment; span, tile: span of every block, tiles ahead of it.
+template <int THREADS>
+struct SharedPlan {
+  int *start, *group, *span, *tile;
+  int blocks, group_blocks;
+  long long tiles;                               // of one kv head
+
+  // -> false where the step does not fit (with a status)
+  __device__ __forceinline__ bool make(const FbSharedStep& st, int R, int kt, int max_group_blocks, int max_seg_blocks, unsigned char* smem, long long* tmp,
+                                       int* status) {
+    const int tid = threadIdx.x;
+    start = reinterpret_cast<int*>(smem);
+    group = start + 2 * SK_SEGS;
+    span = group + SK_SEGS;
+    tile = span + SK_BLOCKS;
+    for (int s = tid; s < st.nseg; s += THREADS) group[s] = -1;
+    __syncthreads();
+    for (int g = tid; g < st.ngrp; g += THREADS) {
+      const int s0 = st.grp_seg0[g], n = st.grp_nsegs[g];
+      int rows = 0;
+      if (s0 < 0 || n < 0 || n > st.nseg - s0) {
+        set_status(status, ST_BOUNDS);
+      } else if (n > 0) {
+        const int slot = st.seg_slot[s0], row0 = st.seg_row0[s0];
+        rows = st.seg_row0[s0 + n - 1] + st.seg_nrows[s0 + n - 1] - row0;
+        if (slot < 0 || slot >= st.slots || !rows_fit(st, row0, rows)) {
+          set_status(status, ST_BOUNDS);
+          rows = 0;
+        }
+        for (int s = s0; s < s0 + n && rows > 0; ++s)
+          if (atomicExch(&group[s], g) >= 0) set_status(status, ST_BOUNDS);      // a segment of two groups
+      }
+      start[g] = (rows + R - 1) / R;
+    }
+    for (int s = tid; s < st.nseg; s += THREADS) {
+      const int n = st.seg_nrows[s], slot = st.seg_slot[s];
+      bool ok = slot >= 0 && slot < st.slots && rows_fit(st, st.seg_row0[s], n);
+      if (!ok) set_status(status, ST_BOUNDS);
+      if (ok && n > st.max_rows) {
+        set_status(status, ST_CAPACITY);
+        ok = false;
+      }
+      start[st.ngrp + s] = ok ? (n + R - 1) / R : 0;
+    }
+    __syncthreads();
+    for (int s = tid + 1; s < st.nseg; s += THREADS)                             // the rows of a group lie side by side
+      if (group[s] >= 0 && group[s] == group[s - 1] && st.seg_row0[s] != st.seg_row0[s - 1] + st.seg_nrows[s - 1]) set_status(status, ST_BOUNDS);
+    const int spans = st.ngrp + st.nseg;
+    const long long all = scan_ahead<THREADS>(start, spans, tmp);
+    blocks = (int)min(all, 0x7fffffffll);
+    group_blocks = st.nseg ? start[st.ngrp] : 0;
+    if (blocks > SK_BLOCKS || group_blocks > max_group_blocks || blocks - group_blocks > max_seg_blocks) {
+      if (tid == 0) set_status(status, ST_CAPACITY);
+      return false;
+    }
+    for (int i = tid; i < spans; i += THREADS) {
+      const int end = i + 1 < spans ? start[i + 1] : blocks;
+      for (int b = start[i]; b < end; ++b) span[b] = i;
+    }
+    __syncthreads();
+    for (int b = tid; b < blocks; b += THREADS) tile[b] = block(st, b, R, kt, status).nt;
+    __syncthreads();
+    tiles = scan_ahead<THREADS>(tile, blocks, tmp);
+    return true;
+  }
+  // block b (without tile0)
+  __device__ __forceinline__ SharedBlock block(const FbSharedStep& st, int b, int R, int kt, int* status) const {
+    const int i = span[b], s = i - st.ngrp, m = b - start[i];
+    SharedBlock e;
+    long most;
+    int rows;
+    if (s < 0) {
+      const int s0 = st.grp_seg0[i], n = st.grp_nsegs[i];
+      e.slot = st.seg_slot[s0];
+      e.row0 = st.seg_row0[s0];
+      rows = st.seg_row0[s0 + n - 1] + st.seg_nrows[s0 + n - 1] - e.row0;
+      e.k0 = 0;
+      most = max(st.grp_len[i], 0);
+    } else {
+      e.slot = st.seg_slot[s];
+      e.row0 = st.seg_row0[s];
+      rows = st.seg_nrows[s];
+      e.k0 = group[s] < 0 ? 0 : max(st.grp_len[group[s]], 0);
+      most = 0x7fffffffl;
+    }
+    e.row0 += m * R;
+    e.nrows = min(R, rows - m * R);
+    int hi = 0, lo = 0x7fffffff;
+#pragma unroll 8
+    for (int r = 0; r < e.nrows; ++r) {
+      const int n = st.kvlen[e.row0 + r];
+      hi = max(hi, n);
+      lo = min(lo, n);
+    }
+    if (hi > table_limit(st)) set_status(status, ST_BOUNDS);
+    e.k1 = (int)min((long)hi, min(most, table_limit(st)));
+    e.kmin = max(0, min(lo, e.k1));
+    e.tile0 = 0;
+    e.nt = e.k1 > e.k0 ? (e.k1 + kt - 1) / kt - e.k0 / kt : 0;
+    return e;
+  }
+  // block that (block, kv head) place `at` of the list of tiles belongs to
+  __device__ __forceinline__ int find(long long at, int heads) const {
+    int lo = 0, hi = blocks - 1;                                                 // the last one that starts at or ahead of it: it has tiles
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if ((long long)tile[mid] * heads <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  }
+};
+
+// Most blocks of a step, from what the host knows.
+inline long shared_group_blocks(long rows, int ngrp, int R) { return ngrp ? rows / R + ngrp : 0; }
+inline long shared_seg_blocks(long rows, int nseg, int max_rows, int R) {
+  const long each = (long)nseg * ((max_rows + R - 1) / R), all = rows / R + nseg;
+  return each < all ? each : all;
+}
+
+// ---- what the kernels of this family use of the tensor cores and barriers ----------------------------------------------------------------------
+__device__ __forceinline__ float sk_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Wait of at most 2^31 cycles (about a second) that leaves the issue slots to others; false where it ran out or another role gave up.
+__device__ __forceinline__ bool sk_poll(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+  return ok;
+}
+__device__ __forceinline__ bool sk_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (sk_poll(bar, parity)) return true;
+  const long long t0 = clock64();
+#pragma unroll 1
+  while (!sk_poll(bar, parity))
+    if (*abort_flag || clock64() - t0 > 1ll << 31) return false;
+  return true;
+}
+// MN-major operand tile with the 128-byte swizzle: rows are K, 64 contiguous MN elements a row; lbo: bytes between chunks of 64 along MN, sbo between eight rows.
+__device__ __forceinline__ uint64_t sk_desc_mn128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
+}
+__device__ __forceinline__ void sk_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// 16 lanes x 32 columns: registers 4 c, 4 c + 1 are columns 8 c + 2 (lane % 4) and the next of TMEM lane lane / 4; 4 c + 2, 4 c + 3 those of lane / 4 + 8.
+__device__ __forceinline__ void sk_tmem_ld16x32(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 
 }  // namespace fb
