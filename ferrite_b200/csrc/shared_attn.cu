@@ -2,7 +2,9 @@
 // prefix are read once for all rows of its group.
 //
 //   S = Q K^T        128 (row, head) pairs of a block x 64 keys; Q and K in shared memory
-//   P = exp2(S - m)  two threads a pair; P as a bf16 value and its bf16 remainder, so that a weight keeps 16 bits, back into TMEM
+//   P = exp2(S - m)  two threads a pair; P as bf16 back into TMEM, its sums in 32 bits. (A weight is off by up to 2^-8 of it, errors that have either sign and
+//                    add up to what rounding the output to bf16 costs: 0.0024 instead of 0.0017 from the result in 64 bits. A second product with the
+//                    remainders would take that away, 512 more cycles of the tensor cores a tile of 128 pairs and 256 columns, 10 % of the whole.)
 //   O += P V         A = P from TMEM, V read along its columns from shared memory, O in TMEM while the CTA stays with the pairs
 //
 // Work (shared_kv.cuh): every CTA takes the same number of consecutive key tiles of the list of all (block, kv head) units. A unit that a CTA leaves or ends
@@ -10,9 +12,12 @@
 // of its own) in the order of the list. Where the contexts are cut follows the step's lengths, so a row may round differently beside other streams; the
 // same call gives the same bits.
 //
-// Warp roles: 0 loads keys, 10 loads values, 1 issues the products, 2..9 run the softmax, bring the queries and write the pieces. The running maximum moves only
-// when a row's new one exceeds it by 2^8. Every wait is bounded: one that runs out sets the status word and an abort flag; the softmax warps then go
-// through their remaining barriers without work, the others leave, and the CTA frees its TMEM.
+// Warp roles: 0 loads keys, 2 loads values, 1 issues the products of S, 3 those of O, 4..19 run the softmax, bring the queries and write the pieces. The
+// softmax of a tile is a chain of waits, and its exponentials alone take 512 cycles of the SM: two sets of eight warps take a tile in turn, each with a
+// buffer of S and P of its own, so that one set's chain hides behind the other's. They share O and the maximum that it belongs to. The maximum moves only
+// when a score of some row exceeds it by 2^16 (a vote of the threads of 32 pairs, who exchange their maxima only then); sets decide in the tiles' order (`turn`), and the one
+// that moves it rescales O between the two products. Every wait is bounded: one that runs out sets the status word and an abort flag; the softmax warps
+// then go through their remaining barriers without work, the others leave, and the CTA frees its TMEM.
 #include <algorithm>
 
 #include "gemm_core.cuh"
@@ -20,7 +25,13 @@
 
 namespace fb {
 
-constexpr int SA_PAIRS = 128, SA_KT = 64, SA_THREADS = 11 * 32;
+constexpr int SA_PAIRS = 128, SA_KT = 64, SA_NEAR = 4;
+#ifndef SA_EXTRA
+#define SA_EXTRA 3
+#endif
+constexpr int SA_SET = 8;                                    // warps of a set: two threads a pair, each with half of a tile's keys
+constexpr int SA_THREADS = (4 + 2 * SA_SET) * 32;
+constexpr int SA_ML = 8;                                     // floats of a pair's statistics: its threads' sums, the maximum
 
 template <int HD, bool OUT>
 struct SaCfg {
@@ -29,60 +40,68 @@ struct SaCfg {
   static constexpr int KS = OUT ? (HD == 256 ? 3 : HD == 128 ? 6 : 8) : (HD == 256 ? 5 : 8);
   static constexpr int VS = OUT ? (HD == 256 ? 2 : HD == 128 ? 5 : 8) : 0;
   static constexpr int TILES = Q_BYTES + (KS + VS) * T_BYTES;
-  static constexpr int MISC_AT = (TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES + 1023) / 1024 * 1024;
-  // TMEM: O | S0 S1 | P0 P1 | remainders
-  static constexpr uint32_t COL_S = OUT ? HD : 0, COL_P = COL_S + 2 * SA_KT, COL_R = COL_P + SA_KT;
+  static constexpr int MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
+  // TMEM: O | S0 S1 | P0 .. P3
+  static constexpr uint32_t COL_S = OUT ? HD : 0, COL_P = COL_S + 2 * SA_KT;
   static constexpr uint32_t COLS = OUT ? 512 : 128;
 };
+template <int STAGES>
 struct SaMisc {
-  float mx[2][2][SA_PAIRS];                      // by the tile's parity and half
-  long long tmp[SA_THREADS / 32 + 1];
-  uint64_t bars[10 + 4 * 8];
-  uint8_t bad[2][8];                             // keys of a tile whose values are no numbers
+  float mx[2][SA_PAIRS], m[SA_PAIRS];            // maxima of a tile's halves (of the set whose turn it is); the maximum that O belongs to (log2)
+  long long tmp[SA_THREADS / 32];
+  uint64_t bars[22 + 2 * STAGES];
+  uint8_t bad[2][2][8];                          // by set and turn: keys of a tile whose values are no numbers
   uint32_t tmem;
   int abort;
+  SharedBlock blocks[SA_NEAR];                   // the first ones of the CTA's share; what follows is in the workspace
 };
 
-// Where things lie in the workspace. ml: maximum (log2), sums of the two halves of the keys; records of 128 pairs for groups, of seg_pairs for segments.
+// Where things lie in the workspace. ml: sums of the pair's threads, maximum (log2); records of 128 pairs for groups, of seg_pairs for segments.
 struct SaSpace {
-  long long* head;                               // tiles a CTA, blocks of groups
+  long long* head;                               // places a CTA, blocks of groups
   SharedBlock* table;
-  int* rows;                                     // [rows][2]: block of a row's group, of its segment, or -1
-  float4 *ml_grp, *ml_seg;
+  int4* rows;                                    // [rows][2]: of a row's group, of its segment: place in the list of one kv head, tiles (0: none), unit, row of the block
+  float *ml_grp, *ml_seg;                        // SA_ML floats a pair
   float *o_grp, *o_seg;
-  int max_blocks, max_group_blocks, seg_pairs;
+  SharedPlanSizes z;
+  int seg_pairs;
 };
 
-// A CTA's way through its share of the list: (block, kv head) after (block, kv head).
+// A CTA's way through its share of the list: (block, kv head) after (block, kv head), as far as tiles of theirs lie in it.
 struct SaWalk {
   SharedBlock e;
-  int b, kvh, t, n;                              // n: tiles of the piece
-  int left;                                      // ... and behind it
-  const SharedBlock* table;
-  __device__ __forceinline__ void take() {
-    n = min(e.nt - t, left);
-    left -= n;
+  int b, kvh, t, n;                              // the piece: n tiles from tile t on
+  int left;                                      // places behind it
+  int b0;
+  const SharedBlock *near, *table;
+  __device__ __forceinline__ SharedBlock block(int i) const { return i - b0 < SA_NEAR ? near[i - b0] : table[i]; }
+  __device__ __forceinline__ void take(int at) {                     // from place `at` of the unit on
+    const int m = min(e.nt + SA_EXTRA - at, left);
+    t = max(at - SA_EXTRA, 0);
+    n = max(at + m - SA_EXTRA, 0) - t;
+    left -= m;
   }
-  __device__ __forceinline__ void start(const SharedBlock* tab, int b0, long long f0, int tiles, int nkv) {
+  // -> whether there is a piece
+  __device__ __forceinline__ bool start(const SharedBlock* close, const SharedBlock* tab, int first, long long f0, int places, int nkv) {
+    near = close;
     table = tab;
-    b = b0;
-    e = table[b];
-    const int at = (int)(f0 - (long long)e.tile0 * nkv);
-    kvh = at / e.nt;
-    t = at - kvh * e.nt;
-    left = tiles;
-    take();
+    b = b0 = first;
+    e = block(b);
+    const int at = (int)(f0 - (long long)e.place0 * nkv);
+    kvh = at / (e.nt + SA_EXTRA);
+    left = places;
+    take(at - kvh * (e.nt + SA_EXTRA));
+    return n > 0 || next(nkv);
   }
   __device__ __forceinline__ bool next(int nkv) {
     if (left == 0) return false;
-    t = 0;
     if (++kvh == nkv) {
       kvh = 0;
-      do e = table[++b];
+      do e = block(++b);
       while (e.nt == 0);
     }
-    take();
-    return true;
+    take(0);
+    return n > 0;                                // (none: the share ends in what lies ahead of the unit's tiles)
   }
   __device__ __forceinline__ int token(int j) const { return (e.k0 / SA_KT + t + j) * SA_KT; }
 };
@@ -95,9 +114,9 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   constexpr int NCH = C::NCH, KS = C::KS, VS = C::VS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *sQ = smem, *sK = smem + C::Q_BYTES, *sV = sK + KS * C::T_BYTES;
-  SaMisc& ms = *reinterpret_cast<SaMisc*>(smem + C::MISC_AT);
-  uint64_t *q_full = ms.bars, *o_empty = q_full + 1, *s_full = q_full + 2, *s_empty = q_full + 4, *p_full = q_full + 6, *p_empty = q_full + 8,
-           *k_full = q_full + 10, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
+  SaMisc<KS + VS>& ms = *reinterpret_cast<SaMisc<KS + VS>*>(smem + C::MISC_AT);
+  uint64_t *q_full = ms.bars, *o_empty = q_full + 1, *s_full = q_full + 2, *s_empty = q_full + 4, *p_full = q_full + 6, *p_empty = q_full + 10,
+           *turn = q_full + 14, *k_full = q_full + 22, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &ms.abort;
   pdl_launch_dependents();
@@ -107,11 +126,13 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   }
   if (tid == 0) {
     ms.abort = 0;
-    mbar_init(q_full, 8);
-    mbar_init(o_empty, 8);
+    mbar_init(q_full, SA_SET);
+    mbar_init(o_empty, 2 * SA_SET);
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 8); mbar_init(&p_full[i], 8); mbar_init(&p_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], SA_SET);
     }
+    for (int i = 0; i < 4; ++i) { mbar_init(&p_full[i], SA_SET); mbar_init(&p_empty[i], 1); }
     for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < VS; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     fence_mbar_init();
@@ -129,46 +150,41 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   // ---- this CTA's share
   const int R = SA_PAIRS / share;
   SharedPlan<SA_THREADS> plan;
-  const bool fits = plan.make(st, R, SA_KT, w.max_group_blocks, w.max_blocks - w.max_group_blocks, smem, ms.tmp, status);
-  const long long all = fits ? plan.tiles * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+  const bool fits = plan.make(st, R, SA_KT, SA_EXTRA, w.z, smem, ms.tmp, status);
+  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
   const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
-  if (blockIdx.x == 0 && tid == 0) {
-    w.head[0] = fits && per < 1ll << 31 ? per : 0;
-    w.head[1] = fits ? plan.group_blocks : 0;
-  }
-  if (fits && blockIdx.x == 0)
-    for (int b = tid; b < plan.blocks; b += SA_THREADS) {            // blocks that have no keys
-      if ((b + 1 < plan.blocks ? (long long)plan.tile[b + 1] : plan.tiles) > plan.tile[b]) continue;
-      const SharedBlock e = plan.block(st, b, R, SA_KT, status);
-      const int s = plan.span[b] - st.ngrp;
-      for (int r = e.row0; r < e.row0 + e.nrows; ++r) {
-        w.rows[2 * r + (s >= 0)] = -1;
-        if (s >= 0 && plan.group[s] < 0) w.rows[2 * r] = -1;
-      }
+  if (blockIdx.x == 0 && tid == 0) w.head[0] = fits && per < 1ll << 31 ? per : 0;
+  // what the second kernel has to know of a row: written by every CTA that has the block's tiles (the same), or by the first one
+  auto note = [&](int b, const SharedBlock& e) {
+    const int s = plan.span[b] - st.ngrp, unit = (b - (s >= 0 ? plan.group_blocks : 0)) * nkv;
+    for (int r = 0; r < e.nrows; ++r) {
+      w.rows[2 * (e.row0 + r) + (s >= 0)] = make_int4(e.place0, e.nt, unit, r);
+      if (s >= 0 && plan.group[s] < 0) w.rows[2 * (e.row0 + r)] = make_int4(0, 0, 0, 0);
     }
+  };
+  if (fits && blockIdx.x == 0)
+    for (int b = tid; b < plan.blocks; b += SA_THREADS)              // blocks that have no keys
+      if ((b + 1 < plan.blocks ? (long long)plan.place[b + 1] : plan.places) == plan.place[b]) note(b, plan.block(st, b, R, SA_KT, status));
   if (f0 == f1 || per >= 1ll << 31) {                                // the same for the whole CTA
     if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
     if (warp == 1) tmem_dealloc(tmem, C::COLS);
     return;
   }
-  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv), tiles = (int)(f1 - f0), group_blocks = plan.group_blocks;
-  for (int b = b0 + tid; b <= b1; b += SA_THREADS) {                 // (other CTAs of a block write the same)
+  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv), group_blocks = plan.group_blocks;
+  for (int b = b0 + tid; b <= b1; b += SA_THREADS) {
     SharedBlock e = plan.block(st, b, R, SA_KT, status);
-    e.tile0 = plan.tile[b];
-    w.table[b] = e;
-    const int s = plan.span[b] - st.ngrp;
-    for (int r = e.row0; r < e.row0 + e.nrows && e.nt; ++r) {
-      w.rows[2 * r + (s >= 0)] = b;
-      if (s >= 0 && plan.group[s] < 0) w.rows[2 * r] = -1;
-    }
+    e.place0 = plan.place[b];
+    if (b - b0 < SA_NEAR) ms.blocks[b - b0] = e;
+    else w.table[b] = e;
+    if (e.nt) note(b, e);
   }
   fence_proxy_async();                                               // tiles take the plan's place
   __syncthreads();
   SaWalk x;
-  x.start(w.table, b0, f0, tiles, nkv);
+  if (!x.start(ms.blocks, w.table, b0, f0, (int)(f1 - f0), nkv)) goto done;    // the same for the whole CTA
 
-  if (warp == 0 || warp == 10) {
-    // ---- keys (warp 0) and values (warp 10): the lanes look up 32 tiles' pages at a time, one of them copies
+  if (warp == 0 || warp == 2) {
+    // ---- keys (warp 0) and values (warp 2): the lanes look up 32 tiles' pages at a time, one of them copies
     const bool keys = warp == 0;
     if (!keys && !OUT) goto done;
     const CUtensorMap* tm = keys ? &tmK : &tmV;
@@ -204,71 +220,66 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     }
     if (*abort_flag && lane == 0)                                    // loads may still be landing: a bounded time before the CTA's memory goes away
       for (int j = max(0, i - S); j < i; ++j) mbar_wait(&full[j % S], (j / S) & 1, 1u << 20);
-  } else if (warp == 1) {
-    // ---- products, issued from the whole warp by one lane's predicate
-    constexpr uint32_t idesc_s = umma_idesc(1, 1, SA_PAIRS, SA_KT);
-    constexpr uint32_t idesc_pv = umma_idesc(1, 1, SA_PAIRS, HD) | (1u << 16);         // B read MN-major
-    const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK), aV = smem_u32(sV);
+  } else if (warp == 1 || warp == 3) {
+    // ---- products, issued from the whole warp by one lane's predicate: S (warp 1), O (warp 3)
+    if (warp == 3 && !OUT) goto done;
     const bool issue = elect_one();
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, sk_wait(bar, parity, abort_flag)); };
-    int kst = 0, kph = 0, vst = 0, vph = 0, i = 0, piece = 0;
-    auto issue_s = [&](int at) -> bool {
-      const int s = at & 1;
-      if (!wait(&k_full[kst], kph)) return false;
-      if (at >= 2 && !wait(&s_empty[s], ((at >> 1) - 1) & 1)) return false;
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) {
-        const uint32_t off = (uint32_t)(kk & 3) * 32u;
-        tc_mma_f16_if(issue, tmem + C::COL_S + s * SA_KT, umma_desc_k128(aQ + (kk >> 2) * C::Q_CH + off),
-                      umma_desc_k128(aK + kst * C::T_BYTES + (kk >> 2) * C::KV_CH + off), idesc_s, kk > 0 ? 1u : 0u);
-      }
-      tc_commit_if(issue, &s_full[s]);
-      tc_commit_if(issue, &k_empty[kst]);
-      if (++kst == KS) {
-        kst = 0;
-        kph ^= 1;
-      }
-      return true;
+    auto wait = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, bool both) {
+      return __all_sync(0xffffffffu, sk_wait2(a, pa, both ? b : a, both ? pb : pa, abort_flag));
     };
-    bool ok = wait(q_full, 0) && issue_s(0);
-    bool more = true;
-    while (ok && more) {
+    bool ok = true;
+    int i = 0, st_i = 0, phase = 0, piece = 0;
+    do {
       for (int j = 0; ok && j < x.n; ++j, ++i) {
-        if (j + 1 < x.n) ok = issue_s(i + 1);
-        if constexpr (OUT) {
-          const int s = i & 1;
-          ok = ok && wait(&p_full[s], (i >> 1) & 1) && wait(&v_full[vst], vph) && (j > 0 || piece == 0 || wait(o_empty, (piece - 1) & 1));
+        const int s = i & 1;
+        if (warp == 1) {
+          constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, SA_KT);
+          const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK) + st_i * C::T_BYTES;
+          ok = j > 0 || wait(q_full, piece & 1, q_full, 0, false);
+          ok = ok && wait(&k_full[st_i], phase, &s_empty[s], ((i >> 1) - 1) & 1, i >= 2);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk & 3) * 32u;
+            tc_mma_f16_if(issue, tmem + C::COL_S + s * SA_KT, umma_desc_k128(aQ + (kk >> 2) * C::Q_CH + off),
+                          umma_desc_k128(aK + (kk >> 2) * C::KV_CH + off), idesc, kk > 0 ? 1u : 0u);
+          }
+          tc_commit_if(issue, &s_full[s]);
+          tc_commit_if(issue, &k_empty[st_i]);
+          if (++st_i == KS) {
+            st_i = 0;
+            phase ^= 1;
+          }
+        } else if constexpr (OUT) {
+          constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, HD) | (1u << 16);      // B read MN-major
+          const uint32_t aV = smem_u32(sV) + st_i * C::T_BYTES;
+          ok = j > 0 || piece == 0 || wait(o_empty, (piece - 1) & 1, o_empty, 0, false);
+          ok = ok && wait(&v_full[st_i], phase, &p_full[i & 3], (i >> 2) & 1, true);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < SA_KT / 16; ++kk)
-            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + s * (SA_KT / 2) + kk * 8,
-                             sk_desc_mn128(aV + vst * C::T_BYTES + kk * 16 * 128, C::KV_CH, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-#pragma unroll
-          for (int kk = 0; kk < SA_KT / 16; ++kk)
-            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_R + s * (SA_KT / 2) + kk * 8,
-                             sk_desc_mn128(aV + vst * C::T_BYTES + kk * 16 * 128, C::KV_CH, 1024), idesc_pv, 1u);
-          tc_commit_if(issue, &v_empty[vst]);
-          tc_commit_if(issue, &p_empty[s]);
-          if (++vst == VS) {
-            vst = 0;
-            vph ^= 1;
+            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + (i & 3) * (SA_KT / 2) + kk * 8, sk_desc_mn128(aV + kk * 16 * 128, C::KV_CH, 1024), idesc,
+                             (j > 0 || kk > 0) ? 1u : 0u);
+          tc_commit_if(issue, &v_empty[st_i]);
+          tc_commit_if(issue, &p_empty[i & 3]);
+          if (++st_i == VS) {
+            st_i = 0;
+            phase ^= 1;
           }
         }
       }
-      if (!ok) break;
-      more = x.next(nkv);
       ++piece;
-      if (more) ok = wait(q_full, piece & 1) && issue_s(i);
-    }
+    } while (ok && x.next(nkv));
     if (!ok) {
       if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
       *abort_flag = 1;
     }
   } else {
-    // ---- softmax, queries, pieces: warps 2..5 take keys 0..31 of a tile, 6..9 the others; a pair's two threads sit in the same lane quadrant
-    const int quad = warp & 3, half = (warp - 2) >> 2, st_tid = tid - 64;
+    // ---- softmax, queries, pieces. Warps 4..11 are set 0, 12..19 set 1; of a set, four have the first 32 keys of a tile, four the others; a pair's threads
+    // sit in the same lane quadrant.
+    const int quad = warp & 3, set = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, st_tid = (tid - 128) & 255;
     const int pair = quad * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     constexpr int HC = SA_KT / 2, OC = HD / 2;
@@ -280,10 +291,17 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         *abort_flag = 1;
       }
     };
+    auto wait2 = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb) {
+      if (!dead && !__all_sync(0xffffffffu, sk_wait2(a, pa, b, pb, abort_flag))) {
+        dead = true;
+        if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+        *abort_flag = 1;
+      }
+    };
     auto copy_q = [&](const SaWalk& y) {                             // 16 bytes at a time, swizzled as the products read them
       const int pieces = y.e.nrows * share * (HD / 8);
       const __nv_bfloat16* src = q + (long)y.e.row0 * q_stride + (long)y.kvh * share * HD;
-      for (int c = st_tid; c < pieces; c += 256) {
+      for (int c = st_tid; c < pieces; c += SA_SET * 32) {
         const int p = c / (HD / 8), d = c % (HD / 8), r = p / share, g = p - r * share;
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                      ::"r"(smem_u32(sQ + (d >> 3) * C::Q_CH + p * 128 + (((d & 7) ^ (p & 7)) << 4))), "l"(src + (long)r * q_stride + g * HD + d * 8)
@@ -296,35 +314,37 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       __syncwarp();
       if (lane == 0 && !dead) mbar_arrive(q_full);
     };
-    copy_q(x);
-    give_q();
-    int i = 0;
+    if (set == 0) {
+      copy_q(x);
+      give_q();
+    }
+    int first = 0;                                                   // number of the piece's first tile
     bool more = true;
     while (more) {
       const SaWalk y = x;
       more = x.next(nkv);
-      const int np = y.e.nrows * share;
+      const int np = y.e.nrows * share, end = first + y.n;
       const int klen = pair < np ? min(st.kvlen[y.e.row0 + pair / share], y.e.k1) : 0;
-      const bool active = quad * 32 < np;                            // (the same for both warps of a quadrant)
-      float m_ref = -INFINITY, l = 0.f;
-      for (int j = 0; j < y.n; ++j, ++i) {
-        const int s = i & 1, t0 = y.token(j);
+      const bool active = quad * 32 < np;                            // (the same for all warps of a quadrant)
+      float m_own = -INFINITY, l = 0.f;
+      for (int i = first + ((first ^ set) & 1); i < end; i += 2) {
+        const int j = i - first, t0 = y.token(j);
         const bool need_mask = t0 < y.e.k0 || t0 + SA_KT > y.e.kmin;
-        wait(&s_full[s], (i >> 1) & 1);
-        if (j + 1 == y.n && more && !dead) copy_q(x);                // every product that reads the queries is through
+        wait(&s_full[set], (i >> 1) & 1);
+        if (i + 1 == end && more && !dead) copy_q(x);                // every product that reads the queries is through
         if constexpr (OUT) if (need_mask) {
           // Values of keys that some row does not see meet weights of zero: those that no row sees become zeros, those that some see are looked at,
           // and where one is no finite number the key's values become zeros and its score NaN for the rows that see it.
-          if (!dead) {
-            wait(&v_full[i % VS], (i / VS) & 1);
-          }
+          // (a wait tells a phase from the one ahead of it only: the values of tile i - VS have to be through)
+          if (i >= 4) wait(&p_empty[i & 3], ((i >> 2) - 1) & 1);
+          if (VS < 4 && i >= VS) wait(&p_empty[(i - VS) & 3], ((i - VS) >> 2) & 1);
+          wait(&v_full[i % VS], (i / VS) & 1);
           if (!dead) {
             const int key = st_tid >> 2, part = st_tid & 3, tok = t0 + key;
             unsigned char* base = sV + (i % VS) * C::T_BYTES;
             constexpr int PER = HD / 32;                             // 16-byte pieces of a thread
             auto at = [&](int e) { return reinterpret_cast<uint4*>(base + ((part * PER + e) >> 3) * C::KV_CH + key * 128 + ((part * PER + e) & 7) * 16); };
-            bool zero = tok < y.e.k0 || tok >= y.e.k1;
-            bool bad = false;
+            bool zero = tok < y.e.k0 || tok >= y.e.k1, bad = false;
             if (!zero && tok >= y.e.kmin) {
 #pragma unroll
               for (int e = 0; e < PER; ++e) {
@@ -335,132 +355,143 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
               }
             }
             const uint32_t bal = __ballot_sync(0xffffffffu, bad);
-            zero |= (bal >> (lane & 28)) & 15u;
+            zero |= (bal >> (lane & 28) & 15u) != 0;
             if (zero)
 #pragma unroll
               for (int e = 0; e < PER; ++e) *at(e) = make_uint4(0, 0, 0, 0);
             if (lane == 0) {
               uint32_t bits = 0;
-              for (int k = 0; k < 8; ++k) bits |= ((bal >> (4 * k)) & 15u) ? 1u << k : 0u;
-              ms.bad[s][st_tid >> 5] = (uint8_t)bits;
+              for (int k = 0; k < 8; ++k) bits |= (bal >> (4 * k) & 15u) ? 1u << k : 0u;
+              ms.bad[set][i >> 1 & 1][st_tid >> 5] = (uint8_t)bits;
             }
             fence_proxy_async();
           }
-          asm volatile("bar.sync 5, 256;" ::: "memory");
-        }
-        if (!active) {
-          __syncwarp();
-          if (lane == 0 && !dead) {
-            mbar_arrive(&s_empty[s]);
-            if (OUT) mbar_arrive(&p_full[s]);
-          }
-          continue;
+          asm volatile("bar.sync %0, 256;" ::"r"(9 + set) : "memory");
         }
         uint32_t sr[HC];
-        float mx = -INFINITY;
-        if (!dead) {
+        float mx = -INFINITY;                                        // of the scores as they are, without the scale
+        if (active && !dead) {
           tc_fence_after();
-          tmem_ld32(tmem + lane_addr + C::COL_S + s * SA_KT + half * HC, sr);
+          tmem_ld32(tmem + lane_addr + C::COL_S + set * SA_KT + sub * HC, sr);
           tmem_ld_wait();
           tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_empty[s]);
+        }
+        __syncwarp();
+        if (lane == 0 && !dead) mbar_arrive(&s_empty[set]);
+        if (active && !dead) {
           if (need_mask) {
-            const int c0 = t0 + half * HC;
-            const uint32_t bad = OUT ? reinterpret_cast<const uint32_t*>(ms.bad[s])[half] : 0u;
+            const int c0 = t0 + sub * HC;
+            const uint32_t bad = OUT ? reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub] : 0u;
 #pragma unroll
             for (int c = 0; c < HC; ++c) {
-              float v = __uint_as_float(sr[c]) * scale_log2;
-              if (bad >> c & 1u) v = NAN;
-              if (c0 + c < y.e.k0 || c0 + c >= klen) v = -INFINITY;
-              sr[c] = __float_as_uint(v);
-              mx = fmaxf(mx, v);
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < HC; ++c) {
-              const float v = __uint_as_float(sr[c]) * scale_log2;
-              sr[c] = __float_as_uint(v);
-              mx = fmaxf(mx, v);
+              if (bad >> c & 1u) sr[c] = 0x7fc00000u;
+              if (c0 + c < y.e.k0 || c0 + c >= klen) sr[c] = 0xff800000u;
             }
           }
+#pragma unroll
+          for (int c = 0; c < HC; c += 4)
+            mx = fmaxf(fmaxf(mx, __uint_as_float(sr[c])), fmaxf(fmaxf(__uint_as_float(sr[c + 1]), __uint_as_float(sr[c + 2])), __uint_as_float(sr[c + 3])));
+          mx = pair < np ? mx * scale_log2 : -INFINITY;              // (what lies behind the pairs moves no maximum)
         }
-        ms.mx[s][half][pair] = mx;
-        asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory");
-        mx = pair < np ? fmaxf(mx, ms.mx[s][half ^ 1][pair]) : -INFINITY;      // (what lies behind the pairs moves no maximum)
-        const bool any = __any_sync(0xffffffffu, mx > m_ref + 8.f);
-        if (OUT) {
-          // P(i - 2) has been read; where O is rescaled, PV(i - 1) is through
-          if (i >= 2) wait(&p_empty[s], ((i >> 1) - 1) & 1);
-          if (any && j > 0) wait(&p_empty[s ^ 1], ((i - 1) >> 1) & 1);
+        // ---- the decision, in the order of the tiles
+        if (OUT && i >= 4) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[i & 3], ((i >> 2) - 1) & 1);    // ... and P(i - 4) has been read
+        else if (i > 0) wait(&turn[2 * quad + set], ((i - 1) >> 1) & 1);
+        float m_new = j > 0 ? ms.m[pair] : -INFINITY;
+        const float m_old = m_new;
+        uint32_t moves;
+        asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.b32 a, %1, 0;\n\tbarrier.cta.red.or.pred b, %2, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+                     : "=r"(moves) : "r"((uint32_t)(!dead && mx > m_old + 16.f)), "r"(1 + 4 * set + quad) : "memory");
+        if (moves) {
+          ms.mx[sub][pair] = mx;
+          asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * set + quad) : "memory");
+          m_new = fmaxf(m_old, fmaxf(mx, ms.mx[sub ^ 1][pair]));
         }
-        if (dead) continue;
+        if (sub == 0 && (moves || j == 0)) ms.m[pair] = m_new;
+        __syncwarp();
+        if (lane == 0 && !dead) mbar_arrive(&turn[2 * quad + (set ^ 1)]);
+        if (OUT && moves && j > 0) wait(&p_empty[(i - 1) & 3], ((i - 1) >> 2) & 1);          // O is rescaled behind PV(i - 1)
+        if (dead || !active) {
+          __syncwarp();
+          if (OUT && lane == 0 && !dead) mbar_arrive(&p_full[i & 3]);
+          continue;
+        }
         if (OUT) tc_fence_after();
-        if (any) {
-          const float m_new = fmaxf(m_ref, mx);
-          const float f = m_ref == -INFINITY ? 0.f : sk_exp2(m_ref - m_new);
-          l = m_ref == -INFINITY ? l : l * f;                        // (a sum that is no number stays one)
-          if (OUT && j > 0) {
+        if (m_new != m_own) {
+          l = m_own == -INFINITY ? l : l * sk_exp2(m_own - m_new);   // (a sum that is no number stays one)
+          m_own = m_new;
+        }
+        if (OUT && moves && j > 0) {
+          const float f = m_old == -INFINITY ? 0.f : sk_exp2(m_old - m_new);
 #pragma unroll 1
-            for (int c0 = 0; c0 < OC; c0 += 32) {
-              uint32_t o[32];
-              tmem_ld32(tmem + lane_addr + half * OC + c0, o);
-              tmem_ld_wait();
+          for (int c0 = 0; c0 < OC; c0 += 16) {
+            uint32_t o[16];
+            tmem_ld16(tmem + lane_addr + sub * OC + c0, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-              tmem_st32(tmem + lane_addr + half * OC + c0, o);
-            }
-            tmem_st_wait();
+            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+            sk_tmem_st16(tmem + lane_addr + sub * OC + c0, o);
           }
-          m_ref = m_new;
+          tmem_st_wait();
         }
-        const float mr = m_ref == -INFINITY ? 0.f : m_ref;
-        float sum = 0.f;
-        uint32_t pr[HC / 2], px[HC / 2];
+        const float mr = m_new == -INFINITY ? 0.f : -m_new;
+        const uint64_t scale2 = f2_pack(scale_log2, scale_log2), mr2 = f2_pack(mr, mr);
+        uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < HC / 2; ++c) {
-          const float p0 = sk_exp2(__uint_as_float(sr[2 * c]) - mr), p1 = sk_exp2(__uint_as_float(sr[2 * c + 1]) - mr);
-          sum += p0 + p1;
-          if constexpr (OUT) {
-            pr[c] = pack_bf2(p0, p1);
-            px[c] = pack_bf2(p0 - bf_lo(pr[c]), p1 - bf_hi(pr[c]));
+        for (int part = 0; part < 2; ++part) {
+          uint32_t pr[HC / 4];
+#pragma unroll
+          for (int c = 0; c < HC / 4; ++c) {
+            const int k = part * (HC / 2) + 2 * c;
+            const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), scale2, mr2));
+            const float p0 = sk_exp2(d.x), p1 = sk_exp2(d.y);
+            sum = f2_add(sum, f2_pack(p0, p1));
+            if constexpr (OUT) pr[c] = pack_bf2(p0, p1);
           }
+          if constexpr (OUT) sk_tmem_st8(tmem + lane_addr + C::COL_P + (i & 3) * (SA_KT / 2) + sub * (HC / 2) + part * (HC / 4), pr);
         }
-        l += sum;
+        const float2 both = f2_unpack(sum);
+        l += both.x + both.y;
         if constexpr (OUT) {
-          sk_tmem_st16(tmem + lane_addr + C::COL_P + s * (SA_KT / 2) + half * (HC / 2), pr);
-          sk_tmem_st16(tmem + lane_addr + C::COL_R + s * (SA_KT / 2) + half * (HC / 2), px);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[s]);
+          if (lane == 0) mbar_arrive(&p_full[i & 3]);
         }
       }
-      if (more) give_q();
+      if (more && ((end - 1) & 1) == set) give_q();
       // ---- the piece: record number = CTA + unit, which no other piece has
       const bool grp = y.b < group_blocks;
       const long rec = (long)blockIdx.x + (long)(y.b - (grp ? 0 : group_blocks)) * nkv + y.kvh;
       const int stride = grp ? SA_PAIRS : w.seg_pairs;
+      if (((end - 1) & 1) != set) {                                  // the last decision was the other set's
+        wait(&turn[2 * quad + set], ((end - 1) >> 1) & 1);
+        const float m = ms.m[pair];
+        l = m_own == -INFINITY ? l : l * sk_exp2(m_own - m);
+        m_own = m;
+      }
       if (active && pair < np && !dead) {
-        float* ml = reinterpret_cast<float*>((grp ? w.ml_grp : w.ml_seg) + rec * stride + pair);
-        if (half == 0) *reinterpret_cast<float2*>(ml) = make_float2(m_ref, l);
-        else ml[2] = l;
+        float* ml = (grp ? w.ml_grp : w.ml_seg) + (rec * stride + pair) * SA_ML;
+        ml[2 * set + sub] = l;
+        if (set == 0 && sub == 0) ml[4] = m_own;
       }
       if constexpr (OUT) {
-        wait(&p_empty[(i - 1) & 1], ((i - 1) >> 1) & 1);
+        if (end >= 2) wait(&p_empty[(end - 2) & 3], ((end - 2) >> 2) & 1);       // (one phase after the other)
+        wait(&p_empty[(end - 1) & 3], ((end - 1) >> 2) & 1);
         if (active && !dead) {
           tc_fence_after();
-          float* o = (grp ? w.o_grp : w.o_seg) + (rec * stride) * HD + half * OC + 2 * (lane & 3);
+          constexpr int QC = HD / 4;
+          const int col = (2 * set + sub) * QC;
+          float* o = (grp ? w.o_grp : w.o_seg) + (rec * stride) * HD + col + 2 * (lane & 3);
 #pragma unroll 1
           for (int r0 = quad * 32; r0 < min(np, quad * 32 + 32); r0 += 16) {
             const int ra = r0 + (lane >> 2), rb = ra + 8;
 #pragma unroll 1
-            for (int c0 = 0; c0 < OC; c0 += 32) {
-              uint32_t v[16];
-              sk_tmem_ld16x32(tmem + ((uint32_t)r0 << 16) + half * OC + c0, v);
+            for (int c0 = 0; c0 < QC; c0 += 16) {
+              uint32_t v[8];
+              sk_tmem_ld16x16(tmem + ((uint32_t)r0 << 16) + col + c0, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
+              for (int k = 0; k < 2; ++k) {
                 if (ra < np) *reinterpret_cast<float2*>(o + (long)ra * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]));
                 if (rb < np) *reinterpret_cast<float2*>(o + (long)rb * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
               }
@@ -471,6 +502,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         __syncwarp();
         if (lane == 0 && !dead) mbar_arrive(o_empty);
       }
+      first = end;
     }
   }
 done:
@@ -479,80 +511,96 @@ done:
   if (warp == 1) tmem_dealloc(tmem, C::COLS);
 }
 
-// Pieces of a row's heads that share a kv head -> output and logarithm. grid: rows x kv heads.
-__global__ void __launch_bounds__(256) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride, FbSharedStep st, SaSpace w,
-                                                          int nkv, int share, int hd, int ctas) {
-  __shared__ float top_s[SA_PAIRS], inv_s[SA_PAIRS];
-  const int row = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+// Pieces of a head's row -> output and logarithm. grid: rows x query heads; a thread has four columns and every fourth (eighth, 16th) piece. Everything that
+// does not depend on the pieces is asked for at once, and the pieces' sums beside their maxima: three trips to memory.
+template <int HD>
+__global__ void __launch_bounds__(256, 4) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride, FbSharedStep st, SaSpace w,
+                                                          int nkv, int share, int ctas) {
+  constexpr int LANES = HD / 4, PARTS = 256 / LANES;
+  __shared__ float top_s[PARTS], sum_s[PARTS];
+  __shared__ float4 o_s[PARTS][LANES];
+  const int row = blockIdx.x, h = blockIdx.y, kvh = h / share, g = h - kvh * share, tid = threadIdx.x, part = tid / LANES, d = tid % LANES * 4;
   pdl_launch_dependents();
   pdl_wait();
   bool mine = false;
   for (int s = tid; s < st.nseg; s += 256) mine |= row >= st.seg_row0[s] && row - st.seg_row0[s] < st.seg_nrows[s];
-  if (!__syncthreads_or(mine)) return;                               // a row of no segment
   const long long per = w.head[0];
-  const int group_blocks = (int)w.head[1], n = st.kvlen[row];
-  if (per <= 0) return;                                              // the step did not fit
-  // a row's two runs of records; checked, since a launch that gave up has not written all of this
-  const float4* ml[2];
-  const float* o[2];
-  int pieces[2], stride[2];
+  const int n = st.kvlen[row];
+  const int4 info[2] = {w.rows[2 * row], w.rows[2 * row + 1]};
+  float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (proj && part == 0) {
+    const __nv_bfloat16* p = proj + (long)row * proj_stride + (long)h * 2 * HD + HD + d;
+    gate = make_float4(bf2f(p[0]), bf2f(p[1]), bf2f(p[2]), bf2f(p[3]));
+  }
+  if (!__syncthreads_or(mine) || per <= 0) return;                   // a row of no segment; a step that did not fit
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    pieces[k] = 0;
-    const int b = w.rows[2 * row + k];
-    if (b < 0 || b >= w.max_blocks || (k == 0) != (b < group_blocks) || group_blocks > w.max_group_blocks) continue;
-    const SharedBlock e = w.table[b];
-    const long long at = (long long)e.tile0 * nkv + (long long)kvh * e.nt;
-    const long long c0 = at / per, c1 = (at + e.nt - 1) / per;
-    const int r = row - e.row0;
-    if (e.nt <= 0 || e.tile0 < 0 || c1 >= ctas || r < 0 || r >= e.nrows || (k && b - group_blocks >= w.max_blocks - w.max_group_blocks)) continue;
-    stride[k] = k == 0 ? SA_PAIRS : w.seg_pairs;
-    const long rec = (long)c0 + (long)(b - (k ? group_blocks : 0)) * nkv + kvh;
-    if ((r + 1) * share > stride[k]) continue;
-    ml[k] = (k == 0 ? w.ml_grp : w.ml_seg) + rec * stride[k] + r * share;
-    o[k] = (k == 0 ? w.o_grp : w.o_seg) + (rec * stride[k] + r * share) * hd;
-    pieces[k] = (int)(c1 - c0) + 1;
-  }
-  const int total = pieces[0] + pieces[1];
-  auto stat = [&](int i, int g) { return i < pieces[0] ? ml[0][(long)i * stride[0] + g] : ml[1][(long)(i - pieces[0]) * stride[1] + g]; };
-  for (int g = warp; g < share; g += 8) {
-    float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < total; i += 32) top = fmaxf(top, stat(i, g).x);
-    top = warp_max(top);
-    for (int i = lane; i < total; i += 32) {
-      const float4 v = stat(i, g);
-      const float l = v.y + v.z;
-      sum += v.x == -INFINITY ? (l != l ? l : 0.f) : l * sk_exp2(v.x - top);
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) {
-      const int h = kvh * share + g;
-      top_s[g] = top;
-      inv_s[g] = n <= 0 ? 0.f : sum == 0.f ? NAN : 1.f / sum;        // (scores of minus infinity only: 0 / 0)
-      if (lse) lse[(long)row * nkv * share + h] = n <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-    }
-  }
-  if (!out) return;
-  __syncthreads();
-  for (int c = tid; c < share * (hd / 4); c += 256) {
-    const int g = c / (hd / 4), d = c % (hd / 4) * 4, h = kvh * share + g;
-    const float top = top_s[g], inv = inv_s[g];
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    // a row's run of records; checked, since a launch that gave up has not written all of this
+    const long long at = (long long)info[k].x * nkv + (long long)kvh * (info[k].y + SA_EXTRA) + SA_EXTRA;
+    const long long c0 = at / per, c1 = (at + info[k].y - 1) / per;
+    const int r = info[k].w, stride = k == 0 ? SA_PAIRS : w.seg_pairs, units = (k == 0 ? w.z.group_blocks : w.z.blocks - w.z.group_blocks) * nkv;
+    if (info[k].y <= 0 || info[k].x < 0 || c1 >= ctas || r < 0 || (r + 1) * share > stride || info[k].z < 0 || info[k].z + kvh >= units) continue;
+    const int pieces = (int)(c1 - c0) + 1;
+    const long rec = (c0 + info[k].z + kvh) * stride + r * share + g;
+    const float* ml = (k == 0 ? w.ml_grp : w.ml_seg) + rec * SA_ML;
+    const float* o = (k == 0 ? w.o_grp : w.o_seg) + rec * HD + d;
+    constexpr int AT_ONCE = 4;
+    for (int i0 = part; i0 < pieces; i0 += PARTS * AT_ONCE) {
+      float2 v[AT_ONCE];                                             // maximum, sum
+      float4 x[AT_ONCE];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll 8
-      for (int i = 0; i < pieces[k]; ++i) {
-        const float4 v = *reinterpret_cast<const float4*>(o[k] + ((long)i * stride[k] + g) * hd + d);
-        const float m = ml[k][(long)i * stride[k] + g].x, f = m == -INFINITY ? 0.f : sk_exp2(m - top);
-        a.x = fmaf(v.x, f, a.x); a.y = fmaf(v.y, f, a.y); a.z = fmaf(v.z, f, a.z); a.w = fmaf(v.w, f, a.w);
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const long i = i0 + e * PARTS;
+        v[e] = make_float2(-INFINITY, 0.f);
+        if (i < pieces) {
+          const float4 l = *reinterpret_cast<const float4*>(ml + i * stride * SA_ML);
+          v[e] = make_float2(ml[i * stride * SA_ML + 4], l.x + l.y + (l.z + l.w));
+        }
+        x[e] = i < pieces && out ? *reinterpret_cast<const float4*>(o + i * stride * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
-    a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
-    if (proj) {
-      const __nv_bfloat16* gate = proj + (long)row * proj_stride + (long)h * 2 * hd + hd + d;
-      a.x *= sigmoidf_(bf2f(gate[0])); a.y *= sigmoidf_(bf2f(gate[1])); a.z *= sigmoidf_(bf2f(gate[2])); a.w *= sigmoidf_(bf2f(gate[3]));
+      float m = top;
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) m = fmaxf(m, v[e].x);
+      const float f0 = top == -INFINITY ? 0.f : sk_exp2(top - m);
+      sum = top == -INFINITY ? sum : sum * f0;                       // (a sum that is no number stays one)
+      a.x *= f0; a.y *= f0; a.z *= f0; a.w *= f0;
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e) {
+        const float l = v[e].y, f = v[e].x == -INFINITY ? 0.f : sk_exp2(v[e].x - m);
+        sum += v[e].x == -INFINITY ? (l != l ? l : 0.f) : l * f;
+        a.x = fmaf(x[e].x, f, a.x); a.y = fmaf(x[e].y, f, a.y); a.z = fmaf(x[e].z, f, a.z); a.w = fmaf(x[e].w, f, a.w);
+      }
+      top = m;
     }
-    *reinterpret_cast<uint2*>(out + ((long)row * nkv * share + h) * hd + d) = make_uint2(pack_bf2(a.x, a.y), pack_bf2(a.z, a.w));
   }
+  if (d == 0) {
+    top_s[part] = top;
+    sum_s[part] = sum;
+  }
+  if (part) o_s[part][d / 4] = a;
+  __syncthreads();
+  if (part) return;
+  float all = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) all = fmaxf(all, top_s[p]);
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    const float m = top_s[p], f = m == -INFINITY ? 0.f : sk_exp2(m - all), s = sum_s[p];
+    const float4 x = p ? o_s[p][d / 4] : a;
+    total += m == -INFINITY ? (s != s ? s : 0.f) : s * f;
+    if (p == 0) a = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+    else a = make_float4(fmaf(x.x, f, a.x), fmaf(x.y, f, a.y), fmaf(x.z, f, a.z), fmaf(x.w, f, a.w));
+  }
+  if (lse && d == 0) lse[(long)row * nkv * share + h] = n <= 0 ? -INFINITY : (all + log2f(total)) * 0.6931471805599453f;
+  if (!out) return;
+  const float inv = n <= 0 ? 0.f : total == 0.f ? NAN : 1.f / total;  // (scores of minus infinity only: 0 / 0)
+  a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
+  if (proj) {
+    a.x *= sigmoidf_(gate.x); a.y *= sigmoidf_(gate.y); a.z *= sigmoidf_(gate.z); a.w *= sigmoidf_(gate.w);
+  }
+  *reinterpret_cast<uint2*>(out + ((long)row * nkv * share + h) * HD + d) = make_uint2(pack_bf2(a.x, a.y), pack_bf2(a.z, a.w));
 }
 
 }  // namespace fb
@@ -573,13 +621,11 @@ static long sa_space(SaSpace* w, float* ws, int rows, int nseg, int max_rows, in
   SaSpace v{};
   v.head = (long long*)take(4);
   v.table = (SharedBlock*)take((gb + sb) * 8);
-  v.rows = (int*)take(2l * rows);
-  v.ml_grp = (float4*)take(recs[0] * 4);
-  v.ml_seg = (float4*)take(recs[1] * 4);
+  v.rows = (int4*)take(8l * rows);
+  v.ml_grp = take(recs[0] * SA_ML);
+  v.ml_seg = take(recs[1] * SA_ML);
   v.o_grp = take(want_out ? recs[0] * hd : 0);
   v.o_seg = take(want_out ? recs[1] * hd : 0);
-  v.max_blocks = (int)std::min(gb + sb, 0x7fffffffl);
-  v.max_group_blocks = (int)std::min(gb, 0x7fffffffl);
   v.seg_pairs = (int)pairs;
   if (w) *w = v;
   return at - ws;
@@ -593,10 +639,11 @@ extern "C" long fb_attention_shared_floats(int rows, int nseg, int max_rows, int
 extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_floats, const void* q, long q_stride, const void* k, const void* v,
                                    const void* proj, long proj_stride, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
   if (st.rows <= 0 || st.nseg <= 0) return 0;
-  if (nkv < 1 || nq % nkv || nq / nkv > SA_PAIRS || st.kv_block % SA_KT || st.nseg > SK_SEGS || st.ngrp > SK_SEGS || ctas < 1) return -1;
+  if (nkv < 1 || nq % nkv || nq / nkv > SA_PAIRS || st.kv_block % SA_KT || ctas < 1) return -1;
   SaSpace w;
   if (ws_floats < sa_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, out != nullptr)) return -3;
-  if (st.rows / (SA_PAIRS / (nq / nkv)) * (st.ngrp ? 2l : 1l) > SK_BLOCKS - st.nseg - st.ngrp) return -2;        // more rows than a plan has room for
+  const int R = SA_PAIRS / (nq / nkv);
+  if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, R), shared_seg_blocks(st.rows, st.nseg, st.max_rows, R), &w.z)) return -2;
   const int share = nq / nkv;
   const float scale = 1.4426950408889634f / sqrtf((float)hd);
   CUtensorMap tmK, tmV;
@@ -608,14 +655,20 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
 #define FB_SA(H, OUTV)                                                                                                                              \
   if (hd == H && (out != nullptr) == OUTV) {                                                                                                        \
     auto kern = shared_attn_kernel<H, OUTV>;                                                                                                        \
-    const size_t smem = SaCfg<H, OUTV>::MISC_AT + sizeof(SaMisc);                                                                                   \
-    static_assert(SaCfg<H, OUTV>::MISC_AT + sizeof(SaMisc) <= 232448, "shared memory of an SM");                                                    \
+    using C = SaCfg<H, OUTV>;                                                                                                                       \
+    const size_t smem = C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>);                                                                                   \
+    static_assert(C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>) <= 232448, "shared memory of an SM");                                                    \
     FB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                                              \
     e = launch_pdl(kern, dim3(ctas), dim3(SA_THREADS), smem, s, tmK, tmV, (const __nv_bfloat16*)q, q_stride, st, w, nkv, share, scale, status);     \
   }
   FB_SA(64, true) FB_SA(128, true) FB_SA(256, true) FB_SA(64, false) FB_SA(128, false) FB_SA(256, false)
 #undef FB_SA
   if (e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(shared_join_kernel, dim3(st.rows, nkv), dim3(256), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj, proj_stride, st, w,
-                         nkv, share, hd, ctas);
+#define FB_SJ(H)                                                                                                                                    \
+  if (hd == H)                                                                                                                                      \
+    return (int)launch_pdl(shared_join_kernel<H>, dim3(st.rows, nq), dim3(256), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj,         \
+                           proj_stride, st, w, nkv, share, ctas);
+  FB_SJ(64) FB_SJ(128) FB_SJ(256)
+#undef FB_SJ
+  return -2;
 }

@@ -10,14 +10,13 @@
 
 namespace fb {
 
-constexpr int SK_SEGS = 4096;                    // segments, and groups, of a step
-constexpr int SK_BLOCKS = 12000;                 // blocks of a step
-constexpr int SK_PLAN_BYTES = (3 * SK_SEGS + 2 * SK_BLOCKS) * 4;   // shared memory that the plan takes while it is made
+constexpr int SK_PLAN_BYTES = 160 << 10;         // shared memory that the plan may take while it is made
 
-// What a block is. kmin: keys that all of its rows see. tile0: key tiles of the blocks ahead of it (of one kv head).
+// What a block is. kmin: keys that all of its rows see. place0: places of the blocks ahead of it (of one kv head): a unit has one for every key tile and,
+// ahead of them, `extra` for what it costs besides.
 struct __align__(16) SharedBlock {
   int row0, nrows, slot, k0;
-  int k1, kmin, tile0, nt;
+  int k1, kmin, place0, nt;
 };
 
 __device__ __forceinline__ long table_limit(const FbSharedStep& st) { return (long)st.max_blocks * st.kv_block; }
@@ -51,7 +50,8 @@ __device__ __forceinline__ int group_of_segment(const FbSharedStep& st, int seg,
   return -1;
 }
 
-// a[0 .. n) -> sums of what lies ahead, in place; returns the sum of all. Every thread of the CTA calls it; tmp: a place for each warp and one more.
+// a[0 .. n) -> sums of what lies ahead, in place; returns the sum of all. Every thread of the CTA calls it, with what it reads written ahead of a barrier;
+// ends with a barrier. tmp: a place for each warp.
 template <int THREADS>
 __device__ __forceinline__ long long scan_ahead(int* a, int n, long long* tmp) {
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, per = (n + THREADS - 1) / THREADS;
@@ -66,135 +66,165 @@ __device__ __forceinline__ long long scan_ahead(int* a, int n, long long* tmp) {
   }
   if (lane == 31) tmp[warp] = x;
   __syncthreads();
-  if (tid == 0) {
-    long long all = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      const long long y = tmp[w];
-      tmp[w] = all;
-      all += y;
-    }
-    tmp[THREADS / 32] = all;
+  const long long own = lane < THREADS / 32 ? tmp[lane] : 0;
+  long long ahead = lane < warp ? own : 0, all = own;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
   }
-  __syncthreads();
-  long long at = tmp[warp] + x - sum;
+  long long at = ahead + x - sum;
   for (int i = lo; i < hi; ++i) {
     const int v = a[i];
     a[i] = (int)min(at, 0x7fffffffll);
     at += v;
   }
-  const long long all = tmp[THREADS / 32];
   __syncthreads();
   return all;
 }
 
-// The plan of a step, made by all threads of a CTA in shared memory. start: first block of every span (groups, then segments) and, behind them, the group of
-// every segment; span, tile: span of every block, tiles ahead of it.
+// Where the plan of a step lies in shared memory: the step's tables, which are read from global memory once, all at the same time, and what is made of them.
+// kv: the rows' contexts too, where there is room for them.
+struct SharedPlanSizes {
+  int blocks, group_blocks;                      // room for: all, those of groups
+  bool kv;
+};
+inline bool shared_plan_sizes(const FbSharedStep& st, long group_blocks, long seg_blocks, SharedPlanSizes* z) {
+  const long words = 5l * st.nseg + 4l * st.ngrp + 2 * (group_blocks + seg_blocks), room = SK_PLAN_BYTES / 4;
+  *z = {(int)(group_blocks + seg_blocks), (int)group_blocks, words + st.rows <= room};
+  return words <= room;
+}
+
 template <int THREADS>
 struct SharedPlan {
-  int *start, *group, *span, *tile;
+  int *slot, *row0, *rows, *group;               // of segments
+  int *seg0, *segs, *len;                        // of groups
+  int *start, *span, *place;                     // first block of every span (groups, then segments); span of every block, places ahead of it
+  const int* kvlen;
   int blocks, group_blocks;
-  long long tiles;                               // of one kv head
+  long long places;                              // of one kv head
 
   // -> false where the step does not fit (with a status)
-  __device__ __forceinline__ bool make(const FbSharedStep& st, int R, int kt, int max_group_blocks, int max_seg_blocks, unsigned char* smem, long long* tmp,
-                                       int* status) {
-    const int tid = threadIdx.x;
-    start = reinterpret_cast<int*>(smem);
-    group = start + 2 * SK_SEGS;
-    span = group + SK_SEGS;
-    tile = span + SK_BLOCKS;
-    for (int s = tid; s < st.nseg; s += THREADS) group[s] = -1;
+  __device__ __forceinline__ bool make(const FbSharedStep& st, int R, int kt, int extra, const SharedPlanSizes& z, unsigned char* smem, long long* tmp, int* status) {
+    const int tid = threadIdx.x, S = st.nseg, G = st.ngrp;
+    slot = reinterpret_cast<int*>(smem); row0 = slot + S; rows = row0 + S; group = rows + S;
+    seg0 = group + S; segs = seg0 + G; len = segs + G;
+    start = len + G; span = start + S + G; place = span + z.blocks;
+    kvlen = z.kv ? place + z.blocks : st.kvlen;
+    if (z.kv) {
+      int* to = place + z.blocks;
+      for (int r = tid; r < st.rows; r += THREADS) to[r] = st.kvlen[r];
+    }
+    for (int s = tid; s < S; s += THREADS) {
+      slot[s] = st.seg_slot[s];
+      row0[s] = st.seg_row0[s];
+      rows[s] = st.seg_nrows[s];
+    }
+    for (int g = tid; g < G; g += THREADS) {
+      seg0[g] = st.grp_seg0[g];
+      segs[g] = st.grp_nsegs[g];
+      len[g] = st.grp_len[g];
+    }
     __syncthreads();
-    for (int g = tid; g < st.ngrp; g += THREADS) {
-      const int s0 = st.grp_seg0[g], n = st.grp_nsegs[g];
-      int rows = 0;
-      if (s0 < 0 || n < 0 || n > st.nseg - s0) {
+    for (int g = tid; g < G; g += THREADS) {
+      const int s0 = seg0[g], n = segs[g];
+      int count = 0;
+      if (s0 < 0 || n < 0 || n > S - s0) {
         set_status(status, ST_BOUNDS);
       } else if (n > 0) {
-        const int slot = st.seg_slot[s0], row0 = st.seg_row0[s0];
-        rows = st.seg_row0[s0 + n - 1] + st.seg_nrows[s0 + n - 1] - row0;
-        if (slot < 0 || slot >= st.slots || !rows_fit(st, row0, rows)) {
+        count = row0[s0 + n - 1] + rows[s0 + n - 1] - row0[s0];
+        if (slot[s0] < 0 || slot[s0] >= st.slots || !rows_fit(st, row0[s0], count)) {
           set_status(status, ST_BOUNDS);
-          rows = 0;
+          count = 0;
         }
-        for (int s = s0; s < s0 + n && rows > 0; ++s)
-          if (atomicExch(&group[s], g) >= 0) set_status(status, ST_BOUNDS);      // a segment of two groups
       }
-      start[g] = (rows + R - 1) / R;
+      start[g] = count;
     }
-    for (int s = tid; s < st.nseg; s += THREADS) {
-      const int n = st.seg_nrows[s], slot = st.seg_slot[s];
-      bool ok = slot >= 0 && slot < st.slots && rows_fit(st, st.seg_row0[s], n);
+    __syncthreads();
+    for (int s = tid; s < S; s += THREADS) {
+      int own = -1;
+      for (int g = 0; g < G; ++g)
+        if (start[g] > 0 && s >= seg0[g] && s - seg0[g] < segs[g]) {
+          if (own >= 0 || (s > seg0[g] && row0[s] != row0[s - 1] + rows[s - 1])) set_status(status, ST_BOUNDS);   // of two groups; rows that lie apart
+          own = g;
+        }
+      group[s] = own;
+      bool ok = slot[s] >= 0 && slot[s] < st.slots && rows_fit(st, row0[s], rows[s]);
       if (!ok) set_status(status, ST_BOUNDS);
-      if (ok && n > st.max_rows) {
+      if (ok && rows[s] > st.max_rows) {
         set_status(status, ST_CAPACITY);
         ok = false;
       }
-      start[st.ngrp + s] = ok ? (n + R - 1) / R : 0;
+      start[G + s] = ok ? (rows[s] + R - 1) / R : 0;
     }
     __syncthreads();
-    for (int s = tid + 1; s < st.nseg; s += THREADS)                             // the rows of a group lie side by side
-      if (group[s] >= 0 && group[s] == group[s - 1] && st.seg_row0[s] != st.seg_row0[s - 1] + st.seg_nrows[s - 1]) set_status(status, ST_BOUNDS);
-    const int spans = st.ngrp + st.nseg;
-    const long long all = scan_ahead<THREADS>(start, spans, tmp);
+    for (int g = tid; g < G; g += THREADS) {
+      segs[g] = start[g];                                                        // (from here on: rows)
+      start[g] = (start[g] + R - 1) / R;
+    }
+    __syncthreads();
+    const long long all = scan_ahead<THREADS>(start, G + S, tmp);
     blocks = (int)min(all, 0x7fffffffll);
-    group_blocks = st.nseg ? start[st.ngrp] : 0;
-    if (blocks > SK_BLOCKS || group_blocks > max_group_blocks || blocks - group_blocks > max_seg_blocks) {
+    group_blocks = start[G];
+    if (blocks > z.blocks || group_blocks > z.group_blocks || blocks - group_blocks > z.blocks - z.group_blocks) {
       if (tid == 0) set_status(status, ST_CAPACITY);
       return false;
     }
-    for (int i = tid; i < spans; i += THREADS) {
-      const int end = i + 1 < spans ? start[i + 1] : blocks;
+    for (int i = tid; i < G + S; i += THREADS) {
+      const int end = i + 1 < G + S ? start[i + 1] : blocks;
       for (int b = start[i]; b < end; ++b) span[b] = i;
     }
     __syncthreads();
-    for (int b = tid; b < blocks; b += THREADS) tile[b] = block(st, b, R, kt, status).nt;
+    for (int b = tid; b < blocks; b += THREADS) {
+      const int nt = block(st, b, R, kt, status).nt;
+      place[b] = nt ? nt + extra : 0;
+    }
     __syncthreads();
-    tiles = scan_ahead<THREADS>(tile, blocks, tmp);
+    places = scan_ahead<THREADS>(place, blocks, tmp);
     return true;
   }
-  // block b (without tile0)
+  // block b (without place0)
   __device__ __forceinline__ SharedBlock block(const FbSharedStep& st, int b, int R, int kt, int* status) const {
     const int i = span[b], s = i - st.ngrp, m = b - start[i];
     SharedBlock e;
     long most;
-    int rows;
+    int count;
     if (s < 0) {
-      const int s0 = st.grp_seg0[i], n = st.grp_nsegs[i];
-      e.slot = st.seg_slot[s0];
-      e.row0 = st.seg_row0[s0];
-      rows = st.seg_row0[s0 + n - 1] + st.seg_nrows[s0 + n - 1] - e.row0;
+      const int s0 = seg0[i];
+      e.slot = slot[s0];
+      e.row0 = row0[s0];
+      count = segs[i];
       e.k0 = 0;
-      most = max(st.grp_len[i], 0);
+      most = max(len[i], 0);
     } else {
-      e.slot = st.seg_slot[s];
-      e.row0 = st.seg_row0[s];
-      rows = st.seg_nrows[s];
-      e.k0 = group[s] < 0 ? 0 : max(st.grp_len[group[s]], 0);
+      e.slot = slot[s];
+      e.row0 = row0[s];
+      count = rows[s];
+      e.k0 = group[s] < 0 ? 0 : max(len[group[s]], 0);
       most = 0x7fffffffl;
     }
     e.row0 += m * R;
-    e.nrows = min(R, rows - m * R);
+    e.nrows = min(R, count - m * R);
     int hi = 0, lo = 0x7fffffff;
 #pragma unroll 8
     for (int r = 0; r < e.nrows; ++r) {
-      const int n = st.kvlen[e.row0 + r];
+      const int n = kvlen[e.row0 + r];
       hi = max(hi, n);
       lo = min(lo, n);
     }
     if (hi > table_limit(st)) set_status(status, ST_BOUNDS);
     e.k1 = (int)min((long)hi, min(most, table_limit(st)));
     e.kmin = max(0, min(lo, e.k1));
-    e.tile0 = 0;
+    e.place0 = 0;
     e.nt = e.k1 > e.k0 ? (e.k1 + kt - 1) / kt - e.k0 / kt : 0;
     return e;
   }
-  // block that (block, kv head) place `at` of the list of tiles belongs to
+  // block that place `at` of the list of all (block, kv head) units belongs to
   __device__ __forceinline__ int find(long long at, int heads) const {
-    int lo = 0, hi = blocks - 1;                                                 // the last one that starts at or ahead of it: it has tiles
+    int lo = 0, hi = blocks - 1;                                                 // the last one that starts at or ahead of it: it has some
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
-      if ((long long)tile[mid] * heads <= at) lo = mid;
+      if ((long long)place[mid] * heads <= at) lo = mid;
       else hi = mid - 1;
     }
     return lo;
@@ -222,12 +252,17 @@ __device__ __forceinline__ bool sk_poll(uint64_t* bar, uint32_t parity) {
   return ok;
 }
 __device__ __forceinline__ bool sk_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (sk_poll(bar, parity)) return true;
+  if (mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
 #pragma unroll 1
   while (!sk_poll(bar, parity))
     if (*abort_flag || clock64() - t0 > 1ll << 31) return false;
   return true;
+}
+// The same for two barriers at once: one that has come by already costs nothing beside the other.
+__device__ __forceinline__ bool sk_wait2(uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, volatile int* abort_flag) {
+  if (mbar_try_wait(a, pa) & mbar_try_wait(b, pb)) return true;
+  return sk_wait(a, pa, abort_flag) && sk_wait(b, pb, abort_flag);
 }
 // MN-major operand tile with the 128-byte swizzle: rows are K, 64 contiguous MN elements a row; lbo: bytes between chunks of 64 along MN, sbo between eight rows.
 __device__ __forceinline__ uint64_t sk_desc_mn128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
@@ -240,13 +275,15 @@ __device__ __forceinline__ void sk_tmem_st16(uint32_t taddr, const uint32_t (&r)
         "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-// 16 lanes x 32 columns: registers 4 c, 4 c + 1 are columns 8 c + 2 (lane % 4) and the next of TMEM lane lane / 4; 4 c + 2, 4 c + 3 those of lane / 4 + 8.
-__device__ __forceinline__ void sk_tmem_ld16x32(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
+__device__ __forceinline__ void sk_tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+// 16 lanes x 16 columns: registers 4 c, 4 c + 1 are columns 8 c + 2 (lane % 4) and the next of TMEM lane lane / 4; 4 c + 2, 4 c + 3 those of lane / 4 + 8.
+__device__ __forceinline__ void sk_tmem_ld16x16(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
 }
 
 }  // namespace fb
