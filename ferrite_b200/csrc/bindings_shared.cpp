@@ -42,7 +42,7 @@ FbSharedStep check_step(const Tensor& q, const Tensor& k, const Tensor& kvlen, c
               q.stride(2) == 1 && aligned(q, 16) && q.device() == k.device(), what, ": q is not [rows, ", nq, ", ", hd, "] bf16 with dense heads");
   TORCH_CHECK(q.size(0) * nq < (1 << 30), what, ": rows");
   TORCH_CHECK(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && table.size(1) * kv_block < std::numeric_limits<int>::max(), what, ": block_table");
-  TORCH_CHECK(max_rows >= 0 && max_rows <= std::numeric_limits<int>::max() && status.scalar_type() == torch::kInt32 && status.device() == k.device(), what,
+  TORCH_CHECK((max_rows >= 1 || seg_slot.numel() == 0 || q.size(0) == 0) && max_rows <= std::numeric_limits<int>::max() && status.scalar_type() == torch::kInt32 && status.device() == k.device(), what,
               ": max_rows, status");
   TORCH_CHECK(grp_seg0.has_value() == grp_nsegs.has_value() && grp_seg0.has_value() == grp_len.has_value(), what, ": groups");
   FbSharedStep st{};
@@ -96,6 +96,7 @@ void attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Tensor
   const char* what = "attention_mass";
   const FbSharedStep st = check_step(q, k, kvlen, table, kv_block, nq, nkv, hd, seg_slot, seg_row0, seg_nrows, max_rows, grp_seg0, grp_nsegs, grp_len,
                                      status, what);
+  TORCH_CHECK(nq / nkv <= 64, what, ": ", nq, " query heads over ", nkv, " (shares of up to 64)");
   for (const Tensor& t : {out, mass})
     TORCH_CHECK(f32(t) && t.is_contiguous() && t.dim() == 3 && t.size(0) == k.size(0) && t.size(1) == nkv && t.size(2) == kv_block &&
                 t.device() == k.device(), what, ": sums are not [pages, ", nkv, ", ", kv_block, "] fp32");

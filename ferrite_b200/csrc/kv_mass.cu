@@ -1,53 +1,656 @@
-// Weight that a step's queries gave to every cached key, added up beside the cache.
+// Weight that a step's queries gave to every cached key, added up beside the cache: out = carry * mass + sum over rows and heads of exp(q k scale - lse).
+//
+//   S^T = K Q^T      128 keys x up to 64 (row, head) pairs on tcgen05, K and Q in shared memory, S^T in TMEM
+//   w  += exp2(S^T scale - lse)    a thread a key: its TMEM lane; the sum over the pairs stays in a register, and nothing passes between threads
+//
+// Few pairs (a decode step): the queries of a group or segment stay in shared memory and its keys stream by; every key tile belongs to one CTA, which writes
+// its sums. Many pairs (a prompt): 256 keys stay and the queries stream by; the stream of a key tile is cut into chunks, whose sums a last kernel joins in
+// their order. The exponentials are 512 cycles of an SM for 128 x 64 scores, the products 768 at 256 columns (the operands' way from shared memory).
+// Every wait is bounded, as in the attention.
 #include <algorithm>
 
+#include "gemm_core.cuh"
 #include "shared_kv.cuh"
 
 namespace fb {
 
-// One CTA per (64 tokens of a group's prefix or of a segment, kv head): a warp has a key at a time and walks the rows that see it.
+constexpr int KM_KEYS = 128, KM_PAIRS = 64, KM_SETS = 4, KM_THREADS = (4 + 4 * KM_SETS) * 32, KM_EXTRA = 2;
+
 template <int HD>
-__global__ void __launch_bounds__(256) kv_mass_kernel(float* out, const float* mass, float carry, const float* lse, const __nv_bfloat16* q, long q_stride,
-                                                      const __nv_bfloat16* k, FbSharedStep st, int nq, int nkv, float scale, int* status) {
-  constexpr int E = HD / 32;
-  const int kvh = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, share = nq / nkv;
-  pdl_launch_dependents();
-  pdl_wait();
-  const int part = blockIdx.z;
-  int slot, seg0, seg1, lo, hi = 0;
-  if (part < st.ngrp) {
-    if (!group_fits(st, part, status) || st.grp_nsegs[part] == 0) return;
-    seg0 = st.grp_seg0[part];
-    seg1 = seg0 + st.grp_nsegs[part];
-    slot = st.seg_slot[seg0];
-    lo = 0;
-    hi = st.grp_len[part];
-  } else {
-    seg0 = part - st.ngrp;
-    seg1 = seg0 + 1;
-    slot = st.seg_slot[seg0];
-    const int grp = group_of_segment(st, seg0, status);
-    lo = grp < 0 ? 0 : st.grp_len[grp];
-    for (int r = st.seg_row0[seg0]; r < st.seg_row0[seg0] + st.seg_nrows[seg0]; ++r) hi = max(hi, st.kvlen[r]);
+struct KmCfg {
+  static constexpr int NCH = HD / 64, K_CH = KM_KEYS * 128, Q_CH = KM_PAIRS * 128, K_BYTES = NCH * K_CH, Q_BYTES = NCH * Q_CH;
+  static constexpr int KS = HD == 256 ? 2 : HD == 128 ? 4 : 6;                    // key tiles in shared memory
+  static constexpr int QS = HD == 256 ? 3 : HD == 128 ? 5 : 8;                    // tiles of queries
+  static constexpr int RS = HD == 256 ? 3 : 8;                                    // ... where they stream
+  static constexpr int TILES = KS * K_BYTES + QS * Q_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
+};
+template <int QS>
+struct KmMisc {
+  float nl[QS][KM_PAIRS];                        // minus a pair's logarithm (log2); minus infinity where there is no pair
+  int kvl[QS][KM_PAIRS];                         // keys that it sees
+  uint64_t bars[40];
+  uint32_t tmem;
+  int abort;
+};
+
+__device__ __forceinline__ void km_load_q(void* dst, const CUtensorMap* tm, uint64_t* bar, int x, int head, int row) {
+  tma_load_3d(dst, tm, bar, x, head, row);
+}
+
+// Sum over a tile's pairs of the weights that they give to this thread's key. cols: 32 or 64.
+template <bool MASKED>
+__device__ __forceinline__ float km_weights(uint32_t taddr, int cols, const float* nl, const int* kvl, int key, uint64_t scale2) {
+  uint64_t acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll 1
+  for (int c0 = 0; c0 < cols; c0 += 32) {
+    uint32_t r[32];
+    tmem_ld32(taddr + c0, r);
+    tmem_ld_wait();
+#pragma unroll
+    for (int c = 0; c < 32; c += 4) {
+      const float4 n = *reinterpret_cast<const float4*>(nl + c0 + c);
+      const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)));
+      const float2 b = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)));
+      float p[4] = {sk_exp2(a.x), sk_exp2(a.y), sk_exp2(b.x), sk_exp2(b.y)};
+      if (MASKED) {
+        const int4 k = *reinterpret_cast<const int4*>(kvl + c0 + c);
+        if (key >= k.x) p[0] = 0.f;
+        if (key >= k.y) p[1] = 0.f;
+        if (key >= k.z) p[2] = 0.f;
+        if (key >= k.w) p[3] = 0.f;
+      }
+      acc[0] = f2_add(acc[0], f2_pack(p[0], p[1]));
+      acc[1] = f2_add(acc[1], f2_pack(p[2], p[3]));
+    }
   }
-  if (hi > (long)st.max_blocks * st.kv_block) set_status(status, ST_BOUNDS);
-  hi = min((long)hi, (long)st.max_blocks * st.kv_block);
-  for (int j = lo + blockIdx.x * 8 + warp; j < hi; j += gridDim.x * 8) {
-    const long at = cache_row(st, slot, j, status);
-    if (at < 0) continue;
-    float kr[E], sum = 0.f;
-    for (int e = 0; e < E; ++e) kr[e] = bf2f(k[(at * nkv + kvh) * HD + e * 32 + lane]);
-    for (int s = seg0; s < seg1; ++s)
-      for (int r = st.seg_row0[s]; r < st.seg_row0[s] + st.seg_nrows[s]; ++r) {
-        if (st.kvlen[r] <= j) continue;
-        for (int h = kvh * share; h < (kvh + 1) * share; ++h) {
-          float x = 0.f;
-          for (int e = 0; e < E; ++e) x += kr[e] * bf2f(q[r * q_stride + (long)h * HD + e * 32 + lane]);
-          sum += expf(warp_sum(x) * scale - lse[(long)r * nq + h]);
+  const float2 s = f2_unpack(f2_add(acc[0], acc[1]));
+  return s.x + s.y;
+}
+
+// What a pair of a tile is: the number that leads from its scores to weights, and the keys that it sees.
+__device__ __forceinline__ void km_pair(const FbSharedStep& st, const float* lse, const SharedBlock& e, int row, int g, int head0, int nq, int share, int Rq, int c,
+                                        float* nl, int* kvl) {
+  const bool there = c < Rq * share && row < e.nrows;
+  *nl = there ? -1.4426950408889634f * lse[(long)(e.row0 + row) * nq + head0 + g] : -INFINITY;
+  *kvl = there ? st.kvlen[e.row0 + row] : 0;
+}
+
+struct KmWalk {
+  SharedBlock e;
+  int b, kvh, t, n, left;
+  const SharedBlock* table;
+  __device__ __forceinline__ void take(int at) {
+    const int m = min(e.nt + KM_EXTRA - at, left);
+    t = max(at - KM_EXTRA, 0);
+    n = max(at + m - KM_EXTRA, 0) - t;
+    left -= m;
+  }
+  __device__ __forceinline__ bool start(const SharedBlock* tab, int first, long long f0, int places, int nkv) {
+    table = tab;
+    b = first;
+    e = table[b];
+    const int at = (int)(f0 - (long long)e.place0 * nkv);
+    kvh = at / (e.nt + KM_EXTRA);
+    left = places;
+    take(at - kvh * (e.nt + KM_EXTRA));
+    return n > 0 || next(nkv);
+  }
+  __device__ __forceinline__ bool next(int nkv) {
+    if (left == 0) return false;
+    if (++kvh == nkv) {
+      kvh = 0;
+      do e = table[++b];
+      while (e.nt == 0);
+    }
+    take(0);
+    return n > 0;
+  }
+};
+
+// ---- few pairs: keys stream by resident queries ---------------------------------------------------------------------------------------------
+template <int HD>
+__global__ void __launch_bounds__(KM_THREADS, 1)
+kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, float* out, const float* mass, float carry,
+                    const float* lse, FbSharedStep st, SharedPlanSizes z, SharedBlock* table, int R, int nq, int nkv, float scale_log2, int* status) {
+  using C = KmCfg<HD>;
+  constexpr int NCH = C::NCH, KS = C::KS;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *sK = smem, *sQ = smem + KS * C::K_BYTES;
+  KmMisc<C::QS>& ms = *reinterpret_cast<KmMisc<C::QS>*>(smem + C::MISC_AT);
+  uint64_t *q_full = ms.bars, *q_done = q_full + 1, *s_full = q_full + 2, *s_empty = s_full + KM_SETS, *k_full = s_empty + KM_SETS, *k_empty = k_full + KS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
+  volatile int* abort_flag = &ms.abort;
+  pdl_launch_dependents();
+  if (smem_u32(smem) & 1023u) {
+    if (tid == 0) set_status(status, ST_BOUNDS);
+    return;
+  }
+  if (tid == 0) {
+    ms.abort = 0;
+    mbar_init(q_full, 1);
+    mbar_init(q_done, 1);
+    for (int i = 0; i < KM_SETS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ms.tmem, KM_SETS * KM_PAIRS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ms.tmem;
+  pdl_wait();
+  SharedPlan<KM_THREADS> plan;
+  const bool fits = plan.make(st, R, KM_KEYS, KM_EXTRA, z, smem, reinterpret_cast<long long*>(ms.nl), status);
+  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+  const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
+  if (f0 == f1 || per >= 1ll << 31) {
+    if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+    if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+    return;
+  }
+  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
+  for (int b = b0 + tid; b <= b1; b += KM_THREADS) {                 // (other CTAs of a block write the same)
+    SharedBlock e = plan.block(st, b, R, KM_KEYS, status);
+    e.place0 = plan.place[b];
+    table[b] = e;
+  }
+  __syncthreads();
+  // rows of a tile of queries that no copy writes are zeros
+  for (int i = tid; i < C::QS * C::Q_BYTES / 16; i += KM_THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+  __syncthreads();
+  KmWalk x;
+  if (!x.start(table, b0, f0, (int)(f1 - f0), nkv)) goto done;       // the same for the whole CTA
+  if (warp == 0) {
+    // ---- keys
+    int i = 0, stage = 0, phase = 0;
+    bool ok = true;
+    do {
+      int rows = 0;
+      for (int j = 0; j < x.n; ++j, ++i) {
+        if (j % 16 == 0) {                                           // 16 tiles' pages (two halves of 64 keys each) at a time
+          const int token = (x.e.k0 / KM_KEYS + x.t + j) * KM_KEYS + lane * 64;
+          rows = j + lane / 2 < x.n && token < x.e.k1 ? tile_row(st, x.e.slot, token, status) : -1024;
+        }
+        const int r0 = __shfl_sync(0xffffffffu, rows, (j % 16) * 2), r1 = __shfl_sync(0xffffffffu, rows, (j % 16) * 2 + 1);
+        if (i >= KS && !__all_sync(0xffffffffu, sk_wait(&k_empty[stage], phase ^ 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(&k_full[stage], C::K_BYTES);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) {
+            tma_load_2d(sK + stage * C::K_BYTES + c * C::K_CH, &tmK, &k_full[stage], x.kvh * HD + c * 64, r0);
+            tma_load_2d(sK + stage * C::K_BYTES + c * C::K_CH + C::K_CH / 2, &tmK, &k_full[stage], x.kvh * HD + c * 64, r1);
+          }
+        }
+        if (++stage == KS) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-    const size_t o = ((size_t)(at / st.kv_block) * nkv + kvh) * st.kv_block + at % st.kv_block;
-    if (lane == 0) out[o] = (carry == 0.f ? 0.f : carry * mass[o]) + sum;
+    } while (ok && x.next(nkv));
+    if (!ok && lane == 0) {
+      if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+    if (*abort_flag && lane == 0)
+      for (int j = max(0, i - KS); j < i; ++j) mbar_wait(&k_full[j % KS], (j / KS) & 1, 1u << 20);
+  } else if (warp == 2) {
+    // ---- queries of a unit, where the products of the one before it are through
+    int unit = 0;
+    bool ok = true;
+    do {
+      ok = unit == 0 || __all_sync(0xffffffffu, sk_wait(q_done, (unit - 1) & 1, abort_flag));
+      if (!ok) break;
+      const int tiles = (x.e.nrows + Rq - 1) / Rq;
+      if (lane == 0) {
+        mbar_expect_tx(q_full, tiles * NCH * Rq * share * 128);
+        for (int i = 0; i < tiles; ++i)
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) km_load_q(sQ + i * C::Q_BYTES + c * C::Q_CH, &tmQ, q_full, c * 64, x.kvh * share, x.e.row0 + i * Rq);
+      }
+      ++unit;
+    } while (x.next(nkv));
+    if (!ok && lane == 0) {
+      if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+    if (*abort_flag && lane == 0 && unit) mbar_wait(q_full, (unit - 1) & 1, 1u << 20);
+  } else if (warp == 1) {
+    // ---- products
+    const bool issue = elect_one();
+    const uint32_t aK = smem_u32(sK), aQ = smem_u32(sQ);
+    int i = 0, stage = 0, phase = 0, unit = 0, turns[KM_SETS] = {0, 0, 0, 0};
+    bool ok = true;
+    do {
+      const int tiles = (x.e.nrows + Rq - 1) / Rq, pairs = x.e.nrows * share;
+      ok = __all_sync(0xffffffffu, sk_wait(q_full, unit & 1, abort_flag));
+      for (int j = 0; ok && j < x.n; ++j, ++i) {
+        const int set = i % KM_SETS;
+        ok = __all_sync(0xffffffffu, sk_wait(&k_full[stage], phase, abort_flag));
+        for (int t = 0; ok && t < tiles; ++t) {
+          const int turn = set == 0 ? turns[0]++ : set == 1 ? turns[1]++ : set == 2 ? turns[2]++ : turns[3]++;
+          ok = turn == 0 || __all_sync(0xffffffffu, sk_wait(&s_empty[set], (turn - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t idesc = umma_idesc(1, 1, KM_KEYS, pairs - t * Rq * share > 32 ? 64 : 32);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            tc_mma_f16_if(issue, tmem + set * KM_PAIRS, umma_desc_k128(aK + stage * C::K_BYTES + (kk >> 2) * C::K_CH + (kk & 3) * 32),
+                          umma_desc_k128(aQ + t * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+          tc_commit_if(issue, &s_full[set]);
+        }
+        if (!ok) break;
+        tc_commit_if(issue, &k_empty[stage]);
+        if (++stage == KS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      tc_commit_if(issue, q_done);
+      ++unit;
+    } while (x.next(nkv));
+    if (!ok) {
+      if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  } else if (warp >= 4) {
+    // ---- weights: set i % 4 of four warps has key tile i with all of its pairs
+    const int quad = warp & 3, set = (warp - 4) >> 2, st_tid = tid - 128, place = quad * 32 + lane;
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + set * KM_PAIRS;
+    const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
+    bool dead = false;
+    int first = 0, turn = 0;
+    do {
+      const int tiles = (x.e.nrows + Rq - 1) / Rq, pairs = x.e.nrows * share;
+      asm volatile("bar.sync 1, 512;" ::: "memory");                 // everyone is through with the pairs before these
+      for (int c = st_tid; c < tiles * KM_PAIRS; c += 512) {
+        const int t = c / KM_PAIRS, p = c % KM_PAIRS, r = p / share;
+        km_pair(st, lse, x.e, t * Rq + r, p - r * share, x.kvh * share, nq, share, Rq, p, &ms.nl[t][p], &ms.kvl[t][p]);
+      }
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      for (int j = (set - first) & (KM_SETS - 1); j < x.n; j += KM_SETS) {
+        const int key0 = (x.e.k0 / KM_KEYS + x.t + j) * KM_KEYS, key = key0 + place;
+        const bool mine = key >= x.e.k0 && key < x.e.k1, masked = key0 + KM_KEYS > x.e.kmin;
+        size_t at = 0;
+        float was = 0.f;
+        bool write = mine;
+        if (mine) {
+          const int page = st.table[(size_t)x.e.slot * st.max_blocks + key / st.kv_block];
+          write = page >= 0 && page < st.pages;                      // (else the loader has set the status)
+          at = ((size_t)(write ? page : 0) * nkv + x.kvh) * st.kv_block + key % st.kv_block;
+          if (carry != 0.f && write) was = carry * mass[at];
+        }
+        float sum = 0.f;
+        for (int t = 0; t < tiles; ++t, ++turn) {
+          if (!dead && !__all_sync(0xffffffffu, sk_wait(&s_full[set], turn & 1, abort_flag))) {
+            dead = true;
+            if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+            *abort_flag = 1;
+          }
+          if (dead) continue;
+          tc_fence_after();
+          const int left = pairs - t * Rq * share, cols = left > 32 ? 64 : 32;
+          sum += masked || left < Rq * share ? km_weights<true>(taddr, cols, ms.nl[t], ms.kvl[t], key, scale2)
+                                             : km_weights<false>(taddr, cols, ms.nl[t], ms.kvl[t], key, scale2);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_empty[set]);
+        }
+        if (write && !dead) out[at] = was + sum;
+      }
+      first += x.n;
+    } while (x.next(nkv));
+  }
+done:
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+}
+
+// ---- many pairs: queries stream by 256 resident keys -----------------------------------------------------------------------------------------
+constexpr int KP_KEYS = 2 * KM_KEYS, KP_PLAN = 1024, KP_CHUNKS = 1024;   // keys of an item; threads of the plan; chunks beside one an item
+
+struct KpItem {                                  // 256 keys of a span
+  int slot, key0, k0, k1;                        // its keys: key0 .. key0 + 255, those of k0 .. k1 count
+  int chunk0, chunks, pad0, pad1;
+};
+struct KpChunk {                                 // of an item: of blocks b0 .. b1 those that see it, `steps` in number
+  int item, b0, b1, steps;
+};
+struct KpSpace {
+  int* head;                                     // items, chunks
+  SharedBlock* blocks;
+  KpItem* items;
+  KpChunk* chunks;
+  float* sums;                                   // [chunks][kv heads][sets][keys of a tile]
+  int max_items;
+  SharedPlanSizes z;
+};
+
+// One CTA: blocks of 64 pairs, items, chunks.
+__global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, KpSpace w, int Rq, int nkv, int ctas, int* status) {
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ long long tmp[32];
+  __shared__ int chunk_s;
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+  SharedPlan<KP_PLAN> plan;
+  const bool fits = plan.make(st, Rq, KP_KEYS, 0, w.z, smem, tmp, status);
+  if (!fits) {
+    if (tid == 0) w.head[0] = w.head[1] = 0;
+    return;
+  }
+  for (int b = tid; b < plan.blocks; b += KP_PLAN) w.blocks[b] = plan.block(st, b, Rq, KP_KEYS, status);
+  __syncthreads();
+  const int spans = st.ngrp + st.nseg;
+  auto first = [&](int i) { return plan.start[i]; };
+  auto behind = [&](int i) { return i + 1 < spans ? plan.start[i + 1] : plan.blocks; };
+  // items of a span: as many as its longest block has (their numbers take the place of the blocks' places)
+  for (int i = tid; i < spans; i += KP_PLAN) {
+    int most = 0;
+    for (int b = first(i); b < behind(i); ++b) most = max(most, w.blocks[b].nt);
+    plan.place[i] = most;
+  }
+  __syncthreads();
+  const long long all = scan_ahead<KP_PLAN>(plan.place, spans, tmp);
+  const int total = (int)min(all, (long long)w.max_items + 1);
+  if (total > w.max_items) {
+    if (tid == 0) {
+      set_status(status, ST_CAPACITY);
+      w.head[0] = w.head[1] = 0;
+    }
+    return;
+  }
+  if (tid == 0) chunk_s = (int)max(8ll, min(64ll, (plan.places * nkv + ctas * 8 - 1) / (ctas * 8)));
+  __syncthreads();
+  // steps of a chunk: eight chunks a CTA where there are enough, no fewer than 8 steps and no more than KP_CHUNKS chunks more than items
+  const int C = (int)max((long long)chunk_s, (plan.places + KP_CHUNKS - 1) / KP_CHUNKS);
+  int base = 0;
+  for (int i0 = 0; i0 < total; i0 += KP_PLAN) {
+    const int it = i0 + tid;
+    int lo = 0, hi = spans - 1, n = 0;
+    KpItem e{};
+    if (it < total) {
+      while (lo < hi) {                                              // the last span that starts at or ahead of the item
+        const int mid = (lo + hi + 1) / 2;
+        if (plan.place[mid] <= it) lo = mid;
+        else hi = mid - 1;
+      }
+      const int j = it - plan.place[lo];
+      int k1 = 0;
+      for (int b = first(lo); b < behind(lo); ++b) {
+        const SharedBlock blk = w.blocks[b];
+        e.slot = blk.slot;
+        e.k0 = blk.k0;
+        k1 = max(k1, blk.k1);
+        n += blk.nt > j;
+      }
+      e.k1 = k1;
+      e.key0 = (e.k0 / KP_KEYS + j) * KP_KEYS;
+      e.chunks = (n + C - 1) / C;
+    }
+    // numbers of the chunks: a scan over the threads
+    const int lane = tid & 31, warp = tid >> 5;
+    int xs = e.chunks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, xs, o);
+      if (lane >= o) xs += y;
+    }
+    if (lane == 31) tmp[warp] = xs;
+    __syncthreads();
+    int ahead = 0, sum = 0;
+    for (int k = 0; k < 32; ++k) {
+      ahead += k < warp ? (int)tmp[k] : 0;
+      sum += (int)tmp[k];
+    }
+    __syncthreads();
+    if (it < total) {
+      e.chunk0 = base + ahead + xs - e.chunks;
+      w.items[it] = e;
+      const int j = it - plan.place[lo];
+      int seen = 0, from = first(lo);
+      for (int b = first(lo); b < behind(lo); ++b)
+        if (w.blocks[b].nt > j) {
+          if (seen % C == 0) from = b;
+          ++seen;
+          if (seen % C == 0 || seen == n) w.chunks[e.chunk0 + (seen - 1) / C] = KpChunk{it, from, b + 1, (seen - 1) % C + 1};
+        }
+    }
+    base += sum;
+  }
+  if (tid == 0) {
+    w.head[0] = total;
+    w.head[1] = base;
+  }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(KM_THREADS, 1)
+kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const float* lse, FbSharedStep st, KpSpace w, int nq,
+                    int nkv, float scale_log2, int* status) {
+  using C = KmCfg<HD>;
+  constexpr int NCH = C::NCH, QS = C::RS;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *sK = smem, *sQ = smem + 2 * C::K_BYTES;
+  KmMisc<QS>& ms = *reinterpret_cast<KmMisc<QS>*>(smem + 2 * C::K_BYTES + QS * C::Q_BYTES);
+  uint64_t *k_full = ms.bars, *k_empty = k_full + 1, *s_full = k_full + 2, *s_empty = s_full + KM_SETS, *q_full = s_empty + KM_SETS, *q_empty = q_full + QS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
+  volatile int* abort_flag = &ms.abort;
+  pdl_launch_dependents();
+  if (smem_u32(smem) & 1023u) {
+    if (tid == 0) set_status(status, ST_BOUNDS);
+    return;
+  }
+  if (tid == 0) {
+    ms.abort = 0;
+    mbar_init(k_full, 1);
+    mbar_init(k_empty, 1);
+    for (int i = 0; i < KM_SETS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); }
+    for (int i = 0; i < QS; ++i) { mbar_init(&q_full[i], 2); mbar_init(&q_empty[i], 9); }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ms.tmem, KM_SETS * KM_PAIRS);
+    tmem_relinquish();
+  }
+  for (int i = tid; i < QS * C::Q_BYTES / 16; i += KM_THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ms.tmem;
+  pdl_wait();
+  const int units = w.head[1] * nkv;
+  // a CTA's chunks: every gridDim-th; steps: the chunk's blocks that see the item
+  auto unit = [&](int u, KpChunk* ch, KpItem* it) {
+    *ch = w.chunks[u / nkv];
+    *it = w.items[ch->item];
+    return u % nkv;
+  };
+  auto sees = [&](const SharedBlock& e, const KpItem& it) { return e.nt > it.key0 / KP_KEYS - it.k0 / KP_KEYS; };
+  if (warp == 0) {
+    // ---- keys
+    int n = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
+      KpChunk ch;
+      KpItem it;
+      const int kvh = unit(u, &ch, &it);
+      const int token = it.key0 + lane * 64, rows = lane < 4 && token < it.k1 ? tile_row(st, it.slot, token, status) : -1024;
+      ok = n == 0 || __all_sync(0xffffffffu, sk_wait(k_empty, (n - 1) & 1, abort_flag));
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(k_full, 2 * C::K_BYTES);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = __shfl_sync(0xffffffffu, rows, k);
+        if (lane == 0)
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+            tma_load_2d(sK + (k / 2) * C::K_BYTES + c * C::K_CH + (k % 2) * (C::K_CH / 2), &tmK, k_full, kvh * HD + c * 64, row);
+      }
+    }
+    if (!ok && lane == 0) {
+      if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+    if (*abort_flag && lane == 0 && n) mbar_wait(k_full, (n - 1) & 1, 1u << 20);
+  } else if (warp == 2 || warp == 3) {
+    // ---- tiles of queries (warp 2), what their pairs are (warp 3)
+    int i = 0, stage = 0, phase = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
+      KpChunk ch;
+      KpItem it;
+      const int kvh = unit(u, &ch, &it);
+      for (int b = ch.b0; b < ch.b1; ++b) {
+        const SharedBlock e = w.blocks[b];
+        if (!sees(e, it)) continue;
+        ok = i < QS || __all_sync(0xffffffffu, sk_wait(&q_empty[stage], phase ^ 1, abort_flag));
+        if (!ok) break;
+        if (warp == 2) {
+          if (lane == 0) {
+            mbar_expect_tx(&q_full[stage], NCH * Rq * share * 128);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) km_load_q(sQ + stage * C::Q_BYTES + c * C::Q_CH, &tmQ, &q_full[stage], c * 64, kvh * share, e.row0);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int p = lane + 32 * h, r = p / share;
+            km_pair(st, lse, e, r, p - r * share, kvh * share, nq, share, Rq, p, &ms.nl[stage][p], &ms.kvl[stage][p]);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[stage]);
+        }
+        ++i;
+        if (++stage == QS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok && lane == 0) {
+      if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+    if (warp == 2 && *abort_flag && lane == 0)
+      for (int j = max(0, i - QS); j < i; ++j) mbar_wait(&q_full[j % QS], (j / QS) & 1, 1u << 20);
+  } else if (warp == 1) {
+    // ---- products: a tile of queries with both tiles of keys
+    const bool issue = elect_one();
+    const uint32_t aK = smem_u32(sK), aQ = smem_u32(sQ), idesc = umma_idesc(1, 1, KM_KEYS, KM_PAIRS);
+    int i = 0, n = 0, stage = 0, phase = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
+      KpChunk ch;
+      KpItem it;
+      unit(u, &ch, &it);
+      ok = __all_sync(0xffffffffu, sk_wait(k_full, n & 1, abort_flag));
+      for (int j = 0; ok && j < ch.steps; ++j, ++i) {
+        ok = __all_sync(0xffffffffu, sk_wait(&q_full[stage], phase, abort_flag));
+        for (int a = 0; ok && a < 2; ++a) {
+          const int f = 2 * i + a, set = f % KM_SETS;
+          ok = f < KM_SETS || __all_sync(0xffffffffu, sk_wait(&s_empty[set], (f / KM_SETS - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            tc_mma_f16_if(issue, tmem + set * KM_PAIRS, umma_desc_k128(aK + a * C::K_BYTES + (kk >> 2) * C::K_CH + (kk & 3) * 32),
+                          umma_desc_k128(aQ + stage * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+          tc_commit_if(issue, &s_full[set]);
+        }
+        if (!ok) break;
+        tc_commit_if(issue, &q_empty[stage]);
+        if (++stage == QS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      tc_commit_if(issue, k_empty);
+    }
+    if (!ok) {
+      if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  } else {
+    // ---- weights: sets 0 and 2 have the first 128 keys, with every other tile of queries each, 1 and 3 the others
+    const int quad = warp & 3, set = (warp - 4) >> 2, place = quad * 32 + lane;
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + set * KM_PAIRS;
+    const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
+    bool dead = false;
+    int i = 0;                                                       // tiles of queries of the CTA so far
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      KpChunk ch;
+      KpItem it;
+      const int kvh = unit(u, &ch, &it);
+      const int key = it.key0 + (set & 1) * KM_KEYS + place, last = key - place + KM_KEYS;
+      float sum = 0.f;
+      int b = ch.b0;
+      SharedBlock e = w.blocks[b];
+      for (int j = 0; j < ch.steps; ++j, ++i, ++b) {
+        while (!sees(e, it)) e = w.blocks[++b];
+        const SharedBlock now = e;
+        if (j + 1 < ch.steps) e = w.blocks[b + 1];
+        if ((i & 1) != set >> 1) continue;
+        const int f = 2 * i + (set & 1), stage = i % QS;
+        if (!dead && !__all_sync(0xffffffffu, sk_wait(&s_full[set], (f / KM_SETS) & 1, abort_flag))) {
+          dead = true;
+          if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+          *abort_flag = 1;
+        }
+        if (dead) continue;
+        tc_fence_after();
+        // (the pairs' numbers came with the tile: the products have waited for both)
+        sum += last > now.kmin || now.nrows < Rq ? km_weights<true>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2)
+                                                 : km_weights<false>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&s_empty[set]);
+          mbar_arrive(&q_empty[stage]);
+        }
+      }
+      if (!dead) w.sums[((size_t)u * KM_SETS + set) * KM_KEYS + place] = sum;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+}
+
+// An item's sums of all chunks, in order, into the cache's. grid: items x kv heads, a thread a key.
+__global__ void __launch_bounds__(KP_KEYS) kv_mass_join_kernel(float* out, const float* mass, float carry, FbSharedStep st, KpSpace w, int nkv, int* status) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int items = w.head[0];
+  for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    const KpItem it = w.items[i];
+    const int kvh = blockIdx.y, key = it.key0 + threadIdx.x;
+    if (key < it.k0 || key >= it.k1) continue;
+    const int page = st.table[(size_t)it.slot * st.max_blocks + key / st.kv_block];
+    if (page < 0 || page >= st.pages) {
+      set_status(status, ST_BOUNDS);
+      continue;
+    }
+    const size_t at = ((size_t)page * nkv + kvh) * st.kv_block + key % st.kv_block;
+    const int set = threadIdx.x / KM_KEYS, place = threadIdx.x % KM_KEYS;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < it.chunks; ++c) {
+      const float* s = w.sums + (((size_t)(it.chunk0 + c) * nkv + kvh) * KM_SETS + set) * KM_KEYS + place;
+      sum += s[0] + s[2 * KM_KEYS];
+    }
+    out[at] = (carry != 0.f ? carry * mass[at] : 0.f) + sum;
   }
 }
 
@@ -55,26 +658,100 @@ __global__ void __launch_bounds__(256) kv_mass_kernel(float* out, const float* m
 
 using namespace fb;
 
-extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int ctas) {
-  return ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, 64, ctas, 0);
+// Tensor map of the queries [rows][heads][HD]: a copy brings 64 columns of Rq rows' heads of a kv head.
+static int make_tmap_queries(CUtensorMap* out, const void* q, int rows, int nq, int hd, long stride, int share, int Rq) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -10;
+  if ((uintptr_t)q % 16 || stride * 2 % 16) return -11;
+  cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)nq, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)share, (cuuint32_t)Rq}, estr[3] = {1, 1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -12;
+}
+// Rows whose queries stay in shared memory
+static int km_resident_rows(int hd, int share) { return (hd == 256 ? KmCfg<256>::QS : hd == 128 ? KmCfg<128>::QS : KmCfg<64>::QS) * (KM_PAIRS / share); }
+static bool km_few(int rows, int max_rows, int ngrp, int hd, int share) { return (ngrp ? rows : std::min(rows, max_rows)) <= km_resident_rows(hd, share); }
+static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room) {
+  const int Rq = KM_PAIRS / share;
+  const long blocks = shared_group_blocks(rows, ngrp, Rq) + shared_seg_blocks(rows, nseg, max_rows, Rq), items = (long)(nseg + ngrp) * ((room + KP_KEYS - 1) / KP_KEYS + 1);
+  float* at = ws;
+  auto take = [&](long floats) {
+    float* p = at;
+    at += (floats + 3) / 4 * 4;
+    return p;
+  };
+  KpSpace v{};
+  v.head = (int*)take(4);
+  v.blocks = (SharedBlock*)take(blocks * 8);
+  v.items = (KpItem*)take(items * 8);
+  v.chunks = (KpChunk*)take((items + KP_CHUNKS) * 4);
+  v.sums = take((items + KP_CHUNKS) * nkv * KM_SETS * KM_KEYS);
+  v.max_items = (int)std::min(items, 0x7fffffffl);
+  if (w) *w = v;
+  return at - ws;
+}
+
+extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, long room, int want_lse, int ctas) {
+  if (rows <= 0 || nseg <= 0 || nkv < 1 || nq / nkv < 1 || nq / nkv > KM_PAIRS) return 0;
+  const int share = nq / nkv;
+  const long logs = want_lse ? ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, 0) : 0;
+  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room));
 }
 
 extern "C" int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride,
                                  const void* k, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
-  if (st.rows <= 0 || st.nseg <= 0) return 0;
+  if (st.rows <= 0 || st.nseg <= 0 || st.max_rows <= 0) return 0;
+  if (nkv < 1 || nq % nkv || nq / nkv > KM_PAIRS || st.kv_block % 64 || ctas < 1 || (hd != 64 && hd != 128 && hd != 256)) return -1;
+  const long room = (long)st.max_blocks * st.kv_block;
+  if (ws_floats < fb_attention_mass_floats(st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, room, !lse, ctas)) return -3;
+  const int share = nq / nkv, Rq = KM_PAIRS / share;
+  int rc;
   if (!lse) {
-    const long used = ((long)st.rows * nq + 3) / 4 * 4;
-    const int rc = fb_attention_shared(nullptr, ws, ws + used, ws_floats - used, q, q_stride, k, k, nullptr, 0, st, nq, nkv, hd, ctas, status, s);
-    if (rc) return rc;
+    const long used = ((long)st.rows * nq + 3) / 4 * 4, more = fb_attention_shared_floats(st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, 0);
+    if ((rc = fb_attention_shared(nullptr, ws, ws + used, more, q, q_stride, k, k, nullptr, 0, st, nq, nkv, hd, ctas, status, s))) return rc;
     lse = ws;
+    ws += used + more;
   }
-  const dim3 grid(std::min(256, (st.max_blocks * st.kv_block + 7) / 8), nkv, st.ngrp + st.nseg);
-  const float scale = 1.f / sqrtf((float)hd);
-#define FB_KM(H)                                                                                                                                  \
-  if (hd == H)                                                                                                                                    \
-    return (int)launch_pdl(kv_mass_kernel<H>, grid, dim3(256), 0, s, out, mass, carry, lse, (const __nv_bfloat16*)q, q_stride,                    \
-                           (const __nv_bfloat16*)k, st, nq, nkv, scale, status);
-  FB_KM(64) FB_KM(128) FB_KM(256)
+  const float scale = 1.4426950408889634f / sqrtf((float)hd);
+  CUtensorMap tmK, tmQ;
+  const uint64_t cache_rows = (uint64_t)st.pages * st.kv_block, width = (uint64_t)nkv * hd;
+  if ((rc = make_tmap_bf16_2d(&tmK, k, cache_rows, width, width, 64))) return rc;
+  if ((rc = make_tmap_queries(&tmQ, q, st.rows, nq, hd, st.rows > 1 ? q_stride : (long)nq * hd, share, Rq))) return rc;
+  cudaError_t e = cudaErrorInvalidValue;
+  if (km_few(st.rows, st.max_rows, st.ngrp, hd, share)) {
+    const int R = km_resident_rows(hd, share);
+    SharedPlanSizes z;
+    if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, R), shared_seg_blocks(st.rows, st.nseg, st.max_rows, R), &z)) return -2;
+#define FB_KM(H)                                                                                                                                       \
+  if (hd == H) {                                                                                                                                       \
+    using C = KmCfg<H>;                                                                                                                                \
+    const size_t smem = C::MISC_AT + sizeof(KmMisc<C::QS>);                                                                                            \
+    static_assert(C::MISC_AT + sizeof(KmMisc<C::QS>) <= 232448, "shared memory of an SM");                                                             \
+    FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_keys_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                               \
+    e = launch_pdl(kv_mass_keys_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, out, mass, carry, lse, st, z, (SharedBlock*)ws, R, nq,     \
+                   nkv, scale, status);                                                                                                                \
+  }
+    FB_KM(64) FB_KM(128) FB_KM(256)
 #undef FB_KM
-  return -2;
+    return (int)e;
+  }
+  KpSpace w;
+  km_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nkv, share, room);
+  if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, Rq), shared_seg_blocks(st.rows, st.nseg, st.max_rows, Rq), &w.z)) return -2;
+  FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_PLAN_BYTES));
+  if ((e = launch_pdl(kv_mass_plan_kernel, dim3(1), dim3(KP_PLAN), SK_PLAN_BYTES, s, st, w, Rq, nkv, ctas, status)) != cudaSuccess) return (int)e;
+#define FB_KP(H)                                                                                                                                       \
+  if (hd == H) {                                                                                                                                       \
+    using C = KmCfg<H>;                                                                                                                                \
+    const size_t smem = 2 * C::K_BYTES + C::RS * C::Q_BYTES + sizeof(KmMisc<C::RS>);                                                                   \
+    static_assert(2 * C::K_BYTES + C::RS * C::Q_BYTES + sizeof(KmMisc<C::RS>) <= 232448, "shared memory of an SM");                                    \
+    FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_rows_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                                \
+    e = launch_pdl(kv_mass_rows_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, lse, st, w, nq, nkv, scale, status);                        \
+  }
+  FB_KP(64) FB_KP(128) FB_KP(256)
+#undef FB_KP
+  if (e != cudaSuccess) return (int)e;
+  return (int)launch_pdl(kv_mass_join_kernel, dim3(std::min(w.max_items, 1024), nkv), dim3(KP_KEYS), 0, s, out, mass, carry, st, w, nkv, status);
 }

@@ -638,7 +638,7 @@ extern "C" long fb_attention_shared_floats(int rows, int nseg, int max_rows, int
 
 extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_floats, const void* q, long q_stride, const void* k, const void* v,
                                    const void* proj, long proj_stride, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
-  if (st.rows <= 0 || st.nseg <= 0) return 0;
+  if (st.rows <= 0 || st.nseg <= 0 || st.max_rows <= 0) return 0;
   if (nkv < 1 || nq % nkv || nq / nkv > SA_PAIRS || st.kv_block % SA_KT || ctas < 1) return -1;
   SaSpace w;
   if (ws_floats < sa_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, out != nullptr)) return -3;

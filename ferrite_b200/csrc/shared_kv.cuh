@@ -31,25 +31,6 @@ __device__ __forceinline__ int tile_row(const FbSharedStep& st, int slot, int to
 }
 __device__ __forceinline__ bool rows_fit(const FbSharedStep& st, int row0, int nrows) { return row0 >= 0 && nrows >= 0 && nrows <= st.rows - row0; }
 
-__device__ __forceinline__ long cache_row(const FbSharedStep& st, int slot, int j, int* status) {
-  const int blk = slot < 0 || slot >= st.slots || j / st.kv_block >= st.max_blocks ? -1 : st.table[(size_t)slot * st.max_blocks + j / st.kv_block];
-  if (blk < 0 || blk >= st.pages) {
-    set_status(status, ST_BOUNDS);
-    return -1;
-  }
-  return (long)blk * st.kv_block + j % st.kv_block;
-}
-__device__ __forceinline__ bool group_fits(const FbSharedStep& st, int g, int* status) {
-  if (st.grp_seg0[g] >= 0 && st.grp_nsegs[g] >= 0 && st.grp_nsegs[g] <= st.nseg - st.grp_seg0[g]) return true;
-  set_status(status, ST_BOUNDS);
-  return false;
-}
-__device__ __forceinline__ int group_of_segment(const FbSharedStep& st, int seg, int* status) {
-  for (int g = 0; g < st.ngrp; ++g)
-    if (group_fits(st, g, status) && seg >= st.grp_seg0[g] && seg < st.grp_seg0[g] + st.grp_nsegs[g]) return g;
-  return -1;
-}
-
 // a[0 .. n) -> sums of what lies ahead, in place; returns the sum of all. Every thread of the CTA calls it, with what it reads written ahead of a barrier;
 // ends with a barrier. tmp: a place for each warp.
 template <int THREADS>

@@ -60,9 +60,9 @@ class TorchShared:
         return (out, lse) if want_lse else out
 
     def attention_mass(self, q, k_cache, mass, row_kvlen, block_table, kv_block, nq, nkv, hd, segs, groups=None, lse=None, carry=1.0, out=None):
-        """Per kv head and key of the step's contexts: out = carry * mass + the sum of exp(q k / sqrt(hd) - lse) over the rows that see the key and the
-        heads that share the kv head; `out` is `mass` itself unless given, other entries stay. `lse` is that of the step's attention, or None: it is
-        computed. With carry 0 `mass` is not read."""
+        """Per kv head and key that some row sees: out = carry * mass + the sum of exp(q k / sqrt(hd) - lse) over the rows that see the key and the heads
+        that share the kv head (64 at most); `out` is `mass` itself unless given, other entries stay. `lse` is that of the step's attention, or None: it
+        is computed. With carry 0 `mass` is not read."""
         out = mass if out is None else out
         kf = k_cache.reshape(-1, nkv, hd)
         sums = torch.zeros(mass.shape[0] * kv_block, nkv, dtype=torch.float32, device=q.device)
@@ -70,8 +70,6 @@ class TorchShared:
         for s, shared_slot, shared in _spans(segs, groups):
             rows = range(int(segs[1][s]), int(segs[1][s]) + int(segs[2][s]))
             longest = max([int(row_kvlen[t]) for t in rows] + [0])
-            if groups is not None and len(rows):
-                longest = max(longest, shared)
             if longest <= 0:
                 continue
             at = _token_rows(block_table, kv_block, int(segs[0][s]), shared_slot, shared, longest)
@@ -144,7 +142,8 @@ class CudaShared:
         q, step = self._shared_step(q, nq, hd, segs, groups)
         out = mass if out is None else out
         G = 0 if groups is None else groups[0].numel()
-        ws = self.empty(self.C.attention_mass_floats(q.shape[0], segs[0].numel(), segs[3], G, nq, nkv, self.sm_count), dtype=torch.float32, device=q.device)
+        ws = self.empty(self.C.attention_mass_floats(q.shape[0], segs[0].numel(), segs[3], G, nq, nkv, hd, block_table.shape[1] * kv_block, lse is None,
+                                                     self.sm_count), dtype=torch.float32, device=q.device)
         self.launches += 1 if lse is not None else 3
         self.C.attention_mass(out, mass, float(carry), lse, ws, q, k_cache, row_kvlen, block_table, kv_block, nq, nkv, hd, *step, self.sm_count,
                               self.status_word)

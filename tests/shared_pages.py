@@ -110,10 +110,6 @@ class Step:
         seen = torch.zeros(self.k.shape[0] * self.page, dtype=torch.bool, device=self.q.device)
         for t in range(self.rows):
             seen[self.at(t)] = True
-        for gi, s in self.first.items():
-            pos = torch.arange(self.shared[gi], device=self.q.device)
-            if any(len(self.streams[i]) for i in range(len(self.streams)) if self.member[i] == gi):
-                seen[self.table[self.slots[s]][pos // self.page].long() * self.page + pos % self.page] = True
         return seen
 
     def masses(self, carry, lse=None, start=None):
