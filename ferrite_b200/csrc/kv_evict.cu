@@ -1,10 +1,11 @@
 // Eviction from a paged cache by accumulated weight: which tokens of a (stream, kv head) stay, and their move into new pages.
 //
-// A cluster of CTAs has a (segment, kv head), each CTA a run of its tokens. The weight of the last token that stays is found digit by digit, 11, 11 and 10
-// bits of the weights as whole numbers in their order: a histogram per CTA in shared memory, added up over the cluster. How many heavier tokens and how
-// many equal ones lie ahead of a token says whether it stays and where it goes (the earliest of equal ones stay), so the order of the tokens is kept without
-// a sort, and nothing depends on the order in which threads run. Then the cluster copies the rows, 32 of them a warp at a time: the lanes look up the pages, then all of
-// them copy one row after another, 16 bytes each. What bounds it is the copy: 512-byte rows from all over the pool.
+// Selection: a cluster of CTAs has a (segment, kv head), each CTA a run of its tokens. The weight of the last token that stays is found digit by digit, 11, 11
+// and 10 bits of the weights as whole numbers in their order: a histogram per CTA in shared memory, added up over the cluster (each CTA adds up a part of the
+// bins). How many heavier tokens and how many equal ones lie ahead of a token says whether it stays and where it goes (the earliest of equal ones stay), so
+// the order of the tokens is kept without a sort, and nothing depends on the order in which threads run.
+//
+// Copy: a warp has up to 32 rows at a time; its lanes look up the pages, then all of them copy row after row, 16 bytes each.
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -31,14 +32,28 @@ struct EvictArgs {
   int segs, slots, max_blocks, dst_blocks;
   long pages;
   int kv_block, nkv, row_bytes, ns, keep, first, recent;
-  int held, row_lanes;                           // weights that fit; lanes that copy a row together (a power of two)
+  int held, page_shift, row_lanes, run;          // weights that fit; log2 of kv_block, or -1; lanes that copy a row together (a power of two); rows of a warp
   int* status;
+
+  __device__ __forceinline__ int page_of(int j) const { return page_shift >= 0 ? j >> page_shift : j / kv_block; }
+  // tokens in the slot's cache, as far as its table reaches
+  __device__ __forceinline__ int tokens(int slot, int seg) const {
+    const int n = max(seg_len[seg], 0);
+    if (slot >= 0 && slot < slots && n <= (long)max_blocks * kv_block) return n;
+    set_status(status, ST_BOUNDS);
+    return slot < 0 || slot >= slots ? 0 : max_blocks * kv_block;
+  }
 };
 
 __device__ __forceinline__ int checked_page(const EvictArgs& a, int page) {
   if (page >= 0 && page < a.pages) return page;
   set_status(a.status, ST_BOUNDS);
   return -1;
+}
+// the same for a weight that no shared memory holds (contexts of more than EV_HELD tokens a CTA)
+__device__ __noinline__ uint32_t weight_of(const EvictArgs& a, const int* table, int h, int j) {
+  const int p = a.page_of(j), page = checked_page(a, table[p]);
+  return page < 0 ? 0u : weight_order(a.mass[((size_t)page * a.nkv + h) * a.kv_block + (j - p * a.kv_block)]);
 }
 // Sums of what lies ahead of a thread (low and high half apart), and of all; tmp: a place for each warp.
 __device__ __forceinline__ uint64_t scan_pairs(uint64_t mine, uint64_t* tmp, uint64_t* all) {
@@ -62,115 +77,158 @@ __device__ __forceinline__ uint64_t scan_pairs(uint64_t mine, uint64_t* tmp, uin
   return ahead;
 }
 
-__global__ void __launch_bounds__(EV_THREADS, 2) kv_evict_kernel(EvictArgs a) {
+__global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
   extern __shared__ uint32_t held_s[];
   __shared__ uint32_t hist[EV_BINS], total[EV_BINS];
   __shared__ uint64_t tmp[EV_WARPS], counts_s;
-  __shared__ uint32_t digit_s[2];
+  __shared__ uint32_t digit_s[3];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int pair = blockIdx.x / ctas, seg = pair / a.nkv, h = pair % a.nkv;
   pdl_launch_dependents();
   pdl_wait();
-  const int slot = a.seg_slot[seg];
-  int n = max(a.seg_len[seg], 0);
-  if (slot < 0 || slot >= a.slots || n > (long)a.max_blocks * a.kv_block) {
-    set_status(a.status, ST_BOUNDS);
-    n = slot < 0 || slot >= a.slots ? 0 : a.max_blocks * a.kv_block;
-  }
+  const int slot = a.seg_slot[seg], n = a.tokens(slot, seg);
   const int* table = a.table + (size_t)max(slot, 0) * a.max_blocks;
   int* kept = a.kept + (size_t)pair * a.keep;
-  const int m = min(n, a.keep);
-  for (int i = m + rank * EV_THREADS + tid; i < a.keep; i += ctas * EV_THREADS) kept[i] = -1;
-  if (n <= a.keep) {
+  for (int i = min(n, a.keep) + rank * EV_THREADS + tid; i < a.keep; i += ctas * EV_THREADS) kept[i] = -1;
+  if (n <= a.keep) {                                                 // (the same for the cluster)
     for (int i = rank * EV_THREADS + tid; i < n; i += ctas * EV_THREADS) kept[i] = i;
-  } else {
-    // ---- this CTA's tokens
-    const int per = (n + ctas - 1) / ctas, t0 = min(n, rank * per), t1 = min(n, t0 + per), lo = a.first, hi = n - a.recent;
-    const bool hold = per <= a.held;
-    auto order = [&](int j) -> uint32_t {
-      const int page = checked_page(a, table[j / a.kv_block]);
-      return page < 0 ? 0u : weight_order(a.mass[((size_t)page * a.nkv + h) * a.kv_block + j % a.kv_block]);
-    };
-    uint32_t need = (uint32_t)(a.keep - a.first - a.recent), prefix = 0, mask = 0;
-    const bool none = need == 0;
-    if (hold && !none)
-#pragma unroll 4
-      for (int j = max(t0, lo) + tid; j < min(t1, hi); j += EV_THREADS) held_s[j - t0] = order(j);
-    for (int pass = 0; pass < 3 && !none; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const uint32_t bins = pass == 2 ? 1024u : 2048u;
-      for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-      __syncthreads();
-      for (int j = max(t0, lo) + tid; j < min(t1, hi); j += EV_THREADS) {
-        const uint32_t u = hold ? held_s[j - t0] : order(j);
-        if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
+    return;
+  }
+  // ---- this CTA's tokens
+  const int per = (n + ctas - 1) / ctas, t0 = min(n, rank * per), t1 = min(n, t0 + per), lo = a.first, hi = n - a.recent;
+  const bool hold = per <= a.held;
+  auto weight = [&](int j) { return weight_of(a, table, h, j); };
+  uint32_t need = (uint32_t)(a.keep - a.first - a.recent), prefix = 0, mask = 0;
+  const bool none = need == 0;
+  const int m0 = max(t0, lo), m1 = min(t1, hi);                      // of the middle, where weights decide
+  if (hold && !none) {
+    // eight a thread: their pages first, then their weights, so that the loads of either are under way together (a page that is none counts as page 0 and
+    // is reported behind the loads)
+    bool bad = false;
+#pragma unroll 1
+    for (int j0 = m0 + tid; j0 < m1; j0 += 8 * EV_THREADS) {
+      int page[8];
+      float w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) page[e] = table[a.page_of(min(j0 + e * EV_THREADS, m1 - 1))];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = min(j0 + e * EV_THREADS, m1 - 1);
+        const bool out = page[e] < 0 || page[e] >= a.pages;
+        bad |= out;
+        w[e] = a.mass[((size_t)(out ? 0 : page[e]) * a.nkv + h) * a.kv_block + (j - a.page_of(j) * a.kv_block)];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j0 + e * EV_THREADS < m1) held_s[j0 + e * EV_THREADS - t0] = weight_order(w[e]);
+    }
+    if (bad) set_status(a.status, ST_BOUNDS);
+  }
+  for (int pass = 0; pass < 3 && !none; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const uint32_t bins = pass == 2 ? 1024u : 2048u;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int j = m0 + tid; j < m1; j += EV_THREADS) {
+      const uint32_t u = hold ? held_s[j - t0] : weight(j);
+      if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
+    }
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+    if (ctas > 1) {
+      // a part of the bins each, handed to everyone
+      const int part = EV_BINS / ctas;
+      for (int i = rank * part + tid; i < (rank + 1) * part; i += EV_THREADS) {
+        uint32_t v[8], sum = 0;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[c] = c < ctas ? cluster.map_shared_rank(hist, c)[i] : 0u;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) sum += v[c];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < ctas) cluster.map_shared_rank(total, c)[i] = sum;
       }
       cluster.sync();
-      for (int i = tid; i < EV_BINS; i += EV_THREADS) {
-        uint32_t sum = 0;
-        for (int c = 0; c < ctas; ++c) sum += cluster.map_shared_rank(hist, c)[i];
-        total[i] = sum;
-      }
-      __syncthreads();
-      // bins from the top, four a thread
-      uint32_t mine = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mine += total[EV_BINS - 1 - 4 * tid - e];
-      uint64_t all;
-      uint32_t ahead = (uint32_t)scan_pairs(mine, tmp, &all);
-      if (ahead < need && need <= ahead + mine) {
-        int d = EV_BINS - 1 - 4 * tid;
-        while (ahead + total[d] < need) ahead += total[d--];
-        digit_s[0] = (uint32_t)d;
-        digit_s[1] = need - ahead;
-      }
-      cluster.sync();                                                // (also: nobody reads these histograms any more)
-      prefix |= digit_s[0] << shift;
-      mask |= (bins - 1) << shift;
-      need = digit_s[1];
     }
-    // need: how many tokens of the weight `prefix` stay. A thread has neighbouring tokens: how many stay for sure (low half) and equal ones (high half)
-    const int each = (t1 - t0 + EV_THREADS - 1) / EV_THREADS, j0 = min(t1, t0 + tid * each), j1 = min(t1, j0 + each);
-    auto kind = [&](int j) -> uint64_t {
-      if (j < lo || j >= hi) return 1;
-      if (none) return 0;
-      const uint32_t u = hold ? held_s[j - t0] : order(j);
-      return u > prefix ? 1ull : u == prefix ? 1ull << 32 : 0ull;
-    };
-    uint64_t mine = 0, all;
-    for (int j = j0; j < j1; ++j) mine += kind(j);
-    uint64_t ahead = scan_pairs(mine, tmp, &all);
+    const uint32_t* all_bins = ctas > 1 ? total : hist;
+    // bins from the top, four a thread
+    const uint4 q = *reinterpret_cast<const uint4*>(all_bins + EV_BINS - 4 - 4 * tid);
+    const uint32_t mine = q.x + q.y + q.z + q.w;
+    uint64_t all;
+    uint32_t ahead = (uint32_t)scan_pairs(mine, tmp, &all);
+    if (ahead < need && need <= ahead + mine) {
+      uint32_t of = q.w, d = EV_BINS - 1 - 4 * tid;
+      if (ahead + of < need) { ahead += of; of = q.z; --d; }
+      if (ahead + of < need) { ahead += of; of = q.y; --d; }
+      if (ahead + of < need) { ahead += of; of = q.x; --d; }
+      digit_s[0] = d;
+      digit_s[1] = need - ahead;
+      digit_s[2] = of;                                               // tokens of this digit
+    }
+    __syncthreads();
+    prefix |= digit_s[0] << shift;
+    mask |= (bins - 1) << shift;
+    need = digit_s[1];
+    if (digit_s[2] == need) break;                                   // all of them stay: the digits behind say nothing
+  }
+  // ---- need: how many tokens whose weight starts with `prefix` stay. A warp has neighbouring tokens, 32 at a time: how many stay for sure (low half), equal ones (high)
+  const int run = ((t1 - t0 + EV_WARPS - 1) / EV_WARPS + 31) / 32 * 32, w0 = min(t1, t0 + warp * run), w1 = min(t1, w0 + run);
+  auto kinds = [&](int j, bool* sure, bool* equal) {
+    const bool there = j < w1, middle = there && j >= lo && j < hi;
+    const uint32_t u = middle && !none ? (hold ? held_s[j - t0] : weight(j)) & mask : 0u;
+    *sure = there && (!middle || (!none && u > prefix));
+    *equal = middle && !none && u == prefix;
+  };
+  uint64_t mine = 0, all;
+  for (int j = w0; j < w1; j += 32) {
+    bool sure, equal;
+    kinds(j + lane, &sure, &equal);
+    mine += (uint64_t)__popc(__ballot_sync(0xffffffffu, sure)) | (uint64_t)__popc(__ballot_sync(0xffffffffu, equal)) << 32;
+  }
+  uint64_t ahead = scan_pairs(lane == 0 ? mine : 0, tmp, &all);
+  ahead = __shfl_sync(0xffffffffu, ahead, 0);
+  if (ctas > 1) {
     if (tid == 0) counts_s = all;
     cluster.sync();
     for (int c = 0; c < rank; ++c) ahead += *cluster.map_shared_rank(&counts_s, c);
-    for (int j = j0; j < j1; ++j) {
-      const uint64_t k = kind(j);
-      const uint32_t sure = (uint32_t)ahead, equal = (uint32_t)(ahead >> 32), at = sure + min(equal, need);
-      if (k == 1 || (k && equal < need)) kept[at] = j;
-      ahead += k;
-    }
+    cluster.sync();                                                  // (a CTA stays as long as its counts are read)
   }
-  __threadfence();
-  cluster.sync();                                                    // the list is complete
-  // ---- the copy
-  const int rows0 = (int)((long)m * rank / ctas), rows1 = (int)((long)m * (rank + 1) / ctas), pieces = a.row_bytes / 16, L = a.row_lanes;
-  for (int i0 = rows0 + warp * 32; i0 < rows1; i0 += EV_THREADS) {
-    const int i = i0 + lane;
+  for (int j = w0; j < w1; j += 32) {
+    bool sure, equal;
+    kinds(j + lane, &sure, &equal);
+    const uint32_t sures = __ballot_sync(0xffffffffu, sure), equals = __ballot_sync(0xffffffffu, equal), below = (1u << lane) - 1;
+    const uint32_t s = (uint32_t)ahead + __popc(sures & below), e = (uint32_t)(ahead >> 32) + __popc(equals & below);
+    if (sure || (equal && e < need)) kept[s + min(e, need)] = j + lane;
+    ahead += (uint64_t)__popc(sures) | (uint64_t)__popc(equals) << 32;
+  }
+}
+
+__global__ void __launch_bounds__(256) kv_copy_kernel(EvictArgs a) {
+  const int lane = threadIdx.x & 31, pieces = a.row_bytes / 16, L = a.row_lanes, step = 32 / L, run = a.run, runs = (a.keep + run - 1) / run;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int* kept_all = after_wait(a.kept);
+  const long u = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (u < (long)a.segs * a.nkv * runs) {
+    const int pair = (int)(u / runs), i0 = (int)(u % runs) * run, seg = pair / a.nkv, h = pair % a.nkv, i = i0 + lane, slot = a.seg_slot[seg];
+    const int j = lane < run && i < a.keep ? kept_all[(size_t)pair * a.keep + i] : -1;
     long from = -1, to = -1;
-    if (i < rows1) {
-      int j = *reinterpret_cast<volatile int*>(kept + i);
-      const int src = checked_page(a, table[j / a.kv_block]), dst = checked_page(a, a.dst[(size_t)seg * a.dst_blocks + i / a.kv_block]);
+    if (j >= 0 && slot >= 0 && slot < a.slots && a.page_of(j) < a.max_blocks) {
+      const int sp = a.page_of(j), dp = a.page_of(i);
+      const int src = checked_page(a, a.table[(size_t)slot * a.max_blocks + sp]), dst = checked_page(a, a.dst[(size_t)seg * a.dst_blocks + dp]);
       if (src >= 0 && dst >= 0) {
-        from = ((long)src * a.kv_block + j % a.kv_block) * a.nkv + h;
-        to = ((long)dst * a.kv_block + i % a.kv_block) * a.nkv + h;
-        a.mass[((size_t)dst * a.nkv + h) * a.kv_block + i % a.kv_block] = a.mass[((size_t)src * a.nkv + h) * a.kv_block + j % a.kv_block];
+        const int so = j - sp * a.kv_block, d0 = i - dp * a.kv_block;
+        from = ((long)src * a.kv_block + so) * a.nkv + h;
+        to = ((long)dst * a.kv_block + d0) * a.nkv + h;
+        a.mass[((size_t)dst * a.nkv + h) * a.kv_block + d0] = a.mass[((size_t)src * a.nkv + h) * a.kv_block + so];
         if (a.scale)
           for (int e = 0; e < a.ns; ++e) a.scale[to * a.ns + e] = a.scale[from * a.ns + e];
       }
     }
-    const int rows = min(32, rows1 - i0), step = 32 / L;
-    for (int r0 = 0; r0 < rows; r0 += 4 * step) {
+    if (!__any_sync(0xffffffffu, to >= 0)) return;
+    for (int r0 = 0; r0 < run; r0 += 4 * step) {
       long f[4], t[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -209,12 +267,21 @@ extern "C" int fb_kv_evict(int* kept, void* k, void* v, float* scale, float* mas
   if (keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || (long)dst_blocks * kv_block < keep || row_bytes % 16 || ns > 32) return -1;
   if ((long)segs * nkv > 0x7fffffffl / 8) return -2;
   const long room = (long)max_blocks * kv_block;
-  const int cluster = 8;
-  int lanes = 1;
+  // CTAs of a cluster: the fewest of 1, 2, 4 and 8 that leave a CTA up to 4096 tokens, as far as all CTAs run at once (what crosses a cluster costs 2 us a digit)
+  int cluster = 1, lanes = 1, shift = -1;
+  while (cluster < 8 && room > 4096l * cluster && (long)segs * nkv * cluster * 2 <= 296) cluster *= 2;
   while (lanes < 32 && lanes * 16 < row_bytes) lanes *= 2;
+  for (int b = 0; b < 31; ++b)
+    if (kv_block == 1 << b) shift = b;
+  // rows of a warp: 32, fewer where that leaves some of the SMs' 148 x 8 x 8 warps without any
+  int run = 32;
+  while (run > 4 && run > 128 / lanes && (long)segs * nkv * ((keep + run - 1) / run) < 148l * 64) run /= 2;
   const EvictArgs a{kept, (unsigned char*)k, (unsigned char*)v, scale, mass, seg_slot, seg_len, table, dst, segs, slots, max_blocks, dst_blocks, pages,
-                    kv_block, nkv, row_bytes, ns, keep, first, recent, (int)std::min((room + cluster - 1) / cluster, (long)EV_HELD), lanes, status};
+                    kv_block, nkv, row_bytes, ns, keep, first, recent, (int)std::min((room + cluster - 1) / cluster, (long)EV_HELD), shift, lanes, run, status};
   const size_t smem = (size_t)a.held * 4;
-  FB_CUDA_CHECK(cudaFuncSetAttribute(kv_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_HELD * 4));
-  return (int)launch_pdl_cluster(cluster, kv_evict_kernel, dim3((unsigned)(segs * nkv * cluster)), dim3(EV_THREADS), smem, s, a);
+  FB_CUDA_CHECK(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_HELD * 4));
+  cudaError_t e = launch_pdl_cluster(cluster, kv_select_kernel, dim3((unsigned)(segs * nkv * cluster)), dim3(EV_THREADS), smem, s, a);
+  if (e != cudaSuccess) return (int)e;
+  const long runs = (long)segs * nkv * ((keep + run - 1) / run);
+  return (int)launch_pdl(kv_copy_kernel, dim3((unsigned)((runs + 7) / 8)), dim3(256), 0, s, a);
 }

@@ -152,6 +152,6 @@ class CudaShared:
     def kv_evict(self, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first=0, recent=0):
         """Eviction by accumulated weight into new pages (see the oracle); rows of every cache form move as they are."""
         kept = self.empty(seg_slot.numel(), k_cache.shape[2], keep, dtype=torch.int32, device=k_cache.device)
-        self.launches += 1
+        self.launches += 2
         self.C.kv_evict(kept, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first, recent, self.status_word)
         return kept
