@@ -21,14 +21,15 @@ struct KmCfg {
   static constexpr int NCH = HD / 64, K_CH = KM_KEYS * 128, Q_CH = KM_PAIRS * 128, K_BYTES = NCH * K_CH, Q_BYTES = NCH * Q_CH;
   static constexpr int KS = HD == 256 ? 2 : HD == 128 ? 4 : 6;                    // key tiles in shared memory
   static constexpr int QS = HD == 256 ? 3 : HD == 128 ? 5 : 8;                    // tiles of queries
-  static constexpr int RS = HD == 256 ? 3 : 8;                                    // ... where they stream
+  static constexpr int RS = HD == 256 ? 3 : 8, AS = HD == 256 ? 5 : 8;            // ... where they stream; of what their pairs are
+  static constexpr int ROWS_AT = 2 * K_BYTES + RS * Q_BYTES;                      // ... what lies behind them then
   static constexpr int TILES = KS * K_BYTES + QS * Q_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
 };
 template <int QS>
 struct KmMisc {
   float nl[QS][KM_PAIRS];                        // minus a pair's logarithm (log2); minus infinity where there is no pair
   int kvl[QS][KM_PAIRS];                         // keys that it sees
-  uint64_t bars[40];
+  uint64_t bars[44];
   uint32_t tmem;
   int abort;
 };
@@ -353,11 +354,20 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
   const int spans = st.ngrp + st.nseg;
   auto first = [&](int i) { return plan.start[i]; };
   auto behind = [&](int i) { return i + 1 < spans ? plan.start[i + 1] : plan.blocks; };
-  // items of a span: as many as its longest block has (their numbers take the place of the blocks' places)
+  // From here on: end of a span's keys in the place of its length or rows, its items (as many as its longest block has) in that of the blocks' places, the
+  // blocks' tiles in that of their spans.
+  auto end = [&](int i) -> int& { return i < st.ngrp ? plan.len[i] : plan.rows[i - st.ngrp]; };
+  int* nts = plan.span;
   for (int i = tid; i < spans; i += KP_PLAN) {
-    int most = 0;
-    for (int b = first(i); b < behind(i); ++b) most = max(most, w.blocks[b].nt);
-    plan.place[i] = most;
+    end(i) = 0;
+    plan.place[i] = 0;
+  }
+  __syncthreads();
+  for (int b = tid; b < plan.blocks; b += KP_PLAN) {
+    const int i = plan.span[b], k1 = w.blocks[b].k1, nt = w.blocks[b].nt;
+    atomicMax(&end(i), k1);
+    atomicMax(&plan.place[i], nt);
+    nts[b] = nt;
   }
   __syncthreads();
   const long long all = scan_ahead<KP_PLAN>(plan.place, spans, tmp);
@@ -385,15 +395,10 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
         else hi = mid - 1;
       }
       const int j = it - plan.place[lo];
-      int k1 = 0;
-      for (int b = first(lo); b < behind(lo); ++b) {
-        const SharedBlock blk = w.blocks[b];
-        e.slot = blk.slot;
-        e.k0 = blk.k0;
-        k1 = max(k1, blk.k1);
-        n += blk.nt > j;
-      }
-      e.k1 = k1;
+      for (int b = first(lo); b < behind(lo); ++b) n += nts[b] > j;
+      e.slot = w.blocks[first(lo)].slot;
+      e.k0 = w.blocks[first(lo)].k0;
+      e.k1 = end(lo);
       e.key0 = (e.k0 / KP_KEYS + j) * KP_KEYS;
       e.chunks = (n + C - 1) / C;
     }
@@ -417,13 +422,17 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
       e.chunk0 = base + ahead + xs - e.chunks;
       w.items[it] = e;
       const int j = it - plan.place[lo];
-      int seen = 0, from = first(lo);
-      for (int b = first(lo); b < behind(lo); ++b)
-        if (w.blocks[b].nt > j) {
-          if (seen % C == 0) from = b;
-          ++seen;
-          if (seen % C == 0 || seen == n) w.chunks[e.chunk0 + (seen - 1) / C] = KpChunk{it, from, b + 1, (seen - 1) % C + 1};
+      int seen = 0, in = 0, from = 0, c = e.chunk0;
+      for (int b = first(lo); b < behind(lo); ++b) {
+        if (nts[b] <= j) continue;
+        if (in == 0) from = b;
+        ++in;
+        ++seen;
+        if (in == C || seen == n) {
+          w.chunks[c++] = KpChunk{it, from, b + 1, in};
+          in = 0;
         }
+      }
     }
     base += sum;
   }
@@ -438,11 +447,12 @@ __global__ void __launch_bounds__(KM_THREADS, 1)
 kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, const float* lse, FbSharedStep st, KpSpace w, int nq,
                     int nkv, float scale_log2, int* status) {
   using C = KmCfg<HD>;
-  constexpr int NCH = C::NCH, QS = C::RS;
+  constexpr int NCH = C::NCH, QS = C::RS, AS = C::AS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *sK = smem, *sQ = smem + 2 * C::K_BYTES;
-  KmMisc<QS>& ms = *reinterpret_cast<KmMisc<QS>*>(smem + 2 * C::K_BYTES + QS * C::Q_BYTES);
-  uint64_t *k_full = ms.bars, *k_empty = k_full + 1, *s_full = k_full + 2, *s_empty = s_full + KM_SETS, *q_full = s_empty + KM_SETS, *q_empty = q_full + QS;
+  KmMisc<AS>& ms = *reinterpret_cast<KmMisc<AS>*>(smem + C::ROWS_AT);
+  uint64_t *k_full = ms.bars, *k_empty = k_full + 1, *s_full = k_full + 2, *s_empty = s_full + KM_SETS, *q_full = s_empty + KM_SETS, *q_empty = q_full + QS,
+           *a_full = q_empty + QS, *a_empty = a_full + AS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
   volatile int* abort_flag = &ms.abort;
   pdl_launch_dependents();
@@ -455,7 +465,8 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     mbar_init(k_full, 1);
     mbar_init(k_empty, 1);
     for (int i = 0; i < KM_SETS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); }
-    for (int i = 0; i < QS; ++i) { mbar_init(&q_full[i], 2); mbar_init(&q_empty[i], 9); }
+    for (int i = 0; i < QS; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
+    for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], 1); mbar_init(&a_empty[i], 8); }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -505,6 +516,8 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (*abort_flag && lane == 0 && n) mbar_wait(k_full, (n - 1) & 1, 1u << 20);
   } else if (warp == 2 || warp == 3) {
     // ---- tiles of queries (warp 2), what their pairs are (warp 3)
+    const int S = warp == 2 ? QS : AS;
+    uint64_t* empty = warp == 2 ? q_empty : a_empty;
     int i = 0, stage = 0, phase = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
@@ -514,7 +527,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       for (int b = ch.b0; b < ch.b1; ++b) {
         const SharedBlock e = w.blocks[b];
         if (!sees(e, it)) continue;
-        ok = i < QS || __all_sync(0xffffffffu, sk_wait(&q_empty[stage], phase ^ 1, abort_flag));
+        ok = i < S || __all_sync(0xffffffffu, sk_wait(&empty[stage], phase ^ 1, abort_flag));
         if (!ok) break;
         if (warp == 2) {
           if (lane == 0) {
@@ -529,10 +542,10 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             km_pair(st, lse, e, r, p - r * share, kvh * share, nq, share, Rq, p, &ms.nl[stage][p], &ms.kvl[stage][p]);
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&q_full[stage]);
+          if (lane == 0) mbar_arrive(&a_full[stage]);
         }
         ++i;
-        if (++stage == QS) {
+        if (++stage == S) {
           stage = 0;
           phase ^= 1;
         }
@@ -556,7 +569,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       unit(u, &ch, &it);
       ok = __all_sync(0xffffffffu, sk_wait(k_full, n & 1, abort_flag));
       for (int j = 0; ok && j < ch.steps; ++j, ++i) {
-        ok = __all_sync(0xffffffffu, sk_wait(&q_full[stage], phase, abort_flag));
+        ok = __all_sync(0xffffffffu, sk_wait2(&q_full[stage], phase, &a_full[i % AS], i / AS & 1, abort_flag));
         for (int a = 0; ok && a < 2; ++a) {
           const int f = 2 * i + a, set = f % KM_SETS;
           ok = f < KM_SETS || __all_sync(0xffffffffu, sk_wait(&s_empty[set], (f / KM_SETS - 1) & 1, abort_flag));
@@ -602,7 +615,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const SharedBlock now = e;
         if (j + 1 < ch.steps) e = w.blocks[b + 1];
         if ((i & 1) != set >> 1) continue;
-        const int f = 2 * i + (set & 1), stage = i % QS;
+        const int f = 2 * i + (set & 1), stage = i % AS;
         if (!dead && !__all_sync(0xffffffffu, sk_wait(&s_full[set], (f / KM_SETS) & 1, abort_flag))) {
           dead = true;
           if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
@@ -617,7 +630,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(&s_empty[set]);
-          mbar_arrive(&q_empty[stage]);
+          mbar_arrive(&a_empty[stage]);
         }
       }
       if (!dead) w.sums[((size_t)u * KM_SETS + set) * KM_KEYS + place] = sum;
@@ -727,8 +740,8 @@ extern "C" int fb_attention_mass(float* out, const float* mass, float carry, con
 #define FB_KM(H)                                                                                                                                       \
   if (hd == H) {                                                                                                                                       \
     using C = KmCfg<H>;                                                                                                                                \
-    const size_t smem = C::MISC_AT + sizeof(KmMisc<C::QS>);                                                                                            \
-    static_assert(C::MISC_AT + sizeof(KmMisc<C::QS>) <= 232448, "shared memory of an SM");                                                             \
+    constexpr size_t smem = C::MISC_AT + sizeof(KmMisc<C::QS>);                                                                                        \
+    static_assert(smem <= 232448, "shared memory of an SM");                                                                                           \
     FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_keys_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                               \
     e = launch_pdl(kv_mass_keys_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, out, mass, carry, lse, st, z, (SharedBlock*)ws, R, nq,     \
                    nkv, scale, status);                                                                                                                \
@@ -745,8 +758,9 @@ extern "C" int fb_attention_mass(float* out, const float* mass, float carry, con
 #define FB_KP(H)                                                                                                                                       \
   if (hd == H) {                                                                                                                                       \
     using C = KmCfg<H>;                                                                                                                                \
-    const size_t smem = 2 * C::K_BYTES + C::RS * C::Q_BYTES + sizeof(KmMisc<C::RS>);                                                                   \
-    static_assert(2 * C::K_BYTES + C::RS * C::Q_BYTES + sizeof(KmMisc<C::RS>) <= 232448, "shared memory of an SM");                                    \
+    using M = KmMisc<C::AS>;                                                                                                                           \
+    constexpr size_t smem = C::ROWS_AT + sizeof(M);                                                                                                    \
+    static_assert(smem <= 232448, "shared memory of an SM");                                                                                           \
     FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_rows_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                                \
     e = launch_pdl(kv_mass_rows_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, lse, st, w, nq, nkv, scale, status);                        \
   }

@@ -33,17 +33,15 @@ constexpr int SA_SET = 8;                                    // warps of a set: 
 constexpr int SA_THREADS = (4 + 2 * SA_SET) * 32;
 constexpr int SA_ML = 8;                                     // floats of a pair's statistics: its threads' sums, the maximum
 
-template <int HD, bool OUT>
+template <int HD>
 struct SaCfg {
   static constexpr int NCH = HD / 64, Q_CH = SA_PAIRS * 128, KV_CH = SA_KT * 128;
   static constexpr int Q_BYTES = NCH * Q_CH, T_BYTES = NCH * KV_CH;
-  static constexpr int KS = OUT ? (HD == 256 ? 3 : HD == 128 ? 6 : 8) : (HD == 256 ? 5 : 8);
-  static constexpr int VS = OUT ? (HD == 256 ? 2 : HD == 128 ? 5 : 8) : 0;
+  static constexpr int KS = HD == 256 ? 3 : HD == 128 ? 6 : 8, VS = HD == 256 ? 2 : HD == 128 ? 5 : 8;
   static constexpr int TILES = Q_BYTES + (KS + VS) * T_BYTES;
   static constexpr int MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
   // TMEM: O | S0 S1 | P0 .. P3
-  static constexpr uint32_t COL_S = OUT ? HD : 0, COL_P = COL_S + 2 * SA_KT;
-  static constexpr uint32_t COLS = OUT ? 512 : 128;
+  static constexpr uint32_t COL_S = HD, COL_P = COL_S + 2 * SA_KT, COLS = 512;
 };
 template <int STAGES>
 struct SaMisc {
@@ -63,9 +61,57 @@ struct SaSpace {
   int4* rows;                                    // [rows][2]: of a row's group, of its segment: place in the list of one kv head, tiles (0: none), unit, row of the block
   float *ml_grp, *ml_seg;                        // SA_ML floats a pair
   float *o_grp, *o_seg;
+  float2* ml;                                    // logarithms alone: [record][half of the pairs][128][thread] maximum, sum
   SharedPlanSizes z;
   int seg_pairs;
 };
+
+// A CTA's share of the list: block that it starts in, blocks of groups, its first place, places.
+struct SaShare {
+  int b0, group_blocks, places;
+  long long f0;
+};
+// -> whether there is any (the same for the whole CTA, whose threads all call this, and which may put tiles in the place of `smem` then)
+template <int THREADS>
+__device__ __forceinline__ bool sa_share(SaShare* mine, const FbSharedStep& st, const SaSpace& w, int R, int nkv, unsigned char* smem, long long* tmp,
+                                         SharedBlock* near, int* status) {
+  const int tid = threadIdx.x;
+  SharedPlan<THREADS> plan;
+  const bool fits = plan.make(st, R, SA_KT, SA_EXTRA, w.z, smem, tmp, status);
+  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+  const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
+  if (blockIdx.x == 0 && tid == 0) {
+    w.head[0] = fits && per < 1ll << 31 ? per : 0;
+    w.head[1] = fits ? plan.group_blocks : 0;
+  }
+  // what the second kernel has to know of a row: written by every CTA that has the block's tiles (the same), or by the first one
+  auto note = [&](int b, const SharedBlock& e) {
+    const int s = plan.span[b] - st.ngrp, unit = (b - (s >= 0 ? plan.group_blocks : 0)) * nkv;
+    for (int r = 0; r < e.nrows; ++r) {
+      w.rows[2 * (e.row0 + r) + (s >= 0)] = make_int4(e.place0, e.nt, unit, r);
+      if (s >= 0 && plan.group[s] < 0) w.rows[2 * (e.row0 + r)] = make_int4(0, 0, 0, 0);
+    }
+  };
+  if (fits && blockIdx.x == 0)
+    for (int b = tid; b < plan.blocks; b += THREADS)                 // blocks that have no keys
+      if ((b + 1 < plan.blocks ? (long long)plan.place[b + 1] : plan.places) == plan.place[b]) note(b, plan.block(st, b, R, SA_KT, status));
+  if (f0 == f1 || per >= 1ll << 31) {
+    if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+    return false;
+  }
+  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
+  for (int b = b0 + tid; b <= b1; b += THREADS) {
+    SharedBlock e = plan.block(st, b, R, SA_KT, status);
+    e.place0 = plan.place[b];
+    if (b - b0 < SA_NEAR) near[b - b0] = e;
+    else w.table[b] = e;
+    if (e.nt) note(b, e);
+  }
+  *mine = {b0, plan.group_blocks, (int)(f1 - f0), f0};
+  fence_proxy_async();                                               // tiles take the plan's place
+  __syncthreads();
+  return true;
+}
 
 // A CTA's way through its share of the list: (block, kv head) after (block, kv head), as far as tiles of theirs lie in it.
 struct SaWalk {
@@ -82,14 +128,14 @@ struct SaWalk {
     left -= m;
   }
   // -> whether there is a piece
-  __device__ __forceinline__ bool start(const SharedBlock* close, const SharedBlock* tab, int first, long long f0, int places, int nkv) {
+  __device__ __forceinline__ bool start(const SharedBlock* close, const SharedBlock* tab, const SaShare& share, int nkv) {
     near = close;
     table = tab;
-    b = b0 = first;
+    b = b0 = share.b0;
     e = block(b);
-    const int at = (int)(f0 - (long long)e.place0 * nkv);
+    const int at = (int)(share.f0 - (long long)e.place0 * nkv);
     kvh = at / (e.nt + SA_EXTRA);
-    left = places;
+    left = share.places;
     take(at - kvh * (e.nt + SA_EXTRA));
     return n > 0 || next(nkv);
   }
@@ -106,11 +152,11 @@ struct SaWalk {
   __device__ __forceinline__ int token(int j) const { return (e.k0 / SA_KT + t + j) * SA_KT; }
 };
 
-template <int HD, bool OUT>
+template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, 1)
 shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __nv_bfloat16* q, long q_stride, FbSharedStep st,
                    SaSpace w, int nkv, int share, float scale_log2, int* status) {
-  using C = SaCfg<HD, OUT>;
+  using C = SaCfg<HD>;
   constexpr int NCH = C::NCH, KS = C::KS, VS = C::VS;
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char *sQ = smem, *sK = smem + C::Q_BYTES, *sV = sK + KS * C::T_BYTES;
@@ -147,46 +193,18 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   const uint32_t tmem = ms.tmem;
   pdl_wait();
 
-  // ---- this CTA's share
-  const int R = SA_PAIRS / share;
-  SharedPlan<SA_THREADS> plan;
-  const bool fits = plan.make(st, R, SA_KT, SA_EXTRA, w.z, smem, ms.tmp, status);
-  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
-  const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
-  if (blockIdx.x == 0 && tid == 0) w.head[0] = fits && per < 1ll << 31 ? per : 0;
-  // what the second kernel has to know of a row: written by every CTA that has the block's tiles (the same), or by the first one
-  auto note = [&](int b, const SharedBlock& e) {
-    const int s = plan.span[b] - st.ngrp, unit = (b - (s >= 0 ? plan.group_blocks : 0)) * nkv;
-    for (int r = 0; r < e.nrows; ++r) {
-      w.rows[2 * (e.row0 + r) + (s >= 0)] = make_int4(e.place0, e.nt, unit, r);
-      if (s >= 0 && plan.group[s] < 0) w.rows[2 * (e.row0 + r)] = make_int4(0, 0, 0, 0);
-    }
-  };
-  if (fits && blockIdx.x == 0)
-    for (int b = tid; b < plan.blocks; b += SA_THREADS)              // blocks that have no keys
-      if ((b + 1 < plan.blocks ? (long long)plan.place[b + 1] : plan.places) == plan.place[b]) note(b, plan.block(st, b, R, SA_KT, status));
-  if (f0 == f1 || per >= 1ll << 31) {                                // the same for the whole CTA
-    if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+  SaShare mine;
+  if (!sa_share<SA_THREADS>(&mine, st, w, SA_PAIRS / share, nkv, smem, ms.tmp, ms.blocks, status)) {
     if (warp == 1) tmem_dealloc(tmem, C::COLS);
     return;
   }
-  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv), group_blocks = plan.group_blocks;
-  for (int b = b0 + tid; b <= b1; b += SA_THREADS) {
-    SharedBlock e = plan.block(st, b, R, SA_KT, status);
-    e.place0 = plan.place[b];
-    if (b - b0 < SA_NEAR) ms.blocks[b - b0] = e;
-    else w.table[b] = e;
-    if (e.nt) note(b, e);
-  }
-  fence_proxy_async();                                               // tiles take the plan's place
-  __syncthreads();
+  const int group_blocks = mine.group_blocks;
   SaWalk x;
-  if (!x.start(ms.blocks, w.table, b0, f0, (int)(f1 - f0), nkv)) goto done;    // the same for the whole CTA
+  if (!x.start(ms.blocks, w.table, mine, nkv)) goto done;            // the same for the whole CTA
 
   if (warp == 0 || warp == 2) {
     // ---- keys (warp 0) and values (warp 2): the lanes look up 32 tiles' pages at a time, one of them copies
     const bool keys = warp == 0;
-    if (!keys && !OUT) goto done;
     const CUtensorMap* tm = keys ? &tmK : &tmV;
     uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
     unsigned char* to = keys ? sK : sV;
@@ -222,7 +240,6 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       for (int j = max(0, i - S); j < i; ++j) mbar_wait(&full[j % S], (j / S) & 1, 1u << 20);
   } else if (warp == 1 || warp == 3) {
     // ---- products, issued from the whole warp by one lane's predicate: S (warp 1), O (warp 3)
-    if (warp == 3 && !OUT) goto done;
     const bool issue = elect_one();
     auto wait = [&](uint64_t* a, uint32_t pa, uint64_t* b, uint32_t pb, bool both) {
       return __all_sync(0xffffffffu, sk_wait2(a, pa, both ? b : a, both ? pb : pa, abort_flag));
@@ -251,7 +268,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             st_i = 0;
             phase ^= 1;
           }
-        } else if constexpr (OUT) {
+        } else {
           constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, HD) | (1u << 16);      // B read MN-major
           const uint32_t aV = smem_u32(sV) + st_i * C::T_BYTES;
           ok = j > 0 || piece == 0 || wait(o_empty, (piece - 1) & 1, o_empty, 0, false);
@@ -332,7 +349,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const bool need_mask = t0 < y.e.k0 || t0 + SA_KT > y.e.kmin;
         wait(&s_full[set], (i >> 1) & 1);
         if (i + 1 == end && more && !dead) copy_q(x);                // every product that reads the queries is through
-        if constexpr (OUT) if (need_mask) {
+        if (need_mask) {
           // Values of keys that some row does not see meet weights of zero: those that no row sees become zeros, those that some see are looked at,
           // and where one is no finite number the key's values become zeros and its score NaN for the rows that see it.
           // (a wait tells a phase from the one ahead of it only: the values of tile i - VS have to be through)
@@ -381,7 +398,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (active && !dead) {
           if (need_mask) {
             const int c0 = t0 + sub * HC;
-            const uint32_t bad = OUT ? reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub] : 0u;
+            const uint32_t bad = reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub];
 #pragma unroll
             for (int c = 0; c < HC; ++c) {
               if (bad >> c & 1u) sr[c] = 0x7fc00000u;
@@ -394,7 +411,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           mx = pair < np ? mx * scale_log2 : -INFINITY;              // (what lies behind the pairs moves no maximum)
         }
         // ---- the decision, in the order of the tiles
-        if (OUT && i >= 4) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[i & 3], ((i >> 2) - 1) & 1);    // ... and P(i - 4) has been read
+        if (i >= 4) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[i & 3], ((i >> 2) - 1) & 1);    // ... and P(i - 4) has been read
         else if (i > 0) wait(&turn[2 * quad + set], ((i - 1) >> 1) & 1);
         float m_new = j > 0 ? ms.m[pair] : -INFINITY;
         const float m_old = m_new;
@@ -409,18 +426,18 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (sub == 0 && (moves || j == 0)) ms.m[pair] = m_new;
         __syncwarp();
         if (lane == 0 && !dead) mbar_arrive(&turn[2 * quad + (set ^ 1)]);
-        if (OUT && moves && j > 0) wait(&p_empty[(i - 1) & 3], ((i - 1) >> 2) & 1);          // O is rescaled behind PV(i - 1)
+        if (moves && j > 0) wait(&p_empty[(i - 1) & 3], ((i - 1) >> 2) & 1);          // O is rescaled behind PV(i - 1)
         if (dead || !active) {
           __syncwarp();
-          if (OUT && lane == 0 && !dead) mbar_arrive(&p_full[i & 3]);
+          if (lane == 0 && !dead) mbar_arrive(&p_full[i & 3]);
           continue;
         }
-        if (OUT) tc_fence_after();
+        tc_fence_after();
         if (m_new != m_own) {
           l = m_own == -INFINITY ? l : l * sk_exp2(m_own - m_new);   // (a sum that is no number stays one)
           m_own = m_new;
         }
-        if (OUT && moves && j > 0) {
+        if (moves && j > 0) {
           const float f = m_old == -INFINITY ? 0.f : sk_exp2(m_old - m_new);
 #pragma unroll 1
           for (int c0 = 0; c0 < OC; c0 += 16) {
@@ -445,18 +462,16 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), scale2, mr2));
             const float p0 = sk_exp2(d.x), p1 = sk_exp2(d.y);
             sum = f2_add(sum, f2_pack(p0, p1));
-            if constexpr (OUT) pr[c] = pack_bf2(p0, p1);
+            pr[c] = pack_bf2(p0, p1);
           }
-          if constexpr (OUT) sk_tmem_st8(tmem + lane_addr + C::COL_P + (i & 3) * (SA_KT / 2) + sub * (HC / 2) + part * (HC / 4), pr);
+          sk_tmem_st8(tmem + lane_addr + C::COL_P + (i & 3) * (SA_KT / 2) + sub * (HC / 2) + part * (HC / 4), pr);
         }
         const float2 both = f2_unpack(sum);
         l += both.x + both.y;
-        if constexpr (OUT) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[i & 3]);
-        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[i & 3]);
       }
       if (more && ((end - 1) & 1) == set) give_q();
       // ---- the piece: record number = CTA + unit, which no other piece has
@@ -474,34 +489,32 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         ml[2 * set + sub] = l;
         if (set == 0 && sub == 0) ml[4] = m_own;
       }
-      if constexpr (OUT) {
-        if (end >= 2) wait(&p_empty[(end - 2) & 3], ((end - 2) >> 2) & 1);       // (one phase after the other)
-        wait(&p_empty[(end - 1) & 3], ((end - 1) >> 2) & 1);
-        if (active && !dead) {
-          tc_fence_after();
-          constexpr int QC = HD / 4;
-          const int col = (2 * set + sub) * QC;
-          float* o = (grp ? w.o_grp : w.o_seg) + (rec * stride) * HD + col + 2 * (lane & 3);
+      if (end >= 2) wait(&p_empty[(end - 2) & 3], ((end - 2) >> 2) & 1);       // (one phase after the other)
+      wait(&p_empty[(end - 1) & 3], ((end - 1) >> 2) & 1);
+      if (active && !dead) {
+        tc_fence_after();
+        constexpr int QC = HD / 4;
+        const int col = (2 * set + sub) * QC;
+        float* o = (grp ? w.o_grp : w.o_seg) + (rec * stride) * HD + col + 2 * (lane & 3);
 #pragma unroll 1
-          for (int r0 = quad * 32; r0 < min(np, quad * 32 + 32); r0 += 16) {
-            const int ra = r0 + (lane >> 2), rb = ra + 8;
+        for (int r0 = quad * 32; r0 < min(np, quad * 32 + 32); r0 += 16) {
+          const int ra = r0 + (lane >> 2), rb = ra + 8;
 #pragma unroll 1
-            for (int c0 = 0; c0 < QC; c0 += 16) {
-              uint32_t v[8];
-              sk_tmem_ld16x16(tmem + ((uint32_t)r0 << 16) + col + c0, v);
-              tmem_ld_wait();
+          for (int c0 = 0; c0 < QC; c0 += 16) {
+            uint32_t v[8];
+            sk_tmem_ld16x16(tmem + ((uint32_t)r0 << 16) + col + c0, v);
+            tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                if (ra < np) *reinterpret_cast<float2*>(o + (long)ra * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]));
-                if (rb < np) *reinterpret_cast<float2*>(o + (long)rb * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
-              }
+            for (int k = 0; k < 2; ++k) {
+              if (ra < np) *reinterpret_cast<float2*>(o + (long)ra * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]));
+              if (rb < np) *reinterpret_cast<float2*>(o + (long)rb * HD + c0 + 8 * k) = make_float2(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3]));
             }
           }
-          tc_fence_before();
         }
-        __syncwarp();
-        if (lane == 0 && !dead) mbar_arrive(o_empty);
+        tc_fence_before();
       }
+      __syncwarp();
+      if (lane == 0 && !dead) mbar_arrive(o_empty);
       first = end;
     }
   }
@@ -509,6 +522,240 @@ done:
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, C::COLS);
+}
+
+// ---- logarithms alone ------------------------------------------------------------------------------------------------------------------------
+// Where a step's weights are wanted and its attention has been something else (a prompt's): S as above, for 256 pairs at a time, so that a key tile serves two
+// products. A set of eight warps has 128 of the pairs; two threads a pair, each with half of every tile's keys and a maximum and sum of its own, which
+// meet in the second kernel only: nothing passes between threads.
+template <int HD>
+struct SlCfg {
+  static constexpr int NCH = HD / 64, Q_CH = SA_PAIRS * 128, KV_CH = SA_KT * 128, Q_BYTES = NCH * Q_CH, T_BYTES = NCH * KV_CH;
+  static constexpr int KS = HD == 256 ? 3 : 8;
+  static constexpr int TILES = 2 * Q_BYTES + KS * T_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
+};
+template <int HD>
+__global__ void __launch_bounds__(SA_THREADS, 1)
+shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* q, long q_stride, FbSharedStep st, SaSpace w, int nkv, int share,
+                  float scale_log2, int* status) {
+  using C = SlCfg<HD>;
+  constexpr int NCH = C::NCH, KS = C::KS;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  unsigned char *sQ = smem, *sK = smem + 2 * C::Q_BYTES;
+  SaMisc<KS>& ms = *reinterpret_cast<SaMisc<KS>*>(smem + C::MISC_AT);
+  uint64_t *q_full = ms.bars, *q_done = q_full + 1, *s_full = q_full + 2, *s_empty = q_full + 6, *k_full = q_full + 10, *k_empty = k_full + KS;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Rh = SA_PAIRS / share;
+  volatile int* abort_flag = &ms.abort;
+  pdl_launch_dependents();
+  if (smem_u32(smem) & 1023u) {
+    if (tid == 0) set_status(status, ST_BOUNDS);
+    return;
+  }
+  if (tid == 0) {
+    ms.abort = 0;
+    mbar_init(q_full, 2 * SA_SET);
+    mbar_init(q_done, 1);
+    for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], SA_SET); }        // [tile of pairs][parity]
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ms.tmem, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = ms.tmem;
+  pdl_wait();
+  SaShare mine;
+  if (!sa_share<SA_THREADS>(&mine, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status)) {
+    if (warp == 1) tmem_dealloc(tmem, 256);
+    return;
+  }
+  SaWalk x;
+  if (!x.start(ms.blocks, w.table, mine, nkv)) goto done;
+  if (warp == 0) {
+    int i = 0, stage = 0, phase = 0;
+    bool ok = true;
+    do {
+      int rows = 0;
+      for (int j = 0; j < x.n; ++j, ++i) {
+        if (j % 32 == 0) rows = j + lane < x.n ? tile_row(st, x.e.slot, x.token(j + lane), status) : 0;
+        const int row = __shfl_sync(0xffffffffu, rows, j % 32);
+        if (i >= KS && !__all_sync(0xffffffffu, sk_wait(&k_empty[stage], phase ^ 1, abort_flag))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          mbar_expect_tx(&k_full[stage], C::T_BYTES);
+#pragma unroll
+          for (int c = 0; c < NCH; ++c) tma_load_2d(sK + stage * C::T_BYTES + c * C::KV_CH, &tmK, &k_full[stage], x.kvh * HD + c * 64, row);
+        }
+        if (++stage == KS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    } while (ok && x.next(nkv));
+    if (!ok && lane == 0) {
+      if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+    if (*abort_flag && lane == 0)
+      for (int j = max(0, i - KS); j < i; ++j) mbar_wait(&k_full[j % KS], (j / KS) & 1, 1u << 20);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, SA_KT);
+    const bool issue = elect_one();
+    const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK);
+    int stage = 0, phase = 0, piece = 0, count[2] = {0, 0};
+    bool ok = true;
+    do {
+      const int tiles = x.e.nrows > Rh ? 2 : 1;
+      ok = __all_sync(0xffffffffu, sk_wait(q_full, piece & 1, abort_flag));
+      for (int j = 0; ok && j < x.n; ++j) {
+        ok = __all_sync(0xffffffffu, sk_wait(&k_full[stage], phase, abort_flag));
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          if (!ok || a >= tiles) break;
+          const int c = count[a]++, b = 2 * a + (c & 1);
+          ok = c < 2 || __all_sync(0xffffffffu, sk_wait(&s_empty[b], (c / 2 - 1) & 1, abort_flag));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            tc_mma_f16_if(issue, tmem + b * SA_KT, umma_desc_k128(aQ + a * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32),
+                          umma_desc_k128(aK + stage * C::T_BYTES + (kk >> 2) * C::KV_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+          tc_commit_if(issue, &s_full[b]);
+        }
+        if (!ok) break;
+        tc_commit_if(issue, &k_empty[stage]);
+        if (++stage == KS) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      tc_commit_if(issue, q_done);
+      ++piece;
+    } while (x.next(nkv));
+    if (!ok) {
+      if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  } else if (warp >= 4) {
+    const int quad = warp & 3, set = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, st_tid = tid - 128, pair = quad * 32 + lane;
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + set * 2 * SA_KT + sub * (SA_KT / 2);
+    const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
+    bool dead = false;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (!dead && !__all_sync(0xffffffffu, sk_wait(bar, parity, abort_flag))) {
+        dead = true;
+        if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+        *abort_flag = 1;
+      }
+    };
+    int piece = 0, count = 0;
+    bool more = true;
+    while (more) {
+      const SaWalk y = x;
+      const int np = min(Rh, y.e.nrows - set * Rh) * share, row0 = y.e.row0 + set * Rh;      // pairs of the set's half
+      const int klen = pair < np ? min(st.kvlen[row0 + pair / share], y.e.k1) : 0;
+      if (piece) wait(q_done, (piece - 1) & 1);                      // the products with the queries ahead of these are through
+      if (!dead) {
+        const int pieces = y.e.nrows * share * (HD / 8);
+        const __nv_bfloat16* src = q + (long)y.e.row0 * q_stride + (long)y.kvh * share * HD;
+        for (int c = st_tid; c < pieces; c += 512) {
+          const int d = c % (HD / 8), all = c / (HD / 8), r = all / share, g = all - r * share, a = r >= Rh, p = (r - a * Rh) * share + g;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                       ::"r"(smem_u32(sQ + a * C::Q_BYTES + (d >> 3) * C::Q_CH + p * 128 + (((d & 7) ^ (p & 7)) << 4))), "l"(src + (long)r * q_stride + g * HD + d * 8)
+                       : "memory");
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0 && !dead) mbar_arrive(q_full);
+      more = x.next(nkv);
+      float m = -INFINITY, l = 0.f;
+      if (np > 0) {
+        for (int j = 0; j < y.n; ++j, ++count) {
+          const int t0 = y.token(j) + sub * (SA_KT / 2), b = count & 1;
+          wait(&s_full[2 * set + b], count / 2 & 1);
+          uint32_t sr[32];
+          if (!dead) {
+            tc_fence_after();
+            tmem_ld32(taddr + b * SA_KT, sr);
+            tmem_ld_wait();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0 && !dead) mbar_arrive(&s_empty[2 * set + b]);
+          if (dead || quad * 32 >= np) continue;
+          if (t0 < y.e.k0 || t0 + SA_KT / 2 > y.e.kmin) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (t0 + c < y.e.k0 || t0 + c >= klen) sr[c] = 0xff800000u;
+          }
+          float mx = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 32; c += 4)
+            mx = fmaxf(fmaxf(mx, __uint_as_float(sr[c])), fmaxf(fmaxf(__uint_as_float(sr[c + 1]), __uint_as_float(sr[c + 2])), __uint_as_float(sr[c + 3])));
+          const float m_new = fmaxf(m, mx * scale_log2), mr = m_new == -INFINITY ? 0.f : -m_new;
+          const uint64_t mr2 = f2_pack(mr, mr);
+          uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * c]), __uint_as_float(sr[2 * c + 1])), scale2, mr2));
+            sum[c & 1] = f2_add(sum[c & 1], f2_pack(sk_exp2(d.x), sk_exp2(d.y)));
+          }
+          const float2 both = f2_unpack(f2_add(sum[0], sum[1]));
+          l = (m == -INFINITY ? l : l * sk_exp2(m - m_new)) + (both.x + both.y);     // (a sum that is no number stays one)
+          m = m_new;
+        }
+      }
+      const long rec = (long)blockIdx.x + (long)y.b * nkv + y.kvh;   // no other piece has this number
+      if (pair < np && !dead) w.ml[((rec * 2 + set) * SA_PAIRS + pair) * 2 + sub] = make_float2(m, l);
+      ++piece;
+    }
+  }
+done:
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, 256);
+}
+
+// A thread a (row, head): its pieces' maxima and sums -> logarithm.
+__global__ void __launch_bounds__(256) shared_lse_join_kernel(float* lse, FbSharedStep st, SaSpace w, int nkv, int share, int ctas) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long id = (long)blockIdx.x * 256 + threadIdx.x, nq = (long)nkv * share;
+  if (id >= st.rows * nq) return;
+  const int row = (int)(id / nq), h = (int)(id % nq), kvh = h / share, g = h - kvh * share, Rh = SA_PAIRS / share;
+  bool mine = false;
+  for (int s = 0; s < st.nseg && !mine; ++s) mine = row >= st.seg_row0[s] && row - st.seg_row0[s] < st.seg_nrows[s];
+  const long long per = w.head[0];
+  if (!mine || per <= 0) return;                                     // a row of no segment; a step that did not fit
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int4 info = w.rows[2 * row + k];
+    const long long at = (long long)info.x * nkv + (long long)kvh * (info.y + SA_EXTRA) + SA_EXTRA;
+    const long long c0 = at / per, c1 = (at + info.y - 1) / per;
+    const int first = k ? (int)w.head[1] : 0, last = k ? w.z.blocks : w.z.group_blocks;
+    // checked, since a launch that gave up has not written all of this
+    if (info.y <= 0 || info.x < 0 || c1 >= ctas || info.w < 0 || info.w >= 2 * Rh || info.z < 0 || info.z + kvh >= (last - (k ? w.z.group_blocks : 0)) * nkv) continue;
+    const int a = info.w >= Rh, pair = (info.w - a * Rh) * share + g;
+    for (long long c = c0; c <= c1; ++c) {
+      const long rec = c + (long)first * nkv + info.z + kvh;
+      const float4 v = *reinterpret_cast<const float4*>(&w.ml[((rec * 2 + a) * SA_PAIRS + pair) * 2]);
+      const float m = fmaxf(top, fmaxf(v.x, v.z));
+      auto part = [&](float mm, float l) { return mm == -INFINITY ? (l != l ? l : 0.f) : l * sk_exp2(mm - m); };
+      sum = part(top, sum) + part(v.x, v.y) + part(v.z, v.w);
+      top = m;
+    }
+  }
+  lse[id] = st.kvlen[row] <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
 // Pieces of a head's row -> output and logarithm. grid: rows x query heads; a thread has four columns and every fourth (eighth, 16th) piece. Everything that
@@ -608,8 +855,8 @@ __global__ void __launch_bounds__(256, 4) shared_join_kernel(__nv_bfloat16* out,
 using namespace fb;
 
 // The workspace: header | table | rows | statistics | sums. -> floats in all
-static long sa_space(SaSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, int ctas, int want_out) {
-  const int share = nq / nkv, R = SA_PAIRS / share;
+static long sa_space(SaSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, int ctas, bool logs_only) {
+  const int share = nq / nkv, R = SA_PAIRS / share * (logs_only ? 2 : 1);
   const long gb = shared_group_blocks(rows, ngrp, R), sb = shared_seg_blocks(rows, nseg, max_rows, R), pairs = std::min(R, std::max(max_rows, 1)) * (long)share;
   const long recs[2] = {gb ? (gb * nkv + ctas) * SA_PAIRS : 0, (sb * nkv + ctas) * pairs};
   float* at = ws;
@@ -622,28 +869,66 @@ static long sa_space(SaSpace* w, float* ws, int rows, int nseg, int max_rows, in
   v.head = (long long*)take(4);
   v.table = (SharedBlock*)take((gb + sb) * 8);
   v.rows = (int4*)take(8l * rows);
-  v.ml_grp = take(recs[0] * SA_ML);
-  v.ml_seg = take(recs[1] * SA_ML);
-  v.o_grp = take(want_out ? recs[0] * hd : 0);
-  v.o_seg = take(want_out ? recs[1] * hd : 0);
+  if (logs_only) {
+    v.ml = (float2*)take(((gb + sb) * nkv + ctas) * 2 * SA_PAIRS * 4);
+  } else {
+    v.ml_grp = take(recs[0] * SA_ML);
+    v.ml_seg = take(recs[1] * SA_ML);
+    v.o_grp = take(recs[0] * hd);
+    v.o_seg = take(recs[1] * hd);
+  }
   v.seg_pairs = (int)pairs;
   if (w) *w = v;
   return at - ws;
 }
+static bool sa_fits(const FbSharedStep& st, int nq, int nkv, int hd, int ctas) {
+  return nkv >= 1 && nq % nkv == 0 && nq / nkv >= 1 && nq / nkv <= SA_PAIRS && st.kv_block % SA_KT == 0 && ctas >= 1 && (hd == 64 || hd == 128 || hd == 256);
+}
+static bool sa_sizes(const FbSharedStep& st, int R, SharedPlanSizes* z) {
+  return shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, R), shared_seg_blocks(st.rows, st.nseg, st.max_rows, R), z);
+}
 
 extern "C" long fb_attention_shared_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, int ctas, int want_out) {
   if (rows <= 0 || nseg <= 0 || nkv < 1 || nq / nkv < 1 || nq / nkv > SA_PAIRS) return 0;
-  return sa_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, want_out);
+  return sa_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, !want_out);
+}
+
+// logarithms alone
+static int sa_logarithms(float* lse, float* ws, const void* q, long q_stride, const void* k, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status,
+                         cudaStream_t s) {
+  SaSpace w;
+  sa_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, true);
+  const int share = nq / nkv;
+  if (!sa_sizes(st, 2 * (SA_PAIRS / share), &w.z)) return -2;
+  const float scale = 1.4426950408889634f / sqrtf((float)hd);
+  CUtensorMap tmK;
+  const uint64_t width = (uint64_t)nkv * hd;
+  if (const int rc = make_tmap_bf16_2d(&tmK, k, (uint64_t)st.pages * st.kv_block, width, width, SA_KT)) return rc;
+  cudaError_t e = cudaErrorInvalidValue;
+#define FB_SL(H)                                                                                                                                    \
+  if (hd == H) {                                                                                                                                    \
+    using C = SlCfg<H>;                                                                                                                             \
+    const size_t smem = C::MISC_AT + sizeof(SaMisc<C::KS>);                                                                                         \
+    static_assert(C::MISC_AT + sizeof(SaMisc<C::KS>) <= 232448, "shared memory of an SM");                                                          \
+    FB_CUDA_CHECK(cudaFuncSetAttribute(shared_lse_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                              \
+    e = launch_pdl(shared_lse_kernel<H>, dim3(ctas), dim3(SA_THREADS), smem, s, tmK, (const __nv_bfloat16*)q, q_stride, st, w, nkv, share, scale,   \
+                   status);                                                                                                                         \
+  }
+  FB_SL(64) FB_SL(128) FB_SL(256)
+#undef FB_SL
+  if (e != cudaSuccess) return (int)e;
+  return (int)launch_pdl(shared_lse_join_kernel, dim3((unsigned)(((long)st.rows * nq + 255) / 256)), dim3(256), 0, s, lse, st, w, nkv, share, ctas);
 }
 
 extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_floats, const void* q, long q_stride, const void* k, const void* v,
                                    const void* proj, long proj_stride, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
   if (st.rows <= 0 || st.nseg <= 0 || st.max_rows <= 0) return 0;
-  if (nkv < 1 || nq % nkv || nq / nkv > SA_PAIRS || st.kv_block % SA_KT || ctas < 1) return -1;
+  if (!sa_fits(st, nq, nkv, hd, ctas)) return -1;
+  if (ws_floats < fb_attention_shared_floats(st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, out != nullptr)) return -3;
+  if (!out) return sa_logarithms(lse, ws, q, q_stride, k, st, nq, nkv, hd, ctas, status, s);
   SaSpace w;
-  if (ws_floats < sa_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, out != nullptr)) return -3;
-  const int R = SA_PAIRS / (nq / nkv);
-  if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, R), shared_seg_blocks(st.rows, st.nseg, st.max_rows, R), &w.z)) return -2;
+  sa_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, ctas, false);
+  if (!sa_sizes(st, SA_PAIRS / (nq / nkv), &w.z)) return -2;
   const int share = nq / nkv;
   const float scale = 1.4426950408889634f / sqrtf((float)hd);
   CUtensorMap tmK, tmV;
@@ -652,16 +937,16 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
   if ((rc = make_tmap_bf16_2d(&tmK, k, cache_rows, width, width, SA_KT))) return rc;
   if ((rc = make_tmap_bf16_2d(&tmV, v, cache_rows, width, width, SA_KT))) return rc;
   cudaError_t e = cudaErrorInvalidValue;
-#define FB_SA(H, OUTV)                                                                                                                              \
-  if (hd == H && (out != nullptr) == OUTV) {                                                                                                        \
-    auto kern = shared_attn_kernel<H, OUTV>;                                                                                                        \
-    using C = SaCfg<H, OUTV>;                                                                                                                       \
-    const size_t smem = C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>);                                                                                   \
-    static_assert(C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>) <= 232448, "shared memory of an SM");                                                    \
-    FB_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                                              \
-    e = launch_pdl(kern, dim3(ctas), dim3(SA_THREADS), smem, s, tmK, tmV, (const __nv_bfloat16*)q, q_stride, st, w, nkv, share, scale, status);     \
+#define FB_SA(H)                                                                                                                                    \
+  if (hd == H) {                                                                                                                                    \
+    using C = SaCfg<H>;                                                                                                                             \
+    const size_t smem = C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>);                                                                                 \
+    static_assert(C::MISC_AT + sizeof(SaMisc<C::KS + C::VS>) <= 232448, "shared memory of an SM");                                                  \
+    FB_CUDA_CHECK(cudaFuncSetAttribute(shared_attn_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                             \
+    e = launch_pdl(shared_attn_kernel<H>, dim3(ctas), dim3(SA_THREADS), smem, s, tmK, tmV, (const __nv_bfloat16*)q, q_stride, st, w, nkv, share,    \
+                   scale, status);                                                                                                                  \
   }
-  FB_SA(64, true) FB_SA(128, true) FB_SA(256, true) FB_SA(64, false) FB_SA(128, false) FB_SA(256, false)
+  FB_SA(64) FB_SA(128) FB_SA(256)
 #undef FB_SA
   if (e != cudaSuccess) return (int)e;
 #define FB_SJ(H)                                                                                                                                    \
