@@ -225,7 +225,7 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   } else if (warp == 1) {
     // ---- products
     const bool issue = elect_one();
-    const uint32_t aK = smem_u32(sK), aQ = smem_u32(sQ);
+    const uint64_t dK = umma_desc_k128(smem_u32(sK)), dQ = umma_desc_k128(smem_u32(sQ));
     int i = 0, stage = 0, phase = 0, unit = 0, turns[KM_SETS] = {0, 0, 0, 0};
     bool ok = true;
     do {
@@ -240,10 +240,7 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           if (!ok) break;
           tc_fence_after();
           const uint32_t idesc = umma_idesc(1, 1, KM_KEYS, pairs - t * Rq * share > 32 ? 64 : 32);
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_f16_if(issue, tmem + set * KM_PAIRS, umma_desc_k128(aK + stage * C::K_BYTES + (kk >> 2) * C::K_CH + (kk & 3) * 32),
-                          umma_desc_k128(aQ + t * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+          sk_products<HD / 16>(issue, tmem + set * KM_PAIRS, dK + (uint32_t)(stage * C::K_BYTES >> 4), dQ + (uint32_t)(t * C::Q_BYTES >> 4), C::K_CH, C::Q_CH, idesc);
           tc_commit_if(issue, &s_full[set]);
         }
         if (!ok) break;
@@ -558,30 +555,30 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (warp == 2 && *abort_flag && lane == 0)
       for (int j = max(0, i - QS); j < i; ++j) mbar_wait(&q_full[j % QS], (j / QS) & 1, 1u << 20);
   } else if (warp == 1) {
-    // ---- products: a tile of queries with both tiles of keys
+    // ---- products: a tile of queries with both tiles of keys, behind one look at everything that they wait for
     const bool issue = elect_one();
-    const uint32_t aK = smem_u32(sK), aQ = smem_u32(sQ), idesc = umma_idesc(1, 1, KM_KEYS, KM_PAIRS);
+    constexpr uint32_t idesc = umma_idesc(1, 1, KM_KEYS, KM_PAIRS);
+    const uint64_t dK = umma_desc_k128(smem_u32(sK)), dQ = umma_desc_k128(smem_u32(sQ));
     int i = 0, n = 0, stage = 0, phase = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
-      KpChunk ch;
-      KpItem it;
-      unit(u, &ch, &it);
+      const int steps = w.chunks[u / nkv].steps;
       ok = __all_sync(0xffffffffu, sk_wait(k_full, n & 1, abort_flag));
-      for (int j = 0; ok && j < ch.steps; ++j, ++i) {
-        ok = __all_sync(0xffffffffu, sk_wait2(&q_full[stage], phase, &a_full[i % AS], i / AS & 1, abort_flag));
-        for (int a = 0; ok && a < 2; ++a) {
-          const int f = 2 * i + a, set = f % KM_SETS;
-          ok = f < KM_SETS || __all_sync(0xffffffffu, sk_wait(&s_empty[set], (f / KM_SETS - 1) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_f16_if(issue, tmem + set * KM_PAIRS, umma_desc_k128(aK + a * C::K_BYTES + (kk >> 2) * C::K_CH + (kk & 3) * 32),
-                          umma_desc_k128(aQ + stage * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
-          tc_commit_if(issue, &s_full[set]);
-        }
+      for (int j = 0; ok && j < steps; ++j, ++i) {
+        const int set = 2 * (i & 1);
+        bool now = mbar_try_wait(&q_full[stage], phase) & mbar_try_wait(&a_full[i % AS], i / AS & 1);
+        if (i >= 2) now = now & mbar_try_wait(&s_empty[set], (i / 2 - 1) & 1) & mbar_try_wait(&s_empty[set + 1], (i / 2 - 1) & 1);
+        if (!now)
+          now = sk_wait2(&q_full[stage], phase, &a_full[i % AS], i / AS & 1, abort_flag) &&
+                (i < 2 || sk_wait2(&s_empty[set], (i / 2 - 1) & 1, &s_empty[set + 1], (i / 2 - 1) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, now);
         if (!ok) break;
+        tc_fence_after();
+        const uint64_t dq = dQ + (uint32_t)(stage * C::Q_BYTES >> 4);
+        sk_products<HD / 16>(issue, tmem + set * KM_PAIRS, dK, dq, C::K_CH, C::Q_CH, idesc);
+        tc_commit_if(issue, &s_full[set]);
+        sk_products<HD / 16>(issue, tmem + (set + 1) * KM_PAIRS, dK + (uint32_t)(C::K_BYTES >> 4), dq, C::K_CH, C::Q_CH, idesc);
+        tc_commit_if(issue, &s_full[set + 1]);
         tc_commit_if(issue, &q_empty[stage]);
         if (++stage == QS) {
           stage = 0;

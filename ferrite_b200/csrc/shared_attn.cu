@@ -256,12 +256,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           ok = ok && wait(&k_full[st_i], phase, &s_empty[s], ((i >> 1) - 1) & 1, i >= 2);
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (uint32_t)(kk & 3) * 32u;
-            tc_mma_f16_if(issue, tmem + C::COL_S + s * SA_KT, umma_desc_k128(aQ + (kk >> 2) * C::Q_CH + off),
-                          umma_desc_k128(aK + (kk >> 2) * C::KV_CH + off), idesc, kk > 0 ? 1u : 0u);
-          }
+          sk_products<HD / 16>(issue, tmem + C::COL_S + s * SA_KT, umma_desc_k128(aQ), umma_desc_k128(aK), C::Q_CH, C::KV_CH, idesc);
           tc_commit_if(issue, &s_full[s]);
           tc_commit_if(issue, &k_empty[st_i]);
           if (++st_i == KS) {
@@ -275,10 +270,10 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           ok = ok && wait(&v_full[st_i], phase, &p_full[i & 3], (i >> 2) & 1, true);
           if (!ok) break;
           tc_fence_after();
+          const uint64_t dV = sk_desc_mn128(aV, C::KV_CH, 1024);
 #pragma unroll
           for (int kk = 0; kk < SA_KT / 16; ++kk)
-            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + (i & 3) * (SA_KT / 2) + kk * 8, sk_desc_mn128(aV + kk * 16 * 128, C::KV_CH, 1024), idesc,
-                             (j > 0 || kk > 0) ? 1u : 0u);
+            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + (i & 3) * (SA_KT / 2) + kk * 8, dV + (uint32_t)(kk * 16 * 128 >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit_if(issue, &v_empty[st_i]);
           tc_commit_if(issue, &p_empty[i & 3]);
           if (++st_i == VS) {
@@ -554,9 +549,9 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
   if (tid == 0) {
     ms.abort = 0;
     mbar_init(q_full, 2 * SA_SET);
-    mbar_init(q_done, 1);
+    mbar_init(q_done, 2);
     for (int i = 0; i < 4; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], SA_SET); }        // [tile of pairs][parity]
-    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
+    for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -604,31 +599,28 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
     }
     if (*abort_flag && lane == 0)
       for (int j = max(0, i - KS); j < i; ++j) mbar_wait(&k_full[j % KS], (j / KS) & 1, 1u << 20);
-  } else if (warp == 1) {
+  } else if (warp < 3) {
+    // ---- products of a tile of keys with the first 128 pairs (warp 1) and the others (warp 2)
     constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, SA_KT);
     const bool issue = elect_one();
-    const uint32_t aQ = smem_u32(sQ), aK = smem_u32(sK);
-    int stage = 0, phase = 0, piece = 0, count[2] = {0, 0};
+    const int a = warp - 1;
+    const uint64_t dQ = umma_desc_k128(smem_u32(sQ) + a * C::Q_BYTES), dK = umma_desc_k128(smem_u32(sK));
+    int stage = 0, phase = 0, piece = 0, count = 0;
     bool ok = true;
     do {
-      const int tiles = x.e.nrows > Rh ? 2 : 1;
+      const bool there = a == 0 || x.e.nrows > Rh;
       ok = __all_sync(0xffffffffu, sk_wait(q_full, piece & 1, abort_flag));
       for (int j = 0; ok && j < x.n; ++j) {
-        ok = __all_sync(0xffffffffu, sk_wait(&k_full[stage], phase, abort_flag));
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          if (!ok || a >= tiles) break;
-          const int c = count[a]++, b = 2 * a + (c & 1);
-          ok = c < 2 || __all_sync(0xffffffffu, sk_wait(&s_empty[b], (c / 2 - 1) & 1, abort_flag));
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            tc_mma_f16_if(issue, tmem + b * SA_KT, umma_desc_k128(aQ + a * C::Q_BYTES + (kk >> 2) * C::Q_CH + (kk & 3) * 32),
-                          umma_desc_k128(aK + stage * C::T_BYTES + (kk >> 2) * C::KV_CH + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
-          tc_commit_if(issue, &s_full[b]);
-        }
+        const int b = 2 * a + (count & 1);
+        ok = __all_sync(0xffffffffu, sk_wait2(&k_full[stage], phase, there && count >= 2 ? &s_empty[b] : &k_full[stage],
+                                              there && count >= 2 ? (count / 2 - 1) & 1 : phase, abort_flag));
         if (!ok) break;
+        if (there) {
+          tc_fence_after();
+          sk_products<HD / 16>(issue, tmem + b * SA_KT, dQ, dK + (uint32_t)(stage * C::T_BYTES >> 4), C::Q_CH, C::KV_CH, idesc);
+          tc_commit_if(issue, &s_full[b]);
+          ++count;
+        }
         tc_commit_if(issue, &k_empty[stage]);
         if (++stage == KS) {
           stage = 0;

@@ -249,6 +249,15 @@ __device__ __forceinline__ bool sk_wait2(uint64_t* a, uint32_t pa, uint64_t* b, 
 __device__ __forceinline__ uint64_t sk_desc_mn128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
 }
+// D = A B^T over 16 NK columns of K-major operands in chunks of 64, chunk_a and chunk_b bytes apart, from the operands' first descriptors. (The issuing warp gets a
+// fifth of its scheduler's slots beside four warps of arithmetic: a descriptor built anew for every product costs as much as the product.)
+template <int NK>
+__device__ __forceinline__ void sk_products(bool issue, uint32_t tmem_d, uint64_t a, uint64_t b, int chunk_a, int chunk_b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk)
+    tc_mma_f16_if(issue, tmem_d, a + (uint32_t)(((kk >> 2) * chunk_a + (kk & 3) * 32) >> 4), b + (uint32_t)(((kk >> 2) * chunk_b + (kk & 3) * 32) >> 4), idesc,
+                  kk > 0 ? 1u : 0u);
+}
 __device__ __forceinline__ void sk_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
