@@ -317,7 +317,7 @@ constexpr int KP_KEYS = 2 * KM_KEYS, KP_PLAN = 1024, KP_CHUNKS = 1024;   // keys
 
 struct KpItem {                                  // 256 keys of a span
   int slot, key0, k0, k1;                        // its keys: key0 .. key0 + 255, those of k0 .. k1 count
-  int chunk0, chunks, pad0, pad1;
+  int chunk0, chunks, seen, pad;                 // seen: blocks that see it
 };
 struct KpChunk {                                 // of an item: of blocks b0 .. b1 those that see it, `steps` in number
   int item, b0, b1, steps;
@@ -380,28 +380,32 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
   __syncthreads();
   // steps of a chunk: eight chunks a CTA where there are enough, no fewer than 8 steps and no more than KP_CHUNKS chunks more than items
   const int C = (int)max((long long)chunk_s, (plan.places + KP_CHUNKS - 1) / KP_CHUNKS);
+  const int lane = tid & 31, warp = tid >> 5;
+  auto span_of = [&](int it) {                                       // the last span that starts at or ahead of the item
+    int lo = 0, hi = spans - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (plan.place[mid] <= it) lo = mid;
+      else hi = mid - 1;
+    }
+    return lo;
+  };
+  // a warp an item: how many blocks see it
+  for (int it = warp; it < total; it += KP_PLAN / 32) {
+    const int i = span_of(it), j = it - plan.place[i];
+    int n = 0;
+    for (int b = first(i); b < behind(i); b += 32) n += __popc(__ballot_sync(0xffffffffu, b + lane < behind(i) && nts[min(b + lane, plan.blocks - 1)] > j));
+    if (lane == 0) {
+      const SharedBlock blk = w.blocks[first(i)];
+      w.items[it] = KpItem{blk.slot, (blk.k0 / KP_KEYS + j) * KP_KEYS, blk.k0, end(i), 0, (n + C - 1) / C, n, 0};
+    }
+  }
+  __syncthreads();
+  // numbers of the chunks
   int base = 0;
   for (int i0 = 0; i0 < total; i0 += KP_PLAN) {
-    const int it = i0 + tid;
-    int lo = 0, hi = spans - 1, n = 0;
-    KpItem e{};
-    if (it < total) {
-      while (lo < hi) {                                              // the last span that starts at or ahead of the item
-        const int mid = (lo + hi + 1) / 2;
-        if (plan.place[mid] <= it) lo = mid;
-        else hi = mid - 1;
-      }
-      const int j = it - plan.place[lo];
-      for (int b = first(lo); b < behind(lo); ++b) n += nts[b] > j;
-      e.slot = w.blocks[first(lo)].slot;
-      e.k0 = w.blocks[first(lo)].k0;
-      e.k1 = end(lo);
-      e.key0 = (e.k0 / KP_KEYS + j) * KP_KEYS;
-      e.chunks = (n + C - 1) / C;
-    }
-    // numbers of the chunks: a scan over the threads
-    const int lane = tid & 31, warp = tid >> 5;
-    int xs = e.chunks;
+    const int it = i0 + tid, mine = it < total ? w.items[it].chunks : 0;
+    int xs = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, xs, o);
@@ -409,29 +413,36 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
     }
     if (lane == 31) tmp[warp] = xs;
     __syncthreads();
-    int ahead = 0, sum = 0;
-    for (int k = 0; k < 32; ++k) {
-      ahead += k < warp ? (int)tmp[k] : 0;
-      sum += (int)tmp[k];
+    const int sum = (int)tmp[lane];
+    int ahead = lane < warp ? sum : 0, all_here = sum;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+      all_here += __shfl_xor_sync(0xffffffffu, all_here, o);
     }
+    if (it < total) w.items[it].chunk0 = base + ahead + xs - mine;
+    base += all_here;
     __syncthreads();
-    if (it < total) {
-      e.chunk0 = base + ahead + xs - e.chunks;
-      w.items[it] = e;
-      const int j = it - plan.place[lo];
-      int seen = 0, in = 0, from = 0, c = e.chunk0;
-      for (int b = first(lo); b < behind(lo); ++b) {
-        if (nts[b] <= j) continue;
-        if (in == 0) from = b;
-        ++in;
-        ++seen;
-        if (in == C || seen == n) {
-          w.chunks[c++] = KpChunk{it, from, b + 1, in};
-          in = 0;
+  }
+  // a warp an item: where its chunks start and end
+  for (int it = warp; it < total; it += KP_PLAN / 32) {
+    const int i = span_of(it), j = it - plan.place[i], n = w.items[it].seen, c0 = w.items[it].chunk0;
+    int rank = 0;
+    for (int b = first(i); b < behind(i); b += 32) {
+      const bool sees = b + lane < behind(i) && nts[min(b + lane, plan.blocks - 1)] > j;
+      const uint32_t bal = __ballot_sync(0xffffffffu, sees);
+      const int r = rank + __popc(bal & ((1u << lane) - 1)), c = r / C;
+      if (sees) {
+        KpChunk* ch = w.chunks + c0 + c;
+        if (r == c * C) {
+          ch->item = it;
+          ch->b0 = b + lane;
+          ch->steps = min(C, n - r);
         }
+        if (r == c * C + C - 1 || r == n - 1) ch->b1 = b + lane + 1;
       }
+      rank += __popc(bal);
     }
-    base += sum;
   }
   if (tid == 0) {
     w.head[0] = total;
