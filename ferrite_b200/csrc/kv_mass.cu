@@ -25,11 +25,16 @@ struct KmCfg {
   static constexpr int ROWS_AT = 2 * K_BYTES + RS * Q_BYTES;                      // ... what lies behind them then
   static constexpr int TILES = KS * K_BYTES + QS * Q_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
 };
+struct KmShare {                                 // a CTA's share: first block, places, the first one
+  int b0, places;
+  long long f0;
+};
 template <int QS>
 struct KmMisc {
   float nl[QS][KM_PAIRS];                        // minus a pair's logarithm (log2); minus infinity where there is no pair
   int kvl[QS][KM_PAIRS];                         // keys that it sees
   uint64_t bars[44];
+  KmShare share;
   uint32_t tmem;
   int abort;
 };
@@ -143,28 +148,55 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = ms.tmem;
   pdl_wait();
-  SharedPlan<KM_THREADS> plan;
-  const bool fits = plan.make(st, R, KM_KEYS, KM_EXTRA, z, smem, reinterpret_cast<long long*>(ms.nl), status);
-  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
-  const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
-  if (f0 == f1 || per >= 1ll << 31) {
-    if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+  SharedPlan<KM_THREADS> plan{};
+  // the CTA's part of the plan, by `count` threads of which this is number `me`: first block, first place, places
+  auto take = [&](bool fits, int me, int count) {
+    const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+    const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
+    if (f0 == f1 || per >= 1ll << 31) {
+      if (me == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+      return KmShare{0, 0, 0};
+    }
+    const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
+    for (int b = b0 + me; b <= b1; b += count) {                     // (other CTAs of a block write the same)
+      SharedBlock e = plan.block(st, b, R, KM_KEYS, status);
+      e.place0 = plan.place[b];
+      table[b] = e;
+    }
+    return KmShare{b0, (int)(f1 - f0), f0};
+  };
+  if (z.few) {
+    plan.load(st, z, smem);
+    if (tid == 0) ms.share = KmShare{0, 0, 0};
+    __syncthreads();
+    if (tid < SK_FEW) {
+      SharedBlock e;
+      int count;
+      const bool fits = plan.make_by_few(st, R, KM_KEYS, KM_EXTRA, z, reinterpret_cast<long long*>(ms.nl), status, &e, &count);
+      const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+      const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per), at = (long long)e.place0 * nkv, end = at + (long long)count * nkv;
+      if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+      if (fits && per < 1ll << 31 && f0 < f1) {
+        if (count > 0 && at <= f0 && end > f0) ms.share = KmShare{tid, (int)(f1 - f0), f0};
+        if (tid < plan.blocks && at < f1 && end >= f0) table[tid] = e;           // (blocks without tiles between others too)
+      }
+    }
+  } else {
+    const KmShare got = take(plan.make(st, R, KM_KEYS, KM_EXTRA, z, smem, reinterpret_cast<long long*>(ms.nl), status), tid, KM_THREADS);
+    if (tid == 0) ms.share = got;
+  }
+  __syncthreads();
+  const KmShare share_of = ms.share;
+  if (share_of.places == 0) {                                        // the same for the whole CTA
     if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
     return;
   }
-  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
-  for (int b = b0 + tid; b <= b1; b += KM_THREADS) {                 // (other CTAs of a block write the same)
-    SharedBlock e = plan.block(st, b, R, KM_KEYS, status);
-    e.place0 = plan.place[b];
-    table[b] = e;
-  }
-  __syncthreads();
   // rows of a tile of queries that no copy writes are zeros
   for (int i = tid; i < C::QS * C::Q_BYTES / 16; i += KM_THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
   __syncthreads();
   KmWalk x;
-  if (!x.start(table, b0, f0, (int)(f1 - f0), nkv)) goto done;       // the same for the whole CTA
+  if (!x.start(table, share_of.b0, share_of.f0, share_of.places, nkv)) goto done;        // the same for the whole CTA
   if (warp == 0) {
     // ---- keys
     int i = 0, stage = 0, phase = 0;

@@ -43,6 +43,11 @@ struct SaCfg {
   // TMEM: O | S0 S1 | P0 .. P3
   static constexpr uint32_t COL_S = HD, COL_P = COL_S + 2 * SA_KT, COLS = 512;
 };
+// A CTA's share of the list: block that it starts in, blocks of groups, its first place, places.
+struct SaShare {
+  int b0, group_blocks, places;
+  long long f0;
+};
 template <int STAGES>
 struct SaMisc {
   float mx[2][SA_PAIRS], m[SA_PAIRS];            // maxima of a tile's halves (of the set whose turn it is); the maximum that O belongs to (log2)
@@ -51,6 +56,7 @@ struct SaMisc {
   uint8_t bad[2][2][8];                          // by set and turn: keys of a tile whose values are no numbers
   uint32_t tmem;
   int abort;
+  SaShare share;
   SharedBlock blocks[SA_NEAR];                   // the first ones of the CTA's share; what follows is in the workspace
 };
 
@@ -66,24 +72,12 @@ struct SaSpace {
   int seg_pairs;
 };
 
-// A CTA's share of the list: block that it starts in, blocks of groups, its first place, places.
-struct SaShare {
-  int b0, group_blocks, places;
-  long long f0;
-};
-// -> whether there is any (the same for the whole CTA, whose threads all call this, and which may put tiles in the place of `smem` then)
+// -> whether there is any (the same for the whole CTA, whose threads all call this, and which may put tiles in the place of `smem` then). kept: shared memory
 template <int THREADS>
-__device__ __forceinline__ bool sa_share(SaShare* mine, const FbSharedStep& st, const SaSpace& w, int R, int nkv, unsigned char* smem, long long* tmp,
-                                         SharedBlock* near, int* status) {
+__device__ __forceinline__ bool sa_share(SaShare* mine, SaShare* kept, const FbSharedStep& st, const SaSpace& w, int R, int nkv, unsigned char* smem,
+                                         long long* tmp, SharedBlock* near, int* status) {
   const int tid = threadIdx.x;
-  SharedPlan<THREADS> plan;
-  const bool fits = plan.make(st, R, SA_KT, SA_EXTRA, w.z, smem, tmp, status);
-  const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
-  const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
-  if (blockIdx.x == 0 && tid == 0) {
-    w.head[0] = fits && per < 1ll << 31 ? per : 0;
-    w.head[1] = fits ? plan.group_blocks : 0;
-  }
+  SharedPlan<THREADS> plan{};
   // what the second kernel has to know of a row: written by every CTA that has the block's tiles (the same), or by the first one
   auto note = [&](int b, const SharedBlock& e) {
     const int s = plan.span[b] - st.ngrp, unit = (b - (s >= 0 ? plan.group_blocks : 0)) * nkv;
@@ -92,25 +86,66 @@ __device__ __forceinline__ bool sa_share(SaShare* mine, const FbSharedStep& st, 
       if (s >= 0 && plan.group[s] < 0) w.rows[2 * (e.row0 + r)] = make_int4(0, 0, 0, 0);
     }
   };
-  if (fits && blockIdx.x == 0)
-    for (int b = tid; b < plan.blocks; b += THREADS)                 // blocks that have no keys
-      if ((b + 1 < plan.blocks ? (long long)plan.place[b + 1] : plan.places) == plan.place[b]) note(b, plan.block(st, b, R, SA_KT, status));
-  if (f0 == f1 || per >= 1ll << 31) {
-    if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
-    return false;
+  // the CTA's part of the plan, by `count` threads of which this is number `me`
+  auto take = [&](bool fits, int me, int count) {
+    const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+    const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per);
+    if (blockIdx.x == 0 && me == 0) {
+      w.head[0] = fits && per < 1ll << 31 ? per : 0;
+      w.head[1] = fits ? plan.group_blocks : 0;
+    }
+    if (fits && blockIdx.x == 0)
+      for (int b = me; b < plan.blocks; b += count)                  // blocks that have no keys
+        if ((b + 1 < plan.blocks ? (long long)plan.place[b + 1] : plan.places) == plan.place[b]) note(b, plan.block(st, b, R, SA_KT, status));
+    if (f0 == f1 || per >= 1ll << 31) {
+      if (me == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+      return SaShare{0, 0, 0, 0};
+    }
+    const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
+    for (int b = b0 + me; b <= b1; b += count) {
+      SharedBlock e = plan.block(st, b, R, SA_KT, status);
+      e.place0 = plan.place[b];
+      if (b - b0 < SA_NEAR) near[b - b0] = e;
+      else w.table[b] = e;
+      if (e.nt) note(b, e);
+    }
+    return SaShare{b0, plan.group_blocks, (int)(f1 - f0), f0};
+  };
+  if (w.z.few) {
+    plan.load(st, w.z, smem);
+    if (tid == 0) *kept = SaShare{0, 0, 0, 0};
+    __syncthreads();
+    if (tid < SK_FEW) {
+      SharedBlock e;
+      int count;
+      const bool fits = plan.make_by_few(st, R, SA_KT, SA_EXTRA, w.z, tmp, status, &e, &count);
+      const long long all = fits ? plan.places * nkv : 0, per = max(1ll, (all + gridDim.x - 1) / gridDim.x);
+      const long long f0 = min(all, blockIdx.x * per), f1 = min(all, f0 + per), at = (long long)e.place0 * nkv, end = at + (long long)count * nkv;
+      if (blockIdx.x == 0 && tid == 0) {
+        w.head[0] = fits && per < 1ll << 31 ? per : 0;
+        w.head[1] = fits ? plan.group_blocks : 0;
+      }
+      if (tid == 0 && per >= 1ll << 31) set_status(status, ST_CAPACITY);
+      if (fits && per < 1ll << 31) {                                 // (the same for all of these threads)
+        const bool here = f0 < f1 && count > 0 && at < f1 && end > f0;
+        if (here && at <= f0) *kept = SaShare{tid, plan.group_blocks, (int)(f1 - f0), f0};
+        asm volatile("bar.sync 11, %0;" ::"n"(SK_FEW) : "memory");
+        if (here || (blockIdx.x == 0 && tid < plan.blocks && count == 0)) note(tid, e);
+        const int b0 = kept->b0;
+        if (f0 < f1 && tid >= b0 && tid < plan.blocks && at < f1) {  // (blocks without tiles between others too)
+          if (tid - b0 < SA_NEAR) near[tid - b0] = e;
+          else w.table[tid] = e;
+        }
+      }
+    }
+  } else {
+    const SaShare got = take(plan.make(st, R, SA_KT, SA_EXTRA, w.z, smem, tmp, status), tid, THREADS);
+    if (tid == 0) *kept = got;
   }
-  const int b0 = plan.find(f0, nkv), b1 = plan.find(f1 - 1, nkv);
-  for (int b = b0 + tid; b <= b1; b += THREADS) {
-    SharedBlock e = plan.block(st, b, R, SA_KT, status);
-    e.place0 = plan.place[b];
-    if (b - b0 < SA_NEAR) near[b - b0] = e;
-    else w.table[b] = e;
-    if (e.nt) note(b, e);
-  }
-  *mine = {b0, plan.group_blocks, (int)(f1 - f0), f0};
   fence_proxy_async();                                               // tiles take the plan's place
   __syncthreads();
-  return true;
+  *mine = *kept;
+  return mine->places > 0;
 }
 
 // A CTA's way through its share of the list: (block, kv head) after (block, kv head), as far as tiles of theirs lie in it.
@@ -151,6 +186,40 @@ struct SaWalk {
   }
   __device__ __forceinline__ int token(int j) const { return (e.k0 / SA_KT + t + j) * SA_KT; }
 };
+
+// Bits lo .. hi - 1 of 32.
+__device__ __forceinline__ uint32_t key_bits(int lo, int hi) {
+  const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1, ahead = lo <= 0 ? 0u : lo >= 32 ? 0xffffffffu : (1u << lo) - 1;
+  return below & ~ahead;
+}
+// Values of a tile's keys that no row sees (outside k0 .. k1) become zeros, and those of a key that some row does not see (from kmin on) where one of them is no
+// finite number. Four of a set's threads have a key. -> such keys of the warp's eight. (Out of line: a few tiles of a unit come by, and what lies between the
+// instructions that every tile runs costs their fetches.)
+template <int HD>
+__device__ __noinline__ uint32_t sa_clean_values(unsigned char* base, int thread, int t0, int k0, int k1, int kmin) {
+  constexpr int CH = SA_KT * 128, PER = HD / 32;                     // bytes of 64 columns; 16-byte pieces of a thread
+  const int key = thread >> 2, part = thread & 3, tok = t0 + key, lane = thread & 31;
+  auto at = [&](int e) { return reinterpret_cast<uint4*>(base + ((part * PER + e) >> 3) * CH + key * 128 + ((part * PER + e) & 7) * 16); };
+  bool zero = tok < k0 || tok >= k1, bad = false;
+  if (!zero && tok >= kmin) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) {
+      const uint4 u = *at(e);
+      const uint32_t a[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) bad |= (a[k] & 0x7f80u) == 0x7f80u || (a[k] & 0x7f800000u) == 0x7f800000u;
+    }
+  }
+  const uint32_t bal = __ballot_sync(0xffffffffu, bad);
+  zero |= (bal >> (lane & 28) & 15u) != 0;
+  if (zero)
+#pragma unroll
+    for (int e = 0; e < PER; ++e) *at(e) = make_uint4(0, 0, 0, 0);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) bits |= (bal >> (4 * k) & 15u) ? 1u << k : 0u;
+  return bits;
+}
 
 template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, 1)
@@ -194,7 +263,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
   pdl_wait();
 
   SaShare mine;
-  if (!sa_share<SA_THREADS>(&mine, st, w, SA_PAIRS / share, nkv, smem, ms.tmp, ms.blocks, status)) {
+  if (!sa_share<SA_THREADS>(&mine, &ms.share, st, w, SA_PAIRS / share, nkv, smem, ms.tmp, ms.blocks, status)) {
     if (warp == 1) tmem_dealloc(tmem, C::COLS);
     return;
   }
@@ -344,7 +413,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         const bool need_mask = t0 < y.e.k0 || t0 + SA_KT > y.e.kmin;
         wait(&s_full[set], (i >> 1) & 1);
         if (i + 1 == end && more && !dead) copy_q(x);                // every product that reads the queries is through
-        if (need_mask) {
+        if (__builtin_expect(need_mask, 0)) {
           // Values of keys that some row does not see meet weights of zero: those that no row sees become zeros, those that some see are looked at,
           // and where one is no finite number the key's values become zeros and its score NaN for the rows that see it.
           // (a wait tells a phase from the one ahead of it only: the values of tile i - VS have to be through)
@@ -352,30 +421,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           if (VS < 4 && i >= VS) wait(&p_empty[(i - VS) & 3], ((i - VS) >> 2) & 1);
           wait(&v_full[i % VS], (i / VS) & 1);
           if (!dead) {
-            const int key = st_tid >> 2, part = st_tid & 3, tok = t0 + key;
-            unsigned char* base = sV + (i % VS) * C::T_BYTES;
-            constexpr int PER = HD / 32;                             // 16-byte pieces of a thread
-            auto at = [&](int e) { return reinterpret_cast<uint4*>(base + ((part * PER + e) >> 3) * C::KV_CH + key * 128 + ((part * PER + e) & 7) * 16); };
-            bool zero = tok < y.e.k0 || tok >= y.e.k1, bad = false;
-            if (!zero && tok >= y.e.kmin) {
-#pragma unroll
-              for (int e = 0; e < PER; ++e) {
-                const uint4 u = *at(e);
-                const uint32_t a[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) bad |= (a[k] & 0x7f80u) == 0x7f80u || (a[k] & 0x7f800000u) == 0x7f800000u;
-              }
-            }
-            const uint32_t bal = __ballot_sync(0xffffffffu, bad);
-            zero |= (bal >> (lane & 28) & 15u) != 0;
-            if (zero)
-#pragma unroll
-              for (int e = 0; e < PER; ++e) *at(e) = make_uint4(0, 0, 0, 0);
-            if (lane == 0) {
-              uint32_t bits = 0;
-              for (int k = 0; k < 8; ++k) bits |= (bal >> (4 * k) & 15u) ? 1u << k : 0u;
-              ms.bad[set][i >> 1 & 1][st_tid >> 5] = (uint8_t)bits;
-            }
+            const uint32_t bits = sa_clean_values<HD>(sV + (i % VS) * C::T_BYTES, st_tid, t0, y.e.k0, y.e.k1, y.e.kmin);
+            if (lane == 0) ms.bad[set][i >> 1 & 1][st_tid >> 5] = (uint8_t)bits;
             fence_proxy_async();
           }
           asm volatile("bar.sync %0, 256;" ::"r"(9 + set) : "memory");
@@ -391,14 +438,11 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         __syncwarp();
         if (lane == 0 && !dead) mbar_arrive(&s_empty[set]);
         if (active && !dead) {
-          if (need_mask) {
+          if (__builtin_expect(need_mask, 0)) {
             const int c0 = t0 + sub * HC;
-            const uint32_t bad = reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub];
+            const uint32_t bad = reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub], sees = key_bits(y.e.k0 - c0, klen - c0);
 #pragma unroll
-            for (int c = 0; c < HC; ++c) {
-              if (bad >> c & 1u) sr[c] = 0x7fc00000u;
-              if (c0 + c < y.e.k0 || c0 + c >= klen) sr[c] = 0xff800000u;
-            }
+            for (int c = 0; c < HC; ++c) sr[c] = sees >> c & 1u ? bad >> c & 1u ? 0x7fc00000u : sr[c] : 0xff800000u;
           }
 #pragma unroll
           for (int c = 0; c < HC; c += 4)
@@ -413,7 +457,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         uint32_t moves;
         asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.b32 a, %1, 0;\n\tbarrier.cta.red.or.pred b, %2, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
                      : "=r"(moves) : "r"((uint32_t)(!dead && mx > m_old + 16.f)), "r"(1 + 4 * set + quad) : "memory");
-        if (moves) {
+        if (__builtin_expect(moves, 0)) {
           ms.mx[sub][pair] = mx;
           asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * set + quad) : "memory");
           m_new = fmaxf(m_old, fmaxf(mx, ms.mx[sub ^ 1][pair]));
@@ -432,7 +476,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           l = m_own == -INFINITY ? l : l * sk_exp2(m_own - m_new);   // (a sum that is no number stays one)
           m_own = m_new;
         }
-        if (moves && j > 0) {
+        if (__builtin_expect(moves && j > 0, 0)) {
           const float f = m_old == -INFINITY ? 0.f : sk_exp2(m_old - m_new);
 #pragma unroll 1
           for (int c0 = 0; c0 < OC; c0 += 16) {
@@ -564,7 +608,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
   const uint32_t tmem = ms.tmem;
   pdl_wait();
   SaShare mine;
-  if (!sa_share<SA_THREADS>(&mine, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status)) {
+  if (!sa_share<SA_THREADS>(&mine, &ms.share, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status)) {
     if (warp == 1) tmem_dealloc(tmem, 256);
     return;
   }
@@ -684,10 +728,10 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
           __syncwarp();
           if (lane == 0 && !dead) mbar_arrive(&s_empty[2 * set + b]);
           if (dead || quad * 32 >= np) continue;
-          if (t0 < y.e.k0 || t0 + SA_KT / 2 > y.e.kmin) {
+          if (__builtin_expect(t0 < y.e.k0 || t0 + SA_KT / 2 > y.e.kmin, 0)) {
+            const uint32_t sees = key_bits(y.e.k0 - t0, klen - t0);
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (t0 + c < y.e.k0 || t0 + c >= klen) sr[c] = 0xff800000u;
+            for (int c = 0; c < 32; ++c) sr[c] = sees >> c & 1u ? sr[c] : 0xff800000u;
           }
           float mx = -INFINITY;
 #pragma unroll

@@ -11,6 +11,7 @@
 namespace fb {
 
 constexpr int SK_PLAN_BYTES = 160 << 10;         // shared memory that the plan may take while it is made
+constexpr int SK_FEW = 128;                      // spans and blocks of a step that SK_FEW threads plan
 
 // What a block is. kmin: keys that all of its rows see. place0: places of the blocks ahead of it (of one kv head): a unit has one for every key tile and,
 // ahead of them, `extra` for what it costs besides.
@@ -69,10 +70,13 @@ __device__ __forceinline__ long long scan_ahead(int* a, int n, long long* tmp) {
 struct SharedPlanSizes {
   int blocks, group_blocks;                      // room for: all, those of groups
   bool kv;
+  bool few;                                      // SK_FEW threads make the plan
 };
 inline bool shared_plan_sizes(const FbSharedStep& st, long group_blocks, long seg_blocks, SharedPlanSizes* z) {
   const long words = 5l * st.nseg + 4l * st.ngrp + 2 * (group_blocks + seg_blocks), room = SK_PLAN_BYTES / 4;
-  *z = {(int)(group_blocks + seg_blocks), (int)group_blocks, words + st.rows <= room};
+  const bool kv = words + st.rows <= room;
+  *z = {(int)(group_blocks + seg_blocks), (int)group_blocks, kv, 
+        kv && group_blocks + seg_blocks <= SK_FEW && st.nseg + st.ngrp <= SK_FEW && (long)st.max_blocks * st.kv_block < 1l << 29};
   return words <= room;
 }
 
@@ -85,8 +89,8 @@ struct SharedPlan {
   int blocks, group_blocks;
   long long places;                              // of one kv head
 
-  // -> false where the step does not fit (with a status)
-  __device__ __forceinline__ bool make(const FbSharedStep& st, int R, int kt, int extra, const SharedPlanSizes& z, unsigned char* smem, long long* tmp, int* status) {
+  // The step's tables into shared memory, by all threads; a barrier has to follow.
+  __device__ __forceinline__ void load(const FbSharedStep& st, const SharedPlanSizes& z, unsigned char* smem) {
     const int tid = threadIdx.x, S = st.nseg, G = st.ngrp;
     slot = reinterpret_cast<int*>(smem); row0 = slot + S; rows = row0 + S; group = rows + S;
     seg0 = group + S; segs = seg0 + G; len = segs + G;
@@ -106,38 +110,101 @@ struct SharedPlan {
       segs[g] = st.grp_nsegs[g];
       len[g] = st.grp_len[g];
     }
-    __syncthreads();
-    for (int g = tid; g < G; g += THREADS) {
-      const int s0 = seg0[g], n = segs[g];
-      int count = 0;
-      if (s0 < 0 || n < 0 || n > S - s0) {
-        set_status(status, ST_BOUNDS);
-      } else if (n > 0) {
-        count = row0[s0 + n - 1] + rows[s0 + n - 1] - row0[s0];
-        if (slot[s0] < 0 || slot[s0] >= st.slots || !rows_fit(st, row0[s0], count)) {
-          set_status(status, ST_BOUNDS);
-          count = 0;
-        }
-      }
-      start[g] = count;
+  }
+  // rows of group g, 0 where it does not fit the step
+  __device__ __forceinline__ int group_rows(const FbSharedStep& st, int g, int* status) const {
+    const int s0 = seg0[g], n = segs[g];
+    if (n == 0) return 0;
+    if (s0 >= 0 && n > 0 && n <= st.nseg - s0) {
+      const int count = row0[s0 + n - 1] + rows[s0 + n - 1] - row0[s0];
+      if (slot[s0] >= 0 && slot[s0] < st.slots && rows_fit(st, row0[s0], count)) return count;
     }
-    __syncthreads();
-    for (int s = tid; s < S; s += THREADS) {
-      int own = -1;
-      for (int g = 0; g < G; ++g)
-        if (start[g] > 0 && s >= seg0[g] && s - seg0[g] < segs[g]) {
-          if (own >= 0 || (s > seg0[g] && row0[s] != row0[s - 1] + rows[s - 1])) set_status(status, ST_BOUNDS);   // of two groups; rows that lie apart
-          own = g;
-        }
-      group[s] = own;
-      bool ok = slot[s] >= 0 && slot[s] < st.slots && rows_fit(st, row0[s], rows[s]);
-      if (!ok) set_status(status, ST_BOUNDS);
-      if (ok && rows[s] > st.max_rows) {
-        set_status(status, ST_CAPACITY);
-        ok = false;
+    set_status(status, ST_BOUNDS);
+    return 0;
+  }
+  // group of segment s and its own blocks (where `start` holds the groups' rows)
+  __device__ __forceinline__ int segment(const FbSharedStep& st, int s, int R, int* status) {
+    int own = -1;
+    for (int g = 0; g < st.ngrp; ++g)
+      if (start[g] > 0 && s >= seg0[g] && s - seg0[g] < segs[g]) {
+        if (own >= 0 || (s > seg0[g] && row0[s] != row0[s - 1] + rows[s - 1])) set_status(status, ST_BOUNDS);   // of two groups; rows that lie apart
+        own = g;
       }
-      start[G + s] = ok ? (rows[s] + R - 1) / R : 0;
+    group[s] = own;
+    if (slot[s] < 0 || slot[s] >= st.slots || !rows_fit(st, row0[s], rows[s])) {
+      set_status(status, ST_BOUNDS);
+      return 0;
     }
+    if (rows[s] > st.max_rows) {
+      set_status(status, ST_CAPACITY);
+      return 0;
+    }
+    return (rows[s] + R - 1) / R;
+  }
+  __device__ __forceinline__ bool fits(const SharedPlanSizes& z) const {
+    return blocks <= z.blocks && group_blocks <= z.group_blocks && blocks - group_blocks <= z.blocks - z.group_blocks;
+  }
+
+  // The plan of a step of up to SK_FEW spans and blocks from the loaded tables, by the first SK_FEW threads: each a span, then a block, which it keeps (`e`, with
+  // its place). What make() does in loops and from shared memory stays in registers: code that an SM sees for the first time costs nine cycles an
+  // instruction, and this comes before everything else.
+  __device__ __forceinline__ bool make_by_few(const FbSharedStep& st, int R, int kt, int extra, const SharedPlanSizes& z, long long* tmp, int* status, SharedBlock* e,
+                                              int* count) {
+    const int me = threadIdx.x, lane = me & 31, warp = me >> 5, S = st.nseg, G = st.ngrp;
+    int* sums = reinterpret_cast<int*>(tmp);
+    auto sync = [] { asm volatile("bar.sync 11, %0;" ::"n"(SK_FEW) : "memory"); };
+    auto scan = [&](int v, int* at, int* all) {                                  // v -> sum of what lies ahead, of all
+      int x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) at[warp] = x;
+      sync();
+      int ahead = x - v, total = 0;
+#pragma unroll
+      for (int w = 0; w < SK_FEW / 32; ++w) {
+        const int y = at[w];
+        if (w < warp) ahead += y;
+        total += y;
+      }
+      *all = total;
+      return ahead;
+    };
+    const int grows = me < G ? group_rows(st, me, status) : 0;
+    if (me < G) start[me] = grows;
+    sync();
+    const int n = me < G ? (grows + R - 1) / R : me < G + S ? segment(st, me - G, R, status) : 0;
+    // (the first barrier of the scan is behind every look at the groups' rows in `start`)
+    const int first = scan(n, sums, &blocks);
+    if (me == G) sums[8] = first;
+    if (me < G) segs[me] = grows;                                                // (from here on: rows)
+    if (me < G + S) start[me] = first;
+    for (int b = 0; b < n && first + b < z.blocks; ++b) span[first + b] = me;
+    sync();
+    group_blocks = sums[8];
+    if (!fits(z)) {
+      if (me == 0) set_status(status, ST_CAPACITY);
+      return false;
+    }
+    *e = SharedBlock{};
+    if (me < blocks) *e = block(st, me, R, kt, status);
+    *count = e->nt ? e->nt + extra : 0;
+    int all;
+    e->place0 = scan(*count, sums + 4, &all);                                    // (fewer than 2^31: 128 blocks of fewer than 2^23 tiles)
+    places = all;
+    return true;
+  }
+
+  // -> false where the step does not fit (with a status)
+  __device__ __forceinline__ bool make(const FbSharedStep& st, int R, int kt, int extra, const SharedPlanSizes& z, unsigned char* smem, long long* tmp, int* status) {
+    const int tid = threadIdx.x, S = st.nseg, G = st.ngrp;
+    load(st, z, smem);
+    __syncthreads();
+    for (int g = tid; g < G; g += THREADS) start[g] = group_rows(st, g, status);
+    __syncthreads();
+    for (int s = tid; s < S; s += THREADS) start[G + s] = segment(st, s, R, status);
     __syncthreads();
     for (int g = tid; g < G; g += THREADS) {
       segs[g] = start[g];                                                        // (from here on: rows)
@@ -147,7 +214,7 @@ struct SharedPlan {
     const long long all = scan_ahead<THREADS>(start, G + S, tmp);
     blocks = (int)min(all, 0x7fffffffll);
     group_blocks = start[G];
-    if (blocks > z.blocks || group_blocks > z.group_blocks || blocks - group_blocks > z.blocks - z.group_blocks) {
+    if (!fits(z)) {
       if (tid == 0) set_status(status, ST_CAPACITY);
       return false;
     }
