@@ -796,17 +796,17 @@ __global__ void __launch_bounds__(256) shared_lse_join_kernel(float* lse, FbShar
 
 // Pieces of a head's row -> output and logarithm. grid: rows x query heads; a thread has four columns and every fourth (eighth, 16th) piece. Everything that
 // does not depend on the pieces is asked for at once, and the pieces' sums beside their maxima: three trips to memory.
-template <int HD>
-__global__ void __launch_bounds__(256, 4) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride, FbSharedStep st, SaSpace w,
+template <int HD, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride, FbSharedStep st, SaSpace w,
                                                           int nkv, int share, int ctas) {
-  constexpr int LANES = HD / 4, PARTS = 256 / LANES;
+  constexpr int LANES = HD / 4, PARTS = THREADS / LANES;
   __shared__ float top_s[PARTS], sum_s[PARTS];
   __shared__ float4 o_s[PARTS][LANES];
   const int row = blockIdx.x, h = blockIdx.y, kvh = h / share, g = h - kvh * share, tid = threadIdx.x, part = tid / LANES, d = tid % LANES * 4;
   pdl_launch_dependents();
   pdl_wait();
   bool mine = false;
-  for (int s = tid; s < st.nseg; s += 256) mine |= row >= st.seg_row0[s] && row - st.seg_row0[s] < st.seg_nrows[s];
+  for (int s = tid; s < st.nseg; s += THREADS) mine |= row >= st.seg_row0[s] && row - st.seg_row0[s] < st.seg_nrows[s];
   const long long per = w.head[0];
   const int n = st.kvlen[row];
   const int4 info[2] = {w.rows[2 * row], w.rows[2 * row + 1]};
@@ -985,11 +985,13 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
   FB_SA(64) FB_SA(128) FB_SA(256)
 #undef FB_SA
   if (e != cudaSuccess) return (int)e;
-#define FB_SJ(H)                                                                                                                                    \
-  if (hd == H)                                                                                                                                      \
-    return (int)launch_pdl(shared_join_kernel<H>, dim3(st.rows, nq), dim3(256), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj,         \
+  // 256 threads a head's row where all of them run at once: more pieces under way; more rows run as twice as many CTAs of 128, since each is a chain of trips to
+  // memory (us, 256 / 128: 48 rows 5.7 / 6.7, 144 6.8 / 8.0, 816 10.9 / 8.5, 2048 17.5 / 11.0)
+#define FB_SJ(H, N)                                                                                                                                 \
+  if (hd == H && (N == 256) == ((long)st.rows * nq <= 4l * ctas))                                                                                   \
+    return (int)launch_pdl(shared_join_kernel<H, N>, dim3(st.rows, nq), dim3(N), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj,        \
                            proj_stride, st, w, nkv, share, ctas);
-  FB_SJ(64) FB_SJ(128) FB_SJ(256)
+  FB_SJ(64, 256) FB_SJ(128, 256) FB_SJ(256, 256) FB_SJ(64, 128) FB_SJ(128, 128) FB_SJ(256, 128)
 #undef FB_SJ
   return -2;
 }
