@@ -42,6 +42,7 @@ FbSharedStep check_step(const Tensor& q, const Tensor& k, const Tensor& kvlen, c
               q.stride(2) == 1 && aligned(q, 16) && q.device() == k.device(), what, ": q is not [rows, ", nq, ", ", hd, "] bf16 with dense heads");
   TORCH_CHECK(q.size(0) * nq < (1 << 30), what, ": rows");
   TORCH_CHECK(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0 && table.size(1) * kv_block < std::numeric_limits<int>::max(), what, ": block_table");
+  TORCH_CHECK(nkv * (table.size(1) * kv_block / 64 + 8) < std::numeric_limits<int>::max(), what, ": block_table of ", table.size(1) * kv_block, " tokens");
   TORCH_CHECK((max_rows >= 1 || seg_slot.numel() == 0 || q.size(0) == 0) && max_rows <= std::numeric_limits<int>::max() && status.scalar_type() == torch::kInt32 && status.device() == k.device(), what,
               ": max_rows, status");
   TORCH_CHECK(grp_seg0.has_value() == grp_nsegs.has_value() && grp_seg0.has_value() == grp_len.has_value(), what, ": groups");
@@ -90,7 +91,7 @@ void attention_shared(Tensor out, OptTensor lse, Tensor ws, Tensor q, Tensor k, 
                             (int)ctas, status.data_ptr<int>(), cur_stream()), what);
 }
 
-void attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Tensor ws, Tensor q, Tensor k, Tensor kvlen, Tensor table, int64_t kv_block,
+int64_t attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Tensor ws, Tensor q, Tensor k, Tensor kvlen, Tensor table, int64_t kv_block,
                     int64_t nq, int64_t nkv, int64_t hd, Tensor seg_slot, Tensor seg_row0, Tensor seg_nrows, int64_t max_rows, OptTensor grp_seg0,
                     OptTensor grp_nsegs, OptTensor grp_len, int64_t ctas, Tensor status) {
   const char* what = "attention_mass";
@@ -107,6 +108,7 @@ void attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Tensor
   check(fb_attention_mass(out.data_ptr<float>(), mass.data_ptr<float>(), (float)carry, lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr<float>(),
                           (long)ws.numel(), q.data_ptr(), (long)q.stride(0), k.data_ptr(), st, (int)nq, (int)nkv, (int)hd, (int)ctas,
                           status.data_ptr<int>(), cur_stream()), what);
+  return fb_attention_mass_launches(st.rows, st.max_rows, st.ngrp, (int)nq, (int)nkv, (int)hd, !lse);
 }
 
 // k, v [pages, kv_block, nkv, ..] of 16-bit values or of codes; scale [pages, kv_block, nkv, ns]

@@ -726,9 +726,11 @@ static int make_tmap_queries(CUtensorMap* out, const void* q, int rows, int nq, 
 // Rows whose queries stay in shared memory
 static int km_resident_rows(int hd, int share) { return (hd == 256 ? KmCfg<256>::QS : hd == 128 ? KmCfg<128>::QS : KmCfg<64>::QS) * (KM_PAIRS / share); }
 static bool km_few(int rows, int max_rows, int ngrp, int hd, int share) { return (ngrp ? rows : std::min(rows, max_rows)) <= km_resident_rows(hd, share); }
-static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room) {
+// (A span of n keys is of up to n / 256 + 2 items, and a key of the pool is of one span.)
+static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room, long keys) {
   const int Rq = KM_PAIRS / share;
-  const long blocks = shared_group_blocks(rows, ngrp, Rq) + shared_seg_blocks(rows, nseg, max_rows, Rq), items = (long)(nseg + ngrp) * ((room + KP_KEYS - 1) / KP_KEYS + 1);
+  const long spans = nseg + ngrp;
+  const long blocks = shared_group_blocks(rows, ngrp, Rq) + shared_seg_blocks(rows, nseg, max_rows, Rq), items = std::min(spans * ((room + KP_KEYS - 1) / KP_KEYS + 1), keys / KP_KEYS + 2 * spans);
   float* at = ws;
   auto take = [&](long floats) {
     float* p = at;
@@ -746,19 +748,23 @@ static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, in
   return at - ws;
 }
 
-extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, long room, int want_lse, int ctas) {
+extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, long room, long keys, int want_lse, int ctas) {
   if (rows <= 0 || nseg <= 0 || nkv < 1 || nq / nkv < 1 || nq / nkv > KM_PAIRS) return 0;
   const int share = nq / nkv;
   const long logs = want_lse ? ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, 0) : 0;
-  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room));
+  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys));
+}
+
+extern "C" int fb_attention_mass_launches(int rows, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse) {
+  return rows <= 0 || max_rows <= 0 ? 0 : (km_few(rows, max_rows, ngrp, hd, nq / nkv) ? 1 : 3) + (want_lse ? 2 : 0);
 }
 
 extern "C" int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride,
                                  const void* k, FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s) {
   if (st.rows <= 0 || st.nseg <= 0 || st.max_rows <= 0) return 0;
   if (nkv < 1 || nq % nkv || nq / nkv > KM_PAIRS || st.kv_block % 64 || ctas < 1 || (hd != 64 && hd != 128 && hd != 256)) return -1;
-  const long room = (long)st.max_blocks * st.kv_block;
-  if (ws_floats < fb_attention_mass_floats(st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, room, !lse, ctas)) return -3;
+  const long room = (long)st.max_blocks * st.kv_block, keys = st.pages * st.kv_block;
+  if (ws_floats < fb_attention_mass_floats(st.rows, st.nseg, st.max_rows, st.ngrp, nq, nkv, hd, room, keys, !lse, ctas)) return -3;
   const int share = nq / nkv, Rq = KM_PAIRS / share;
   int rc;
   if (!lse) {
@@ -791,7 +797,7 @@ extern "C" int fb_attention_mass(float* out, const float* mass, float carry, con
     return (int)e;
   }
   KpSpace w;
-  km_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nkv, share, room);
+  km_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nkv, share, room, keys);
   if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, Rq), shared_seg_blocks(st.rows, st.nseg, st.max_rows, Rq), &w.z)) return -2;
   FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_PLAN_BYTES));
   if ((e = launch_pdl(kv_mass_plan_kernel, dim3(1), dim3(KP_PLAN), SK_PLAN_BYTES, s, st, w, Rq, nkv, ctas, status)) != cudaSuccess) return (int)e;

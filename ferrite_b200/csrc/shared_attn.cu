@@ -26,9 +26,7 @@
 namespace fb {
 
 constexpr int SA_PAIRS = 128, SA_KT = 64, SA_NEAR = 4;
-#ifndef SA_EXTRA
-#define SA_EXTRA 3
-#endif
+constexpr int SA_EXTRA = 3;                                  // places of a unit's queries and piece, in key tiles (2 to 5 measure alike)
 constexpr int SA_SET = 8;                                    // warps of a set: two threads a pair, each with half of a tile's keys
 constexpr int SA_THREADS = (4 + 2 * SA_SET) * 32;
 constexpr int SA_ML = 8;                                     // floats of a pair's statistics: its threads' sums, the maximum
@@ -776,11 +774,11 @@ __global__ void __launch_bounds__(256) shared_lse_join_kernel(float* lse, FbShar
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int4 info = w.rows[2 * row + k];
-    const long long at = (long long)info.x * nkv + (long long)kvh * (info.y + SA_EXTRA) + SA_EXTRA;
+    const long long at = (long long)info.x * nkv + kvh * ((long long)info.y + SA_EXTRA) + SA_EXTRA;
     const long long c0 = at / per, c1 = (at + info.y - 1) / per;
     const int first = k ? (int)w.head[1] : 0, last = k ? w.z.blocks : w.z.group_blocks;
-    // checked, since a launch that gave up has not written all of this
-    if (info.y <= 0 || info.x < 0 || c1 >= ctas || info.w < 0 || info.w >= 2 * Rh || info.z < 0 || info.z + kvh >= (last - (k ? w.z.group_blocks : 0)) * nkv) continue;
+    // checked, since this is not written for rows of a segment that was refused, nor by a launch that gave up
+    if (info.y <= 0 || info.x < 0 || c1 >= ctas || info.w < 0 || info.w >= 2 * Rh || info.z < 0 || info.z >= (last - (k ? w.z.group_blocks : 0)) * nkv - kvh) continue;
     const int a = info.w >= Rh, pair = (info.w - a * Rh) * share + g;
     for (long long c = c0; c <= c1; ++c) {
       const long rec = c + (long)first * nkv + info.z + kvh;
@@ -820,11 +818,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   float top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    // a row's run of records; checked, since a launch that gave up has not written all of this
-    const long long at = (long long)info[k].x * nkv + (long long)kvh * (info[k].y + SA_EXTRA) + SA_EXTRA;
+    // a row's run of records; checked, since this is not written for rows of a segment that was refused, nor by a launch that gave up
+    const long long at = (long long)info[k].x * nkv + kvh * ((long long)info[k].y + SA_EXTRA) + SA_EXTRA;
     const long long c0 = at / per, c1 = (at + info[k].y - 1) / per;
     const int r = info[k].w, stride = k == 0 ? SA_PAIRS : w.seg_pairs, units = (k == 0 ? w.z.group_blocks : w.z.blocks - w.z.group_blocks) * nkv;
-    if (info[k].y <= 0 || info[k].x < 0 || c1 >= ctas || r < 0 || (r + 1) * share > stride || info[k].z < 0 || info[k].z + kvh >= units) continue;
+    if (info[k].y <= 0 || info[k].x < 0 || c1 >= ctas || r < 0 || r >= stride / share || info[k].z < 0 || info[k].z >= units - kvh) continue;
     const int pieces = (int)(c1 - c0) + 1;
     const long rec = (c0 + info[k].z + kvh) * stride + r * share + g;
     const float* ml = (k == 0 ? w.ml_grp : w.ml_seg) + rec * SA_ML;

@@ -131,6 +131,7 @@ struct SharedPlan {
         own = g;
       }
     group[s] = own;
+    if (rows[s] == 0) return 0;                                                  // (padding: its slot says nothing)
     if (slot[s] < 0 || slot[s] >= st.slots || !rows_fit(st, row0[s], rows[s])) {
       set_status(status, ST_BOUNDS);
       return 0;
@@ -229,6 +230,10 @@ struct SharedPlan {
     }
     __syncthreads();
     places = scan_ahead<THREADS>(place, blocks, tmp);
+    if (places > 0x7fffffffll) {                                                 // (what a place's number holds)
+      if (tid == 0) set_status(status, ST_CAPACITY);
+      return false;
+    }
     return true;
   }
   // block b (without place0)

@@ -5,8 +5,10 @@ kernels of `csrc/shared_attn.cu`, `csrc/kv_mass.cu` and `csrc/kv_evict.cu`. Both
 A step's rows come in segments of one slot each, `segs` = (seg_slot, seg_row0, seg_nrows, rows of the longest): rows seg_row0 .. seg_row0 + seg_nrows, in any
 order; row i sees the first row_kvlen[i] tokens. `groups` = (grp_seg0, grp_nsegs, grp_len), or None: the rows of grp_nsegs consecutive segments from grp_seg0
 on lie side by side and read their first grp_len tokens, any number, through the table of the first of these segments, and what follows through their
-own. A segment belongs to one group at most. Streams that share pages (a forked conversation, samples of one prompt) are a group, so that their common keys and values are read
-once. A row of no segment is left out: its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a multiple of 64.
+own. A segment belongs to one group at most; one of no rows is padding, whatever its slot (but that of a group's first). Streams that share pages (a forked
+conversation, samples of one prompt) are a group, so that their common keys and values are read once. A row is of one segment; of none, it is left out and
+its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a multiple of 64. What the kernels find wrong in the tables on the
+device (a page or slot that is none, a context beyond its table, a segment of more rows than was said) sets the op class's status word.
 
 Sums of weights are [pages, kv heads, kv_block] in fp32, beside the cache: they follow the pages through forks and parking.
 """
@@ -126,6 +128,8 @@ class CudaShared:
     def attention_shared(self, q, proj, k_cache, v_cache, row_kvlen, block_table, kv_block, nq, nkv, hd, gated, segs, groups=None, want_lse=False):
         """Attention of a step's rows over a cache whose streams share pages; the oracle's docstring and the top of this file say what of. `proj` is read
         for the output gate only."""
+        if gated and proj is None:
+            raise RuntimeError("attention_shared: no proj to gate with")
         q, step = self._shared_step(q, nq, hd, segs, groups)
         T, G = q.shape[0], 0 if groups is None else groups[0].numel()
         out = self.empty(T, nq * hd, dtype=torch.bfloat16, device=q.device)
@@ -142,11 +146,10 @@ class CudaShared:
         q, step = self._shared_step(q, nq, hd, segs, groups)
         out = mass if out is None else out
         G = 0 if groups is None else groups[0].numel()
-        ws = self.empty(self.C.attention_mass_floats(q.shape[0], segs[0].numel(), segs[3], G, nq, nkv, hd, block_table.shape[1] * kv_block, lse is None,
-                                                     self.sm_count), dtype=torch.float32, device=q.device)
-        self.launches += 1 if lse is not None else 3
-        self.C.attention_mass(out, mass, float(carry), lse, ws, q, k_cache, row_kvlen, block_table, kv_block, nq, nkv, hd, *step, self.sm_count,
-                              self.status_word)
+        ws = self.empty(self.C.attention_mass_floats(q.shape[0], segs[0].numel(), segs[3], G, nq, nkv, hd, block_table.shape[1] * kv_block,
+                                                     k_cache.shape[0] * kv_block, lse is None, self.sm_count), dtype=torch.float32, device=q.device)
+        self.launches += self.C.attention_mass(out, mass, float(carry), lse, ws, q, k_cache, row_kvlen, block_table, kv_block, nq, nkv, hd, *step,
+                                               self.sm_count, self.status_word)
         return out
 
     def kv_evict(self, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first=0, recent=0):

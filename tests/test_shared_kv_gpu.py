@@ -186,6 +186,65 @@ def test_captured_steps_follow_their_tables(ops):
         t.copy_(h)
 
 
+MANY = {
+    "hundreds of streams": ([(200 + 7 * i, [[230 + 7 * i + j] for j in range(5)]) for i in range(30)], [[1 + i % 90] for i in range(170)]),
+    "a thousand short ones": ([], [[1 + i % 3] for i in range(1000)]),
+    "long rows among padding": ([(64, [[], [70], []]), (5, [[9]] * 9)], [[]] * 150 + [[2000, 1999], []]),
+}
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(4, 2, 64), (24, 1, 256), (8, 8, 128)])
+@pytest.mark.parametrize("name", MANY)
+def test_steps_of_many_streams(ops, name, nq, nkv, hd):
+    """More streams than one pass of threads plans, and more blocks than a CTA keeps beside it."""
+    groups, alone = MANY[name]
+    st = shared_pages.Step(gen("many", name, nq), DEV, nq, nkv, hd, 64, groups, alone)
+    out, lse = attend(ops, st)
+    check_attend(st, out, lse)
+    for known in (lse, None):
+        check_mass(st, ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), st.segs, st.groups, lse=known, carry=0.25, out=st.mass.clone()), 0.25)
+
+
+@pytest.mark.parametrize("fill", [0x7fffffff, -1, 1 << 20])
+def test_rows_of_refused_segments(ops, fill):
+    """A segment that does not fit the step sets the status; its rows' places in the workspace were never written, whatever lies there, and the other rows are right."""
+    for spoil in ("rows", "slot"):
+        st = shared_pages.Step(gen("refused", spoil), DEV, 6, 2, 128, 64, ((130, [[140], [200]]),), [[9], [30, 31, 32], [77]])
+        segs = st.segs
+        if spoil == "rows":
+            segs = (*segs[:3], 2)
+        else:
+            segs = (i32([*segs[0][:3].tolist(), -5, int(segs[0][4])]), *segs[1:])
+        want, wl, tol, ltol = st.attend()
+        ok = [0, 1, 2, 6]
+        for lse_only in (False, True):
+            n = ops.C.attention_shared_floats(st.rows, 5, segs[3], 1, 6, 2, 128, ops.sm_count, 0 if lse_only else 1)
+            torch.full((n,), fill, dtype=torch.int32, device=DEV)      # what the allocator hands out next
+            if lse_only:
+                ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), segs, st.groups, out=st.mass.clone())
+            else:
+                out, lse = ops.attention_shared(st.q, None, st.k, st.v, st.kvlen, *st.args(), False, segs, st.groups, want_lse=True)
+                assert ((out.view_as(want).double() - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol) + 1e-30)[ok].all()
+                assert ((lse - wl).abs() <= ltol)[ok].all()
+            assert ops.status() != 0
+            ops.status_word.zero_()
+
+
+def test_padding_has_any_slot(ops):
+    st = shared_pages.Step(gen("padding"), DEV, 6, 2, 128, 64, ((130, [[140], [], [200]]),), [[9], [], [77]])
+    segs = (torch.where(st.segs[2] == 0, i32(-1), st.segs[0]).int(), *st.segs[1:])
+    out, lse = ops.attention_shared(st.q, None, st.k, st.v, st.kvlen, *st.args(), False, segs, st.groups, want_lse=True)
+    check_attend(st, out, lse)
+    check_mass(st, ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), segs, st.groups, out=st.mass.clone()), 1.0)
+
+
+def test_sums_of_a_pool_with_wide_tables(ops):
+    """Tables with room for far more tokens than the pool has: the workspace follows the pool."""
+    st = shared_pages.Step(gen("wide"), DEV, 4, 2, 64, 64, ((300, [list(range(290, 690)), [301]]),), [list(range(1, 500))], width=8000)
+    assert ops.C.attention_mass_floats(st.rows, 3, 499, 1, 4, 2, 64, st.table.shape[1] * 64, st.k.shape[0] * 64, 0, ops.sm_count) < 1 << 23
+    check_mass(st, ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), st.segs, st.groups, out=st.mass.clone()), 1.0)
+
+
 def test_two_streams_at_once(ops):
     sts = [shared_pages.Step(gen("stream", i), DEV, 24, 4, 256, 64, ((2000, [[2100 + i], [2500], [2001]]),), [[900]]) for i in range(2)]
     want = [attend(ops, st) for st in sts]
@@ -371,6 +430,13 @@ def test_refusals(ops):
                    dict(groups=(st.groups[0], st.groups[1], st.groups[2].float())), dict(k_cache=st.k.transpose(1, 2).contiguous().transpose(1, 2))):
         with pytest.raises(RuntimeError):
             ops.attention_shared(**{**base, **change})
+    with pytest.raises(RuntimeError):
+        ops.attention_shared(**{**base, "gated": True})                # no proj
+    many = 4097
+    with pytest.raises(RuntimeError):
+        ops.attention_shared(**{**base, "segs": (*(torch.zeros(many, dtype=torch.int32, device=DEV) for _ in range(3)), 1), "groups": None})
+    with pytest.raises(RuntimeError):
+        ops.attention_mass(torch.zeros(3, 130, 128, dtype=torch.bfloat16, device=DEV), st.k, st.mass, st.kvlen, st.table, 64, 130, 2, 128, st.segs, st.groups)   # share 65
     mbase = dict(q=st.q, k_cache=st.k, mass=st.mass, row_kvlen=st.kvlen, block_table=st.table, kv_block=64, nq=6, nkv=2, hd=128, segs=st.segs, groups=st.groups)
     for change in (dict(mass=st.mass.half()), dict(mass=st.mass.transpose(1, 2).contiguous()), dict(out=st.mass[:1]), dict(lse=torch.zeros(2, 6, device=DEV)),
                    dict(lse=torch.zeros(3, 6, device=DEV, dtype=torch.bfloat16)), dict(k_cache=st.k.float())):
