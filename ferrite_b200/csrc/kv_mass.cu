@@ -345,6 +345,7 @@ done:
 }
 
 // ---- many pairs: queries stream by 256 resident keys -----------------------------------------------------------------------------------------
+constexpr uint32_t KP_COL_K = KM_SETS * KM_PAIRS, KP_COLS = 512;          // TMEM: S of the sets | keys of both tiles
 constexpr int KP_KEYS = 2 * KM_KEYS, KP_PLAN = 1024, KP_CHUNKS = 1024;   // keys of an item; threads of the plan; chunks beside one an item
 
 struct KpItem {                                  // 256 keys of a span
@@ -492,7 +493,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   unsigned char *sK = smem, *sQ = smem + 2 * C::K_BYTES;
   KmMisc<AS>& ms = *reinterpret_cast<KmMisc<AS>*>(smem + C::ROWS_AT);
   uint64_t *k_full = ms.bars, *k_empty = k_full + 1, *s_full = k_full + 2, *s_empty = s_full + KM_SETS, *q_full = s_empty + KM_SETS, *q_empty = q_full + QS,
-           *a_full = q_empty + QS, *a_empty = a_full + AS;
+           *a_full = q_empty + QS, *a_empty = a_full + AS, *t_full = a_empty + AS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
   volatile int* abort_flag = &ms.abort;
   pdl_launch_dependents();
@@ -503,14 +504,15 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   if (tid == 0) {
     ms.abort = 0;
     mbar_init(k_full, 1);
-    mbar_init(k_empty, 1);
+    mbar_init(k_empty, 4 * KM_SETS);
+    mbar_init(t_full, 4 * KM_SETS);
     for (int i = 0; i < KM_SETS; ++i) { mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], 4); }
     for (int i = 0; i < QS; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], 1); }
     for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], 1); mbar_init(&a_empty[i], 8); }
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&ms.tmem, KM_SETS * KM_PAIRS);
+    tmem_alloc(&ms.tmem, KP_COLS);
     tmem_relinquish();
   }
   for (int i = tid; i < QS * C::Q_BYTES / 16; i += KM_THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
@@ -601,12 +603,12 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // ---- products: a tile of queries with both tiles of keys, behind one look at everything that they wait for
     const bool issue = elect_one();
     constexpr uint32_t idesc = umma_idesc(1, 1, KM_KEYS, KM_PAIRS);
-    const uint64_t dK = umma_desc_k128(smem_u32(sK)), dQ = umma_desc_k128(smem_u32(sQ));
+    const uint64_t dQ = umma_desc_k128(smem_u32(sQ));
     int i = 0, n = 0, stage = 0, phase = 0;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
       const int steps = w.chunks[u / nkv].steps;
-      ok = __all_sync(0xffffffffu, sk_wait(k_full, n & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, sk_wait(t_full, n & 1, abort_flag));
       for (int j = 0; ok && j < steps; ++j, ++i) {
         const int set = 2 * (i & 1);
         bool now = mbar_try_wait(&q_full[stage], phase) & mbar_try_wait(&a_full[i % AS], i / AS & 1);
@@ -618,9 +620,9 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (!ok) break;
         tc_fence_after();
         const uint64_t dq = dQ + (uint32_t)(stage * C::Q_BYTES >> 4);
-        sk_products<HD / 16>(issue, tmem + set * KM_PAIRS, dK, dq, C::K_CH, C::Q_CH, idesc);
+        sk_products_ts<HD / 16>(issue, tmem + set * KM_PAIRS, tmem + KP_COL_K, dq, C::Q_CH, idesc);
         tc_commit_if(issue, &s_full[set]);
-        sk_products<HD / 16>(issue, tmem + (set + 1) * KM_PAIRS, dK + (uint32_t)(C::K_BYTES >> 4), dq, C::K_CH, C::Q_CH, idesc);
+        sk_products_ts<HD / 16>(issue, tmem + (set + 1) * KM_PAIRS, tmem + KP_COL_K + HD / 2, dq, C::Q_CH, idesc);
         tc_commit_if(issue, &s_full[set + 1]);
         tc_commit_if(issue, &q_empty[stage]);
         if (++stage == QS) {
@@ -629,7 +631,6 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
       }
       if (!ok) break;
-      tc_commit_if(issue, k_empty);
     }
     if (!ok) {
       if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
@@ -641,8 +642,39 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + set * KM_PAIRS;
     const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
     bool dead = false;
-    int i = 0;                                                       // tiles of queries of the CTA so far
-    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    int i = 0, n = 0;                                                // tiles of queries, units of the CTA so far
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      // Half of a key each from shared memory into its lane of tensor memory, where every product with the keys ahead of these is through: each set has waited
+      // for its own. The next unit's keys land meanwhile.
+      asm volatile("bar.sync 1, %0;" ::"n"(KM_SETS * 128) : "memory");
+      if (!dead && !__all_sync(0xffffffffu, sk_wait(k_full, n & 1, abort_flag))) {
+        dead = true;
+        if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
+        *abort_flag = 1;
+      }
+      if (!dead) {
+        tc_fence_after();
+#pragma unroll
+        for (int e = 0; e < HD / 64; ++e) {
+          const int x0 = (set >> 1) * (HD / 2) + e * 32;
+          const unsigned char* from = sK + (set & 1) * C::K_BYTES + (x0 >> 6) * C::K_CH + place * 128;
+          uint32_t c[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from + ((((x0 & 63) >> 3) + k) ^ (place & 7)) * 16);
+            c[4 * k] = v.x; c[4 * k + 1] = v.y; c[4 * k + 2] = v.z; c[4 * k + 3] = v.w;
+          }
+          sk_tmem_st16(tmem + ((uint32_t)(quad * 32) << 16) + KP_COL_K + (set & 1) * (HD / 2) + x0 / 2, c);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+      }
+      __syncwarp();
+      if (lane == 0 && !dead) {
+        mbar_arrive(k_empty);
+        mbar_arrive(t_full);
+      }
+
       KpChunk ch;
       KpItem it;
       const int kvh = unit(u, &ch, &it);
@@ -678,7 +710,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+  if (warp == 1) tmem_dealloc(tmem, KP_COLS);
 }
 
 // An item's sums of all chunks, in order, into the cache's. grid: items x kv heads, a thread a key.

@@ -567,9 +567,11 @@ done:
 // meet in the second kernel only: nothing passes between threads.
 template <int HD>
 struct SlCfg {
-  static constexpr int NCH = HD / 64, Q_CH = SA_PAIRS * 128, KV_CH = SA_KT * 128, Q_BYTES = NCH * Q_CH, T_BYTES = NCH * KV_CH;
-  static constexpr int KS = HD == 256 ? 3 : 8;
-  static constexpr int TILES = 2 * Q_BYTES + KS * T_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
+  static constexpr int NCH = HD / 64, KV_CH = SA_KT * 128, T_BYTES = NCH * KV_CH;
+  static constexpr int KS = HD == 256 ? 6 : 8;
+  static constexpr int TILES = KS * T_BYTES, MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
+  // TMEM: S [tile of pairs][parity] | queries of both tiles
+  static constexpr uint32_t COL_Q = 4 * SA_KT, COLS = 512;
 };
 template <int HD>
 __global__ void __launch_bounds__(SA_THREADS, 1)
@@ -578,7 +580,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
   using C = SlCfg<HD>;
   constexpr int NCH = C::NCH, KS = C::KS;
   extern __shared__ __align__(1024) unsigned char smem[];
-  unsigned char *sQ = smem, *sK = smem + 2 * C::Q_BYTES;
+  unsigned char* sK = smem;
   SaMisc<KS>& ms = *reinterpret_cast<SaMisc<KS>*>(smem + C::MISC_AT);
   uint64_t *q_full = ms.bars, *q_done = q_full + 1, *s_full = q_full + 2, *s_empty = q_full + 6, *k_full = q_full + 10, *k_empty = k_full + KS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Rh = SA_PAIRS / share;
@@ -597,7 +599,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(&ms.tmem, 256);
+    tmem_alloc(&ms.tmem, C::COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -607,7 +609,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
   pdl_wait();
   SaShare mine;
   if (!sa_share<SA_THREADS>(&mine, &ms.share, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status)) {
-    if (warp == 1) tmem_dealloc(tmem, 256);
+    if (warp == 1) tmem_dealloc(tmem, C::COLS);
     return;
   }
   SaWalk x;
@@ -646,7 +648,8 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
     constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, SA_KT);
     const bool issue = elect_one();
     const int a = warp - 1;
-    const uint64_t dQ = umma_desc_k128(smem_u32(sQ) + a * C::Q_BYTES), dK = umma_desc_k128(smem_u32(sK));
+    const uint32_t tQ = tmem + C::COL_Q + a * (HD / 2);
+    const uint64_t dK = umma_desc_k128(smem_u32(sK));
     int stage = 0, phase = 0, piece = 0, count = 0;
     bool ok = true;
     do {
@@ -659,7 +662,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
         if (!ok) break;
         if (there) {
           tc_fence_after();
-          sk_products<HD / 16>(issue, tmem + b * SA_KT, dQ, dK + (uint32_t)(stage * C::T_BYTES >> 4), C::Q_CH, C::KV_CH, idesc);
+          sk_products_ts<HD / 16>(issue, tmem + b * SA_KT, tQ, dK + (uint32_t)(stage * C::T_BYTES >> 4), C::KV_CH, idesc);
           tc_commit_if(issue, &s_full[b]);
           ++count;
         }
@@ -678,8 +681,8 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
       *abort_flag = 1;
     }
   } else if (warp >= 4) {
-    const int quad = warp & 3, set = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, st_tid = tid - 128, pair = quad * 32 + lane;
-    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + set * 2 * SA_KT + sub * (SA_KT / 2);
+    const int quad = warp & 3, set = (warp - 4) >> 3, sub = ((warp - 4) >> 2) & 1, pair = quad * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16), taddr = lanes + set * 2 * SA_KT + sub * (SA_KT / 2);
     const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
     bool dead = false;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -695,19 +698,29 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
       const SaWalk y = x;
       const int np = min(Rh, y.e.nrows - set * Rh) * share, row0 = y.e.row0 + set * Rh;      // pairs of the set's half
       const int klen = pair < np ? min(st.kvlen[row0 + pair / share], y.e.k1) : 0;
-      if (piece) wait(q_done, (piece - 1) & 1);                      // the products with the queries ahead of these are through
-      if (!dead) {
-        const int pieces = y.e.nrows * share * (HD / 8);
-        const __nv_bfloat16* src = q + (long)y.e.row0 * q_stride + (long)y.kvh * share * HD;
-        for (int c = st_tid; c < pieces; c += 512) {
-          const int d = c % (HD / 8), all = c / (HD / 8), r = all / share, g = all - r * share, a = r >= Rh, p = (r - a * Rh) * share + g;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       ::"r"(smem_u32(sQ + a * C::Q_BYTES + (d >> 3) * C::Q_CH + p * 128 + (((d & 7) ^ (p & 7)) << 4))), "l"(src + (long)r * q_stride + g * HD + d * 8)
-                       : "memory");
+      // half of the pair's query into its TMEM lane, 64 columns at a time (fewer registers than all at once)
+      constexpr int AT_ONCE = HD == 64 ? 4 : 8;
+      const int r = pair < np ? pair / share : 0;
+      const uint4* src = reinterpret_cast<const uint4*>(q + (long)(row0 + r) * q_stride + (long)(y.kvh * share + pair - r * share) * HD + sub * (HD / 2));
+#pragma unroll
+      for (int e0 = 0; e0 < HD / 16; e0 += AT_ONCE) {
+        uint4 v[AT_ONCE];
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) v[e] = pair < np ? src[e0 + e] : make_uint4(0, 0, 0, 0);
+        if (e0 == 0 && piece) wait(q_done, (piece - 1) & 1);         // the products with the queries ahead of these are through
+        if (dead) continue;
+        tc_fence_after();
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; e += 4) {
+          const uint32_t c[16] = {v[e].x,     v[e].y,     v[e].z,     v[e].w,     v[e + 1].x, v[e + 1].y, v[e + 1].z, v[e + 1].w,
+                                  v[e + 2].x, v[e + 2].y, v[e + 2].z, v[e + 2].w, v[e + 3].x, v[e + 3].y, v[e + 3].z, v[e + 3].w};
+          sk_tmem_st16(lanes + C::COL_Q + set * (HD / 2) + sub * (HD / 4) + (e0 + e) * 4, c);
         }
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async();
+      if (!dead) {
+        tmem_st_wait();
+        tc_fence_before();
+      }
       __syncwarp();
       if (lane == 0 && !dead) mbar_arrive(q_full);
       more = x.next(nkv);
@@ -756,7 +769,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
 done:
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, 256);
+  if (warp == 1) tmem_dealloc(tmem, C::COLS);
 }
 
 // A thread a (row, head): its pieces' maxima and sums -> logarithm.

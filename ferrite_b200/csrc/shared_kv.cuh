@@ -330,6 +330,14 @@ __device__ __forceinline__ void sk_products(bool issue, uint32_t tmem_d, uint64_
     tc_mma_f16_if(issue, tmem_d, a + (uint32_t)(((kk >> 2) * chunk_a + (kk & 3) * 32) >> 4), b + (uint32_t)(((kk >> 2) * chunk_b + (kk & 3) * 32) >> 4), idesc,
                   kk > 0 ? 1u : 0u);
 }
+// The same with A in tensor memory: a lane a row, a column two of its values, K-major. Products of few columns are bound by what they read of shared memory, 128
+// bytes a cycle: 128 x 64 x 256 takes 768 cycles with both operands there and 512, what its operations take, with B alone.
+template <int NK>
+__device__ __forceinline__ void sk_products_ts(bool issue, uint32_t tmem_d, uint32_t tmem_a, uint64_t b, int chunk_b, uint32_t idesc) {
+#pragma unroll
+  for (int kk = 0; kk < NK; ++kk)
+    tc_mma_f16_ts_if(issue, tmem_d, tmem_a + kk * 8, b + (uint32_t)(((kk >> 2) * chunk_b + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
+}
 __device__ __forceinline__ void sk_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
