@@ -4,8 +4,9 @@
 //   w  += exp2(S^T scale - lse)    a thread a key: its TMEM lane; the sum over the pairs stays in a register, and nothing passes between threads
 //
 // Few pairs (a decode step): the queries of a group or segment stay in shared memory and its keys stream by; every key tile belongs to one CTA, which writes
-// its sums. Many pairs (a prompt): 256 keys stay and the queries stream by; the stream of a key tile is cut into chunks, whose sums a last kernel joins in
-// their order. The exponentials are 512 cycles of an SM for 128 x 64 scores, the products 768 at 256 columns (the operands' way from shared memory).
+// its sums. Many pairs (a prompt): 256 keys stay in tensor memory and the queries stream by; every CTA has the same number of (256 keys, 64 pairs) steps, and a
+// last kernel joins the sums of a key's pieces in their order. The exponentials are 512 cycles of an SM for 128 x 64 scores, the products 512 at 256 columns
+// (768 with the keys in shared memory: what the operands take from there).
 // Every wait is bounded, as in the attention.
 #include <algorithm>
 
@@ -33,6 +34,7 @@ template <int QS>
 struct KmMisc {
   float nl[QS][KM_PAIRS];                        // minus a pair's logarithm (log2); minus infinity where there is no pair
   int kvl[QS][KM_PAIRS];                         // keys that it sees
+  int edge[QS];                                  // keys that every pair of a full tile sees
   uint64_t bars[44];
   KmShare share;
   uint32_t tmem;
@@ -346,30 +348,58 @@ done:
 
 // ---- many pairs: queries stream by 256 resident keys -----------------------------------------------------------------------------------------
 constexpr uint32_t KP_COL_K = KM_SETS * KM_PAIRS, KP_COLS = 512;          // TMEM: S of the sets | keys of both tiles
-constexpr int KP_KEYS = 2 * KM_KEYS, KP_PLAN = 1024, KP_CHUNKS = 1024;   // keys of an item; threads of the plan; chunks beside one an item
+constexpr int KP_KEYS = 2 * KM_KEYS, KP_PLAN = 1024;                      // keys of an item; threads of the plan
 
+// The list of all steps: item after item, kv head after kv head, the blocks of queries that see it. Each CTA has the same number of consecutive steps; what it has of
+// an (item, kv head) is a piece.
 struct KpItem {                                  // 256 keys of a span
   int slot, key0, k0, k1;                        // its keys: key0 .. key0 + 255, those of k0 .. k1 count
-  int chunk0, chunks, seen, pad;                 // seen: blocks that see it
+  int place0, seen, first, pad;                  // steps ahead of it (of one kv head), blocks that see it, the span's first block
 };
-struct KpChunk {                                 // of an item: of blocks b0 .. b1 those that see it, `steps` in number
-  int item, b0, b1, steps;
+struct KpStart {                                 // of a CTA: the block and step where it starts, steps in all
+  int item, kvh, block, step;
+  int left, pad[3];
 };
 struct KpSpace {
-  int* head;                                     // items, chunks
+  int* head;                                     // items, steps of a CTA
   SharedBlock* blocks;
   KpItem* items;
-  KpChunk* chunks;
-  float* sums;                                   // [chunks][kv heads][sets][keys of a tile]
+  KpStart* starts;
+  float* sums;                                   // [pieces][sets][keys of a tile]; piece: CTA + item * kv heads + kv head
   int max_items;
   SharedPlanSizes z;
 };
+struct KpWalk {
+  KpItem it;
+  int item, kvh, block, n, left;                 // n steps from `block` on, places behind them
+  __device__ __forceinline__ bool start(const KpSpace& w) {
+    const KpStart s = w.starts[blockIdx.x];
+    if (s.left == 0) return false;
+    item = s.item;
+    kvh = s.kvh;
+    block = s.block;
+    it = w.items[item];
+    n = min(it.seen - s.step, s.left);
+    left = s.left - n;
+    return true;
+  }
+  __device__ __forceinline__ bool next(const KpSpace& w, int nkv) {
+    if (left == 0) return false;
+    if (++kvh == nkv) {
+      kvh = 0;
+      it = w.items[++item];
+    }
+    block = it.first;
+    n = min(it.seen, left);
+    left -= n;
+    return true;
+  }
+};
 
-// One CTA: blocks of 64 pairs, items, chunks.
+// One CTA: blocks of 64 pairs, items, where the CTAs start.
 __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, KpSpace w, int Rq, int nkv, int ctas, int* status) {
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ long long tmp[32];
-  __shared__ int chunk_s;
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
@@ -409,10 +439,6 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
     }
     return;
   }
-  if (tid == 0) chunk_s = (int)max(8ll, min(64ll, (plan.places * nkv + ctas * 8 - 1) / (ctas * 8)));
-  __syncthreads();
-  // steps of a chunk: eight chunks a CTA where there are enough, no fewer than 8 steps and no more than KP_CHUNKS chunks more than items
-  const int C = (int)max((long long)chunk_s, (plan.places + KP_CHUNKS - 1) / KP_CHUNKS);
   const int lane = tid & 31, warp = tid >> 5;
   auto span_of = [&](int it) {                                       // the last span that starts at or ahead of the item
     int lo = 0, hi = spans - 1;
@@ -430,14 +456,14 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
     for (int b = first(i); b < behind(i); b += 32) n += __popc(__ballot_sync(0xffffffffu, b + lane < behind(i) && nts[min(b + lane, plan.blocks - 1)] > j));
     if (lane == 0) {
       const SharedBlock blk = w.blocks[first(i)];
-      w.items[it] = KpItem{blk.slot, (blk.k0 / KP_KEYS + j) * KP_KEYS, blk.k0, end(i), 0, (n + C - 1) / C, n, 0};
+      w.items[it] = KpItem{blk.slot, (blk.k0 / KP_KEYS + j) * KP_KEYS, blk.k0, end(i), 0, n, first(i), 0};
     }
   }
   __syncthreads();
-  // numbers of the chunks
+  // steps ahead of the items
   int base = 0;
   for (int i0 = 0; i0 < total; i0 += KP_PLAN) {
-    const int it = i0 + tid, mine = it < total ? w.items[it].chunks : 0;
+    const int it = i0 + tid, mine = it < total ? w.items[it].seen : 0;
     int xs = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -453,33 +479,42 @@ __global__ void __launch_bounds__(KP_PLAN) kv_mass_plan_kernel(FbSharedStep st, 
       ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
       all_here += __shfl_xor_sync(0xffffffffu, all_here, o);
     }
-    if (it < total) w.items[it].chunk0 = base + ahead + xs - mine;
+    if (it < total) w.items[it].place0 = base + ahead + xs - mine;
     base += all_here;
     __syncthreads();
   }
-  // a warp an item: where its chunks start and end
+  const long long steps = (long long)base * nkv, per = max(1ll, (steps + ctas - 1) / ctas);
+  if (per >= 1ll << 31) {                                            // (the same for all)
+    if (tid == 0) {
+      set_status(status, ST_CAPACITY);
+      w.head[0] = w.head[1] = 0;
+    }
+    return;
+  }
+  for (int c = tid; c < ctas; c += KP_PLAN)
+    if (c * per >= steps) w.starts[c].left = 0;
+  // a warp an item: the CTAs that start in it
   for (int it = warp; it < total; it += KP_PLAN / 32) {
-    const int i = span_of(it), j = it - plan.place[i], n = w.items[it].seen, c0 = w.items[it].chunk0;
-    int rank = 0;
-    for (int b = first(i); b < behind(i); b += 32) {
-      const bool sees = b + lane < behind(i) && nts[min(b + lane, plan.blocks - 1)] > j;
-      const uint32_t bal = __ballot_sync(0xffffffffu, sees);
-      const int r = rank + __popc(bal & ((1u << lane) - 1)), c = r / C;
-      if (sees) {
-        KpChunk* ch = w.chunks + c0 + c;
-        if (r == c * C) {
-          ch->item = it;
-          ch->b0 = b + lane;
-          ch->steps = min(C, n - r);
+    const int i = span_of(it), j = it - plan.place[i], n = w.items[it].seen;
+    const long long at = (long long)w.items[it].place0 * nkv, last = at + (long long)n * nkv - 1;
+    for (long long c = (at + per - 1) / per; c <= last / per; ++c) {
+      const long long ahead = c * per - at;
+      const int kvh = (int)(ahead / n), step = (int)(ahead - (long long)kvh * n);
+      int b = first(i), before = 0;                                  // the block that is number `step` of those that see the item
+      for (;; b += 32) {
+        const uint32_t bal = __ballot_sync(0xffffffffu, b + lane < behind(i) && nts[min(b + lane, plan.blocks - 1)] > j);
+        if (before + __popc(bal) > step || b + 32 >= behind(i)) {
+          b += (int)__fns(bal, 0, step - before + 1);
+          break;
         }
-        if (r == c * C + C - 1 || r == n - 1) ch->b1 = b + lane + 1;
+        before += __popc(bal);
       }
-      rank += __popc(bal);
+      if (lane == 0) w.starts[c] = KpStart{it, kvh, b, step, (int)min(per, steps - c * per), {0, 0, 0}};
     }
   }
   if (tid == 0) {
     w.head[0] = total;
-    w.head[1] = base;
+    w.head[1] = (int)per;
   }
 }
 
@@ -522,23 +557,15 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = ms.tmem;
   pdl_wait();
-  const int units = w.head[1] * nkv;
-  // a CTA's chunks: every gridDim-th; steps: the chunk's blocks that see the item
-  auto unit = [&](int u, KpChunk* ch, KpItem* it) {
-    *ch = w.chunks[u / nkv];
-    *it = w.items[ch->item];
-    return u % nkv;
-  };
+  const bool any = w.head[0] > 0;
+  KpWalk x;
   auto sees = [&](const SharedBlock& e, const KpItem& it) { return e.nt > it.key0 / KP_KEYS - it.k0 / KP_KEYS; };
   if (warp == 0) {
     // ---- keys
     int n = 0;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
-      KpChunk ch;
-      KpItem it;
-      const int kvh = unit(u, &ch, &it);
-      const int token = it.key0 + lane * 64, rows = lane < 4 && token < it.k1 ? tile_row(st, it.slot, token, status) : -1024;
+    for (bool more = any && x.start(w); ok && more; more = x.next(w, nkv), ++n) {
+      const int token = x.it.key0 + lane * 64, rows = lane < 4 && token < x.it.k1 ? tile_row(st, x.it.slot, token, status) : -1024;
       ok = n == 0 || __all_sync(0xffffffffu, sk_wait(k_empty, (n - 1) & 1, abort_flag));
       if (!ok) break;
       if (lane == 0) mbar_expect_tx(k_full, 2 * C::K_BYTES);
@@ -548,7 +575,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (lane == 0)
 #pragma unroll
           for (int c = 0; c < NCH; ++c)
-            tma_load_2d(sK + (k / 2) * C::K_BYTES + c * C::K_CH + (k % 2) * (C::K_CH / 2), &tmK, k_full, kvh * HD + c * 64, row);
+            tma_load_2d(sK + (k / 2) * C::K_BYTES + c * C::K_CH + (k % 2) * (C::K_CH / 2), &tmK, k_full, x.kvh * HD + c * 64, row);
       }
     }
     if (!ok && lane == 0) {
@@ -557,42 +584,78 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     }
     if (*abort_flag && lane == 0 && n) mbar_wait(k_full, (n - 1) & 1, 1u << 20);
   } else if (warp == 2 || warp == 3) {
-    // ---- tiles of queries (warp 2), what their pairs are (warp 3)
+    // ---- tiles of queries (warp 2), what their pairs are (warp 3). The lanes look at 32 blocks at a time.
     const int S = warp == 2 ? QS : AS;
     uint64_t* empty = warp == 2 ? q_empty : a_empty;
     int i = 0, stage = 0, phase = 0;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
-      KpChunk ch;
-      KpItem it;
-      const int kvh = unit(u, &ch, &it);
-      for (int b = ch.b0; b < ch.b1; ++b) {
-        const SharedBlock e = w.blocks[b];
-        if (!sees(e, it)) continue;
-        ok = i < S || __all_sync(0xffffffffu, sk_wait(&empty[stage], phase ^ 1, abort_flag));
-        if (!ok) break;
+    auto room = [&] { return ok = i < S || __all_sync(0xffffffffu, sk_wait(&empty[stage], phase ^ 1, abort_flag)); };
+    auto step = [&] {
+      ++i;
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1;
+      }
+    };
+    // warp 3: its lanes' two pairs of a tile; a tile's numbers are asked for ahead of the one before it being handed on
+    const int r2[2] = {lane / share, (lane + 32) / share}, g2[2] = {lane - r2[0] * share, lane + 32 - r2[1] * share};
+    float nl[2] = {0.f, 0.f};
+    int kvl[2] = {0, 0}, edge = -1;
+    auto give = [&] {
+      if (!room()) return;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ms.nl[stage][lane + 32 * h] = nl[h] * -1.4426950408889634f;
+        ms.kvl[stage][lane + 32 * h] = kvl[h];
+      }
+      if (lane == 0) ms.edge[stage] = edge;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[stage]);
+      step();
+    };
+    for (bool more = any && x.start(w); ok && more; more = x.next(w, nkv)) {
+      int b = x.block;
+      SharedBlock e{};
+      uint32_t bits = 0;
+      for (int left = x.n; ok && left > 0;) {
+        if (bits == 0) {                                             // (of the span's last blocks on, `left` says where it ends)
+          e = w.blocks[min(b + lane, w.z.blocks - 1)];
+          bits = __ballot_sync(0xffffffffu, b + lane < w.z.blocks && sees(e, x.it));
+          b += 32;
+          if (bits == 0) {
+            if (b >= w.z.blocks) ok = false;
+            continue;
+          }
+        }
+        const int from = __ffs(bits) - 1, row0 = __shfl_sync(0xffffffffu, e.row0, from), nrows = __shfl_sync(0xffffffffu, e.nrows, from),
+                  kmin = __shfl_sync(0xffffffffu, e.kmin, from);
+        bits &= bits - 1;
+        --left;
         if (warp == 2) {
+          if (!room()) break;
           if (lane == 0) {
             mbar_expect_tx(&q_full[stage], NCH * Rq * share * 128);
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) km_load_q(sQ + stage * C::Q_BYTES + c * C::Q_CH, &tmQ, &q_full[stage], c * 64, kvh * share, e.row0);
+            for (int c = 0; c < NCH; ++c) km_load_q(sQ + stage * C::Q_BYTES + c * C::Q_CH, &tmQ, &q_full[stage], c * 64, x.kvh * share, row0);
           }
+          step();
         } else {
+          float l[2];
+          int k[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int p = lane + 32 * h, r = p / share;
-            km_pair(st, lse, e, r, p - r * share, kvh * share, nq, share, Rq, p, &ms.nl[stage][p], &ms.kvl[stage][p]);
+            const bool there = lane + 32 * h < Rq * share && r2[h] < nrows;
+            l[h] = there ? lse[(long)(row0 + r2[h]) * nq + x.kvh * share + g2[h]] : INFINITY;
+            k[h] = there ? st.kvlen[row0 + r2[h]] : 0;
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&a_full[stage]);
-        }
-        ++i;
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1;
+          if (edge >= 0) give();
+          nl[0] = l[0]; nl[1] = l[1];
+          kvl[0] = k[0]; kvl[1] = k[1];
+          edge = nrows < Rq ? 0 : kmin;
         }
       }
     }
+    if (ok && warp == 3 && edge >= 0) give();
     if (!ok && lane == 0) {
       if (!*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
       *abort_flag = 1;
@@ -606,10 +669,9 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint64_t dQ = umma_desc_k128(smem_u32(sQ));
     int i = 0, n = 0, stage = 0, phase = 0;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < units; u += gridDim.x, ++n) {
-      const int steps = w.chunks[u / nkv].steps;
+    for (bool more = any && x.start(w); ok && more; more = x.next(w, nkv), ++n) {
       ok = __all_sync(0xffffffffu, sk_wait(t_full, n & 1, abort_flag));
-      for (int j = 0; ok && j < steps; ++j, ++i) {
+      for (int j = 0; ok && j < x.n; ++j, ++i) {
         const int set = 2 * (i & 1);
         bool now = mbar_try_wait(&q_full[stage], phase) & mbar_try_wait(&a_full[i % AS], i / AS & 1);
         if (i >= 2) now = now & mbar_try_wait(&s_empty[set], (i / 2 - 1) & 1) & mbar_try_wait(&s_empty[set + 1], (i / 2 - 1) & 1);
@@ -643,7 +705,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     const uint64_t scale2 = f2_pack(scale_log2, scale_log2);
     bool dead = false;
     int i = 0, n = 0;                                                // tiles of queries, units of the CTA so far
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+    for (bool more = any && x.start(w); more; ++n) {
       // Half of a key each from shared memory into its lane of tensor memory, where every product with the keys ahead of these is through: each set has waited
       // for its own. The next unit's keys land meanwhile.
       asm volatile("bar.sync 1, %0;" ::"n"(KM_SETS * 128) : "memory");
@@ -675,17 +737,9 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         mbar_arrive(t_full);
       }
 
-      KpChunk ch;
-      KpItem it;
-      const int kvh = unit(u, &ch, &it);
-      const int key = it.key0 + (set & 1) * KM_KEYS + place, last = key - place + KM_KEYS;
+      const int key = x.it.key0 + (set & 1) * KM_KEYS + place, last = key - place + KM_KEYS;
       float sum = 0.f;
-      int b = ch.b0;
-      SharedBlock e = w.blocks[b];
-      for (int j = 0; j < ch.steps; ++j, ++i, ++b) {
-        while (!sees(e, it)) e = w.blocks[++b];
-        const SharedBlock now = e;
-        if (j + 1 < ch.steps) e = w.blocks[b + 1];
+      for (int j = 0; j < x.n; ++j, ++i) {
         if ((i & 1) != set >> 1) continue;
         const int f = 2 * i + (set & 1), stage = i % AS;
         if (!dead && !__all_sync(0xffffffffu, sk_wait(&s_full[set], (f / KM_SETS) & 1, abort_flag))) {
@@ -696,8 +750,8 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (dead) continue;
         tc_fence_after();
         // (the pairs' numbers came with the tile: the products have waited for both)
-        sum += last > now.kmin || now.nrows < Rq ? km_weights<true>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2)
-                                                 : km_weights<false>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2);
+        sum += last > ms.edge[stage] ? km_weights<true>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2)
+                                     : km_weights<false>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -705,7 +759,8 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           mbar_arrive(&a_empty[stage]);
         }
       }
-      if (!dead) w.sums[((size_t)u * KM_SETS + set) * KM_KEYS + place] = sum;
+      if (!dead) w.sums[((blockIdx.x + (size_t)x.item * nkv + x.kvh) * KM_SETS + set) * KM_KEYS + place] = sum;
+      more = x.next(w, nkv);
     }
   }
   tc_fence_before();
@@ -713,11 +768,11 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   if (warp == 1) tmem_dealloc(tmem, KP_COLS);
 }
 
-// An item's sums of all chunks, in order, into the cache's. grid: items x kv heads, a thread a key.
+// An item's sums of all pieces, in order, into the cache's. grid: items x kv heads, a thread a key.
 __global__ void __launch_bounds__(KP_KEYS) kv_mass_join_kernel(float* out, const float* mass, float carry, FbSharedStep st, KpSpace w, int nkv, int* status) {
   pdl_launch_dependents();
   pdl_wait();
-  const int items = w.head[0];
+  const int items = w.head[0], per = w.head[1];
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
     const KpItem it = w.items[i];
     const int kvh = blockIdx.y, key = it.key0 + threadIdx.x;
@@ -730,9 +785,11 @@ __global__ void __launch_bounds__(KP_KEYS) kv_mass_join_kernel(float* out, const
     const size_t at = ((size_t)page * nkv + kvh) * st.kv_block + key % st.kv_block;
     const int set = threadIdx.x / KM_KEYS, place = threadIdx.x % KM_KEYS;
     float sum = 0.f;
+    const long long p0 = (long long)it.place0 * nkv + (long long)kvh * it.seen;
+    const int c0 = (int)(p0 / per), c1 = (int)((p0 + it.seen - 1) / per);
 #pragma unroll 4
-    for (int c = 0; c < it.chunks; ++c) {
-      const float* s = w.sums + (((size_t)(it.chunk0 + c) * nkv + kvh) * KM_SETS + set) * KM_KEYS + place;
+    for (int c = c0; c <= c1; ++c) {
+      const float* s = w.sums + ((c + (size_t)i * nkv + kvh) * KM_SETS + set) * KM_KEYS + place;
       sum += s[0] + s[2 * KM_KEYS];
     }
     out[at] = (carry != 0.f ? carry * mass[at] : 0.f) + sum;
@@ -759,7 +816,7 @@ static int make_tmap_queries(CUtensorMap* out, const void* q, int rows, int nq, 
 static int km_resident_rows(int hd, int share) { return (hd == 256 ? KmCfg<256>::QS : hd == 128 ? KmCfg<128>::QS : KmCfg<64>::QS) * (KM_PAIRS / share); }
 static bool km_few(int rows, int max_rows, int ngrp, int hd, int share) { return (ngrp ? rows : std::min(rows, max_rows)) <= km_resident_rows(hd, share); }
 // (A span of n keys is of up to n / 256 + 2 items, and a key of the pool is of one span.)
-static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room, long keys) {
+static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room, long keys, int ctas) {
   const int Rq = KM_PAIRS / share;
   const long spans = nseg + ngrp;
   const long blocks = shared_group_blocks(rows, ngrp, Rq) + shared_seg_blocks(rows, nseg, max_rows, Rq), items = std::min(spans * ((room + KP_KEYS - 1) / KP_KEYS + 1), keys / KP_KEYS + 2 * spans);
@@ -773,8 +830,8 @@ static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, in
   v.head = (int*)take(4);
   v.blocks = (SharedBlock*)take(blocks * 8);
   v.items = (KpItem*)take(items * 8);
-  v.chunks = (KpChunk*)take((items + KP_CHUNKS) * 4);
-  v.sums = take((items + KP_CHUNKS) * nkv * KM_SETS * KM_KEYS);
+  v.starts = (KpStart*)take(ctas * 8l);
+  v.sums = take((items * nkv + ctas) * KM_SETS * KM_KEYS);
   v.max_items = (int)std::min(items, 0x7fffffffl);
   if (w) *w = v;
   return at - ws;
@@ -784,7 +841,7 @@ extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int n
   if (rows <= 0 || nseg <= 0 || nkv < 1 || nq / nkv < 1 || nq / nkv > KM_PAIRS) return 0;
   const int share = nq / nkv;
   const long logs = want_lse ? ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, 0) : 0;
-  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys));
+  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys, ctas));
 }
 
 extern "C" int fb_attention_mass_launches(int rows, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse) {
@@ -829,7 +886,7 @@ extern "C" int fb_attention_mass(float* out, const float* mass, float carry, con
     return (int)e;
   }
   KpSpace w;
-  km_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nkv, share, room, keys);
+  km_space(&w, ws, st.rows, st.nseg, st.max_rows, st.ngrp, nkv, share, room, keys, ctas);
   if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, Rq), shared_seg_blocks(st.rows, st.nseg, st.max_rows, Rq), &w.z)) return -2;
   FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SK_PLAN_BYTES));
   if ((e = launch_pdl(kv_mass_plan_kernel, dim3(1), dim3(KP_PLAN), SK_PLAN_BYTES, s, st, w, Rq, nkv, ctas, status)) != cudaSuccess) return (int)e;
