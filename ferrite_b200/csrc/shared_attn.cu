@@ -18,6 +18,10 @@
 // when a score of some row exceeds it by 2^16 (a vote of the threads of 32 pairs, who exchange their maxima only then); sets decide in the tiles' order (`turn`), and the one
 // that moves it rescales O between the two products. Every wait is bounded: one that runs out sets the status word and an abort flag; the softmax warps
 // then go through their remaining barriers without work, the others leave, and the CTA frees its TMEM.
+//
+// Measured (B200, us a call): 34 rows x 24 heads of 256 over 30000 shared and 2000 own tokens each 94 (bytes alone 48), 64 x 32 of 128 over 60000 and 500 125 (52),
+// six over 8000 and 900 25 (7.5). A tile takes 1325 cycles at 256 columns, of which the products are 1280 if they never wait; 18 us are the plan, the first loads, the
+// pieces and the join. Four sets of four warps (twice the scores a thread) spill and are slower.
 #include <algorithm>
 
 #include "gemm_core.cuh"
@@ -564,7 +568,8 @@ done:
 // ---- logarithms alone ------------------------------------------------------------------------------------------------------------------------
 // Where a step's weights are wanted and its attention has been something else (a prompt's): S as above, for 256 pairs at a time, so that a key tile serves two
 // products. A set of eight warps has 128 of the pairs; two threads a pair, each with half of every tile's keys and a maximum and sum of its own, which
-// meet in the second kernel only: nothing passes between threads.
+// meet in the second kernel only: nothing passes between threads. The queries are in tensor memory, so that a product reads the keys alone from shared memory.
+// Measured: 2048 rows x 24 heads of 256 over 16000 keys 300 us (340 with the queries in shared memory), tensor pipe 72 % busy under the power cap.
 template <int HD>
 struct SlCfg {
   static constexpr int NCH = HD / 64, KV_CH = SA_KT * 128, T_BYTES = NCH * KV_CH;
