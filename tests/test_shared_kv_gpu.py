@@ -245,6 +245,46 @@ def test_sums_of_a_pool_with_wide_tables(ops):
     check_mass(st, ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), st.segs, st.groups, out=st.mass.clone()), 1.0)
 
 
+def test_large_pages_and_slots_that_come_twice(ops):
+    """Two segments of one slot read the same pages, each with its own rows; pages of 1024 tokens."""
+    st = shared_pages.Step(gen("twice"), DEV, 24, 4, 256, 1024, ((1500, [[1600, 1601], [1510]]),), [[2300, 2299], [40]])
+    out, lse = attend(ops, st)
+    check_attend(st, out, lse)
+    slots, row0, nrows, most = st.segs                                  # the two rows of the third stream as a segment each
+    twice = (i32([*slots[:3].tolist(), *slots[2:].tolist()]), i32([*row0[:3].tolist(), int(row0[2]) + 1, int(row0[3])]), i32([2, 1, 1, 1, 1]), most)
+    out, lse = ops.attention_shared(st.q, None, st.k, st.v, st.kvlen, *st.args(), False, twice, st.groups, want_lse=True)
+    check_attend(st, out, lse)
+
+
+def test_pools_past_32_bits(ops):
+    """A pool of more than 2^31 elements a cache: the bits of a small one with the same pages."""
+    far, page, nkv, hd = 33200, 64, 4, 256
+    small = shared_pages.Step(gen("far"), DEV, 24, nkv, hd, page, ((1200, [[1300], [1201, 1202]]),), [list(range(300, 700))], poison=None)
+    n = small.k.shape[0]
+    k, v = (torch.zeros(far, page, nkv, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    mass = torch.zeros(far, nkv, page, device=DEV)
+    assert k.numel() > 1 << 31
+    k[far - n:], v[far - n:], mass[far - n:] = small.k, small.v, small.mass
+    table = torch.where(small.table >= 0, small.table + far - n, small.table)
+    args = (table, *small.args()[1:])
+    out, lse = attend(ops, small)
+    far_out, far_lse = ops.attention_shared(small.q, None, k, v, small.kvlen, *args, False, small.segs, small.groups, want_lse=True)
+    assert torch.equal(out, far_out) and torch.equal(lse, far_lse)
+    for known in (lse, None):
+        got = ops.attention_mass(small.q, small.k, small.mass, small.kvlen, *small.args(), small.segs, small.groups, lse=known, out=small.mass.clone())
+        check_mass(small, got, 1.0)
+        far_got = ops.attention_mass(small.q, k, mass, small.kvlen, *args, small.segs, small.groups, lse=known, out=mass.clone())
+        assert torch.equal(got, far_got[far - n:])
+    spare = sorted(set(range(n)) - set(small.table[small.table >= 0].tolist()))[:1]
+    keep = page
+    slot, length = small.segs[0][2:3], i32([699])
+    kept = ops.kv_evict(small.k, small.v, None, small.mass, slot, length, small.table, i32([spare]), page, keep, 3, 20)
+    far_kept = ops.kv_evict(k, v, None, mass, slot, length, table, i32([spare]) + far - n, page, keep, 3, 20)
+    assert torch.equal(kept, far_kept)
+    for a, b in ((small.k, k), (small.v, v), (small.mass, mass)):
+        assert torch.equal(a, b[far - n:])
+
+
 def test_two_streams_at_once(ops):
     sts = [shared_pages.Step(gen("stream", i), DEV, 24, 4, 256, 64, ((2000, [[2100 + i], [2500], [2001]]),), [[900]]) for i in range(2)]
     want = [attend(ops, st) for st in sts]
