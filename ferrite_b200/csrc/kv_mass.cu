@@ -130,7 +130,6 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   uint64_t *q_full = ms.bars, *q_done = q_full + 1, *s_full = q_full + 2, *s_empty = s_full + KM_SETS, *k_full = s_empty + KM_SETS, *k_empty = k_full + KS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
   volatile int* abort_flag = &ms.abort;
-  pdl_launch_dependents();
   if (smem_u32(smem) & 1023u) {
     if (tid == 0) set_status(status, ST_BOUNDS);
     return;
@@ -143,15 +142,8 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc(&ms.tmem, KM_SETS * KM_PAIRS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ms.tmem;
   pdl_wait();
+  sk_tmem_alloc(&ms.tmem, KM_SETS * KM_PAIRS);
   SharedPlan<KM_THREADS> plan{};
   // the CTA's part of the plan, by `count` threads of which this is number `me`: first block, first place, places
   auto take = [&](bool fits, int me, int count) {
@@ -190,9 +182,10 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     if (tid == 0) ms.share = got;
   }
   __syncthreads();
+  const uint32_t tmem = sk_tmem_ready(&ms.tmem);
   const KmShare share_of = ms.share;
   if (share_of.places == 0) {                                        // the same for the whole CTA
-    if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+    if (warp == SK_ALLOC) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
     return;
   }
   // rows of a tile of queries that no copy writes are zeros
@@ -345,7 +338,7 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 done:
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
+  if (warp == SK_ALLOC) tmem_dealloc(tmem, KM_SETS * KM_PAIRS);
 }
 
 // ---- many pairs: queries stream by 256 resident keys -----------------------------------------------------------------------------------------
@@ -551,7 +544,6 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
            *a_full = q_empty + QS, *a_empty = a_full + AS, *t_full = a_empty + AS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, share = nq / nkv, Rq = KM_PAIRS / share;
   volatile int* abort_flag = &ms.abort;
-  pdl_launch_dependents();
   if (smem_u32(smem) & 1023u) {
     if (tid == 0) set_status(status, ST_BOUNDS);
     return;
@@ -566,17 +558,12 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     for (int i = 0; i < AS; ++i) { mbar_init(&a_full[i], 1); mbar_init(&a_empty[i], 8); }
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc(&ms.tmem, KP_COLS);
-    tmem_relinquish();
-  }
   for (int i = tid; i < QS * C::Q_BYTES / 16; i += KM_THREADS) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ms.tmem;
   pdl_wait();
+  sk_tmem_alloc(&ms.tmem, KP_COLS);
+  __syncthreads();
+  const uint32_t tmem = sk_tmem_ready(&ms.tmem);
   const bool any = w.head[0] > 0;
   KpWalk x;
   auto sees = [&](const SharedBlock& e, const KpItem& it) { return e.nt > it.key0 / KP_KEYS - it.k0 / KP_KEYS; };
@@ -785,7 +772,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, KP_COLS);
+  if (warp == SK_ALLOC) tmem_dealloc(tmem, KP_COLS);
 }
 
 // An item's sums of all pieces, in order, into the cache's. grid: items x kv heads, a thread a key.

@@ -236,7 +236,6 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
            *turn = q_full + 14, *k_full = q_full + 22, *k_empty = k_full + KS, *v_full = k_empty + KS, *v_empty = v_full + VS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort_flag = &ms.abort;
-  pdl_launch_dependents();
   if (smem_u32(smem) & 1023u) {                                      // the swizzled tiles need the 1024-byte base
     if (tid == 0) set_status(status, ST_BOUNDS);
     return;
@@ -254,19 +253,14 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int i = 0; i < VS; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc(&ms.tmem, C::COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ms.tmem;
   pdl_wait();
+  sk_tmem_alloc(&ms.tmem, C::COLS);
 
   SaShare mine;
-  if (!sa_share<SA_THREADS>(&mine, &ms.share, st, w, SA_PAIRS / share, nkv, smem, ms.tmp, ms.blocks, status)) {
-    if (warp == 1) tmem_dealloc(tmem, C::COLS);
+  const bool any = sa_share<SA_THREADS>(&mine, &ms.share, st, w, SA_PAIRS / share, nkv, smem, ms.tmp, ms.blocks, status);
+  const uint32_t tmem = sk_tmem_ready(&ms.tmem);
+  if (!any) {
+    if (warp == SK_ALLOC) tmem_dealloc(tmem, C::COLS);
     return;
   }
   const int group_blocks = mine.group_blocks;
@@ -562,7 +556,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 done:
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, C::COLS);
+  if (warp == SK_ALLOC) tmem_dealloc(tmem, C::COLS);
 }
 
 // ---- logarithms alone ------------------------------------------------------------------------------------------------------------------------
@@ -590,7 +584,6 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
   uint64_t *q_full = ms.bars, *q_done = q_full + 1, *s_full = q_full + 2, *s_empty = q_full + 6, *k_full = q_full + 10, *k_empty = k_full + KS;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, Rh = SA_PAIRS / share;
   volatile int* abort_flag = &ms.abort;
-  pdl_launch_dependents();
   if (smem_u32(smem) & 1023u) {
     if (tid == 0) set_status(status, ST_BOUNDS);
     return;
@@ -603,18 +596,13 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
     for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 2); }
     fence_mbar_init();
   }
-  if (warp == 1) {
-    tmem_alloc(&ms.tmem, C::COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = ms.tmem;
   pdl_wait();
+  sk_tmem_alloc(&ms.tmem, C::COLS);
   SaShare mine;
-  if (!sa_share<SA_THREADS>(&mine, &ms.share, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status)) {
-    if (warp == 1) tmem_dealloc(tmem, C::COLS);
+  const bool any = sa_share<SA_THREADS>(&mine, &ms.share, st, w, 2 * Rh, nkv, smem, ms.tmp, ms.blocks, status);
+  const uint32_t tmem = sk_tmem_ready(&ms.tmem);
+  if (!any) {
+    if (warp == SK_ALLOC) tmem_dealloc(tmem, C::COLS);
     return;
   }
   SaWalk x;
@@ -774,7 +762,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
 done:
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, C::COLS);
+  if (warp == SK_ALLOC) tmem_dealloc(tmem, C::COLS);
 }
 
 // A thread a (row, head): its pieces' maxima and sums -> logarithm.

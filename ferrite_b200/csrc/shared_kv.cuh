@@ -321,6 +321,21 @@ __device__ __forceinline__ bool sk_wait2(uint64_t* a, uint32_t pa, uint64_t* b, 
 __device__ __forceinline__ uint64_t sk_desc_mn128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
   return (uint64_t)((smem_addr & 0x3ffffu) >> 4) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 | (uint64_t)((sbo >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
 }
+// Tensor memory, by a warp that plans nothing, behind the wait for the kernels ahead: one of them whose CTA has yet to ask for its columns would never get them from a
+// CTA that waits for it. For the same reason the kernels behind start only where this CTA has its columns. A barrier has to lie between the two.
+constexpr int SK_ALLOC = 4;
+__device__ __forceinline__ void sk_tmem_alloc(uint32_t* to, uint32_t cols) {
+  if (threadIdx.x >> 5 == SK_ALLOC) {
+    tmem_alloc(to, cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+}
+__device__ __forceinline__ uint32_t sk_tmem_ready(const uint32_t* at) {
+  tc_fence_after();
+  pdl_launch_dependents();
+  return *at;
+}
 // D = A B^T over 16 NK columns of K-major operands in chunks of 64, chunk_a and chunk_b bytes apart, from the operands' first descriptors. (The issuing warp gets a
 // fifth of its scheduler's slots beside four warps of arithmetic: a descriptor built anew for every product costs as much as the product.)
 template <int NK>
