@@ -102,14 +102,17 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
   // ---- this CTA's tokens
   const int per = (n + ctas - 1) / ctas, t0 = min(n, rank * per), t1 = min(n, t0 + per), lo = a.first, hi = n - a.recent;
   const bool hold = per <= a.held;
-  auto weight = [&](int j) { return weight_of(a, table, h, j); };
+  auto far = [&](int j) { return weight_of(a, table, h, j); };
+  auto near = [&](int j) { return held_s[j - t0]; };
   uint32_t need = (uint32_t)(a.keep - a.first - a.recent), prefix = 0, mask = 0;
   const bool none = need == 0;
   const int m0 = max(t0, lo), m1 = min(t1, hi);                      // of the middle, where weights decide
   if (hold && !none) {
     // eight a thread: their pages first, then their weights, so that the loads of either are under way together (a page that is none counts as page 0 and
-    // is reported behind the loads)
+    // is reported behind the loads). The first digits are counted on the way.
     bool bad = false;
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
 #pragma unroll 1
     for (int j0 = m0 + tid; j0 < m1; j0 += 8 * EV_THREADS) {
       int page[8];
@@ -125,19 +128,29 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (j0 + e * EV_THREADS < m1) held_s[j0 + e * EV_THREADS - t0] = weight_order(w[e]);
+        if (j0 + e * EV_THREADS < m1) {
+          const uint32_t u = weight_order(w[e]);
+          held_s[j0 + e * EV_THREADS - t0] = u;
+          atomicAdd(&hist[u >> 21], 1u);
+        }
     }
     if (bad) set_status(a.status, ST_BOUNDS);
   }
   for (int pass = 0; pass < 3 && !none; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bins = pass == 2 ? 1024u : 2048u;
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
-#pragma unroll 1
-    for (int j = m0 + tid; j < m1; j += EV_THREADS) {
-      const uint32_t u = hold ? held_s[j - t0] : weight(j);
-      if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
+    auto count = [&](auto read) {
+#pragma unroll 4
+      for (int j = m0 + tid; j < m1; j += EV_THREADS) {
+        const uint32_t u = read(j);
+        if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
+      }
+    };
+    if (pass > 0 || !hold) {
+      for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+      __syncthreads();
+      if (hold) count(near);
+      else count(far);
     }
     if (ctas > 1) cluster.sync();
     else __syncthreads();
@@ -179,18 +192,28 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
   }
   // ---- need: how many tokens whose weight starts with `prefix` stay. A warp has neighbouring tokens, 32 at a time: how many stay for sure (low half), equal ones (high)
   const int run = ((t1 - t0 + EV_WARPS - 1) / EV_WARPS + 31) / 32 * 32, w0 = min(t1, t0 + warp * run), w1 = min(t1, w0 + run);
-  auto kinds = [&](int j, bool* sure, bool* equal) {
+  // (without weights to decide, mask and prefix are zero: all of the middle is equal, and none of it stays)
+  auto kinds = [&](int j, uint32_t* sures, uint32_t* equals) {
     const bool there = j < w1, middle = there && j >= lo && j < hi;
-    const uint32_t u = middle && !none ? (hold ? held_s[j - t0] : weight(j)) & mask : 0u;
-    *sure = there && (!middle || (!none && u > prefix));
-    *equal = middle && !none && u == prefix;
+    const uint32_t u = middle ? (hold ? near(j) : far(j)) & mask : 0u;
+    *sures = __ballot_sync(0xffffffffu, there && (!middle || u > prefix));
+    *equals = __ballot_sync(0xffffffffu, middle && u == prefix);
   };
-  uint64_t mine = 0, all;
-  for (int j = w0; j < w1; j += 32) {
-    bool sure, equal;
-    kinds(j + lane, &sure, &equal);
-    mine += (uint64_t)__popc(__ballot_sync(0xffffffffu, sure)) | (uint64_t)__popc(__ballot_sync(0xffffffffu, equal)) << 32;
+  // (a lane keeps what its number's 32 tokens are, for the first 1024 of the warp)
+  uint32_t sure_of = 0, equal_of = 0, sure_sum = 0, equal_sum = 0;
+  int at = 0;
+  for (int j = w0; j < w1; j += 32, ++at) {
+    uint32_t sures, equals;
+    kinds(j + lane, &sures, &equals);
+    if (at == lane) {
+      sure_of = sures;
+      equal_of = equals;
+    }
+    sure_sum += __popc(sures);
+    equal_sum += __popc(equals);
   }
+  const uint64_t mine = (uint64_t)sure_sum | (uint64_t)equal_sum << 32;
+  uint64_t all;
   uint64_t ahead = scan_pairs(lane == 0 ? mine : 0, tmp, &all);
   ahead = __shfl_sync(0xffffffffu, ahead, 0);
   if (ctas > 1) {
@@ -199,13 +222,15 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
     for (int c = 0; c < rank; ++c) ahead += *cluster.map_shared_rank(&counts_s, c);
     cluster.sync();                                                  // (a CTA stays as long as its counts are read)
   }
-  for (int j = w0; j < w1; j += 32) {
-    bool sure, equal;
-    kinds(j + lane, &sure, &equal);
-    const uint32_t sures = __ballot_sync(0xffffffffu, sure), equals = __ballot_sync(0xffffffffu, equal), below = (1u << lane) - 1;
-    const uint32_t s = (uint32_t)ahead + __popc(sures & below), e = (uint32_t)(ahead >> 32) + __popc(equals & below);
-    if (sure || (equal && e < need)) kept[s + min(e, need)] = j + lane;
-    ahead += (uint64_t)__popc(sures) | (uint64_t)__popc(equals) << 32;
+  uint32_t sures_ahead = (uint32_t)ahead, equals_ahead = (uint32_t)(ahead >> 32);
+  at = 0;
+  for (int j = w0; j < w1; j += 32, ++at) {
+    uint32_t sures = __shfl_sync(0xffffffffu, sure_of, at & 31), equals = __shfl_sync(0xffffffffu, equal_of, at & 31);
+    if (at >= 32) kinds(j + lane, &sures, &equals);
+    const uint32_t below = (1u << lane) - 1, e = equals_ahead + __popc(equals & below), s = sures_ahead + __popc(sures & below);
+    if ((sures >> lane & 1u) || ((equals >> lane & 1u) && e < need)) kept[s + min(e, need)] = j + lane;
+    sures_ahead += __popc(sures);
+    equals_ahead += __popc(equals);
   }
 }
 
