@@ -7,9 +7,10 @@
 //
 // Copy: a warp has up to 32 rows at a time; its lanes look up the pages, then all of them copy row after row, 16 bytes each.
 //
-// Measured (B200, us): 24 streams of 12000 tokens, 4 heads of 256 in bf16, 2048 stay: selection 28, copy 70 (408 MB read and written, 5.8 TB/s: HBM); two of 100000 in
-// 8 bits, 8192 stay: 36 in all, nearly all of it selection (12500 weights a CTA, three passes with a sum over the cluster each); one of 4000, 1024 stay: 17 to 19, the
-// call's path on the host.
+// Measured (B200, us): 24 streams of 12000 tokens, 4 heads of 256 in bf16, 2048 stay: selection 22, copy 70 (408 MB read and written, 5.8 TB/s: HBM); two of 100000 in
+// 8 bits, 8192 stay: 30 in all, selection 23 (12500 weights a CTA, digits added up over the cluster); one of 4000, 1024 stay: 16, selection 12 of it.
+// Selection is bound by its instructions (issue slots of its SMs 40 % busy between the digits' barriers); 1024 threads a CTA take 16 for 4000 tokens and 24 for 12000, and
+// one lane a bin adding for its warp 15 to 20 % more than an addition a lane.
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -296,9 +297,10 @@ extern "C" int fb_kv_evict(int* kept, void* k, void* v, float* scale, float* mas
   if (keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || (long)dst_blocks * kv_block < keep || row_bytes % 16 || ns > 32) return -1;
   if ((long)segs * nkv > 0x7fffffffl / 8) return -2;
   const long room = (long)max_blocks * kv_block;
-  // CTAs of a cluster: the fewest of 1, 2, 4 and 8 that leave a CTA up to 4096 tokens, as far as all CTAs run at once (what crosses a cluster costs 2 us a digit)
+  // CTAs of a cluster: the fewest of 1, 2, 4 and 8 that leave a CTA up to 8192 tokens, as far as each has an SM for itself. (A CTA alone takes 12 us for 4000 tokens and
+  // 22 for 12000; what crosses a cluster costs 2 us a digit, and 96 clusters of two, some SMs with two CTAs, take 25 for 12000 where 96 CTAs take 22.)
   int cluster = 1, lanes = 1, shift = -1;
-  while (cluster < 8 && room > 4096l * cluster && (long)segs * nkv * cluster * 2 <= 296) cluster *= 2;
+  while (cluster < 8 && room > 8192l * cluster && (long)segs * nkv * cluster * 2 <= 148) cluster *= 2;
   while (lanes < 32 && lanes * 16 < row_bytes) lanes *= 2;
   for (int b = 0; b < 31; ++b)
     if (kv_block == 1 << b) shift = b;
