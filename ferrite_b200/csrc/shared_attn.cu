@@ -2,9 +2,9 @@
 // prefix are read once for all rows of its group.
 //
 //   S = Q K^T        128 (row, head) pairs of a block x 64 keys; Q and K in shared memory
-//   P = exp2(S - m)  two threads a pair; P as bf16 back into TMEM, its sums in 32 bits. (A weight is off by up to 2^-8 of it, errors that have either sign and
-//                    add up to what rounding the output to bf16 costs: 0.0024 instead of 0.0017 from the result in 64 bits. A second product with the
-//                    remainders would take that away, 512 more cycles of the tensor cores a tile of 128 pairs and 256 columns, 10 % of the whole.)
+//   P = exp2(S - m)  two threads a pair; P as bf16 and what that leaves, as bf16 too, back into TMEM, its sums in 32 bits. (Without the remainders a weight is off by up
+//                    to 2^-8 of it, errors of either sign that add up to what rounding the output costs once more: 0.0024 instead of 0.0017 from the result
+//                    in 64 bits. Their product costs 512 cycles of the tensor cores a tile of 128 pairs and 256 columns, 6 to 14 % of a long call.)
 //   O += P V         A = P from TMEM, V read along its columns from shared memory, O in TMEM while the CTA stays with the pairs
 //
 // Work (shared_kv.cuh): every CTA takes the same number of consecutive key tiles of the list of all (block, kv head) units. A unit that a CTA leaves or ends
@@ -19,9 +19,9 @@
 // that moves it rescales O between the two products. Every wait is bounded: one that runs out sets the status word and an abort flag; the softmax warps
 // then go through their remaining barriers without work, the others leave, and the CTA frees its TMEM.
 //
-// Measured (B200, us a call): 34 rows x 24 heads of 256 over 30000 shared and 2000 own tokens each 94 (bytes alone 48), 64 x 32 of 128 over 60000 and 500 125 (52),
-// six over 8000 and 900 25 (7.5). A tile takes 1325 cycles at 256 columns, of which the products are 1280 if they never wait; 18 us are the plan, the first loads, the
-// pieces and the join. Four sets of four warps (twice the scores a thread) spill and are slower.
+// Measured (B200, us a call): 34 rows x 24 heads of 256 over 30000 shared and 2000 own tokens each 100 (bytes alone 48), 64 x 32 of 128 over 60000 and 500 142 (52),
+// six over 8000 and 900 27 (7.5). The products of a tile are 1536 cycles at 256 columns, 63 us of the first; plan, first loads, pieces and join are 27 of it. Four sets of
+// four warps (twice the scores a thread) spill and are slower.
 #include <algorithm>
 
 #include "gemm_core.cuh"
@@ -42,7 +42,7 @@ struct SaCfg {
   static constexpr int KS = HD == 256 ? 3 : HD == 128 ? 6 : 8, VS = HD == 256 ? 2 : HD == 128 ? 5 : 8;
   static constexpr int TILES = Q_BYTES + (KS + VS) * T_BYTES;
   static constexpr int MISC_AT = TILES > SK_PLAN_BYTES ? TILES : SK_PLAN_BYTES;
-  // TMEM: O | S0 S1 | P0 .. P3
+  // TMEM: O | S0 S1 | P0 and its remainders, P1 and its
   static constexpr uint32_t COL_S = HD, COL_P = COL_S + 2 * SA_KT, COLS = 512;
 };
 // A CTA's share of the list: block that it starts in, blocks of groups, its first place, places.
@@ -248,7 +248,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1); mbar_init(&s_empty[i], SA_SET);
     }
-    for (int i = 0; i < 4; ++i) { mbar_init(&p_full[i], SA_SET); mbar_init(&p_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&p_full[i], SA_SET); mbar_init(&p_empty[i], 1); }
     for (int i = 0; i < KS; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); }
     for (int i = 0; i < VS; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
     fence_mbar_init();
@@ -332,15 +332,15 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           constexpr uint32_t idesc = umma_idesc(1, 1, SA_PAIRS, HD) | (1u << 16);      // B read MN-major
           const uint32_t aV = smem_u32(sV) + st_i * C::T_BYTES;
           ok = j > 0 || piece == 0 || wait(o_empty, (piece - 1) & 1, o_empty, 0, false);
-          ok = ok && wait(&v_full[st_i], phase, &p_full[i & 3], (i >> 2) & 1, true);
+          ok = ok && wait(&v_full[st_i], phase, &p_full[s], (i >> 1) & 1, true);
           if (!ok) break;
           tc_fence_after();
           const uint64_t dV = sk_desc_mn128(aV, C::KV_CH, 1024);
 #pragma unroll
-          for (int kk = 0; kk < SA_KT / 16; ++kk)
-            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + (i & 3) * (SA_KT / 2) + kk * 8, dV + (uint32_t)(kk * 16 * 128 >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < SA_KT / 8; ++kk)                      // weights, remainders
+            tc_mma_f16_ts_if(issue, tmem, tmem + C::COL_P + s * SA_KT + kk * 8, dV + (uint32_t)((kk & 3) * 16 * 128 >> 4), idesc, (j > 0 || kk > 0) ? 1u : 0u);
           tc_commit_if(issue, &v_empty[st_i]);
-          tc_commit_if(issue, &p_empty[i & 3]);
+          tc_commit_if(issue, &p_empty[s]);
           if (++st_i == VS) {
             st_i = 0;
             phase ^= 1;
@@ -413,8 +413,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           // Values of keys that some row does not see meet weights of zero: those that no row sees become zeros, those that some see are looked at,
           // and where one is no finite number the key's values become zeros and its score NaN for the rows that see it.
           // (a wait tells a phase from the one ahead of it only: the values of tile i - VS have to be through)
-          if (i >= 4) wait(&p_empty[i & 3], ((i >> 2) - 1) & 1);
-          if (VS < 4 && i >= VS) wait(&p_empty[(i - VS) & 3], ((i - VS) >> 2) & 1);
+          if (i >= 2) wait(&p_empty[set], ((i >> 1) - 1) & 1);
           wait(&v_full[i % VS], (i / VS) & 1);
           if (!dead) {
             const uint32_t bits = sa_clean_values<HD>(sV + (i % VS) * C::T_BYTES, st_tid, t0, y.e.k0, y.e.k1, y.e.kmin);
@@ -446,7 +445,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           mx = pair < np ? mx * scale_log2 : -INFINITY;              // (what lies behind the pairs moves no maximum)
         }
         // ---- the decision, in the order of the tiles
-        if (i >= 4) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[i & 3], ((i >> 2) - 1) & 1);    // ... and P(i - 4) has been read
+        if (i >= 2) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[set], ((i >> 1) - 1) & 1);      // ... and P(i - 2) has been read
         else if (i > 0) wait(&turn[2 * quad + set], ((i - 1) >> 1) & 1);
         float m_new = j > 0 ? ms.m[pair] : -INFINITY;
         const float m_old = m_new;
@@ -461,10 +460,10 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         if (sub == 0 && (moves || j == 0)) ms.m[pair] = m_new;
         __syncwarp();
         if (lane == 0 && !dead) mbar_arrive(&turn[2 * quad + (set ^ 1)]);
-        if (moves && j > 0) wait(&p_empty[(i - 1) & 3], ((i - 1) >> 2) & 1);          // O is rescaled behind PV(i - 1)
+        if (moves && j > 0) wait(&p_empty[set ^ 1], ((i - 1) >> 1) & 1);               // O is rescaled behind PV(i - 1)
         if (dead || !active) {
           __syncwarp();
-          if (lane == 0 && !dead) mbar_arrive(&p_full[i & 3]);
+          if (lane == 0 && !dead) mbar_arrive(&p_full[set]);
           continue;
         }
         tc_fence_after();
@@ -490,7 +489,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
-          uint32_t pr[HC / 4];
+          uint32_t pr[HC / 4], px[HC / 4];
 #pragma unroll
           for (int c = 0; c < HC / 4; ++c) {
             const int k = part * (HC / 2) + 2 * c;
@@ -498,15 +497,18 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const float p0 = sk_exp2(d.x), p1 = sk_exp2(d.y);
             sum = f2_add(sum, f2_pack(p0, p1));
             pr[c] = pack_bf2(p0, p1);
+            px[c] = pack_bf2(p0 - __uint_as_float(pr[c] << 16), p1 - __uint_as_float(pr[c] & 0xffff0000u));
           }
-          sk_tmem_st8(tmem + lane_addr + C::COL_P + (i & 3) * (SA_KT / 2) + sub * (HC / 2) + part * (HC / 4), pr);
+          const uint32_t to = tmem + lane_addr + C::COL_P + set * SA_KT + sub * (HC / 2) + part * (HC / 4);
+          sk_tmem_st8(to, pr);
+          sk_tmem_st8(to + SA_KT / 2, px);
         }
         const float2 both = f2_unpack(sum);
         l += both.x + both.y;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[i & 3]);
+        if (lane == 0) mbar_arrive(&p_full[set]);
       }
       if (more && ((end - 1) & 1) == set) give_q();
       // ---- the piece: record number = CTA + unit, which no other piece has
@@ -524,8 +526,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
         ml[2 * set + sub] = l;
         if (set == 0 && sub == 0) ml[4] = m_own;
       }
-      if (end >= 2) wait(&p_empty[(end - 2) & 3], ((end - 2) >> 2) & 1);       // (one phase after the other)
-      wait(&p_empty[(end - 1) & 3], ((end - 1) >> 2) & 1);
+      if (end >= 2) wait(&p_empty[end & 1], ((end - 2) >> 1) & 1);             // (one phase after the other)
+      wait(&p_empty[(end - 1) & 1], ((end - 1) >> 1) & 1);
       if (active && !dead) {
         tc_fence_after();
         constexpr int QC = HD / 4;
