@@ -86,7 +86,7 @@ class Step:
         return x, l, off
 
     def attend(self):
-        """out [rows, nq, hd], lse [rows, nq] and how far each may be off in 32-bit arithmetic with weights rounded to bf16, before out is rounded."""
+        """out [rows, nq, hd], lse [rows, nq] and how far each may be off in 32-bit arithmetic with weights of twice eight bits, before out is rounded."""
         dev = self.q.device
         out = torch.zeros(self.rows, self.nq, self.hd, dtype=torch.float64, device=dev)
         lse = torch.full((self.rows, self.nq), -math.inf, dtype=torch.float64, device=dev)
@@ -99,9 +99,9 @@ class Step:
             v = self.v.reshape(-1, self.nkv, self.hd)[self.at(t)].double()
             out[t] = torch.einsum("kgt,tkd->kgd", p, v).reshape(self.nq, self.hd)
             lse[t] = l.reshape(-1)
-            # a weight: its score's error and 2^-21 of the exponential, once above and once below the fraction; above it the weight is a bf16 number, off by
-            # half a step, 2^-8 of it at most
-            tol[t] = (torch.einsum("kgt,tkd->kgd", p, v.abs()) * (2 * (off[..., None] + 2.0 ** -20) + 2.0 ** -8)).reshape(self.nq, self.hd)
+            # a weight: its score's error and 2^-21 of the exponential, once above and once below the fraction; above it the weight is a bf16 number and what that
+            # leaves, at most 2^-8 of it, another one: off by 2^-16 of it. Its product is added in fewer than 2^10 steps (eight for 64 keys), 2^-22 each.
+            tol[t] = (torch.einsum("kgt,tkd->kgd", p, v.abs()) * (2 * (off[..., None] + 2.0 ** -20) + 2.0 ** -16 + 2.0 ** -12)).reshape(self.nq, self.hd)
             ltol[t] = (off + 2.0 ** -22 * l.abs() + 2.0 ** -20).reshape(-1)
         return out, lse, tol, ltol
 
