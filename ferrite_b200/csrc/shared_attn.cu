@@ -485,7 +485,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
           tmem_st_wait();
         }
         const float mr = m_new == -INFINITY ? 0.f : -m_new;
-        const uint64_t scale2 = f2_pack(scale_log2, scale_log2), mr2 = f2_pack(mr, mr);
+        const uint64_t scale2 = f2_pack(scale_log2, scale_log2), mr2 = f2_pack(mr, mr), minus = f2_pack(-1.f, -1.f);
         uint64_t sum = f2_pack(0.f, 0.f);
 #pragma unroll
         for (int part = 0; part < 2; ++part) {
@@ -495,9 +495,11 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const int k = part * (HC / 2) + 2 * c;
             const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), scale2, mr2));
             const float p0 = sk_exp2(d.x), p1 = sk_exp2(d.y);
-            sum = f2_add(sum, f2_pack(p0, p1));
+            const uint64_t pp = f2_pack(p0, p1);
+            sum = f2_add(sum, pp);
             pr[c] = pack_bf2(p0, p1);
-            px[c] = pack_bf2(p0 - __uint_as_float(pr[c] << 16), p1 - __uint_as_float(pr[c] & 0xffff0000u));
+            const float2 rest = f2_unpack(f2_fma(f2_pack(__uint_as_float(pr[c] << 16), __uint_as_float(pr[c] & 0xffff0000u)), minus, pp));
+            px[c] = pack_bf2(rest.x, rest.y);
           }
           const uint32_t to = tmem + lane_addr + C::COL_P + set * SA_KT + sub * (HC / 2) + part * (HC / 4);
           sk_tmem_st8(to, pr);
