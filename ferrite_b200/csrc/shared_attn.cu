@@ -33,7 +33,7 @@ constexpr int SA_PAIRS = 128, SA_KT = 64, SA_NEAR = 4;
 constexpr int SA_EXTRA = 3;                                  // places of a unit's queries and piece, in key tiles (2 to 5 measure alike)
 constexpr int SA_SET = 8;                                    // warps of a set: two threads a pair, each with half of a tile's keys
 constexpr int SA_THREADS = (4 + 2 * SA_SET) * 32;
-constexpr int SA_ML = 8;                                     // floats of a pair's statistics: its threads' sums, the maximum
+constexpr int SA_ML = 8;                                     // floats of a pair's statistics: its threads' sums, the maximum, a byte a thread (see `hidden`)
 
 template <int HD>
 struct SaCfg {
@@ -55,7 +55,7 @@ struct SaMisc {
   float mx[2][SA_PAIRS], m[SA_PAIRS];            // maxima of a tile's halves (of the set whose turn it is); the maximum that O belongs to (log2)
   long long tmp[SA_THREADS / 32];
   uint64_t bars[22 + 2 * STAGES];
-  uint8_t bad[2][2][8];                          // by set and turn: keys of a tile whose values are no numbers
+  uint8_t bad[2][2][8];                          // by set and turn: keys of a tile that lost values which are no finite numbers
   uint32_t tmem;
   int abort;
   SaShare share;
@@ -194,29 +194,33 @@ __device__ __forceinline__ uint32_t key_bits(int lo, int hi) {
   const uint32_t below = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1, ahead = lo <= 0 ? 0u : lo >= 32 ? 0xffffffffu : (1u << lo) - 1;
   return below & ~ahead;
 }
-// Values of a tile's keys that no row sees (outside k0 .. k1) become zeros, and those of a key that some row does not see (from kmin on) where one of them is no
-// finite number. Four of a set's threads have a key. -> such keys of the warp's eight. (Out of line: a few tiles of a unit come by, and what lies between the
-// instructions that every tile runs costs their fetches.)
+// Two bf16 values with zeros in the place of those that are no finite numbers.
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t u) {
+  return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u);
+}
+// What meets weights of zero in a tile becomes zeros: values of keys that no row sees (outside k0 .. k1), and what is no finite number in those of a key that some row
+// does not see (from kmin on). Four of a set's threads have a key. -> which of the warp's eight keys had such numbers: the second kernel looks at them for the
+// rows that see them. (Out of line: a few tiles of a unit come by, and what lies between the instructions that every tile runs costs their fetches.)
 template <int HD>
 __device__ __noinline__ uint32_t sa_clean_values(unsigned char* base, int thread, int t0, int k0, int k1, int kmin) {
   constexpr int CH = SA_KT * 128, PER = HD / 32;                     // bytes of 64 columns; 16-byte pieces of a thread
-  const int key = thread >> 2, part = thread & 3, tok = t0 + key, lane = thread & 31;
+  const int key = thread >> 2, part = thread & 3, tok = t0 + key;
   auto at = [&](int e) { return reinterpret_cast<uint4*>(base + ((part * PER + e) >> 3) * CH + key * 128 + ((part * PER + e) & 7) * 16); };
-  bool zero = tok < k0 || tok >= k1, bad = false;
-  if (!zero && tok >= kmin) {
+  const bool none = tok < k0 || tok >= k1;
+  bool bad = false;
+  if (none) {
+#pragma unroll
+    for (int e = 0; e < PER; ++e) *at(e) = make_uint4(0, 0, 0, 0);
+  } else if (tok >= kmin) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const uint4 u = *at(e);
-      const uint32_t a[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) bad |= (a[k] & 0x7f80u) == 0x7f80u || (a[k] & 0x7f800000u) == 0x7f800000u;
+      const uint4 u = *at(e), c = make_uint4(finite_or_zero(u.x), finite_or_zero(u.y), finite_or_zero(u.z), finite_or_zero(u.w));
+      const bool other = ((u.x ^ c.x) | (u.y ^ c.y) | (u.z ^ c.z) | (u.w ^ c.w)) != 0;
+      bad |= other;
+      if (other) *at(e) = c;
     }
   }
   const uint32_t bal = __ballot_sync(0xffffffffu, bad);
-  zero |= (bal >> (lane & 28) & 15u) != 0;
-  if (zero)
-#pragma unroll
-    for (int e = 0; e < PER; ++e) *at(e) = make_uint4(0, 0, 0, 0);
   uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) bits |= (bal >> (4 * k) & 15u) ? 1u << k : 0u;
@@ -404,14 +408,15 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       const int klen = pair < np ? min(st.kvlen[y.e.row0 + pair / share], y.e.k1) : 0;
       const bool active = quad * 32 < np;                            // (the same for all warps of a quadrant)
       float m_own = -INFINITY, l = 0.f;
+      bool hidden = false;                                           // whether such a value of a key that the pair sees was taken out
       for (int i = first + ((first ^ set) & 1); i < end; i += 2) {
         const int j = i - first, t0 = y.token(j);
         const bool need_mask = t0 < y.e.k0 || t0 + SA_KT > y.e.kmin;
         wait(&s_full[set], (i >> 1) & 1);
         if (i + 1 == end && more && !dead) copy_q(x);                // every product that reads the queries is through
         if (__builtin_expect(need_mask, 0)) {
-          // Values of keys that some row does not see meet weights of zero: those that no row sees become zeros, those that some see are looked at,
-          // and where one is no finite number the key's values become zeros and its score NaN for the rows that see it.
+          // Values of keys that some row does not see meet weights of zero, which an infinity or NaN would not leave at that: zeros take their place, and
+          // what they mean for the rows that see the key is found behind the join (sa_odd_columns).
           // (a wait tells a phase from the one ahead of it only: the values of tile i - VS have to be through)
           if (i >= 2) wait(&p_empty[set], ((i >> 1) - 1) & 1);
           wait(&v_full[i % VS], (i / VS) & 1);
@@ -437,7 +442,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
             const int c0 = t0 + sub * HC;
             const uint32_t bad = reinterpret_cast<const uint32_t*>(ms.bad[set][i >> 1 & 1])[sub], sees = key_bits(y.e.k0 - c0, klen - c0);
 #pragma unroll
-            for (int c = 0; c < HC; ++c) sr[c] = sees >> c & 1u ? bad >> c & 1u ? 0x7fc00000u : sr[c] : 0xff800000u;
+            for (int c = 0; c < HC; ++c) sr[c] = sees >> c & 1u ? sr[c] : 0xff800000u;
+            hidden |= (bad & sees) != 0;
           }
 #pragma unroll
           for (int c = 0; c < HC; c += 4)
@@ -526,6 +532,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
       if (active && pair < np && !dead) {
         float* ml = (grp ? w.ml_grp : w.ml_seg) + (rec * stride + pair) * SA_ML;
         ml[2 * set + sub] = l;
+        reinterpret_cast<uint8_t*>(ml + 5)[2 * set + sub] = hidden;
         if (set == 0 && sub == 0) ml[4] = m_own;
       }
       if (end >= 2) wait(&p_empty[end & 1], ((end - 2) >> 1) & 1);             // (one phase after the other)
@@ -802,13 +809,64 @@ __global__ void __launch_bounds__(256) shared_lse_join_kernel(float* lse, FbShar
   lse[id] = st.kvlen[row] <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
+// Columns d .. d + 3 of a head's row in which keys that the row sees have values that are no finite numbers: an infinity, if they are alike, else NaN. (A weight is
+// larger than zero, however small, but that of a score of minus infinity.) Out of line, for the rows that come across such values.
+template <int HD>
+__device__ __noinline__ float4 sa_odd_columns(float4 a, const FbSharedStep& st, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, int row,
+                                              int kvh, int nkv, int d) {
+  int s = 0, shared = 0;
+  while (s < st.nseg && (row < st.seg_row0[s] || row - st.seg_row0[s] >= st.seg_nrows[s])) ++s;
+  if (s == st.nseg) return a;
+  int first = -1;
+  const int slot = st.seg_slot[s];
+  for (int g = 0; g < st.ngrp; ++g)
+    if (s >= st.grp_seg0[g] && s - st.grp_seg0[g] < st.grp_nsegs[g] && st.grp_seg0[g] >= 0) {
+      first = st.seg_slot[st.grp_seg0[g]];
+      shared = max(st.grp_len[g], 0);
+    }
+  const int n = (int)min((long)st.kvlen[row], table_limit(st));
+  uint32_t seen = 0;                                                 // of column c: bit c an infinity above zero, bit 4 + c one below; NaN is both
+#pragma unroll 1
+  for (int run = 0; run < 2; ++run) {
+    const int from = run ? min(shared, n) : 0, to = run ? n : min(shared, n), via = run ? slot : first;
+    if (via < 0 || via >= st.slots) continue;
+#pragma unroll 1
+    for (int j0 = from / 8 * 8; j0 < to; j0 += 8) {                  // (eight tokens of one page)
+      const int page = st.table[(size_t)via * st.max_blocks + j0 / st.kv_block];
+      if (page < 0 || page >= st.pages) continue;
+      const size_t r0 = ((size_t)page * st.kv_block + j0 % st.kv_block) * nkv + kvh;
+      uint2 u[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] = *reinterpret_cast<const uint2*>(v + (r0 + (size_t)e * nkv) * HD + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t odd = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t x = (c & 2 ? u[e].y : u[e].x) >> (c & 1) * 16 & 0xffffu;
+          if ((x & 0x7f80u) == 0x7f80u) odd |= (x & 0x7fu ? 0x11u : x & 0x8000u ? 0x10u : 0x01u) << c;
+        }
+        if (odd == 0 || j0 + e < from || j0 + e >= to) continue;
+        float score = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < HD; ++i) score = fmaf(bf2f(q[i]), bf2f(k[(r0 + (size_t)e * nkv) * HD + i]), score);
+        seen |= score == -INFINITY ? (odd | odd >> 4 | odd << 4) & 0xffu : odd;
+      }
+    }
+  }
+  auto column = [&](int c, float x) { return seen >> c & 1u ? (seen >> (4 + c) & 1u ? NAN : INFINITY) : seen >> (4 + c) & 1u ? -INFINITY : x; };
+  return make_float4(column(0, a.x), column(1, a.y), column(2, a.z), column(3, a.w));
+}
+
 // Pieces of a head's row -> output and logarithm. grid: rows x query heads; a thread has four columns and every fourth (eighth, 16th) piece. Everything that
 // does not depend on the pieces is asked for at once, and the pieces' sums beside their maxima: three trips to memory.
 template <int HD, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride, FbSharedStep st, SaSpace w,
-                                                          int nkv, int share, int ctas) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride,
+                                                          const __nv_bfloat16* q, long q_stride, const __nv_bfloat16* keys, const __nv_bfloat16* values,
+                                                          const __grid_constant__ FbSharedStep st, SaSpace w, int nkv, int share, int ctas) {
   constexpr int LANES = HD / 4, PARTS = THREADS / LANES;
   __shared__ float top_s[PARTS], sum_s[PARTS];
+  __shared__ uint32_t hidden_s[PARTS];
   __shared__ float4 o_s[PARTS][LANES];
   const int row = blockIdx.x, h = blockIdx.y, kvh = h / share, g = h - kvh * share, tid = threadIdx.x, part = tid / LANES, d = tid % LANES * 4;
   pdl_launch_dependents();
@@ -826,6 +884,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   if (!__syncthreads_or(mine) || per <= 0) return;                   // a row of no segment; a step that did not fit
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   float top = -INFINITY, sum = 0.f;
+  uint32_t hidden = 0;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     // a row's run of records; checked, since this is not written for rows of a segment that was refused, nor by a launch that gave up
@@ -847,7 +906,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
         v[e] = make_float2(-INFINITY, 0.f);
         if (i < pieces) {
           const float4 l = *reinterpret_cast<const float4*>(ml + i * stride * SA_ML);
-          v[e] = make_float2(ml[i * stride * SA_ML + 4], l.x + l.y + (l.z + l.w));
+          const float2 m = *reinterpret_cast<const float2*>(ml + i * stride * SA_ML + 4);
+          v[e] = make_float2(m.x, l.x + l.y + (l.z + l.w));
+          hidden |= __float_as_uint(m.y);
         }
         x[e] = i < pieces && out ? *reinterpret_cast<const float4*>(o + i * stride * HD) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -869,13 +930,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   if (d == 0) {
     top_s[part] = top;
     sum_s[part] = sum;
+    hidden_s[part] = hidden;
   }
   if (part) o_s[part][d / 4] = a;
   __syncthreads();
   if (part) return;
   float all = -INFINITY, total = 0.f;
 #pragma unroll
-  for (int p = 0; p < PARTS; ++p) all = fmaxf(all, top_s[p]);
+  for (int p = 0; p < PARTS; ++p) {
+    all = fmaxf(all, top_s[p]);
+    hidden |= hidden_s[p];
+  }
 #pragma unroll
   for (int p = 0; p < PARTS; ++p) {
     const float m = top_s[p], f = m == -INFINITY ? 0.f : sk_exp2(m - all), s = sum_s[p];
@@ -888,6 +953,9 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   if (!out) return;
   const float inv = n <= 0 ? 0.f : total == 0.f ? NAN : 1.f / total;  // (scores of minus infinity only: 0 / 0)
   a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
+  const bool finite = fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) < INFINITY;
+  if (__builtin_expect((hidden || !finite) && total > 0.f && total < INFINITY, 0))       // weights that are numbers, of values that are none
+    a = sa_odd_columns<HD>(a, st, q + (long)row * q_stride + (long)h * HD, keys, values, row, kvh, nkv, d);
   if (proj) {
     a.x *= sigmoidf_(gate.x); a.y *= sigmoidf_(gate.y); a.z *= sigmoidf_(gate.z); a.w *= sigmoidf_(gate.w);
   }
@@ -998,7 +1066,7 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
 #define FB_SJ(H, N)                                                                                                                                 \
   if (hd == H && (N == 256) == ((long)st.rows * nq <= 4l * ctas))                                                                                   \
     return (int)launch_pdl(shared_join_kernel<H, N>, dim3(st.rows, nq), dim3(N), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj,        \
-                           proj_stride, st, w, nkv, share, ctas);
+                           proj_stride, (const __nv_bfloat16*)q, q_stride, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, st, w, nkv, share, ctas);
   FB_SJ(64, 256) FB_SJ(128, 256) FB_SJ(256, 256) FB_SJ(64, 128) FB_SJ(128, 128) FB_SJ(256, 128)
 #undef FB_SJ
   return -2;
