@@ -23,6 +23,7 @@
 // six over 8000 and 900 27 (7.5). The products of a tile are 1536 cycles at 256 columns, 63 us of the first; plan, first loads, pieces and join are 27 of it. Four sets of
 // four warps (twice the scores a thread) spill and are slower.
 #include <algorithm>
+#include <cfloat>
 
 #include "gemm_core.cuh"
 #include "shared_kv.cuh"
@@ -448,7 +449,9 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constan
 #pragma unroll
           for (int c = 0; c < HC; c += 4)
             mx = fmaxf(fmaxf(mx, __uint_as_float(sr[c])), fmaxf(fmaxf(__uint_as_float(sr[c + 1]), __uint_as_float(sr[c + 2])), __uint_as_float(sr[c + 3])));
-          mx = pair < np ? mx * scale_log2 : -INFINITY;              // (what lies behind the pairs moves no maximum)
+          // (what lies behind the pairs moves no maximum; of a score of infinity the largest number stands for it, so that the sum becomes infinity, and NaN only
+          // where a score is)
+          mx = pair < np ? fminf(mx * scale_log2, FLT_MAX) : -INFINITY;
         }
         // ---- the decision, in the order of the tiles
         if (i >= 2) wait2(&turn[2 * quad + set], ((i - 1) >> 1) & 1, &p_empty[set], ((i >> 1) - 1) & 1);      // ... and P(i - 2) has been read
@@ -752,7 +755,7 @@ shared_lse_kernel(const __grid_constant__ CUtensorMap tmK, const __nv_bfloat16* 
 #pragma unroll
           for (int c = 0; c < 32; c += 4)
             mx = fmaxf(fmaxf(mx, __uint_as_float(sr[c])), fmaxf(fmaxf(__uint_as_float(sr[c + 1]), __uint_as_float(sr[c + 2])), __uint_as_float(sr[c + 3])));
-          const float m_new = fmaxf(m, mx * scale_log2), mr = m_new == -INFINITY ? 0.f : -m_new;
+          const float m_new = fmaxf(m, fminf(mx * scale_log2, FLT_MAX)), mr = m_new == -INFINITY ? 0.f : -m_new;
           const uint64_t mr2 = f2_pack(mr, mr);
           uint64_t sum[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll

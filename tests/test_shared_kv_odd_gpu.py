@@ -102,3 +102,44 @@ def test_rows_whose_values_are_all_infinite(ops):
     proj = torch.randn(st.rows, 6 * 256, generator=gen("gate"), device=DEV).to(torch.bfloat16)
     got = ops.attention_shared(st.q, proj, st.k, st.v, st.kvlen, *st.args(), True, st.segs, st.groups)
     assert torch.equal(got.view(-1, 6, 128)[:, :3].float().nan_to_num(7, 8, 9), attend(ops, st)[0].view(-1, 6, 128)[:, :3].float().nan_to_num(7, 8, 9))
+
+
+class OddKeys(shared_pages.Step):
+    """A step with keys that are no finite numbers: rounding leaves what it leaves of the scores of the others."""
+
+    def weights(self, t):
+        x, l, _ = super().weights(t)
+        k = self.k.reshape(-1, self.nkv, self.hd)[self.at(t)].double().nan_to_num(0, 0, 0)
+        off = (torch.einsum("kgd,tkd->kgt", self.q[t].reshape(self.nkv, -1, self.hd).double().abs(), k.abs()) / self.hd ** 0.5).amax(-1) * 2.0 ** -20
+        return x, l, off
+
+    def check_sums(self, got, carry, lse=None):
+        want, tol, seen = self.masses(carry, lse)
+        assert torch.equal(got[~seen], self.mass[~seen])
+        alike(got, want, torch.where(torch.isnan(tol), 2.0 ** -22 * want.abs(), tol))       # (where a score is minus infinity for every row: nothing is added)
+
+
+def odd_keys(nq, nkv, hd):
+    """Heads that look at column 0 all the same way, and keys with infinities there: scores of infinity, minus infinity, NaN."""
+    st = OddKeys(gen("scores", nq, hd), DEV, nq, nkv, hd, 64, ((200, [[230, 210, 226], [260]]), (3000, [[3100, 3060]])), [[40, 30, 35], [700]])
+    st.q[:, :, 0] = st.q[:, :, 0].abs() + 0.1
+    flat = st.k.view(-1, nkv, hd)
+    for s, token, head, value in [(0, 220, 0, INF), (1, 255, 1, -INF), (2, 100, 0, INF), (2, 2990, 1, -INF), (2, 3090, 1, NAN), (3, 33, 1, INF), (3, 31, 1, NAN),
+                                  (4, 650, 0, -INF), (4, 65, 1, INF)]:
+        flat[stream_row(st, s, token), head, 0] = value
+    return st
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(6, 2, 128), (24, 4, 256), (4, 2, 64)])
+def test_scores_of_infinity(ops, nq, nkv, hd):
+    """A score of infinity makes the logarithm infinity, NaN only where another score of the row is NaN; the row's output is NaN. Scores of minus infinity weigh nothing."""
+    st = odd_keys(nq, nkv, hd)
+    wl = st.attend()[1]
+    assert torch.isposinf(wl).any() and torch.isnan(wl).any() and torch.isfinite(wl).any()
+    check_attend(st, *attend(ops, st))
+
+
+def test_sums_of_scores_of_infinity(ops):
+    st = odd_keys(4, 2, 64)
+    for lse in (None, attend(ops, st)[1]):
+        st.check_sums(sums(ops, st, lse), 0.5)
