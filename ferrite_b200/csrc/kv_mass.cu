@@ -202,8 +202,9 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       int rows = 0;
       for (int j = 0; j < x.n; ++j, ++i) {
         if (j % 16 == 0) {                                           // 16 tiles' pages (two halves of 64 keys each) at a time
+          // (the table of a group's stream need not have what lies whole in the shared tokens)
           const int token = (x.e.k0 / KM_KEYS + x.t + j) * KM_KEYS + lane * 64;
-          rows = j + lane / 2 < x.n && token < x.e.k1 ? tile_row(st, x.e.slot, token, status) : -1024;
+          rows = j + lane / 2 < x.n && token + 64 > x.e.k0 && token < x.e.k1 ? tile_row(st, x.e.slot, token, status) : -1024;
         }
         const int r0 = __shfl_sync(0xffffffffu, rows, (j % 16) * 2), r1 = __shfl_sync(0xffffffffu, rows, (j % 16) * 2 + 1);
         if (i >= KS && !__all_sync(0xffffffffu, sk_wait(&k_empty[stage], phase ^ 1, abort_flag))) {
@@ -572,7 +573,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     int n = 0;
     bool ok = true;
     for (bool more = any && x.start(w); ok && more; more = x.next(w, nkv), ++n) {
-      const int token = x.it.key0 + lane * 64, rows = lane < 4 && token < x.it.k1 ? tile_row(st, x.it.slot, token, status) : -1024;
+      const int token = x.it.key0 + lane * 64, rows = lane < 4 && token + 64 > x.it.k0 && token < x.it.k1 ? tile_row(st, x.it.slot, token, status) : -1024;
       ok = n == 0 || __all_sync(0xffffffffu, sk_wait(k_empty, (n - 1) & 1, abort_flag));
       if (!ok) break;
       if (lane == 0) mbar_expect_tx(k_full, 2 * C::K_BYTES);

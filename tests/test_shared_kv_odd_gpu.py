@@ -143,3 +143,23 @@ def test_sums_of_scores_of_infinity(ops):
     st = odd_keys(4, 2, 64)
     for lse in (None, attend(ops, st)[1]):
         st.check_sums(sums(ops, st, lse), 0.5)
+
+
+# ---- tables ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("nq,nkv,hd", [(6, 2, 128), (24, 4, 256), (4, 2, 64)])
+@pytest.mark.parametrize("shared", [64, 192, 320, 321])
+@pytest.mark.parametrize("rows", [1, 300])
+def test_streams_need_no_entries_for_shared_pages(ops, nq, nkv, hd, shared, rows):
+    """Shared tokens are read through the table of a group's first stream: whole pages of them are missing from the others' tables."""
+    members = [[shared + 5], [max(0, shared + 100 - i) for i in range(rows)], [shared + 1]]
+    st = shared_pages.Step(gen("no entries", nq, shared, rows), DEV, nq, nkv, hd, 64, ((shared, members),), [[70]])
+    full = st.table.clone()
+    st.table[st.slots[1]:st.slots[2] + 1, :shared // 64] = -1
+    out, lse = attend(ops, st)
+    got = [sums(ops, st), sums(ops, st, lse)]
+    assert ops.status() == 0
+    st.table.copy_(full)                                                 # (the statement in 64 bits is the same for both)
+    check_attend(st, out, lse)
+    for g in got:
+        check_sums(st, g, 0.5)
