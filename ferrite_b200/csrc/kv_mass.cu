@@ -18,6 +18,7 @@
 namespace fb {
 
 constexpr int KM_KEYS = 128, KM_PAIRS = 64, KM_SETS = 4, KM_THREADS = (4 + 4 * KM_SETS) * 32, KM_EXTRA = 2;
+constexpr int KM_NEAR = KM_PAIRS - 4;             // pairs of a full tile from which on the unmasked form takes it
 
 template <int HD>
 struct KmCfg {
@@ -47,9 +48,11 @@ __device__ __forceinline__ void km_load_q(void* dst, const CUtensorMap* tm, uint
   tma_load_3d(dst, tm, bar, x, head, row);
 }
 
-// Sum over a tile's pairs of the weights that they give to this thread's key. cols: 32 or 64.
+// Sum over a tile's pairs of the weights that they give to this thread's key. cols: 32 or 64. Columns from `pairs` on (query heads that do not divide 64) are
+// scores of zeros, and NaN where a key has an infinity: they are masked as keys that a pair does not see are, up to four of them by themselves, more (shares of 11,
+// 13, 14 and some above 16) with the whole tile.
 template <bool MASKED>
-__device__ __forceinline__ float km_weights(uint32_t taddr, int cols, const float* nl, const int* kvl, int key, uint64_t scale2) {
+__device__ __forceinline__ float km_weights(uint32_t taddr, int cols, int pairs, const float* nl, const int* kvl, int key, uint64_t scale2) {
   uint64_t acc[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
 #pragma unroll 1
   for (int c0 = 0; c0 < cols; c0 += 32) {
@@ -62,7 +65,7 @@ __device__ __forceinline__ float km_weights(uint32_t taddr, int cols, const floa
       const float2 a = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, f2_pack(n.x, n.y)));
       const float2 b = f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c + 2]), __uint_as_float(r[c + 3])), scale2, f2_pack(n.z, n.w)));
       float p[4] = {sk_exp2(a.x), sk_exp2(a.y), sk_exp2(b.x), sk_exp2(b.y)};
-      if (MASKED) {
+      if (MASKED || (c == 28 && c0 + 32 > pairs)) {
         const int4 k = *reinterpret_cast<const int4*>(kvl + c0 + c);
         if (key >= k.x) p[0] = 0.f;
         if (key >= k.y) p[1] = 0.f;
@@ -325,8 +328,8 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           if (dead) continue;
           tc_fence_after();
           const int left = pairs - t * Rq * share, cols = left > 32 ? 64 : 32;
-          sum += masked || left < Rq * share ? km_weights<true>(taddr, cols, ms.nl[t], ms.kvl[t], key, scale2)
-                                             : km_weights<false>(taddr, cols, ms.nl[t], ms.kvl[t], key, scale2);
+          sum += masked || left < Rq * share || Rq * share < KM_NEAR ? km_weights<true>(taddr, cols, Rq * share, ms.nl[t], ms.kvl[t], key, scale2)
+                                                                     : km_weights<false>(taddr, cols, Rq * share, ms.nl[t], ms.kvl[t], key, scale2);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[set]);
@@ -758,8 +761,8 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (dead) continue;
         tc_fence_after();
         // (the pairs' numbers came with the tile: the products have waited for both)
-        sum += last > ms.edge[stage] ? km_weights<true>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2)
-                                     : km_weights<false>(taddr, KM_PAIRS, ms.nl[stage], ms.kvl[stage], key, scale2);
+        sum += last > ms.edge[stage] || Rq * share < KM_NEAR ? km_weights<true>(taddr, KM_PAIRS, Rq * share, ms.nl[stage], ms.kvl[stage], key, scale2)
+                                                             : km_weights<false>(taddr, KM_PAIRS, Rq * share, ms.nl[stage], ms.kvl[stage], key, scale2);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) {

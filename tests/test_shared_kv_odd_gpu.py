@@ -163,3 +163,17 @@ def test_streams_need_no_entries_for_shared_pages(ops, nq, nkv, hd, shared, rows
     check_attend(st, out, lse)
     for g in got:
         check_sums(st, g, 0.5)
+
+
+@pytest.mark.parametrize("nq,nkv,hd", [(24, 4, 256), (6, 2, 128), (5, 1, 128), (11, 1, 64), (33, 1, 64), (4, 2, 64)])
+@pytest.mark.parametrize("rows", [8, 24, 300])
+def test_sums_beside_keys_of_minus_infinity(ops, nq, nkv, hd, rows):
+    """A key whose score is minus infinity for every row gets nothing, also where the query heads of whole rows leave some of a product's columns without a pair."""
+    st = OddKeys(gen("minus", nq, hd, rows), DEV, nq, nkv, hd, 64, alone=[[700 - r for r in range(rows)]])
+    st.q[:, :, 0] = st.q[:, :, 0].abs() + 0.1
+    for token in (0, 50, 127, 200, 399):
+        st.k.view(-1, nkv, hd)[stream_row(st, 0, token), :, 0] = -INF
+    for lse in (None, attend(ops, st)[1]):
+        got = sums(ops, st, lse)
+        assert torch.isfinite(got).all()
+        st.check_sums(got, 0.5)
