@@ -37,10 +37,10 @@ int fb_attention_mass(float* out, const float* mass, float carry, const float* l
                       FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s);
 
 // ---- kv_evict.cu ----
-// kept [segs, nkv, keep]; k, v: rows of nkv * row_bytes bytes; scale: nkv * ns floats a row, or null; mass [pages, nkv, kv_block]
+// kept [segs, nkv, keep]; k, v: rows of nkv * row_bytes bytes; scale: nkv * ns floats a row, or null; mass [pages, nkv, kv_block]; ctas: SMs
 int fb_kv_evict(int* kept, void* k, void* v, float* scale, float* mass, const int* seg_slot, const int* seg_len, int segs, const int* table, int slots,
                 int max_blocks, const int* dst, int dst_blocks, long pages, int kv_block, int nkv, int row_bytes, int ns, int keep, int first, int recent,
-                int* status, cudaStream_t s);
+                int ctas, int* status, cudaStream_t s);
 
 #ifdef __cplusplus
 }

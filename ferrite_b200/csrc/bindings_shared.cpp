@@ -113,7 +113,7 @@ int64_t attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Ten
 
 // k, v [pages, kv_block, nkv, ..] of 16-bit values or of codes; scale [pages, kv_block, nkv, ns]
 void kv_evict(Tensor kept, Tensor k, Tensor v, OptTensor scale, Tensor mass, Tensor seg_slot, Tensor seg_len, Tensor table, Tensor dst, int64_t kv_block,
-              int64_t keep, int64_t first, int64_t recent, Tensor status) {
+              int64_t keep, int64_t first, int64_t recent, int64_t ctas, Tensor status) {
   const char* what = "kv_evict";
   TORCH_CHECK(k.is_cuda() && k.is_contiguous() && k.dim() == 4 && kv_block > 0 && k.size(1) == kv_block && k.size(0) > 0 &&
               k.size(0) * kv_block < std::numeric_limits<int>::max() && aligned(k, 16), what, ": cache is not [pages, ", kv_block, ", kv heads, ..]");
@@ -137,7 +137,8 @@ void kv_evict(Tensor kept, Tensor k, Tensor v, OptTensor scale, Tensor mass, Ten
   check(fb_kv_evict(kept.data_ptr<int>(), k.data_ptr(), v.data_ptr(), scale ? scale->data_ptr<float>() : nullptr, mass.data_ptr<float>(),
                     ints(seg_slot, S, k, what, "seg_slot"), ints(seg_len, S, k, what, "seg_len"), (int)S, ints(table, table.numel(), k, what, "block_table"),
                     (int)table.size(0), (int)table.size(1), ints(dst, dst.numel(), k, what, "dst_table"), (int)dst.size(1), (long)k.size(0), (int)kv_block,
-                    (int)nkv, (int)row, scale ? (int)scale->size(3) : 0, (int)keep, (int)first, (int)recent, status.data_ptr<int>(), cur_stream()), what);
+                    (int)nkv, (int)row, scale ? (int)scale->size(3) : 0, (int)keep, (int)first, (int)recent, (int)ctas, status.data_ptr<int>(),
+                    cur_stream()), what);
 }
 
 }  // namespace

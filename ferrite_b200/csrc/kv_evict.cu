@@ -9,10 +9,13 @@
 //
 // Measured (B200, us): 24 streams of 12000 tokens, 4 heads of 256 in bf16, 2048 stay: selection 22, copy 70 (408 MB read and written, 5.8 TB/s: HBM); two of 100000 in
 // 8 bits, 8192 stay: 30 in all, selection 23 (12500 weights a CTA, digits added up over the cluster); one of 4000, 1024 stay: 16, selection 12 of it.
+// The same in tables of 131072 tokens: one of 4000 13, four of 4000 20 (15 in tables that fit), 24 of 12000 91. 40 of 50000, whose last 5000 weights a CTA do not fit its
+// shared memory, 2048 stay: 234 (heads of 32).
 // Selection is bound by its instructions (issue slots of its SMs 40 % busy between the digits' barriers); 1024 threads a CTA take 16 for 4000 tokens and 24 for 12000, and
 // one lane a bin adding for its warp 15 to 20 % more than an addition a lane.
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <type_traits>
 
 #include "api_shared.h"
 #include "common.cuh"
@@ -21,6 +24,7 @@ namespace fb {
 
 namespace cg = cooperative_groups;
 constexpr int EV_THREADS = 512, EV_WARPS = EV_THREADS / 32, EV_BINS = 2048, EV_HELD = 44 << 10;   // weights that a CTA holds in shared memory
+constexpr int EV_PART = 8192;                    // tokens of a CTA where another one could have an SM for itself
 
 // Order of weights as whole numbers: a larger weight is a larger number; no number counts as the largest, -0 as 0.
 __device__ __forceinline__ uint32_t weight_order(float x) {
@@ -55,7 +59,7 @@ __device__ __forceinline__ int checked_page(const EvictArgs& a, int page) {
   set_status(a.status, ST_BOUNDS);
   return -1;
 }
-// the same for a weight that no shared memory holds (contexts of more than EV_HELD tokens a CTA)
+// the weight of a token that shared memory does not hold (behind the first EV_HELD of a CTA)
 __device__ __noinline__ uint32_t weight_of(const EvictArgs& a, const int* table, int h, int j) {
   const int p = a.page_of(j), page = checked_page(a, table[p]);
   return page < 0 ? 0u : weight_order(a.mass[((size_t)page * a.nkv + h) * a.kv_block + (j - p * a.kv_block)]);
@@ -88,11 +92,16 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
   __shared__ uint64_t tmp[EV_WARPS], counts_s;
   __shared__ uint32_t digit_s[3];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int pair = blockIdx.x / ctas, seg = pair / a.nkv, h = pair % a.nkv;
+  const int rank = (int)cluster.block_rank(), most = (int)cluster.num_blocks(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int pair = blockIdx.x / most, seg = pair / a.nkv, h = pair % a.nkv;
   pdl_launch_dependents();
   pdl_wait();
   const int slot = a.seg_slot[seg], n = a.tokens(slot, seg);
+  // The cluster is for what the table has room for; the context says how many of its CTAs there is work for, and the others leave (its barriers wait for those that have
+  // not left).
+  int ctas = 1;
+  while (ctas < most && n > EV_PART * ctas) ctas *= 2;
+  if (rank >= ctas) return;
   const int* table = a.table + (size_t)max(slot, 0) * a.max_blocks;
   int* kept = a.kept + (size_t)pair * a.keep;
   for (int i = min(n, a.keep) + rank * EV_THREADS + tid; i < a.keep; i += ctas * EV_THREADS) kept[i] = -1;
@@ -102,57 +111,58 @@ __global__ void __launch_bounds__(EV_THREADS, 2) kv_select_kernel(EvictArgs a) {
   }
   // ---- this CTA's tokens
   const int per = (n + ctas - 1) / ctas, t0 = min(n, rank * per), t1 = min(n, t0 + per), lo = a.first, hi = n - a.recent;
-  const bool hold = per <= a.held;
-  auto far = [&](int j) { return weight_of(a, table, h, j); };
+  const int th = min(t1, t0 + a.held);                               // shared memory holds the weights of those ahead of this one
+  const bool hold = th == t1;
   auto near = [&](int j) { return held_s[j - t0]; };
+  auto far = [&](int j) { return j < th ? near(j) : weight_of(a, table, h, j); };
   uint32_t need = (uint32_t)(a.keep - a.first - a.recent), prefix = 0, mask = 0;
   const bool none = need == 0;
-  const int m0 = max(t0, lo), m1 = min(t1, hi);                      // of the middle, where weights decide
-  if (hold && !none) {
-    // eight a thread: their pages first, then their weights, so that the loads of either are under way together (a page that is none counts as page 0 and
-    // is reported behind the loads). The first digits are counted on the way.
+  const int m0 = max(t0, lo), m1 = min(t1, hi), mh = min(m1, max(m0, th));       // of the middle, where weights decide; held ones ahead of mh
+  // N a thread: their pages first, then their weights, so that the loads of either are under way together (a page that is none is reported behind them; what counts for
+  // its weight is the same for every digit).
+  auto load = [&](auto at_once, auto far_ones, int from, int to, auto use) {
+    constexpr int N = decltype(at_once)::value;
     bool bad = false;
-    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
-    __syncthreads();
 #pragma unroll 1
-    for (int j0 = m0 + tid; j0 < m1; j0 += 8 * EV_THREADS) {
-      int page[8];
-      float w[8];
+    for (int j0 = from + tid; j0 < to; j0 += N * EV_THREADS) {
+      int page[N];
+      float w[N];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) page[e] = table[a.page_of(min(j0 + e * EV_THREADS, m1 - 1))];
+      for (int e = 0; e < N; ++e) page[e] = table[a.page_of(min(j0 + e * EV_THREADS, to - 1))];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = min(j0 + e * EV_THREADS, m1 - 1);
+      for (int e = 0; e < N; ++e) {
+        const int j = min(j0 + e * EV_THREADS, to - 1);
         const bool out = page[e] < 0 || page[e] >= a.pages;
         bad |= out;
         w[e] = a.mass[((size_t)(out ? 0 : page[e]) * a.nkv + h) * a.kv_block + (j - a.page_of(j) * a.kv_block)];
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (j0 + e * EV_THREADS < m1) {
-          const uint32_t u = weight_order(w[e]);
-          held_s[j0 + e * EV_THREADS - t0] = u;
-          atomicAdd(&hist[u >> 21], 1u);
-        }
+      for (int e = 0; e < N; ++e)
+        if (j0 + e * EV_THREADS < to) use(j0 + e * EV_THREADS, far_ones.value && (page[e] < 0 || page[e] >= a.pages) ? 0u : weight_order(w[e]));
     }
     if (bad) set_status(a.status, ST_BOUNDS);
+  };
+  if (!none) {
+    for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
+    __syncthreads();
+    load(std::integral_constant<int, 8>{}, std::false_type{}, m0, mh, [&](int j, uint32_t u) {                            // (the first digits are counted on the way)
+      held_s[j - t0] = u;
+      atomicAdd(&hist[u >> 21], 1u);
+    });
   }
   for (int pass = 0; pass < 3 && !none; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
     const uint32_t bins = pass == 2 ? 1024u : 2048u;
-    auto count = [&](auto read) {
-#pragma unroll 4
-      for (int j = m0 + tid; j < m1; j += EV_THREADS) {
-        const uint32_t u = read(j);
-        if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
-      }
+    auto count = [&](int, uint32_t u) {
+      if ((u & mask) == prefix) atomicAdd(&hist[u >> shift & (bins - 1)], 1u);
     };
-    if (pass > 0 || !hold) {
+    if (pass > 0) {
       for (int i = tid; i < EV_BINS; i += EV_THREADS) hist[i] = 0;
       __syncthreads();
-      if (hold) count(near);
-      else count(far);
+#pragma unroll 4
+      for (int j = m0 + tid; j < mh; j += EV_THREADS) count(j, held_s[j - t0]);
     }
+    if (mh < m1) load(std::integral_constant<int, 4>{}, std::true_type{}, mh, m1, count);
     if (ctas > 1) cluster.sync();
     else __syncthreads();
     if (ctas > 1) {
@@ -292,23 +302,25 @@ using namespace fb;
 
 extern "C" int fb_kv_evict(int* kept, void* k, void* v, float* scale, float* mass, const int* seg_slot, const int* seg_len, int segs, const int* table,
                            int slots, int max_blocks, const int* dst, int dst_blocks, long pages, int kv_block, int nkv, int row_bytes, int ns, int keep,
-                           int first, int recent, int* status, cudaStream_t s) {
+                           int first, int recent, int ctas, int* status, cudaStream_t s) {
   if (segs <= 0) return 0;
-  if (keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || (long)dst_blocks * kv_block < keep || row_bytes % 16 || ns > 32) return -1;
+  if (ctas < 1 || keep < 1 || first < 0 || recent < 0 || (long)first + recent > keep || (long)dst_blocks * kv_block < keep || row_bytes % 16 || ns > 32) return -1;
   if ((long)segs * nkv > 0x7fffffffl / 8) return -2;
   const long room = (long)max_blocks * kv_block;
   // CTAs of a cluster: the fewest of 1, 2, 4 and 8 that leave a CTA up to 8192 tokens, as far as each has an SM for itself. (A CTA alone takes 12 us for 4000 tokens and
-  // 22 for 12000; what crosses a cluster costs 2 us a digit, and 96 clusters of two, some SMs with two CTAs, take 25 for 12000 where 96 CTAs take 22.)
+  // 22 for 12000; what crosses a cluster costs 2 us a digit, and 96 clusters of two, some SMs with two CTAs, take 25 for 12000 where 96 CTAs take 22.) Tables are as
+  // wide as contexts may get: a shorter one uses fewer of its CTAs. Weights of contexts past EV_HELD a CTA are partly read anew for every digit.
   int cluster = 1, lanes = 1, shift = -1;
-  while (cluster < 8 && room > 8192l * cluster && (long)segs * nkv * cluster * 2 <= 148) cluster *= 2;
+  while (cluster < 8 && room > (long)EV_PART * cluster && (long)segs * nkv * cluster * 2 <= ctas) cluster *= 2;
+  const long held = std::min(std::max((room + cluster - 1) / cluster, std::min(room, (long)EV_PART)), (long)EV_HELD);
   while (lanes < 32 && lanes * 16 < row_bytes) lanes *= 2;
   for (int b = 0; b < 31; ++b)
     if (kv_block == 1 << b) shift = b;
-  // rows of a warp: 32, fewer where that leaves some of the SMs' 148 x 8 x 8 warps without any
+  // rows of a warp: 32, fewer where that leaves some of the SMs' 64 warps without any
   int run = 32;
-  while (run > 4 && run > 128 / lanes && (long)segs * nkv * ((keep + run - 1) / run) < 148l * 64) run /= 2;
+  while (run > 4 && run > 128 / lanes && (long)segs * nkv * ((keep + run - 1) / run) < 64l * ctas) run /= 2;
   const EvictArgs a{kept, (unsigned char*)k, (unsigned char*)v, scale, mass, seg_slot, seg_len, table, dst, segs, slots, max_blocks, dst_blocks, pages,
-                    kv_block, nkv, row_bytes, ns, keep, first, recent, (int)std::min((room + cluster - 1) / cluster, (long)EV_HELD), shift, lanes, run, status};
+                    kv_block, nkv, row_bytes, ns, keep, first, recent, (int)held, shift, lanes, run, status};
   const size_t smem = (size_t)a.held * 4;
   FB_CUDA_CHECK(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_HELD * 4));
   cudaError_t e = launch_pdl_cluster(cluster, kv_select_kernel, dim3((unsigned)(segs * nkv * cluster)), dim3(EV_THREADS), smem, s, a);

@@ -156,5 +156,6 @@ class CudaShared:
         """Eviction by accumulated weight into new pages (see the oracle); rows of every cache form move as they are."""
         kept = self.empty(seg_slot.numel(), k_cache.shape[2], keep, dtype=torch.int32, device=k_cache.device)
         self.launches += 2
-        self.C.kv_evict(kept, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first, recent, self.status_word)
+        self.C.kv_evict(kept, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first, recent,
+                        self.sm_count, self.status_word)
         return kept

@@ -177,3 +177,59 @@ def test_sums_beside_keys_of_minus_infinity(ops, nq, nkv, hd, rows):
         got = sums(ops, st, lse)
         assert torch.isfinite(got).all()
         st.check_sums(got, 0.5)
+
+
+# ---- eviction ----------------------------------------------------------------------------------------------------------
+
+def pool(g, lens, keep, page, nkv, row, width=0, levels=0):
+    """A pool of bf16 rows with streams of `lens` tokens in tables of `width` entries, or as many as the longest has; sums of few levels where said."""
+    need, per = [-(-n // page) for n in lens], -(-keep // page)
+    total = sum(need) + len(lens) * per + 1
+    order = torch.randperm(total, generator=g, device=DEV).int()
+    table, at = torch.full((len(lens), max(need + [width])), -1, dtype=torch.int32, device=DEV), 0
+    for s, n in enumerate(need):
+        table[s, :n] = order[at:at + n]
+        at += n
+    dst = order[at:at + len(lens) * per].view(len(lens), per).contiguous()
+    k, v = (torch.randn(total, page, nkv, row, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    mass = (torch.randint(0, levels, (total, nkv, page), generator=g, device=DEV).float() if levels else torch.randn(total, nkv, page, generator=g, device=DEV).exp())
+    return table, dst, k, v, mass
+
+
+def check_evict(ops, lens, keep, first, recent, page, nkv, table, dst, k, v, mass):
+    """Against a sort of every context, whole pools compared."""
+    old = [x.clone() for x in (k, v, mass)]
+    kept = ops.kv_evict(k, v, None, mass, i32(list(range(len(lens)))), i32(lens), table, dst, page, keep, first, recent)
+    want = [x.clone() for x in old]
+    for s, n in enumerate(lens):
+        pos, i = torch.arange(n, device=DEV), torch.arange(min(n, keep), device=DEV)
+        w = old[2].transpose(1, 2)[table[s, pos // page].long(), pos % page]                     # [tokens, heads]
+        for h in range(nkv):
+            ids = pos
+            if n > keep:
+                best = torch.sort(w[first:n - recent, h], descending=True, stable=True).indices[:keep - first - recent] + first
+                ids = torch.cat([pos[:first], best.sort().values, pos[n - recent:]])
+            assert torch.equal(kept[s, h], torch.cat([ids.int(), i32([-1] * (keep - len(ids)))]))
+            a, b, c, d = table[s].long()[ids // page], ids % page, dst[s].long()[i // page], i % page
+            for x, was in zip(want[:2], old[:2]):
+                x[c, d, h] = was[a, b, h]
+            want[2][c, h, d] = old[2][a, h, b]
+    for x, y in zip((k, v, mass), want):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("streams,nkv", [(1, 1), (1, 4), (5, 4), (24, 4), (40, 4)])
+@pytest.mark.parametrize("width", [70, 300, 2048, 20000])
+def test_evict_with_wide_tables(ops, streams, nkv, width):
+    """Tables with room for far more than the contexts: the same tokens, however many CTAs the room asks for."""
+    lens = [1 + (1237 * i + 4000) % 4400 for i in range(streams)]
+    for levels in (0, 3):
+        check_evict(ops, lens, 500, 3, 101, 64, nkv, *pool(gen("wide", streams, width, levels), lens, 500, 64, nkv, 8, width, levels))
+
+
+@pytest.mark.parametrize("streams,nkv,longest,levels", [(1, 1, 200000, 0), (1, 1, 200000, 4), (1, 1, 400000, 0), (1, 1, 400000, 4), (19, 4, 50000, 0), (19, 4, 50000, 3),
+                                                        (38, 4, 22000, 4)])
+def test_evict_of_very_long_contexts(ops, streams, nkv, longest, levels):
+    """More tokens a CTA than a warp keeps track of in registers, and more than shared memory holds the weights of; equal ones across all of it."""
+    lens = [max(1, longest - 997 * i) for i in range(streams)]
+    check_evict(ops, lens, 3001, 5, 700, 64, nkv, *pool(gen("very long", streams, longest, levels), lens, 3001, 64, nkv, 8, 0, levels))
