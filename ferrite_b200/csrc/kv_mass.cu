@@ -9,6 +9,7 @@
 // (768 with the keys in shared memory: what the operands take from there).
 // Measured (B200, us): one row of 24 heads of 256 over 100000 keys 39, 5.3 TB/s; six over 8000 shared and 900 own keys each 12; 2048 rows over 16000 keys 345, tensor
 // pipe 72 % busy under the power cap, and 1111 rows of 32 heads of 128 over 5000 keys 66.
+// A key's sum is written once, so a key is of one span: a bit a key says that one has taken it, and a second one sets the status (idle warps ask, or those that join).
 // Every wait is bounded, as in the attention.
 #include <algorithm>
 
@@ -80,6 +81,25 @@ __device__ __forceinline__ float km_weights(uint32_t taddr, int cols, int pairs,
   return s.x + s.y;
 }
 
+// Words of 32 keys' bits, cleared ahead of the kernel that takes them.
+__device__ __forceinline__ void km_clear(uint32_t* taken, long words) {
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < words / 4; i += (long)gridDim.x * blockDim.x) reinterpret_cast<uint4*>(taken)[i] = make_uint4(0, 0, 0, 0);
+}
+__global__ void __launch_bounds__(256) kv_mass_clear_kernel(uint32_t* taken, long words) {
+  pdl_launch_dependents();
+  pdl_wait();
+  km_clear(taken, words);
+}
+// Takes those of k0 .. k1 of the 32 keys from `key` on (a multiple of 32; what reads the page reports one that is none).
+__device__ __forceinline__ void km_take(const FbSharedStep& st, uint32_t* taken, int slot, int key, int k0, int k1, int* status) {
+  const int lo = max(k0 - key, 0), hi = min(k1 - key, 32);
+  if (lo >= hi) return;
+  const int page = st.table[(size_t)slot * st.max_blocks + key / st.kv_block];
+  if (page < 0 || page >= st.pages) return;
+  const uint32_t bits = (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+  if (atomicOr(taken + ((size_t)page * st.kv_block + key % st.kv_block) / 32, bits) & bits) set_status(status, ST_BOUNDS);
+}
+
 // What a pair of a tile is: the number that leads from its scores to weights, and the keys that it sees.
 __device__ __forceinline__ void km_pair(const FbSharedStep& st, const float* lse, const SharedBlock& e, int row, int g, int head0, int nq, int share, int Rq, int c,
                                         float* nl, int* kvl) {
@@ -124,7 +144,8 @@ struct KmWalk {
 template <int HD>
 __global__ void __launch_bounds__(KM_THREADS, 1)
 kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ, float* out, const float* mass, float carry,
-                    const float* lse, FbSharedStep st, SharedPlanSizes z, SharedBlock* table, int R, int nq, int nkv, float scale_log2, int* status) {
+                    const float* lse, FbSharedStep st, SharedPlanSizes z, SharedBlock* table, uint32_t* taken, int R, int nq, int nkv, float scale_log2,
+                    int* status) {
   using C = KmCfg<HD>;
   constexpr int NCH = C::NCH, KS = C::KS;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -291,6 +312,12 @@ kv_mass_keys_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (lane == 0 && !*abort_flag) set_status(status, ST_MBAR_TIMEOUT);
       *abort_flag = 1;
     }
+  } else if (warp == 3) {
+    // ---- keys of the CTA's tiles are taken
+    do
+      for (int w = lane; x.kvh == 0 && w < x.n * (KM_KEYS / 32); w += 32)
+        km_take(st, taken, x.e.slot, (x.e.k0 / KM_KEYS + x.t) * KM_KEYS + 32 * w, x.e.k0, x.e.k1, status);
+    while (x.next(nkv));
   } else if (warp >= 4) {
     // ---- weights: set i % 4 of four warps has key tile i with all of its pairs
     const int quad = warp & 3, set = (warp - 4) >> 2, st_tid = tid - 128, place = quad * 32 + lane;
@@ -365,6 +392,8 @@ struct KpSpace {
   KpItem* items;
   KpStart* starts;
   float* sums;                                   // [pieces][sets][keys of a tile]; piece: CTA + item * kv heads + kv head
+  uint32_t* taken;
+  long words;
   int max_items;
   SharedPlanSizes z;
 };
@@ -568,6 +597,7 @@ kv_mass_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   sk_tmem_alloc(&ms.tmem, KP_COLS);
   __syncthreads();
   const uint32_t tmem = sk_tmem_ready(&ms.tmem);
+  km_clear(w.taken, w.words);                                        // (for the kernel that joins the sums)
   const bool any = w.head[0] > 0;
   KpWalk x;
   auto sees = [&](const SharedBlock& e, const KpItem& it) { return e.nt > it.key0 / KP_KEYS - it.k0 / KP_KEYS; };
@@ -787,6 +817,7 @@ __global__ void __launch_bounds__(KP_KEYS) kv_mass_join_kernel(float* out, const
   for (int i = blockIdx.x; i < items; i += gridDim.x) {
     const KpItem it = w.items[i];
     const int kvh = blockIdx.y, key = it.key0 + threadIdx.x;
+    if (kvh == 0 && threadIdx.x % 32 == 0) km_take(st, w.taken, it.slot, key, it.k0, it.k1, status);
     if (key < it.k0 || key >= it.k1) continue;
     const int page = st.table[(size_t)it.slot * st.max_blocks + key / st.kv_block];
     if (page < 0 || page >= st.pages) {
@@ -828,6 +859,7 @@ static int km_resident_rows(int hd, int share) { return (hd == 256 ? KmCfg<256>:
 // The form for few pairs takes all that fit (us, the most rows that stay / one row more, at 500, 16000, 60000 keys: 24 heads of 256, 30 rows 11 / 25, 20 / 34, 51 / 68;
 // 32 of 128, 80 rows 11 / 37, 36 / 41, 114 / 103; 4 of 64, 256 rows 14 / 24, 20 / 29, 47 / 51).
 static bool km_few(int rows, int max_rows, int ngrp, int hd, int share) { return (ngrp ? rows : std::min(rows, max_rows)) <= km_resident_rows(hd, share); }
+static long km_words(long keys) { return (keys / 32 + 3) / 4 * 4; }
 // (A span of n keys is of up to n / 256 + 2 items, and a key of the pool is of one span.)
 static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, int ngrp, int nkv, int share, long room, long keys, int ctas) {
   const int Rq = KM_PAIRS / share;
@@ -845,6 +877,8 @@ static long km_space(KpSpace* w, float* ws, int rows, int nseg, int max_rows, in
   v.items = (KpItem*)take(items * 8);
   v.starts = (KpStart*)take(ctas * 8l);
   v.sums = take((items * nkv + ctas) * KM_SETS * KM_KEYS);
+  v.words = km_words(keys);
+  v.taken = (uint32_t*)take(v.words);
   v.max_items = (int)std::min(items, 0x7fffffffl);
   if (w) *w = v;
   return at - ws;
@@ -854,11 +888,11 @@ extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int n
   if (rows <= 0 || nseg <= 0 || nkv < 1 || nq / nkv < 1 || nq / nkv > KM_PAIRS) return 0;
   const int share = nq / nkv;
   const long logs = want_lse ? ((long)rows * nq + 3) / 4 * 4 + fb_attention_shared_floats(rows, nseg, max_rows, ngrp, nq, nkv, hd, ctas, 0) : 0;
-  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys, ctas));
+  return logs + (km_few(rows, max_rows, ngrp, hd, share) ? km_words(keys) + 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys, ctas));
 }
 
 extern "C" int fb_attention_mass_launches(int rows, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse) {
-  return rows <= 0 || max_rows <= 0 ? 0 : (km_few(rows, max_rows, ngrp, hd, nq / nkv) ? 1 : 3) + (want_lse ? 2 : 0);
+  return rows <= 0 || max_rows <= 0 ? 0 : (km_few(rows, max_rows, ngrp, hd, nq / nkv) ? 2 : 3) + (want_lse ? 2 : 0);
 }
 
 extern "C" int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride,
@@ -885,14 +919,17 @@ extern "C" int fb_attention_mass(float* out, const float* mass, float carry, con
     const int R = km_resident_rows(hd, share);
     SharedPlanSizes z;
     if (!shared_plan_sizes(st, shared_group_blocks(st.rows, st.ngrp, R), shared_seg_blocks(st.rows, st.nseg, st.max_rows, R), &z)) return -2;
+    const long words = km_words(keys);
+    if ((e = launch_pdl(kv_mass_clear_kernel, dim3((unsigned)std::min((words + 1023) / 1024, (long)ctas)), dim3(256), 0, s, (uint32_t*)ws, words)) != cudaSuccess)
+      return (int)e;
 #define FB_KM(H)                                                                                                                                       \
   if (hd == H) {                                                                                                                                       \
     using C = KmCfg<H>;                                                                                                                                \
     constexpr size_t smem = C::MISC_AT + sizeof(KmMisc<C::QS>);                                                                                        \
     static_assert(smem <= 232448, "shared memory of an SM");                                                                                           \
     FB_CUDA_CHECK(cudaFuncSetAttribute(kv_mass_keys_kernel<H>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));                               \
-    e = launch_pdl(kv_mass_keys_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, out, mass, carry, lse, st, z, (SharedBlock*)ws, R, nq,     \
-                   nkv, scale, status);                                                                                                                \
+    e = launch_pdl(kv_mass_keys_kernel<H>, dim3(ctas), dim3(KM_THREADS), smem, s, tmK, tmQ, out, mass, carry, lse, st, z, (SharedBlock*)(ws + words),  \
+                   (uint32_t*)ws, R, nq, nkv, scale, status);                                                                                                                \
   }
     FB_KM(64) FB_KM(128) FB_KM(256)
 #undef FB_KM

@@ -20,15 +20,15 @@ import torch
 
 
 def _spans(segs, groups):
-    """(segment, slot that the shared tokens are read through, shared tokens) of every segment."""
+    """(segment, slot that the shared tokens are read through, shared tokens, group or -1) of every segment."""
     out = []
     for s in range(len(segs[0])):
-        slot, shared = int(segs[0][s]), 0
+        slot, shared, group = int(segs[0][s]), 0, -1
         for g in range(0 if groups is None else len(groups[0])):
             lo = int(groups[0][g])
             if lo <= s < lo + int(groups[1][g]):
-                slot, shared = int(segs[0][lo]), int(groups[2][g])
-        out.append((s, slot, shared))
+                slot, shared, group = int(segs[0][lo]), int(groups[2][g]), g
+        out.append((s, slot, shared, group))
     return out
 
 
@@ -47,7 +47,7 @@ class TorchShared:
         out = torch.zeros(T, nq, hd, dtype=torch.float32, device=q.device)
         lse = torch.full((T, nq), -math.inf, dtype=torch.float32, device=q.device)
         kf, vf = k_cache.reshape(-1, nkv, hd), v_cache.reshape(-1, nkv, hd)
-        for s, shared_slot, shared in _spans(segs, groups):
+        for s, shared_slot, shared, _ in _spans(segs, groups):
             for t in range(int(segs[1][s]), int(segs[1][s]) + int(segs[2][s])):
                 n = int(row_kvlen[t])
                 if n <= 0:
@@ -64,18 +64,24 @@ class TorchShared:
     def attention_mass(self, q, k_cache, mass, row_kvlen, block_table, kv_block, nq, nkv, hd, segs, groups=None, lse=None, carry=1.0, out=None):
         """Per kv head and key that some row sees: out = carry * mass + the sum of exp(q k / sqrt(hd) - lse) over the rows that see the key and the heads
         that share the kv head (64 at most); `out` is `mass` itself unless given, other entries stay. `lse` is that of the step's attention, or None: it
-        is computed. With carry 0 `mass` is not read."""
+        is computed. With carry 0 `mass` is not read. A key is of one segment, or of one group's shared tokens: one that two of them hold is an error (of streams
+        that were forked at different tokens; a call for each of them, with carry 1, adds their weights up)."""
         out = mass if out is None else out
         kf = k_cache.reshape(-1, nkv, hd)
         sums = torch.zeros(mass.shape[0] * kv_block, nkv, dtype=torch.float32, device=q.device)
         seen = torch.zeros(sums.shape[0], dtype=torch.bool, device=q.device)
-        for s, shared_slot, shared in _spans(segs, groups):
+        holder = torch.full((sums.shape[0],), -1, dtype=torch.int64, device=q.device)
+        for s, shared_slot, shared, group in _spans(segs, groups):
             rows = range(int(segs[1][s]), int(segs[1][s]) + int(segs[2][s]))
             longest = max([int(row_kvlen[t]) for t in rows] + [0])
             if longest <= 0:
                 continue
             at = _token_rows(block_table, kv_block, int(segs[0][s]), shared_slot, shared, longest)
             seen[at] = True
+            for part, who in ((at[:max(shared, 0)], group), (at[max(shared, 0):], -2 - s)):
+                if part.unique().numel() < part.numel() or not ((holder[part] == -1) | (holder[part] == who)).all():
+                    raise RuntimeError("attention_mass: a key of two segments, or of a segment and a group's shared tokens")
+                holder[part] = who
             for t in rows:
                 n = int(row_kvlen[t])
                 if n <= 0:
@@ -141,8 +147,8 @@ class CudaShared:
         return (out, lse) if want_lse else out
 
     def attention_mass(self, q, k_cache, mass, row_kvlen, block_table, kv_block, nq, nkv, hd, segs, groups=None, lse=None, carry=1.0, out=None):
-        """Weight that the step's rows gave to every key of their contexts, added to `carry` times the sums so far (see the oracle). Every page of the
-        step belongs to one segment or to one group's shared tokens: its sums are written once."""
+        """Weight that the step's rows gave to every key of their contexts, added to `carry` times the sums so far (see the oracle). A key that
+        two segments hold, or a segment and a group's shared tokens, sets the status, and its sum says nothing."""
         q, step = self._shared_step(q, nq, hd, segs, groups)
         out = mass if out is None else out
         G = 0 if groups is None else groups[0].numel()

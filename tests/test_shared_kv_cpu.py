@@ -93,3 +93,24 @@ def test_evict_refuses():
     for keep, first, recent in ((0, 0, 0), (9, 0, 0), (4, 3, 2), (4, -1, 0), (4, 0, -1)):
         with pytest.raises(RuntimeError):
             OPS.kv_evict(z, z, None, torch.zeros(4, 2, 8), one, one, one[None], one[None], 8, keep, first, recent)
+
+
+def test_sums_refuse_keys_that_two_segments_hold():
+    """Streams that were forked twice, a slot that comes twice, a page that comes twice in a table: a key's sum is written once."""
+    for spoil in ("forked twice", "slot", "page"):
+        st = step(6, groups=[(16, [[17], [41], [45]])], alone=[[33]])
+        if spoil == "forked twice":
+            st.table[2, 2:4] = st.table[1, 2:4]
+        elif spoil == "slot":
+            st.segs[0][3] = 2
+        else:
+            st.table[3, 3] = st.table[3, 1]
+        with pytest.raises(RuntimeError):
+            OPS.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), st.segs, st.groups)
+    st = step(6, groups=[(16, [[17], [41], [45]])], alone=[[33]])
+    st.table[2, 2:4] = st.table[1, 2:4]                                   # one by one
+    whole = torch.zeros_like(st.mass)
+    for s in range(4):
+        segs = tuple(t[s:s + 1] for t in st.segs[:3]) + (1,)
+        OPS.attention_mass(st.q, st.k, whole, st.kvlen, *st.args(), segs)
+    assert torch.allclose(whole.sum((0, 2)), torch.full((2,), 4.0 * 3), rtol=1e-5)

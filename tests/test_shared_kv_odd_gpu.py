@@ -233,3 +233,36 @@ def test_evict_of_very_long_contexts(ops, streams, nkv, longest, levels):
     """More tokens a CTA than a warp keeps track of in registers, and more than shared memory holds the weights of; equal ones across all of it."""
     lens = [max(1, longest - 997 * i) for i in range(streams)]
     check_evict(ops, lens, 3001, 5, 700, 64, nkv, *pool(gen("very long", streams, longest, levels), lens, 3001, 64, nkv, 8, 0, levels))
+
+
+# ---- keys of two segments ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [1, 300])
+@pytest.mark.parametrize("spoil", ["forked twice", "forked in a page", "slot", "page", "group"])
+def test_sums_of_keys_that_two_segments_hold(ops, rows, spoil):
+    """A key's sum is written once: one that two segments hold, or a segment and a group's shared tokens, is reported. The attention takes such steps."""
+    def some(n):
+        return [max(1, n - i) for i in range(rows)]
+
+    def step():
+        return shared_pages.Step(gen("forked", rows), DEV, 6, 2, 128, 64, ((128, [[130], some(900), [1000]]),), [[333], [64]], poison=None)
+    st = step()
+    attend(ops, st)
+    check_sums(st, sums(ops, st), 0.5)                                   # nothing held twice, nothing reported
+    assert ops.status() == 0
+    if spoil == "forked twice":
+        st.table[2, 2:13] = st.table[1, 2:13]
+    elif spoil == "forked in a page":
+        st.table[2, 14] = st.table[1, 14]                                # token 896 .. 899 of one, 896 .. 959 of the other
+    elif spoil == "slot":
+        st.segs[0][3] = 2
+    elif spoil == "page":
+        st.table[3, 5] = st.table[3, 2]                                  # its last page again, ahead of the last tokens
+    else:
+        st.table[4, 0] = st.table[0, 1]                                  # a shared page as another stream's own
+    lse = attend(ops, st)[1]
+    assert ops.status() == 0
+    for known in (lse, None):
+        sums(ops, st, known)
+        assert ops.status() != 0
+        ops.status_word.zero_()
