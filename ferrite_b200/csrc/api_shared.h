@@ -32,7 +32,7 @@ int fb_attention_shared(void* out, float* lse, float* ws, long ws_floats, const 
 // out[page, kv head, place] = carry * mass[..] + sum over rows and heads of exp(score - lse), for the keys of the step's contexts
 // (lse null: computed); one that two spans hold sets the status. room: tokens that a table has room for; keys: tokens of the pool
 long fb_attention_mass_floats(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, long room, long keys, int want_lse, int ctas);
-int fb_attention_mass_launches(int rows, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse);
+int fb_attention_mass_launches(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse);
 int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride, const void* k,
                       FbSharedStep st, int nq, int nkv, int hd, int ctas, int* status, cudaStream_t s);
 

@@ -108,7 +108,7 @@ int64_t attention_mass(Tensor out, Tensor mass, double carry, OptTensor lse, Ten
   check(fb_attention_mass(out.data_ptr<float>(), mass.data_ptr<float>(), (float)carry, lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr<float>(),
                           (long)ws.numel(), q.data_ptr(), (long)q.stride(0), k.data_ptr(), st, (int)nq, (int)nkv, (int)hd, (int)ctas,
                           status.data_ptr<int>(), cur_stream()), what);
-  return fb_attention_mass_launches(st.rows, st.max_rows, st.ngrp, (int)nq, (int)nkv, (int)hd, !lse);
+  return fb_attention_mass_launches(st.rows, st.nseg, st.max_rows, st.ngrp, (int)nq, (int)nkv, (int)hd, !lse);
 }
 
 // k, v [pages, kv_block, nkv, ..] of 16-bit values or of codes; scale [pages, kv_block, nkv, ns]

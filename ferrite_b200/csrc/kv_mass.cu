@@ -891,8 +891,8 @@ extern "C" long fb_attention_mass_floats(int rows, int nseg, int max_rows, int n
   return logs + (km_few(rows, max_rows, ngrp, hd, share) ? km_words(keys) + 8l * (nseg + ngrp) : km_space(nullptr, nullptr, rows, nseg, max_rows, ngrp, nkv, share, room, keys, ctas));
 }
 
-extern "C" int fb_attention_mass_launches(int rows, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse) {
-  return rows <= 0 || max_rows <= 0 ? 0 : (km_few(rows, max_rows, ngrp, hd, nq / nkv) ? 2 : 3) + (want_lse ? 2 : 0);
+extern "C" int fb_attention_mass_launches(int rows, int nseg, int max_rows, int ngrp, int nq, int nkv, int hd, int want_lse) {
+  return rows <= 0 || nseg <= 0 || max_rows <= 0 ? 0 : (km_few(rows, max_rows, ngrp, hd, nq / nkv) ? 2 : 3) + (want_lse ? 2 : 0);
 }
 
 extern "C" int fb_attention_mass(float* out, const float* mass, float carry, const float* lse, float* ws, long ws_floats, const void* q, long q_stride,

@@ -141,7 +141,7 @@ class CudaShared:
         out = self.empty(T, nq * hd, dtype=torch.bfloat16, device=q.device)
         lse = self.empty(T, nq, dtype=torch.float32, device=q.device) if want_lse else None
         ws = self.empty(self.C.attention_shared_floats(T, segs[0].numel(), segs[3], G, nq, nkv, hd, self.sm_count, 1), dtype=torch.float32, device=q.device)
-        self.launches += 2
+        self.launches += 2 if T and segs[0].numel() else 0
         self.C.attention_shared(out, lse, ws, q, k_cache, v_cache, proj if gated else None, row_kvlen, block_table, kv_block, nq, nkv, hd, *step,
                                 self.sm_count, self.status_word)
         return (out, lse) if want_lse else out
@@ -161,7 +161,7 @@ class CudaShared:
     def kv_evict(self, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first=0, recent=0):
         """Eviction by accumulated weight into new pages (see the oracle); rows of every cache form move as they are."""
         kept = self.empty(seg_slot.numel(), k_cache.shape[2], keep, dtype=torch.int32, device=k_cache.device)
-        self.launches += 2
+        self.launches += 2 if seg_slot.numel() else 0
         self.C.kv_evict(kept, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first, recent,
                         self.sm_count, self.status_word)
         return kept

@@ -266,3 +266,22 @@ def test_sums_of_keys_that_two_segments_hold(ops, rows, spoil):
         sums(ops, st, known)
         assert ops.status() != 0
         ops.status_word.zero_()
+
+
+# ---- empty calls -------------------------------------------------------------------------------------------------------
+
+def test_calls_without_rows_or_segments(ops):
+    """Steps of no rows and of no segments launch nothing, count nothing and leave everything as it was."""
+    st = shared_pages.Step(gen("empty"), DEV, 6, 2, 128, 64, ((130, [[140], [200]]),), [[9]])
+    table, dst, k, v, mass = pool(gen("empty evict"), [100], 32, 64, 2, 8)
+    none = i32([])
+    before, launches = [x.clone() for x in (st.mass, k, v, mass)], ops.launches
+    for q, kvlen, segs in ((st.q[:0], none, st.segs), (st.q, st.kvlen, (none, none, none, 0)), (st.q[:0], none, (none, none, none, 0))):
+        out, lse = ops.attention_shared(q, None, st.k, st.v, kvlen, *st.args(), False, segs, want_lse=True)
+        assert out.shape == (len(q), 768) and lse.shape == (len(q), 6)
+        for known in (None, lse):
+            ops.attention_mass(q, st.k, st.mass, kvlen, *st.args(), segs, lse=known)
+    assert ops.kv_evict(k, v, None, mass, none, none, table, dst[:0], 64, 32).shape == (0, 2, 32)
+    assert ops.launches == launches
+    for x, y in zip((st.mass, k, v, mass), before):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
