@@ -17,6 +17,7 @@ inline cudaStream_t cur_stream() { return c10::cuda::getCurrentCUDAStream().stre
 inline void check(int rc, const char* what) {
   if (rc == 0) return;
   if (rc > 0) TORCH_CHECK(false, what, ": CUDA error ", rc, " (", cudaGetErrorString((cudaError_t)rc), ")");
+  TORCH_CHECK(rc != -2, what, ": more segments or rows than a call plans");
   TORCH_CHECK(false, what, ": unsupported arguments (code ", rc, ")");
 }
 bool aligned(const Tensor& t, int64_t bytes) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % bytes == 0; }

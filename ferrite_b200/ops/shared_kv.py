@@ -5,12 +5,20 @@ kernels of `csrc/shared_attn.cu`, `csrc/kv_mass.cu` and `csrc/kv_evict.cu`. Both
 A step's rows come in segments of one slot each, `segs` = (seg_slot, seg_row0, seg_nrows, rows of the longest): rows seg_row0 .. seg_row0 + seg_nrows, in any
 order; row i sees the first row_kvlen[i] tokens. `groups` = (grp_seg0, grp_nsegs, grp_len), or None: the rows of grp_nsegs consecutive segments from grp_seg0
 on lie side by side and read their first grp_len tokens, any number, through the table of the first of these segments, and what follows through their
-own. A segment belongs to one group at most; one of no rows is padding, whatever its slot (but that of a group's first). Streams that share pages (a forked
-conversation, samples of one prompt) are a group, so that their common keys and values are read once. A row is of one segment; of none, it is left out and
-its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a multiple of 64. What the kernels find wrong in the tables on the
-device (a page or slot that is none, a context beyond its table, a segment of more rows than was said) sets the op class's status word.
+own (whose entries for whole shared pages are not looked at). A segment belongs to one group at most; one of no rows is padding, whatever its slot (but that of
+a group's first). Streams whose tables hold the same pages (a pool whose owner lets several streams have a page: samples of one prompt, forks of one
+conversation) are a group, so that their common keys and values are read once for every 128 (row, head) pairs of it. A row is of one segment; of none, it is
+left out and its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a multiple of 64. What the kernels find wrong in the
+tables on the device (a page or slot that is none, a context beyond its table, a segment of more rows than was said) sets the op class's status word.
 
-Sums of weights are [pages, kv heads, kv_block] in fp32, beside the cache: they follow the pages through forks and parking.
+Where contexts are cut follows the lengths of the whole step: a row may round otherwise beside other streams, decoded or verified, than by itself (the paged
+attention of every stream by itself does not). The same call gives the same bits. A call plans 5 words a segment, 4 a group and 2 a block of rows (128 pairs of a row
+and a query head of one kv head for the attention, 64 for the sums), 40960 in all, and is refused beyond: from about 20000 rows on where 128 query heads share a kv
+head, 320000 where 8 do (160000 for the sums), half as many in groups.
+
+Sums of weights are [pages, kv heads, kv_block] in fp32, beside the cache: they follow the pages through forks and parking. Whoever writes a key into a page sets its sum,
+to zero or what it is to start from: the ops change the sums of keys that a step sees and of places that tokens are moved to, and leave those behind a page's last token, a
+former owner's among them, as they are.
 """
 from __future__ import annotations
 
@@ -97,8 +105,9 @@ class TorchShared:
     def kv_evict(self, k_cache, v_cache, kv_scale, mass, seg_slot, seg_len, block_table, dst_table, kv_block, keep, first=0, recent=0):
         """Per slot of `seg_slot` (with seg_len tokens) and kv head, `keep` tokens move to the pages dst_table[segment], in their order: the `first` first
         ones, the `recent` last ones, and of the others those with the largest sums (the earlier of equal ones; a sum that is no number counts as the
-        largest). Keys, values, scales and sums are copied; contexts of up to `keep` tokens whole. The new pages are none of the old ones. Returns the
-        tokens kept, int32 [segments, kv heads, keep], ascending, -1 behind the last."""
+        largest). Keys, values, scales and sums are copied; contexts of up to `keep` tokens whole. The new pages are none of the old ones; places of theirs
+        behind the last token kept stay as they were, sums too. Returns the tokens kept, int32 [segments, kv heads, keep], ascending, -1 behind the last.
+        Caches of codes move as they are, with sums that their owner has: `attention_mass` reads bf16 caches."""
         nkv = k_cache.shape[2]
         if not 0 <= first <= keep - recent <= keep or keep < 1 or dst_table.shape[1] * kv_block < keep:
             raise RuntimeError(f"kv_evict: first {first} and recent {recent} of {keep}, pages for {dst_table.shape[1] * kv_block}")

@@ -285,3 +285,49 @@ def test_calls_without_rows_or_segments(ops):
     assert ops.launches == launches
     for x, y in zip((st.mass, k, v, mass), before):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+# ---- steps of very many rows -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("nq,hd", [(1, 64), (3, 128)])
+def test_steps_whose_lengths_do_not_fit_beside_the_plan(ops, nq, hd):
+    """More rows than the plan has room for the lengths of: they are read where they lie."""
+    rows, n, page = 41500, 300, 64
+    g = gen("rows", nq)
+    k, v = (torch.randn(8, page, 1, hd, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    table = torch.randperm(8, generator=g, device=DEV).int()[:5].view(1, 5).contiguous()
+    q = torch.randn(rows, nq, hd, generator=g, device=DEV).to(torch.bfloat16)
+    kvlen = torch.randint(0, n + 1, (rows,), generator=g, device=DEV, dtype=torch.int32)
+    segs = (i32([0]), i32([0]), i32([rows]), rows)
+    out, lse = ops.attention_shared(q, None, k, v, kvlen, table, page, nq, 1, hd, False, segs, want_lse=True)
+    at = table[0].long()[torch.arange(n, device=DEV) // page] * page + torch.arange(n, device=DEV) % page
+    keys, values = k.view(-1, hd)[at].double(), v.view(-1, hd)[at].double()
+    sees = torch.arange(n, device=DEV) < kvlen[:, None, None]
+    x = torch.where(sees, q.double() @ keys.t() / hd ** 0.5, -INF)
+    wl = torch.logsumexp(x, -1)
+    p = torch.where(sees, torch.exp(x - wl[..., None]), 0.0)
+    # as in shared_pages.Step: scores in 32 bits, weights of twice eight bits
+    off = torch.where(sees, q.double().abs() @ keys.abs().t(), 0.0).amax(-1) / hd ** 0.5 * 2.0 ** -20
+    tol = (p @ values.abs()) * (2 * (off[..., None] + 2.0 ** -20) + 2.0 ** -16 + 2.0 ** -12)
+    want = p @ values
+    alike(out.view_as(want), want, tol + 2.0 ** -8 * (want.abs() + tol) + 1e-30)
+    alike(lse, wl, off + 2.0 ** -22 * wl.abs().nan_to_num(0, 0, 0) + 2.0 ** -20)
+    rel = off[..., None] * 2 + 2.0 ** -20 + 2.0 ** -22 * (x.abs().nan_to_num(0, 0, 0) + wl.abs().nan_to_num(0, 0, 0)[..., None])
+    new, mtol = p.sum((0, 1)), (p * rel).sum((0, 1))
+    mtol += new * (rows * nq) * 2.0 ** -24 + 2.0 ** -22 * new
+    for known in (lse, None):
+        got = ops.attention_mass(q, k, torch.zeros(8, 1, page, device=DEV), kvlen, table, page, nq, 1, hd, segs, lse=known)
+        alike(got.view(-1)[at], new, mtol)
+        assert float(got.sum()) == float(got.view(-1)[at].sum())
+
+
+def test_steps_of_more_rows_than_a_call_plans(ops):
+    """Refused, with what the bound is for."""
+    rows = 20600
+    q = torch.zeros(rows, 128, 64, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(2, 64, 1, 64, dtype=torch.bfloat16, device=DEV)
+    kvlen, table, segs = i32([10] * rows), i32([[0, 1]]), (i32([0]), i32([0]), i32([rows]), rows)
+    with pytest.raises(RuntimeError, match="more segments or rows than a call plans"):
+        ops.attention_shared(q, None, k, k, kvlen, table, 64, 128, 1, 64, False, segs)
+    with pytest.raises(RuntimeError, match="more segments or rows than a call plans"):
+        ops.attention_mass(q[:, :64], k, torch.zeros(2, 1, 64, device=DEV), kvlen, table, 64, 64, 1, 64, segs, lse=torch.zeros(rows, 64, device=DEV))
