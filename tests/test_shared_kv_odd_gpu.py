@@ -287,6 +287,22 @@ def test_calls_without_rows_or_segments(ops):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
+# ---- layouts ----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_one_query_for_all_rows(ops, rows):
+    """A query expanded over the rows, and rows that overlap: the same as a copy of them."""
+    st = shared_pages.Step(gen("expanded", rows), DEV, 6, 2, 128, 64, ((130, [[140], [200]]),), [[500 - i for i in range(rows - 2)]])
+    flat = torch.randn(6 * 128 + 8 * rows, generator=gen("overlap"), device=DEV).to(torch.bfloat16)
+    for q in (st.q[:1].expand(rows, 6, 128), flat.as_strided((rows, 6, 128), (8, 128, 1))):
+        st.q = q
+        got = [attend(ops, st), sums(ops, st)]
+        st.q = q.contiguous()
+        want = [attend(ops, st), sums(ops, st)]
+        assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[0][1], want[0][1]) and torch.equal(got[1], want[1])
+        check_sums(st, got[1], 0.5)
+
+
 # ---- steps of very many rows -------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("nq,hd", [(1, 64), (3, 128)])
@@ -331,3 +347,183 @@ def test_steps_of_more_rows_than_a_call_plans(ops):
         ops.attention_shared(q, None, k, k, kvlen, table, 64, 128, 1, 64, False, segs)
     with pytest.raises(RuntimeError, match="more segments or rows than a call plans"):
         ops.attention_mass(q[:, :64], k, torch.zeros(2, 1, 64, device=DEV), kvlen, table, 64, 64, 1, 64, segs, lse=torch.zeros(rows, 64, device=DEV))
+
+
+# ---- steps that are wrong in a part ------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("fill", [0x7fffffff, -1, 1 << 20])
+@pytest.mark.parametrize("spoil", ["rows", "slot"])
+@pytest.mark.parametrize("many", [False, True])
+def test_sums_beside_refused_segments(ops, fill, spoil, many):
+    """A segment that does not fit the step sets the status. The sums of the others' keys are right, whatever the workspace held, and nothing else changes."""
+    rows = 150 if many else 3
+    st = shared_pages.Step(gen("refused sums", spoil, many), DEV, 6, 2, 128, 64, ((130, [[140], [200]]),), [[9], [31 + i for i in range(rows)], [77]], spare=20)
+    bad = 3
+    if spoil == "rows":
+        segs = (*st.segs[:3], rows - 1)
+    else:
+        segs = (i32([*st.segs[0][:bad].tolist(), -5, int(st.segs[0][4])]), *st.segs[1:])
+    lse = attend(ops, st)[1]
+    ops.status_word.zero_()
+    want, tol, seen = st.masses(0.5)
+    other = torch.ones(st.k.shape[0], dtype=torch.bool, device=DEV)      # pages of the other streams and of none
+    other[st.table[st.slots[bad]][st.table[st.slots[bad]] >= 0].long()] = False
+    for known in (lse, None):
+        n = ops.C.attention_mass_floats(st.rows, 5, segs[3], 1, 6, 2, 128, st.table.shape[1] * 64, st.k.shape[0] * 64, known is None, ops.sm_count)
+        out = st.mass.clone()
+        torch.full((n,), fill, dtype=torch.int32, device=DEV)            # what the allocator hands out next
+        ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), segs, st.groups, lse=known, carry=0.5, out=out)
+        assert ops.status() != 0
+        ops.status_word.zero_()
+        assert ((out - want).abs() <= tol)[seen & other[:, None, None]].all()
+        assert torch.equal(out[~seen], st.mass[~seen]) and torch.equal(out[~other], st.mass[~other])
+
+
+def test_wrong_tables_touch_nothing_else(ops):
+    """Pages that are none, contexts beyond the table, slots that are none: caches, tables and sums that the step does not name stay as they were."""
+    for spoil in ("page", "far page", "length", "slot", "group"):
+        st = shared_pages.Step(gen("wrong", spoil), DEV, 6, 2, 128, 64, ((130, [[140], [200]]),), [[9]], spare=30, poison=None)
+        named = torch.zeros(st.k.shape[0], dtype=torch.bool, device=DEV)
+        named[st.table[st.table >= 0].long()] = True
+        if spoil == "page":
+            st.table[0, 1] = -1
+        elif spoil == "far page":
+            st.table[1, 3] = 1 << 30
+        elif spoil == "length":
+            st.kvlen[2] = 100000
+        elif spoil == "slot":
+            st.segs[0][2] = 77
+        else:
+            st.groups[0][0] = 3
+        held = [t.clone() for t in (st.k, st.v, st.mass, st.table, st.kvlen, st.q)]
+        lse = attend(ops, st)[1]
+        outs = [sums(ops, st, known) for known in (lse, None)]
+        assert ops.status() != 0, spoil
+        ops.status_word.zero_()
+        for t, h in zip((st.k, st.v, st.mass, st.table, st.kvlen, st.q), held):
+            assert torch.equal(t, h), spoil
+        for out in outs:
+            assert torch.equal(out[~named], st.mass[~named]), spoil
+    for spoil in ("page", "dst", "length", "slot"):
+        table, dst, k, v, mass = pool(gen("wrong evict", spoil), [200, 150], 64, 64, 2, 8)
+        new = torch.zeros(k.shape[0], dtype=torch.bool, device=DEV)
+        new[dst.long()] = True
+        n, slot = i32([200, 150]), i32([0, 1])
+        if spoil == "page":
+            table[0, 2] = 1 << 20
+        elif spoil == "dst":
+            new[dst[0, 0].long()] = False
+            dst[0, 0] = -1
+        elif spoil == "length":
+            n[0] = 1 << 20
+        else:
+            slot[0] = -1
+        held = [t.clone() for t in (k, v, mass)]
+        ops.kv_evict(k, v, None, mass, slot, n, table, dst, 64, 64, 2, 10)
+        assert ops.status() != 0, spoil
+        ops.status_word.zero_()
+        for t, h in zip((k, v, mass), held):
+            assert torch.equal(t[~new], h[~new]), spoil
+
+
+# ---- captured calls ----------------------------------------------------------------------------------------------------
+
+def captured(call):
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        res = call()
+    return graph, res
+
+
+def test_captured_sums_follow_their_tables(ops):
+    """Attention, the sums of a step's few rows and those of a prompt, their logarithms in hand and not, each captured and replayed with other pages, lengths and queries."""
+    few = lambda seed, lens: shared_pages.Step(gen("captured few", seed), DEV, 8, 2, 128, 64, ((256, [[lens[0]], [lens[1]], [lens[2]]]),), [[lens[3]]], poison=None, spare=12,
+                                               width=4)
+    many = lambda seed, lens: shared_pages.Step(gen("captured many", seed), DEV, 24, 4, 256, 64, (), [list(range(n - r + 1, n + 1)) for n, r in zip(lens, (200, 70))],
+                                                poison=None, spare=14, width=4)
+    for make, lens, more in ((few, (400, 310, 555, 70), ((290, 600, 257, 1), (256, 480, 301, 190))), (many, (700, 300), ((200, 640), (650, 90)))):
+        st = make(0, lens)
+        st.mass.fill_(1.0)
+        out = torch.zeros_like(st.mass)
+
+        def call():
+            o, lse = attend(ops, st)
+            ops.attention_mass(st.q, st.k, st.mass, st.kvlen, *st.args(), st.segs, st.groups, lse=lse, carry=0.5, out=out)
+            alone = ops.attention_mass(st.q, st.k, torch.zeros_like(st.mass), st.kvlen, *st.args(), st.segs, st.groups, carry=0.0)
+            return o, lse, alone
+        graphs = [captured(call) for _ in range(2)]
+        for i, now in enumerate((lens, *more)):
+            if i:
+                nxt = make(i, now)
+                pages = min(st.k.shape[0], nxt.k.shape[0])
+                width = min(st.table.shape[1], nxt.table.shape[1])
+                assert int(nxt.table.max()) < st.k.shape[0] and (nxt.table[:, width:] < 0).all()
+                st.k[:pages], st.v[:pages] = nxt.k[:pages], nxt.v[:pages]
+                st.q.copy_(nxt.q); st.kvlen.copy_(nxt.kvlen)
+                st.table.fill_(-1)
+                st.table[:, :width] = nxt.table[:, :width]
+                st.streams = nxt.streams
+            want, tol, seen = st.masses(0.5)
+            zero, ztol, _ = st.masses(0.0)
+            for graph, (o, lse, alone) in graphs:
+                out.fill_(7.0)
+                graph.replay()
+                torch.cuda.synchronize()
+                check_attend(st, o, lse)
+                assert ((out - want).abs() <= tol)[seen].all() and (out[~seen] == 7).all()
+                assert ((alone - zero).abs() <= ztol)[seen].all() and (alone[~seen] == 0).all()
+
+
+def test_captured_eviction_follows_its_tables(ops):
+    """A captured eviction replayed with other lengths, pages and sums, in a table wider than any context."""
+    keep, page, nkv = 300, 64, 2
+    first = pool(gen("captured evict", 0), [299, 301, 10000], keep, page, nkv, 8, 400)
+    table, dst, k, v, mass = (t.clone() for t in first)
+    lens, slots = i32([299, 301, 10000]), i32([0, 1, 2])
+    graph, kept = captured(lambda: ops.kv_evict(k, v, None, mass, slots, lens, table, dst, page, keep, 4, 50))
+    for i, now in enumerate(([299, 301, 10000], [8000, 1200, 1], [1000, 300, 9000], [0, 5000, 4000])):
+        nt, nd, nk, nv, nm = pool(gen("captured evict", i), now, keep, page, nkv, 8, 400)
+        n = nk.shape[0]
+        assert n <= k.shape[0] and nt.shape == table.shape
+        table.copy_(nt); dst.copy_(nd); lens.copy_(i32(now))
+        for t, x in zip((k, v, mass), (nk, nv, nm)):
+            t[:n] = x
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = ops.kv_evict(nk, nv, None, nm, slots, i32(now), nt, nd, page, keep, 4, 50)
+        assert torch.equal(kept, eager)
+        for t, x in zip((k, v, mass), (nk, nv, nm)):
+            assert torch.equal(t[:n].view(torch.uint8), x.view(torch.uint8))
+        check_evict(ops, now, keep, 4, 50, page, nkv, *pool(gen("captured evict", i), now, keep, page, nkv, 8, 400))
+
+
+def test_contexts_that_were_shrunk(ops):
+    """Sums of a step, eviction by them, attention over what stayed, to the precision of weights of twice eight bits; then a token is appended, whose sum its writer clears."""
+    nq, nkv, hd, page, keep = 8, 2, 128, 64, 200
+    st = shared_pages.Step(gen("shrunk"), DEV, nq, nkv, hd, page, ((640, [[900], [700], [1000]]),), [[333]], spare=4 * 4 + 2, poison=None, q_scale=2.0)
+    mass = torch.full_like(st.mass, 5.0)                                 # what former owners left
+    out, lse = attend(ops, st)
+    ops.attention_mass(st.q, st.k, mass, st.kvlen, *st.args(), st.segs, st.groups, lse=lse, carry=0.0)
+    used = torch.zeros(st.k.shape[0], dtype=torch.bool, device=DEV)
+    used[st.table[st.table >= 0].long()] = True
+    dst = torch.nonzero(~used).flatten()[:16].int().view(4, 4).contiguous()
+    kept = ops.kv_evict(st.k, st.v, None, mass, i32(st.slots), i32([900, 700, 1000, 333]), st.table, dst, page, keep, 4, 64)
+    assert (mass[dst[:, 3].long()][:, :, keep % page:] == 5).all()       # behind the last token: as it was
+    new = shared_pages.Step.__new__(shared_pages.Step)
+    new.__dict__.update(st.__dict__)
+    new.table, new.slots, new.member, new.groups, new.first = dst, [0, 1, 2, 3], [None] * 4, None, {}
+    new.segs = (i32([0, 1, 2, 3]), *st.segs[1:])
+    new.streams, new.kvlen = [[keep]] * 4, i32([keep] * 4)
+    check_attend(new, *attend(ops, new))
+    # the next token
+    page_of, place = dst[:, keep // page].long(), keep % page
+    st.k[page_of, place], st.v[page_of, place] = st.q[:, :nkv], st.q[:, nkv:2 * nkv]
+    mass[page_of, :, place] = 0
+    new.streams, new.kvlen, new.mass = [[keep + 1]] * 4, i32([keep + 1] * 4), mass.clone()
+    out, lse = attend(ops, new)
+    check_attend(new, out, lse)
+    check_sums(new, sums(ops, new, lse, 1.0), 1.0)
