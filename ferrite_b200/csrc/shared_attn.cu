@@ -812,14 +812,20 @@ __global__ void __launch_bounds__(256) shared_lse_join_kernel(float* lse, FbShar
   lse[id] = st.kvlen[row] <= 0 ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
 }
 
-// Columns d .. d + 3 of a head's row in which keys that the row sees have values that are no finite numbers: an infinity, if they are alike, else NaN. (A weight is
-// larger than zero, however small, but that of a score of minus infinity.) Out of line, for the rows that come across such values.
+struct SaInputs {                                // what the step's kernels read besides its tables
+  const __nv_bfloat16 *q, *k, *v, *proj;
+  long q_stride, proj_stride;
+};
+// A thread's columns d .. d + 3 of a head's row in which keys that the row sees have values that are no finite numbers: an infinity, if they are alike, else NaN, into the
+// output. (A weight is larger than zero, however small, but that of a score of minus infinity.) A walk over the context, out of line and the
+// last thing that a thread does: the rows that come across no such values keep nothing in registers for it.
 template <int HD>
-__device__ __noinline__ float4 sa_odd_columns(float4 a, const FbSharedStep& st, const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* v, int row,
-                                              int kvh, int nkv, int d) {
+__device__ __noinline__ void sa_odd_columns(__nv_bfloat16* out, const FbSharedStep& st, const SaInputs& in, int nkv, int share) {
+  const int row = blockIdx.x, h = blockIdx.y, kvh = h / share, d = threadIdx.x % (HD / 4) * 4;
+  const __nv_bfloat16 *q = in.q + (long)row * in.q_stride + (long)h * HD, *k = in.k, *v = in.v;
   int s = 0, shared = 0;
   while (s < st.nseg && (row < st.seg_row0[s] || row - st.seg_row0[s] >= st.seg_nrows[s])) ++s;
-  if (s == st.nseg) return a;
+  if (s == st.nseg) return;
   int first = -1;
   const int slot = st.seg_slot[s];
   for (int g = 0; g < st.ngrp; ++g)
@@ -857,16 +863,21 @@ __device__ __noinline__ float4 sa_odd_columns(float4 a, const FbSharedStep& st, 
       }
     }
   }
-  auto column = [&](int c, float x) { return seen >> c & 1u ? (seen >> (4 + c) & 1u ? NAN : INFINITY) : seen >> (4 + c) & 1u ? -INFINITY : x; };
-  return make_float4(column(0, a.x), column(1, a.y), column(2, a.z), column(3, a.w));
+  out += ((long)row * nkv * share + h) * HD + d;
+  for (int c = 0; c < 4; ++c) {
+    const bool above = seen >> c & 1u, below = seen >> (4 + c) & 1u;
+    float x = above && below ? NAN : above ? INFINITY : -INFINITY;
+    if (in.proj) x *= sigmoidf_(bf2f(in.proj[(long)row * in.proj_stride + (long)h * 2 * HD + HD + d + c]));
+    if (above || below) out[c] = __float2bfloat16(x);
+  }
 }
 
 // Pieces of a head's row -> output and logarithm. grid: rows x query heads; a thread has four columns and every fourth (eighth, 16th) piece. Everything that
 // does not depend on the pieces is asked for at once, and the pieces' sums beside their maxima: three trips to memory.
 template <int HD, int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__nv_bfloat16* out, float* lse, const __nv_bfloat16* proj, long proj_stride,
-                                                          const __nv_bfloat16* q, long q_stride, const __nv_bfloat16* keys, const __nv_bfloat16* values,
-                                                          const __grid_constant__ FbSharedStep st, SaSpace w, int nkv, int share, int ctas) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS)
+shared_join_kernel(__nv_bfloat16* out, float* lse, const __grid_constant__ SaInputs in, const __grid_constant__ FbSharedStep st, SaSpace w, int nkv, int share,
+                   int ctas) {
   constexpr int LANES = HD / 4, PARTS = THREADS / LANES;
   __shared__ float top_s[PARTS], sum_s[PARTS];
   __shared__ uint32_t hidden_s[PARTS];
@@ -880,8 +891,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   const int n = st.kvlen[row];
   const int4 info[2] = {w.rows[2 * row], w.rows[2 * row + 1]};
   float4 gate = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (proj && part == 0) {
-    const __nv_bfloat16* p = proj + (long)row * proj_stride + (long)h * 2 * HD + HD + d;
+  if (in.proj && part == 0) {
+    const __nv_bfloat16* p = in.proj + (long)row * in.proj_stride + (long)h * 2 * HD + HD + d;
     gate = make_float4(bf2f(p[0]), bf2f(p[1]), bf2f(p[2]), bf2f(p[3]));
   }
   if (!__syncthreads_or(mine) || per <= 0) return;                   // a row of no segment; a step that did not fit
@@ -956,13 +967,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) shared_join_kernel(__
   if (!out) return;
   const float inv = n <= 0 ? 0.f : total == 0.f ? NAN : 1.f / total;  // (scores of minus infinity only: 0 / 0)
   a.x *= inv; a.y *= inv; a.z *= inv; a.w *= inv;
-  const bool finite = fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) < INFINITY;
-  if (__builtin_expect((hidden || !finite) && total > 0.f && total < INFINITY, 0))       // weights that are numbers, of values that are none
-    a = sa_odd_columns<HD>(a, st, q + (long)row * q_stride + (long)h * HD, keys, values, row, kvh, nkv, d);
-  if (proj) {
+  const bool odd = (hidden || !(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) < INFINITY)) && total > 0.f && total < INFINITY;
+  if (in.proj) {
     a.x *= sigmoidf_(gate.x); a.y *= sigmoidf_(gate.y); a.z *= sigmoidf_(gate.z); a.w *= sigmoidf_(gate.w);
   }
   *reinterpret_cast<uint2*>(out + ((long)row * nkv * share + h) * HD + d) = make_uint2(pack_bf2(a.x, a.y), pack_bf2(a.z, a.w));
+  if (__builtin_expect(odd, 0)) sa_odd_columns<HD>(out, st, in, nkv, share);             // weights that are numbers, of values that are none
 }
 
 }  // namespace fb
@@ -1066,11 +1076,11 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
   if (e != cudaSuccess) return (int)e;
   // 256 threads a head's row where all of them run at once: more pieces under way; more rows run as twice as many CTAs of 128, since each is a chain of trips to
   // memory (us, 256 / 128: 48 rows 5.7 / 6.7, 144 6.8 / 8.0, 816 10.9 / 8.5, 2048 17.5 / 11.0)
+  const SaInputs in{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)proj, q_stride, proj_stride};
 #define FB_SJ(H, N)                                                                                                                                 \
   if (hd == H && (N == 256) == ((long)st.rows * nq <= 4l * ctas))                                                                                   \
-    return (int)launch_pdl(shared_join_kernel<H, N>, dim3(st.rows, nq), dim3(N), 0, s, (__nv_bfloat16*)out, lse, (const __nv_bfloat16*)proj,        \
-                           proj_stride, (const __nv_bfloat16*)q, q_stride, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, st, w, nkv, share, ctas);
+    return (int)launch_pdl(shared_join_kernel<H, N>, dim3(st.rows, nq), dim3(N), 0, s, (__nv_bfloat16*)out, lse, in, st, w, nkv, share, ctas);
   FB_SJ(64, 256) FB_SJ(128, 256) FB_SJ(256, 256) FB_SJ(64, 128) FB_SJ(128, 128) FB_SJ(256, 128)
 #undef FB_SJ
-  return -2;
+  return -1;
 }
