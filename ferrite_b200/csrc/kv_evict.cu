@@ -7,8 +7,9 @@
 //
 // Copy: a warp has up to 32 rows at a time; its lanes look up the pages, then all of them copy row after row, 16 bytes each.
 //
-// Measured (B200, us): 24 streams of 12000 tokens, 4 heads of 256 in bf16, 2048 stay: selection 22, copy 70 (408 MB read and written, 5.8 TB/s: HBM); two of 100000 in
-// 8 bits, 8192 stay: 30 in all, selection 23 (12500 weights a CTA, digits added up over the cluster); one of 4000, 1024 stay: 16, selection 12 of it.
+// Measured (B200, us): 24 streams of 12000 tokens, 4 heads of 256 in bf16, 2048 stay: 92, selection 22, copy 70 (408 MB read and written, 5.8 TB/s: HBM); two of 100000 in
+// 8 bits, 8192 stay: 31 in all, 36 on other inputs each time, selection 23 (12500 weights a CTA, digits added up over the cluster); one of 4000, 1024 stay: 13 to 16,
+// selection 12 of it.
 // The same in tables of 131072 tokens: one of 4000 13, four of 4000 20 (15 in tables that fit), 24 of 12000 91. 40 of 50000, whose last 5000 weights a CTA do not fit its
 // shared memory, 2048 stay: 234 (heads of 32).
 // Selection is bound by its instructions (issue slots of its SMs 40 % busy between the digits' barriers); 1024 threads a CTA take 16 for 4000 tokens and 24 for 12000, and

@@ -7,8 +7,8 @@
 // its sums. Many pairs (a prompt): 256 keys stay in tensor memory and the queries stream by; every CTA has the same number of (256 keys, 64 pairs) steps, and a
 // last kernel joins the sums of a key's pieces in their order. The exponentials are 512 cycles of an SM for 128 x 64 scores, the products 512 at 256 columns
 // (768 with the keys in shared memory: what the operands take from there).
-// Measured (B200, us): one row of 24 heads of 256 over 100000 keys 39, 5.3 TB/s; six over 8000 shared and 900 own keys each 12; 2048 rows over 16000 keys 345, tensor
-// pipe 72 % busy under the power cap, and 1111 rows of 32 heads of 128 over 5000 keys 66.
+// Measured (B200, us): one row of 24 heads of 256 over 100000 keys 41, 5.1 TB/s; six over 8000 shared and 900 own keys each 13; 2048 rows over 16000 keys 346, tensor
+// pipe 67 % busy under the power cap, and 1111 rows of 32 heads of 128 over 5000 keys 69. Clearing the keys' bits is 1 to 2 of the first two.
 // A key's sum is written once, so a key is of one span: a bit a key says that one has taken it, and a second one sets the status (idle warps ask, or those that join).
 // Every wait is bounded, as in the attention.
 #include <algorithm>
@@ -856,8 +856,8 @@ static int make_tmap_queries(CUtensorMap* out, const void* q, int rows, int nq, 
 }
 // Rows whose queries stay in shared memory
 static int km_resident_rows(int hd, int share) { return (hd == 256 ? KmCfg<256>::QS : hd == 128 ? KmCfg<128>::QS : KmCfg<64>::QS) * (KM_PAIRS / share); }
-// The form for few pairs takes all that fit (us, the most rows that stay / one row more, at 500, 16000, 60000 keys: 24 heads of 256, 30 rows 11 / 25, 20 / 34, 51 / 68;
-// 32 of 128, 80 rows 11 / 37, 36 / 41, 114 / 103; 4 of 64, 256 rows 14 / 24, 20 / 29, 47 / 51).
+// The form for few pairs takes all that fit (us, the most rows that stay / one row more, at 500, 16000, 60000 keys: 24 heads of 256, 30 rows 11 / 23, 21 / 33, 52 / 67;
+// 32 of 128, 80 rows 12 / 36, 37 / 41, 118 / 102; 4 of 64, 256 rows 14 / 23, 20 / 29, 48 / 51).
 static bool km_few(int rows, int max_rows, int ngrp, int hd, int share) { return (ngrp ? rows : std::min(rows, max_rows)) <= km_resident_rows(hd, share); }
 static long km_words(long keys) { return (keys / 32 + 3) / 4 * 4; }
 // (A span of n keys is of up to n / 256 + 2 items, and a key of the pool is of one span.)

@@ -1,5 +1,5 @@
 // Attention of a step's rows over a paged cache in which streams share the pages of a prefix, on the 5th-generation tensor cores: the keys and values of a
-// prefix are read once for all rows of its group.
+// prefix are read once for every 128 (row, head) pairs of its group.
 //
 //   S = Q K^T        128 (row, head) pairs of a block x 64 keys; Q and K in shared memory
 //   P = exp2(S - m)  two threads a pair; P as bf16 and what that leaves, as bf16 too, back into TMEM, its sums in 32 bits. (Without the remainders a weight is off by up
@@ -19,9 +19,11 @@
 // that moves it rescales O between the two products. Every wait is bounded: one that runs out sets the status word and an abort flag; the softmax warps
 // then go through their remaining barriers without work, the others leave, and the CTA frees its TMEM.
 //
-// Measured (B200, us a call): 34 rows x 24 heads of 256 over 30000 shared and 2000 own tokens each 100 (bytes alone 48), 64 x 32 of 128 over 60000 and 500 142 (52),
-// six over 8000 and 900 27 (7.5). The products of a tile are 1536 cycles at 256 columns, 63 us of the first; plan, first loads, pieces and join are 27 of it. Four sets of
-// four warps (twice the scores a thread) spill and are slower.
+// Measured (B200, us a call, on the same inputs again / on others each time): 34 rows x 24 heads of 256 over 30000 shared and 2000 own tokens each 100 / 115 (bytes alone
+// 48), 64 x 32 of 128 over 60000 and 500 141 / 166 (52), six over 8000 and 900 27 / 29 (7.5). The first is 45 tiles a CTA, 3040 cycles each with plan, first loads and
+// pieces, of which the tensor pipe is busy for the 1536 that the operations take; the second 122 of 1830 and 768. What the sets hand over to each other for every tile
+// sets the pace, and a tile of a stream's own tokens takes as long with its few pairs as one with 128. Four sets of four warps (twice the scores a thread) spill and are
+// slower.
 #include <algorithm>
 #include <cfloat>
 
@@ -1075,7 +1077,7 @@ extern "C" int fb_attention_shared(void* out, float* lse, float* ws, long ws_flo
 #undef FB_SA
   if (e != cudaSuccess) return (int)e;
   // 256 threads a head's row where all of them run at once: more pieces under way; more rows run as twice as many CTAs of 128, since each is a chain of trips to
-  // memory (us, 256 / 128: 48 rows 5.7 / 6.7, 144 6.8 / 8.0, 816 10.9 / 8.5, 2048 17.5 / 11.0)
+  // memory (us, 256 / 128: 48 heads' rows 5.7 / 6.7, 144 6.8 / 8.0, 816 10.9 / 8.5, 2048 17.5 / 11.0)
   const SaInputs in{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, (const __nv_bfloat16*)proj, q_stride, proj_stride};
 #define FB_SJ(H, N)                                                                                                                                 \
   if (hd == H && (N == 256) == ((long)st.rows * nq <= 4l * ctas))                                                                                   \

@@ -6,10 +6,11 @@ A step's rows come in segments of one slot each, `segs` = (seg_slot, seg_row0, s
 order; row i sees the first row_kvlen[i] tokens. `groups` = (grp_seg0, grp_nsegs, grp_len), or None: the rows of grp_nsegs consecutive segments from grp_seg0
 on lie side by side and read their first grp_len tokens, any number, through the table of the first of these segments, and what follows through their
 own (whose entries for whole shared pages are not looked at). A segment belongs to one group at most; one of no rows is padding, whatever its slot (but that of
-a group's first). Streams whose tables hold the same pages (a pool whose owner lets several streams have a page: samples of one prompt, forks of one
-conversation) are a group, so that their common keys and values are read once for every 128 (row, head) pairs of it. A row is of one segment; of none, it is
-left out and its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a multiple of 64. What the kernels find wrong in the
-tables on the device (a page or slot that is none, a context beyond its table, a segment of more rows than was said) sets the op class's status word.
+a group's first; inside a group it lies between the rows of its neighbours). Streams whose tables hold the same pages (a pool whose owner lets several streams
+have a page: samples of one prompt, forks of one conversation) are a group, so that their common keys and values are read once for every 128 (row, head) pairs
+of it. A row is of one segment; of none, it is left out and its output says nothing. Caches are [pages, kv_block, kv heads, head dim] in bf16, kv_block a
+multiple of 64. What the kernels find wrong in the tables on the device (a page or slot that is none, a context beyond its table, a segment of more rows than
+was said) sets the op class's status word.
 
 Where contexts are cut follows the lengths of the whole step: a row may round otherwise beside other streams, decoded or verified, than by itself (the paged
 attention of every stream by itself does not). The same call gives the same bits. A call plans 5 words a segment, 4 a group and 2 a block of rows (128 pairs of a row
@@ -142,7 +143,9 @@ class CudaShared:
 
     def attention_shared(self, q, proj, k_cache, v_cache, row_kvlen, block_table, kv_block, nq, nkv, hd, gated, segs, groups=None, want_lse=False):
         """Attention of a step's rows over a cache whose streams share pages; the oracle's docstring and the top of this file say what of. `proj` is read
-        for the output gate only."""
+        for the output gate only. It takes less time than the paged attention of every stream by itself from about 4 streams of 1024 shared tokens on, or 2 of
+        4096 (24 query heads of 256 columns over 4; 32 of 128 over 8: 16 of 1024, 4 of 4096, 2 of 16000): at 32 of 16000 55 us instead of 529. Below that,
+        and for up to four streams without groups, it takes up to 8 us more."""
         if gated and proj is None:
             raise RuntimeError("attention_shared: no proj to gate with")
         q, step = self._shared_step(q, nq, hd, segs, groups)
