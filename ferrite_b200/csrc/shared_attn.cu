@@ -831,7 +831,7 @@ __device__ __noinline__ void sa_odd_columns(__nv_bfloat16* out, const FbSharedSt
   int first = -1;
   const int slot = st.seg_slot[s];
   for (int g = 0; g < st.ngrp; ++g)
-    if (s >= st.grp_seg0[g] && s - st.grp_seg0[g] < st.grp_nsegs[g] && st.grp_seg0[g] >= 0) {
+    if (st.grp_seg0[g] >= 0 && s >= st.grp_seg0[g] && s - st.grp_seg0[g] < st.grp_nsegs[g]) {
       first = st.seg_slot[st.grp_seg0[g]];
       shared = max(st.grp_len[g], 0);
     }
